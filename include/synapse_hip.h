@@ -614,6 +614,141 @@ syn_status_t syn_hip_hlm_set_options(syn_hip_hlm_t *m, int fused, int graph);
 syn_status_t syn_hip_hlm_fused_active(syn_hip_hlm_t *m, int *active);
 syn_status_t syn_hip_hlm_destroy(syn_hip_hlm_t *m);
 
+/* =====================================================================
+ * 3. Beam decoding over a paged key/value cache (no reference counterpart):
+ *    several continuations of one or more prompts decoded together.  All
+ *    buffers are the caller's, on the current device; calls are asynchronous
+ *    on `stream` (NULL = the library's stream), allocate nothing and may be
+ *    captured into a graph: lengths, positions, tables and parents are read
+ *    on the device.  Two calls that overlap (streams, captured graphs) need a
+ *    workspace each.
+ * =================================================================== */
+#define SYN_HIP_KV_F32 0
+#define SYN_HIP_KV_F16 1
+#define SYN_HIP_KV_BF16 2
+/* A pool of pages, each page_size positions of every kv head:
+ *   k [n_layers][n_pages][n_kv_heads][head_dim / 8][page_size][8]
+ *   v [n_layers][n_pages][n_kv_heads][page_size / 8][head_dim][8]
+ * page_size: a power of two, 8 to 1024; head_dim: a multiple of 8 up to 256;
+ * k and v 16-byte aligned.  A sequence's positions are found through its row
+ * of a page table: position i in page table[i / page_size], slot
+ * i % page_size.  Entries outside [0, n_pages) name no page. */
+typedef struct {
+  int32_t dtype; /* SYN_HIP_KV_* */
+  uint32_t page_size, n_pages, n_layers, n_kv_heads, head_dim;
+  void *k, *v;
+} syn_hip_kv_pages;
+
+/* Keys and values of n_tokens tokens into the pages of one layer, with the
+ * decoders' q/k head norms (x * gain / sqrt(mean x^2 + eps); NULL gains: none)
+ * and position rotation on the way; the query heads are normed and rotated
+ * into d_q_out.  d_q [n_tokens][n_heads][head_dim], d_k and d_v
+ * [n_tokens][n_kv_heads][head_dim], rows ldq, ldk and ldv floats apart (a
+ * stacked q|k|v row has one stride for the three), d_q_out rows ldo apart.
+ * The first rotary_dim dims of a head are rotated (even, 0 to head_dim) in
+ * pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved: a' = a cos
+ * - b sin, b' = b cos + a sin with d_cos, d_sin [n_positions][rotary_dim / 2]
+ * at row d_pos[t].  Token t belongs to sequence d_seq[t] (NULL: t), row of
+ * d_table [n_seqs][ld_table], and is stored at that sequence's position
+ * d_index[t].  A token with d_pos outside [0, n_positions) is skipped
+ * altogether; one whose d_index is negative or past the table, or whose page
+ * is outside the pool, is rotated but not stored (padding).  Tokens stored at
+ * the same place leave either's values there.  n_heads = 0: no queries (d_q
+ * and d_q_out unused).  d_q_out may be d_q with ldo == ldq. */
+typedef struct {
+  uint32_t layer, n_heads, n_seqs, rotary_dim;
+  int32_t interleaved;
+  uint32_t n_positions;
+  float eps;
+  size_t ldq, ldk, ldv, ldo, ld_table;
+} syn_hip_kv_append_params;
+syn_status_t syn_hip_kv_append(const syn_hip_kv_pages *pages, const syn_hip_kv_append_params *p,
+                               size_t n_tokens, const float *d_q, const float *d_k,
+                               const float *d_v, const float *d_q_norm, const float *d_k_norm,
+                               const float *d_cos, const float *d_sin, const int32_t *d_pos,
+                               const int32_t *d_seq, const int32_t *d_index,
+                               const int32_t *d_table, float *d_q_out, void *stream);
+
+/* Attention of one query token per sequence, for n_groups groups of group_size
+ * sequences that share a prefix: out = softmax(scale q K^T) V over the
+ * group's prefix (d_prefix_len[g] positions found through row g of
+ * d_prefix_table [n_groups][ld_prefix_table]) and the sequence's own suffix
+ * (d_len[s] positions, from slot 0 of the first page of row s of d_table
+ * [n_groups * group_size][ld_table]).  The prefix is read once for the whole
+ * group.  d_q and d_out [sequences][n_heads][head_dim], rows ldq and ldo
+ * apart, n_heads a multiple of n_kv_heads (query head h reads kv head
+ * h / (n_heads / n_kv_heads)); scale 0: 1 / sqrt(head_dim).  max_prefix and
+ * max_suffix bound the lengths, which are cut to them (they and the table
+ * widths decide the split of the work, so a captured call keeps them);
+ * a negative length is 0.  Positions in pages outside the pool are left out;
+ * a sequence with no position gives zeros.  Scores, softmax and sums are f32;
+ * 16-bit pools are read as stored.  The workspace holds the parts of a split
+ * prefix or suffix (size from syn_hip_prefix_attention_workspace, which may
+ * be 0; 16-byte aligned). */
+typedef struct {
+  uint32_t layer, n_heads, n_groups, group_size, max_prefix, max_suffix;
+  float scale;
+  size_t ldq, ldo, ld_prefix_table, ld_table;
+} syn_hip_prefix_attention_params;
+syn_status_t syn_hip_prefix_attention_workspace(const syn_hip_kv_pages *pages,
+                                                const syn_hip_prefix_attention_params *p,
+                                                size_t *bytes);
+syn_status_t syn_hip_prefix_attention(const syn_hip_kv_pages *pages,
+                                      const syn_hip_prefix_attention_params *p, const float *d_q,
+                                      const int32_t *d_prefix_table, const int32_t *d_prefix_len,
+                                      const int32_t *d_table, const int32_t *d_len, float *d_out,
+                                      void *d_workspace, size_t workspace_bytes, void *stream);
+
+/* Beam search's choice: for each of n_groups groups the n_select best of its
+ * n_beams * vocab continuations, best first.  The value of token t after beam
+ * b is d_scores[b] + d_logits[b][t] - log(sum of exp(d_logits[b])), with
+ * d_scores and d_finished [n_groups * n_beams] and d_logits rows ld_logits
+ * floats apart.  Equal values go to the lower beam, then the lower token; the
+ * tokens of one beam are ordered by their logits, beams against each other by
+ * values formed in f64 (d_score: rounded once to f32).  A NaN logit counts as
+ * -inf; a row whose largest logit is +inf shares its probability among the
+ * infinities; every continuation of a beam whose score is NaN or infinite is
+ * -inf.  A beam whose d_finished is not 0 (NULL: none) is not
+ * read: its one continuation is `pad` at its score, every other one -inf.
+ * d_parent gets the beam within the group, d_token the token, d_finished_out
+ * (nullable) whether the parent was finished or the token is eos (-1: none).
+ * 1 <= n_beams <= 64, 1 <= n_select <= 128, n_select <= n_beams * vocab;
+ * d_score may be d_scores and d_finished_out d_finished when n_select ==
+ * n_beams.  The workspace (16-byte aligned) is needed by every call. */
+typedef struct {
+  uint32_t n_groups, n_beams, n_select;
+  int32_t eos, pad;
+  size_t vocab, ld_logits;
+} syn_hip_beam_select_params;
+syn_status_t syn_hip_beam_select_workspace(const syn_hip_beam_select_params *p, size_t *bytes);
+syn_status_t syn_hip_beam_select(const syn_hip_beam_select_params *p, const float *d_logits,
+                                 const float *d_scores, const int32_t *d_finished,
+                                 int32_t *d_parent, uint32_t *d_token, float *d_score,
+                                 int32_t *d_finished_out, void *d_workspace,
+                                 size_t workspace_bytes, void *stream);
+
+/* States follow the chosen beams, in place: in each of n_buffers buffers
+ * (buffer_stride bytes apart), row g * n_beams + b becomes what row
+ * g * n_beams + d_parent[g * n_beams + b] was.  row_bytes of every row_stride
+ * bytes are moved; a parent outside [0, n_beams) leaves its row as it is. */
+syn_status_t syn_hip_beam_reorder_rows(size_t n_groups, size_t n_beams, const int32_t *d_parent,
+                                       void *d_rows, size_t row_bytes, size_t row_stride,
+                                       size_t n_buffers, size_t buffer_stride, void *stream);
+/* The same for paged caches, every layer of the pool, without moving what is
+ * already a whole page.  d_len[g] is the number of positions that each beam of
+ * group g holds (cut to the table's), d_table [n_groups * n_beams][ld_table].
+ * A row takes its parent's entries for the pages that are full; the page that
+ * is not is copied (positions up to the next multiple of 8) into the page
+ * d_spare[row], which becomes the row's, and the row's own old one becomes its
+ * spare.  The entries after it stay the row's.  So if every entry from column
+ * d_len[g] / page_size on and every spare name distinct pages that nothing
+ * else refers to, that stays so, with no allocator and no count of references:
+ * pages are filled by one row at a time and never written again once full. */
+syn_status_t syn_hip_beam_reorder_pages(const syn_hip_kv_pages *pages, size_t n_groups,
+                                        size_t n_beams, const int32_t *d_parent,
+                                        const int32_t *d_len, int32_t *d_table, size_t ld_table,
+                                        int32_t *d_spare, void *stream);
+
 /* -- harness helpers (no reference counterpart) -- */
 /* Encode f32 [n,k] into Q8_0 / Q4_K / Q6_K block bytes.  The reference has no
  * encoder for these formats (only dequantizers); any encoding is valid since

@@ -63,6 +63,40 @@ class HybridConfig(C.Structure):
                 ("conv_bias", C.c_int32), ("layer_kinds", C.c_uint8 * 64)]
 
 
+KV_F32, KV_F16, KV_BF16 = 0, 1, 2
+
+
+class KvPages(C.Structure):
+    """syn_hip_kv_pages: a pool of key/value pages on the device."""
+    _fields_ = [("dtype", C.c_int32), ("page_size", C.c_uint32), ("n_pages", C.c_uint32),
+                ("n_layers", C.c_uint32), ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("k", C.c_void_p), ("v", C.c_void_p)]
+
+
+class KvAppend(C.Structure):
+    """syn_hip_kv_append_params"""
+    _fields_ = [("layer", C.c_uint32), ("n_heads", C.c_uint32), ("n_seqs", C.c_uint32),
+                ("rotary_dim", C.c_uint32), ("interleaved", C.c_int32),
+                ("n_positions", C.c_uint32), ("eps", C.c_float), ("ldq", C.c_size_t),
+                ("ldk", C.c_size_t), ("ldv", C.c_size_t), ("ldo", C.c_size_t),
+                ("ld_table", C.c_size_t)]
+
+
+class PrefixAttention(C.Structure):
+    """syn_hip_prefix_attention_params"""
+    _fields_ = [("layer", C.c_uint32), ("n_heads", C.c_uint32), ("n_groups", C.c_uint32),
+                ("group_size", C.c_uint32), ("max_prefix", C.c_uint32),
+                ("max_suffix", C.c_uint32), ("scale", C.c_float), ("ldq", C.c_size_t),
+                ("ldo", C.c_size_t), ("ld_prefix_table", C.c_size_t), ("ld_table", C.c_size_t)]
+
+
+class BeamSelect(C.Structure):
+    """syn_hip_beam_select_params"""
+    _fields_ = [("n_groups", C.c_uint32), ("n_beams", C.c_uint32), ("n_select", C.c_uint32),
+                ("eos", C.c_int32), ("pad", C.c_int32), ("vocab", C.c_size_t),
+                ("ld_logits", C.c_size_t)]
+
+
 SIGNATURES = {
     "syn_quantize_per_channel_int8": (ST, [P, SZ, SZ, P, P]),
     "syn_qgemm_int8": (ST, [SZ, SZ, SZ, P, SZ, P, SZ, P, SZ, P, P]),
@@ -123,6 +157,15 @@ SIGNATURES = {
     "syn_hip_qlm_set_options": (ST, [P, C.c_int, C.c_int]),
     "syn_hip_qlm_set_sampler": (ST, [P, C.POINTER(SamplerParams), C.c_uint64]),
     "syn_hip_sample": (ST, [P, SZ, P, SZ, C.POINTER(SamplerParams), C.c_float, P, P, P]),
+    "syn_hip_kv_append": (ST, [C.POINTER(KvPages), C.POINTER(KvAppend), SZ] + [P] * 13),
+    "syn_hip_prefix_attention_workspace": (ST, [C.POINTER(KvPages), C.POINTER(PrefixAttention),
+                                                C.POINTER(SZ)]),
+    "syn_hip_prefix_attention": (ST, [C.POINTER(KvPages), C.POINTER(PrefixAttention)] + [P] * 7
+                                 + [SZ, P]),
+    "syn_hip_beam_select_workspace": (ST, [C.POINTER(BeamSelect), C.POINTER(SZ)]),
+    "syn_hip_beam_select": (ST, [C.POINTER(BeamSelect)] + [P] * 8 + [SZ, P]),
+    "syn_hip_beam_reorder_rows": (ST, [SZ, SZ, P, P, SZ, SZ, SZ, SZ, P]),
+    "syn_hip_beam_reorder_pages": (ST, [C.POINTER(KvPages), SZ, SZ, P, P, P, SZ, P, P]),
     "syn_hip_stdrng_f32": (ST, [C.c_uint64, SZ, P]),
     "syn_hip_qlm_time_lm_head_rotating": (ST, [P, SZ, C.POINTER(C.c_float)]),
     "syn_hip_qlm_time_step_kernels": (ST, [P, SZ, P, P]),
