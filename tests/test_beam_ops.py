@@ -76,7 +76,7 @@ def attention(pg=None, ptrs=None, ws=None, ws_bytes=None, **kw):
     a.update(ptrs or {})
     got = hip.lib().syn_hip_prefix_attention(
         C.byref(pg), C.byref(p), *[a[x] for x in ("q", "pt", "pl", "t", "l", "out")],
-        FAKE if ws is None else ws, need.value if ws_bytes is None else ws_bytes, None)
+        FAKE if ws is None else (ws or None), need.value if ws_bytes is None else ws_bytes, None)
     if st != OK:
         assert got == st  # the size and the call refuse the same descriptions
     return got
@@ -97,6 +97,16 @@ def test_attention_refuses_pages(kw, want):
     (dict(ptrs=dict(l=None)), NULL), (dict(n_groups=0), OK), (dict(group_size=0), OK)])
 def test_attention_refuses(kw, want):
     assert attention(**kw) == want
+
+
+LONG = dict(max_prefix=4000, max_suffix=900, ld_prefix_table=250, ld_table=57)
+
+
+@pytest.mark.parametrize("kw,want", [(dict(ws_bytes=64), ARG), (dict(ws=FAKE + 4), ARG),
+                                     (dict(ws=0), NULL)])
+def test_attention_refuses_workspaces(kw, want):
+    """lengths that are split need one"""
+    assert attention(**LONG, **kw) == want
 
 
 def test_attention_null_structs():
