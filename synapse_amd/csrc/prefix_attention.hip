@@ -29,6 +29,10 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr int kWaves = 4;
 constexpr int kTile = 32;  // positions a wave takes at a time
+#ifndef KWANT
+#define KWANT 512
+#endif
+constexpr size_t kWant = KWANT;
 
 struct AttnArgs {
   const float *q;
@@ -40,8 +44,9 @@ struct AttnArgs {
   // the split: positions of a part (a multiple of kTile * kWaves), parts of
   // the longest prefix and suffix; parts of query row (sequence, head) are
   // po[(sequence * nh + head) * (npp + nsp) + part][hd], pml[..][2] (max, sum)
-  int pchunk, schunk, npp, nsp;
+  int pchunk, schunk, npp, nsp, prefix_wgs;
   float *po, *pml;
+  bool q16;  // rows of queries are 16-byte aligned
 };
 
 // ---------------------------------------------------------------- products
@@ -135,11 +140,11 @@ __device__ __forceinline__ float groups_sum(float x) {
   return x + __shfl_xor(x, 32);
 }
 
-// What a workgroup works on: query rows row0 .. row0 + rows of kv head `head`
-// (row = member * rep + its query head), and up to two runs of positions.
+// Positions from .. to of a page table, dealt to the waves by tiles, the first
+// to wave `first`.
 struct Run {
   const int32_t *table;
-  int from, to, len;  // positions from .. min(to, len)
+  int from, to, first;
 };
 
 // RT: tiles of 16 query rows; NC: 32 dims each (hd <= 32 NC)
@@ -147,85 +152,165 @@ template <class T, int NC, int RT> struct Attend {
   using F = Frag<T>;
   using V = typename F::V;
   static constexpr int DT = 2 * NC;
-  V q[RT][NC][F::kParts];
+  static constexpr int kLd = 32 * NC + 4;  // f32 rows on different banks
+  static constexpr size_t kQueryBytes = (size_t)RT * NC * F::kParts * 64 * sizeof(V);
+  static constexpr size_t kJoinBytes = (size_t)kWaves * 16 * kLd * 4;
+  static constexpr size_t kLdsBytes = kQueryBytes > kJoinBytes ? kQueryBytes : kJoinBytes;
+  // the queries' parts stay in LDS where registers would not hold them
+  static constexpr bool kKeep = RT * NC * F::kParts * sizeof(V) <= 64 * 4;
+  V q[kKeep ? RT : 1][NC][F::kParts], kf[2][NC], vf[DT];
+  const V *qs;  // [RT][NC][parts][64 lanes]
   f32x4 o[RT][DT];
   float m[RT], l[RT], unscale[RT];
+  int page_k, page_v;  // of the tile whose K and V are loaded next
 
-  // the rows' queries times scale, each row of an f16 pool times the power of
+  // The rows' queries times scale, each row for an f16 pool times the power of
   // two that puts its largest element into [2^11, 2^12): both parts of every
-  // element that matters are normal
+  // element that matters are normal.  Wave t splits tile t for all.
   __device__ __forceinline__ void load_queries(const AttnArgs &a, int hd, int seq0, int head, int row0,
-                                               int rows) {
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int t = 0; t < RT; t++) {
-      const int r = row0 + t * 16 + n;
+                                               int rows, uint8_t *lds, float *scales) {
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, t = threadIdx.x >> 6;
+    V *to = reinterpret_cast<V *>(lds);
+    qs = to;
+    if (t < RT) {
       const bool on = t * 16 + n < rows;
-      const int member = on ? r / a.rep : 0;
+      const int r = row0 + min(t * 16 + n, rows - 1), member = r / a.rep;
       const float *src = a.q + (size_t)(seq0 + member) * a.ldq +
-                         (size_t)(head * a.rep + (on ? r - member * a.rep : 0)) * hd;
+                         (size_t)(head * a.rep + (r - member * a.rep)) * hd;
       float x[NC][8], top = 0.0f;
+      if (a.q16) {
 #pragma unroll
-      for (int c = 0; c < NC; c++) {
-        const int d = (c * 4 + g) * 8;
+        for (int c = 0; c < NC; c++) {
+          const f32x4 *p = reinterpret_cast<const f32x4 *>(src + min((c * 4 + g) * 8, hd - 8));
+          const f32x4 u = p[0], v = p[1];
+#pragma unroll
+          for (int j = 0; j < 4; j++) x[c][j] = u[j], x[c][j + 4] = v[j];
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+          for (int j = 0; j < 8; j++) x[c][j] = src[min((c * 4 + g) * 8, hd - 8) + j];
+      }
+#pragma unroll
+      for (int c = 0; c < NC; c++)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-          x[c][j] = on && d < hd ? src[d + j] * a.scale : 0.0f;
+          x[c][j] = on && (c * 4 + g) * 8 < hd ? x[c][j] * a.scale : 0.0f;
           top = fmaxf(top, fabsf(x[c][j]));
         }
-      }
       int e = 0;
       if constexpr (F::kParts == 2) {
         top = groups_max(top);
         if (top > 0.0f && top < __builtin_huge_valf()) e = 11 - ilogbf(top);
-        // a power of two within f32's own range either way
-        e = min(max(e, -120), 120);
+        e = min(max(e, -120), 120);  // a power of two within f32's own range either way
       }
       const float up = __builtin_ldexpf(1.0f, e);
-      unscale[t] = __builtin_ldexpf(1.0f, -e);
+      if (g == 0) scales[t * 16 + n] = __builtin_ldexpf(1.0f, -e);
 #pragma unroll
       for (int c = 0; c < NC; c++) {
         if constexpr (F::kParts == 2)
 #pragma unroll
           for (int j = 0; j < 8; j++) x[c][j] *= up;
-        F::split(x[c], q[t][c]);
-      }
-      m[t] = kNegInf;
-      l[t] = 0.0f;
+        V part[F::kParts];
+        F::split(x[c], part);
 #pragma unroll
-      for (int d = 0; d < DT; d++) o[t][d] = f32x4{0, 0, 0, 0};
+        for (int k = 0; k < F::kParts; k++) to[((t * NC + c) * F::kParts + k) * 64 + lane] = part[k];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < RT; u++) {
+      if constexpr (kKeep)
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+          for (int k = 0; k < F::kParts; k++) q[u][c][k] = qs[((u * NC + c) * F::kParts + k) * 64 + lane];
+      unscale[u] = scales[u * 16 + n];
+      m[u] = kNegInf;
+      l[u] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DT; d++) o[u][d] = f32x4{0, 0, 0, 0};
     }
   }
 
-  // the wave's tiles of a run: kTile positions every kTile * kWaves
-  __device__ __forceinline__ void run(const KvPool<T> &pool, int head, int rows, const Run &r) {
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
-    const int to = min(r.to, r.len), hd = pool.hd, d8 = hd >> 3;
-    const int last = (to - 1) & ~7;  // the last group of 8 positions
-    for (int k0 = r.from + wave * kTile; k0 < to; k0 += kTile * kWaves) {
-      // lane (g, n): K of the 8 positions of group n / 4, V of those of group g
-      const int kk = min(k0 + 8 * (n >> 2), last), kv = min(k0 + 8 * g, last);
-      int pk = r.table[kk >> pool.ps_shift], pv = r.table[kv >> pool.ps_shift];
-      const bool has_k = pool.has(pk), has_v = pool.has(pv);
-      // whole: every position of the tile is there
+  // Lane (g, n) reads K of the group of 8 positions n / 4 of a tile and V of
+  // group g.  Positions past the end are read at the last group there is.
+  __device__ __forceinline__ int spot(int k0, int group, int to) { return min(k0 + 8 * group, (to - 1) & ~7); }
+  __device__ __forceinline__ void load_pages(const KvPool<T> &pool, const Run &r, int k0) {
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    page_k = r.table[spot(k0, n >> 2, r.to) >> pool.ps_shift];
+    page_v = r.table[spot(k0, g, r.to) >> pool.ps_shift];
+  }
+  __device__ __forceinline__ void load_k(const KvPool<T> &pool, int head, const Run &r, int k0) {
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int slot = (spot(k0, n >> 2, r.to) & (pool.ps - 1)) + (n & 3);
+    const T *kp = pool.k + pool.base(pool.has(page_k) ? page_k : 0, head) + (size_t)slot * 8;
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+      const size_t at = (size_t)min(c * 4 + g, (pool.hd >> 3) - 1) * pool.ps * 8;
+      kf[0][c] = F::load(kp + at);
+      kf[1][c] = F::load(kp + at + 32);
+    }
+  }
+  __device__ __forceinline__ void load_v(const KvPool<T> &pool, int head, const Run &r, int k0) {
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int group = (spot(k0, g, r.to) & (pool.ps - 1)) >> 3;
+    const T *vp = pool.v + pool.base(pool.has(page_v) ? page_v : 0, head) + (size_t)group * pool.hd * 8;
+#pragma unroll
+    for (int d = 0; d < DT; d++) vf[d] = F::load(vp + (size_t)min(d * 16 + n, pool.hd - 1) * 8);
+  }
+
+  // The wave's tiles of a run.  One set of registers: the next tile's K is
+  // requested when this one's scores are formed, its V when this one's product
+  // is, its pages a tile ahead of both.
+  template <int ACT>  // tiles of query rows in use
+  __device__ __forceinline__ void run_tiles(const KvPool<T> &pool, int head, const Run &r) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
+    constexpr int kStep = kTile * kWaves;
+    const int to = r.to;
+    int k0 = r.from + ((wave - r.first) & (kWaves - 1)) * kTile;
+    if (k0 >= to) return;
+    load_pages(pool, r, k0);
+    bool has_k = pool.has(page_k), has_v = pool.has(page_v);
+    load_k(pool, head, r, k0);
+    load_v(pool, head, r, k0);
+    load_pages(pool, r, k0 + kStep);
+    for (;;) {
+      const int k1 = k0 + kStep;
       const bool whole = __all(k0 + kTile <= to && has_k && has_v);
-      pk = has_k ? pk : 0;
-      pv = has_v ? pv : 0;
-      const T *kp = pool.k + pool.base(pk, head) + (size_t)((kk & (pool.ps - 1)) + (n & 3)) * 8;
-      const T *vp = pool.v + pool.base(pv, head) + (size_t)((kv & (pool.ps - 1)) >> 3) * hd * 8;
-      V kf[2][NC], vf[DT];
-#pragma unroll
-      for (int c = 0; c < NC; c++) {
-        const size_t at = (size_t)min(c * 4 + g, d8 - 1) * pool.ps * 8;
-        kf[0][c] = F::load(kp + at);
-        kf[1][c] = F::load(kp + at + 32);
-      }
-#pragma unroll
-      for (int d = 0; d < DT; d++) vf[d] = F::load(vp + (size_t)min(d * 16 + n, hd - 1) * 8);
       uint32_t there = 0xff;  // of the positions 8g .. 8g+7 whose weights this lane holds
       if (!whole) {
         const int left = has_v ? to - (k0 + 8 * g) : 0;
         there = left >= 8 ? 0xff : (left <= 0 ? 0 : (1u << left) - 1);
+      }
+      f32x4 s[ACT][2];
+#pragma unroll
+      for (int t = 0; t < ACT; t++) {
+        s[t][0] = s[t][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+          if constexpr (kKeep) {
+            s[t][0] = F::mma(kf[0][c], q[t][c], s[t][0]);
+            s[t][1] = F::mma(kf[1][c], q[t][c], s[t][1]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < F::kParts; k++) q[0][c][k] = qs[((t * NC + c) * F::kParts + k) * 64 + lane];
+            s[t][0] = F::mma(kf[0][c], q[0][c], s[t][0]);
+            s[t][1] = F::mma(kf[1][c], q[0][c], s[t][1]);
+          }
+        }
+      }
+      // Read the sums before the next branch: where a conditional region lies
+      // between, the compiler pads the matrix instruction's latency on the
+      // longer way only.
+#pragma unroll
+      for (int t = 0; t < ACT; t++) asm volatile("" : "+v"(s[t][0]), "+v"(s[t][1]));
+      if (k1 < to) {
+        has_k = pool.has(page_k);
+        load_k(pool, head, r, k1);
+      }
+      if (!whole) {  // what is not there may hold anything: 0 times NaN is NaN
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -233,17 +318,10 @@ template <class T, int NC, int RT> struct Attend {
             if (!(there >> j & 1)) F::clear(vf[d], j);
       }
 #pragma unroll
-      for (int t = 0; t < RT; t++) {
-        if (RT > 1 && t * 16 >= rows) break;
-        f32x4 s0{0, 0, 0, 0}, s1{0, 0, 0, 0};
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-          s0 = F::mma(kf[0][c], q[t][c], s0);
-          s1 = F::mma(kf[1][c], q[t][c], s1);
-        }
+      for (int t = 0; t < ACT; t++) {
         float x[8];
 #pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = s0[j] * unscale[t], x[j + 4] = s1[j] * unscale[t];
+        for (int j = 0; j < 4; j++) x[j] = s[t][0][j] * unscale[t], x[j + 4] = s[t][1][j] * unscale[t];
         if (!whole)
 #pragma unroll
           for (int j = 0; j < 8; j++) x[j] = there >> j & 1 ? x[j] : kNegInf;
@@ -268,51 +346,71 @@ template <class T, int NC, int RT> struct Attend {
           o[t][d] = F::mma(vf[d], p, o[t][d]);
         }
       }
+      if (k1 >= to) break;
+      const bool next_v = pool.has(page_v);
+      const int pv = page_v;
+      load_pages(pool, r, k1 + kStep);
+      const int ahead = page_v;
+      page_v = pv;
+      load_v(pool, head, r, k1);
+      page_v = ahead;
+      has_v = next_v;
+      k0 = k1;
     }
   }
 
-  // the four waves' results joined, in the order of the waves; a row's goes to
-  // the output, or to its part of the workspace
+  __device__ __forceinline__ void run(const KvPool<T> &pool, int head, int rows, const Run &r) {
+    if (RT == 1 || rows <= 16)
+      run_tiles<1>(pool, head, r);
+    else if (RT == 2 || rows <= 32)
+      run_tiles<RT < 2 ? RT : 2>(pool, head, r);
+    else
+      run_tiles<RT>(pool, head, r);
+  }
+
+  // The four waves' results joined, in the order of the waves; a row's goes to
+  // the output, or to its part of the workspace.
   __device__ __forceinline__ void finish(const AttnArgs &a, int hd, int seq0, int head, int row0, int rows,
                                          int part, float *buf, float *ml) {
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4, wave = tid >> 6;
-    constexpr int LD = 32 * NC + 4;  // rows on different banks
+    constexpr int kCols = 8 * NC;  // of four dims
 #pragma unroll
     for (int t = 0; t < RT; t++) {
       if (t * 16 >= rows) break;
       const float sum = groups_sum(l[t]);
       __syncthreads();
       if (g == 0) ml[(wave * 16 + n) * 2] = m[t], ml[(wave * 16 + n) * 2 + 1] = sum;
-      __syncthreads();
-      float top = ml[n * 2];
-#pragma unroll
-      for (int w = 1; w < kWaves; w++) top = fmaxf(top, ml[(w * 16 + n) * 2]);
-      const float f = m[t] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m[t] - top);
 #pragma unroll
       for (int d = 0; d < DT; d++)
-        *reinterpret_cast<f32x4 *>(buf + (wave * 16 + n) * LD + d * 16 + g * 4) = o[t][d] * f;
+        *reinterpret_cast<f32x4 *>(buf + (wave * 16 + n) * kLd + d * 16 + g * 4) = o[t][d];
       __syncthreads();
-      for (int i = tid; i < 16 * hd; i += 64 * kWaves) {
-        const int r = i / hd, d = i - r * hd;
-        if (t * 16 + r >= rows) break;
-        float mx = ml[r * 2], ls = 0.0f, x = 0.0f;
 #pragma unroll
-        for (int w = 1; w < kWaves; w++) mx = fmaxf(mx, ml[(w * 16 + r) * 2]);
+      for (int i = tid; i < 16 * kCols; i += 64 * kWaves) {
+        const int r = i / kCols, c = i % kCols;
+        if (t * 16 + r >= rows || 4 * c >= hd) continue;
+        float mw[kWaves], ls = 0.0f, mx = kNegInf;
+        f32x4 x{0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) mx = fmaxf(mx, mw[w] = ml[(w * 16 + r) * 2]);
 #pragma unroll
         for (int w = 0; w < kWaves; w++) {
-          const float mw = ml[(w * 16 + r) * 2];
-          x += buf[(w * 16 + r) * LD + d];
-          // (the sum of a wave with no position is 0, or NaN if its scores were)
-          ls += ml[(w * 16 + r) * 2 + 1] * (mw == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(mw - mx));
+          // (a wave with no position has sums of 0, or of NaN if its scores were)
+          const float f = mw[w] == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(mw[w] - mx);
+          const f32x4 y = *reinterpret_cast<const f32x4 *>(buf + (w * 16 + r) * kLd + 4 * c);
+          ls = __builtin_fmaf(ml[(w * 16 + r) * 2 + 1], f, ls);
+#pragma unroll
+          for (int k = 0; k < 4; k++) x[k] = __builtin_fmaf(y[k], f, x[k]);
         }
         const int row = row0 + t * 16 + r, member = row / a.rep;
         const size_t qh = (size_t)head * a.rep + (row - member * a.rep), seq = seq0 + member;
         if (part < 0) {
-          a.out[seq * a.ldo + qh * hd + d] = ls == 0.0f ? 0.0f : x / ls;
+          float *out = a.out + seq * a.ldo + qh * hd + 4 * c;
+#pragma unroll
+          for (int k = 0; k < 4; k++) out[k] = ls == 0.0f ? 0.0f : x[k] / ls;
         } else {
           const size_t at = (seq * a.nh + qh) * (a.npp + a.nsp) + part;
-          a.po[at * hd + d] = x;
-          if (d == 0) a.pml[at * 2] = mx, a.pml[at * 2 + 1] = ls;
+          *reinterpret_cast<f32x4 *>(a.po + at * hd + 4 * c) = x;
+          if (c == 0) a.pml[at * 2] = mx, a.pml[at * 2 + 1] = ls;
         }
       }
     }
@@ -323,83 +421,103 @@ __device__ __forceinline__ int clamped(const int32_t *len, int i, int most) {
   return most ? max(0, min(len[i], most)) : 0;
 }
 
-// kJoined: one workgroup has both runs of a sequence whole; else the parts of
-// the prefixes, or of the suffixes
-enum { kJoined, kPrefix, kSuffix };
-
-template <class T, int NC, int RT, int WHAT>
+// JOINED: a workgroup has both runs of a sequence's rows whole.  Else the
+// first workgroups have the parts of the prefixes, the others those of the
+// suffixes.
+template <class T, int NC, int RT, bool JOINED>
 __global__ void __launch_bounds__(64 * kWaves) k_attend(AttnArgs a, KvPool<T> pool) {
-  __shared__ __align__(16) float buf[kWaves * 16 * (32 * NC + 4)];
-  __shared__ float ml[kWaves * 16 * 2];
-  const int members = WHAT == kPrefix ? a.group_size : 1;  // sequences whose rows go together
+  using W = Attend<T, NC, RT>;
+  __shared__ __align__(16) uint8_t lds[W::kLdsBytes];
+  __shared__ float ml[kWaves * 16 * 2], scales[RT * 16];
+  const bool prefix = !JOINED && (int)blockIdx.x < a.prefix_wgs;
+  const int i = JOINED || prefix ? blockIdx.x : blockIdx.x - a.prefix_wgs;
+  const int members = prefix ? a.group_size : 1;  // sequences whose rows go together
   const int all = members * a.rep, blocks = (all + RT * 16 - 1) / (RT * 16);
-  const int parts = WHAT == kPrefix ? a.npp : (WHAT == kSuffix ? a.nsp : 1);
+  const int parts = JOINED ? 1 : (prefix ? a.npp : a.nsp);
   // workgroup i runs on XCD i % 8: the blocks of rows that read the same
   // positions come 8 apart and share that XCD's L2
-  const int i = blockIdx.x, j = i >> 3;
-  const int unit = (j / blocks) * 8 + (i & 7), block = j % blocks;
+  const int j = i >> 3, unit = (j / blocks) * 8 + (i & 7), block = j % blocks;
   const int head = unit % pool.nkv, u = unit / pool.nkv;
   const int part = u % parts, owner = u / parts;  // group or sequence
   if (owner * members >= a.n_seqs) return;
   const int seq0 = owner * members, row0 = block * RT * 16, rows = min(RT * 16, all - row0);
-  const int group = WHAT == kPrefix ? owner : owner / a.group_size;
-  const int plen = WHAT == kSuffix ? 0 : clamped(a.plen, group, a.max_prefix);
-  const int slen = WHAT == kPrefix ? 0 : clamped(a.slen, seq0, a.max_suffix);
+  const int group = prefix ? owner : owner / a.group_size;
   const int32_t *pt = a.ptable + (size_t)group * a.ld_ptable;
   const int32_t *st = a.table + (size_t)seq0 * a.ld_table;
-  Attend<T, NC, RT> w;
-  if (WHAT != kJoined) {
-    const int len = WHAT == kPrefix ? plen : slen, chunk = WHAT == kPrefix ? a.pchunk : a.schunk;
-    const int from = part * chunk;
+  W w;
+  if (JOINED) {
+    const int plen = clamped(a.plen, group, a.max_prefix), slen = clamped(a.slen, seq0, a.max_suffix);
+    w.load_queries(a, pool.hd, seq0, head, row0, rows, lds, scales);
+    w.run(pool, head, rows, Run{pt, 0, plen, 0});
+    w.run(pool, head, rows, Run{st, 0, slen, (plen + kTile - 1) / kTile});
+    w.finish(a, pool.hd, seq0, head, row0, rows, -1, reinterpret_cast<float *>(lds), ml);
+  } else {
+    const int len = prefix ? clamped(a.plen, group, a.max_prefix) : clamped(a.slen, seq0, a.max_suffix);
+    const int chunk = prefix ? a.pchunk : a.schunk, from = part * chunk, at = prefix ? part : a.npp + part;
     if (from >= len) {  // nothing here: no rows to write, a sum of 0
       for (int r = threadIdx.x; r < rows; r += 64 * kWaves) {
         const int row = row0 + r, member = row / a.rep;
-        const size_t at = ((size_t)(seq0 + member) * a.nh + (size_t)head * a.rep +
-                           (row - member * a.rep)) * (a.npp + a.nsp) +
-                          (WHAT == kPrefix ? part : a.npp + part);
-        a.pml[at * 2] = kNegInf;
-        a.pml[at * 2 + 1] = 0.0f;
+        const size_t p = ((size_t)(seq0 + member) * a.nh + (size_t)head * a.rep + (row - member * a.rep)) *
+                             (a.npp + a.nsp) + at;
+        a.pml[p * 2] = kNegInf;
+        a.pml[p * 2 + 1] = 0.0f;
       }
       return;
     }
-    w.load_queries(a, pool.hd, seq0, head, row0, rows);
-    w.run(pool, head, rows, Run{WHAT == kPrefix ? pt : st, from, min(from + chunk, len), len});
-    w.finish(a, pool.hd, seq0, head, row0, rows, WHAT == kPrefix ? part : a.npp + part, buf, ml);
-  } else {
-    w.load_queries(a, pool.hd, seq0, head, row0, rows);
-    for (int k = 0; k < 2; k++) {
-      const int len = k ? slen : plen;
-      w.run(pool, head, rows, Run{k ? st : pt, 0, len, len});
-    }
-    w.finish(a, pool.hd, seq0, head, row0, rows, -1, buf, ml);
+    w.load_queries(a, pool.hd, seq0, head, row0, rows, lds, scales);
+    w.run(pool, head, rows, Run{prefix ? pt : st, from, min(from + chunk, len), 0});
+    w.finish(a, pool.hd, seq0, head, row0, rows, at, reinterpret_cast<float *>(lds), ml);
   }
 }
 
-// one wave a query row: the parts in order
+// One workgroup a query row: the factors of 64 parts at a time by lanes, the
+// parts' rows four to a step over the waves (all loads of a step in flight),
+// the waves' sums joined in order.
 __global__ void __launch_bounds__(256) k_join_parts(AttnArgs a, int hd) {
-  const int lane = threadIdx.x & 63;
-  const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (size_t)a.n_seqs * a.nh) return;
+  __shared__ float xs[3][kKvMaxHeadDim];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const size_t row = blockIdx.x;
   const int n = a.npp + a.nsp;
   const float *ml = a.pml + row * n * 2, *po = a.po + row * n * hd;
   float top = kNegInf;
   for (int i = lane; i < n; i += 64) top = fmaxf(top, ml[2 * i]);
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  float x[4] = {0, 0, 0, 0}, l = 0.0f;
-  for (int i = 0; i < n; i++) {
-    const float lp = ml[2 * i + 1];
-    if (lp == 0.0f) continue;
-    const float f = __builtin_amdgcn_exp2f(ml[2 * i] - top);
+  f32x4 x{0, 0, 0, 0};
+  const int d0 = min(4 * lane, hd - 4);
+  float l = 0.0f;
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    const int i = i0 + lane;
+    const float lp = i < n ? ml[2 * i + 1] : 0.0f;
+    const float f = lp == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml[2 * i] - top);
     l += lp * f;
+    const int most = min(64, n - i0);
+    for (int k = 4 * wave; k < most; k += 16) {
+      f32x4 y[4];
 #pragma unroll
-    for (int k = 0; k < 4; k++)
-      if (lane + 64 * k < hd) x[k] = __builtin_fmaf(po[(size_t)i * hd + lane + 64 * k], f, x[k]);
+      for (int u = 0; u < 4; u++)
+        y[u] = *reinterpret_cast<const f32x4 *>(po + (size_t)(i0 + min(k + u, most - 1)) * hd + d0);
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const float fu = __shfl(f, (k + u) & 63);
+        // (a part with no position has left its row unwritten)
+        if (k + u < most && fu != 0.0f)
+#pragma unroll
+          for (int c = 0; c < 4; c++) x[c] = __builtin_fmaf(y[u][c], fu, x[c]);
+      }
+    }
   }
-  const size_t seq = row / a.nh, head = row - seq * a.nh;
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+  if (wave > 0 && 4 * lane < hd) *reinterpret_cast<f32x4 *>(&xs[wave - 1][4 * lane]) = x;
+  __syncthreads();
+  if (wave == 0 && 4 * lane < hd) {
+    const size_t seq = row / a.nh, head = row - seq * a.nh;
+    float *out = a.out + seq * a.ldo + head * hd + 4 * lane;
 #pragma unroll
-  for (int k = 0; k < 4; k++)
-    if (lane + 64 * k < hd)
-      a.out[seq * a.ldo + head * hd + lane + 64 * k] = l == 0.0f ? 0.0f : x[k] / l;
+    for (int c = 0; c < 4; c++) {
+      const float v = x[c] + xs[0][4 * lane + c] + xs[1][4 * lane + c] + xs[2][4 * lane + c];
+      out[c] = l == 0.0f ? 0.0f : v / l;
+    }
+  }
 }
 
 // ---------------------------------------------------------------- host
@@ -426,79 +544,74 @@ syn_status_t check_attention(const syn_hip_kv_pages *pages,
   return SYN_OK;
 }
 
-// tiles of 16 query rows that a workgroup holds: the registers allow 4 (two
-// parts of 64 dims) to 1
-int row_tiles(int nc, int parts, int rows) {
-  const int most = nc * parts <= 8 ? 4 : (nc <= 4 ? 2 : 1);
-  const int need = (rows + 15) / 16;
-  return need >= 3 && most == 4 ? 4 : (need >= 2 && most >= 2 ? 2 : 1);
+// tiles of 16 query rows that a workgroup holds, as many as there are up to
+// what the registers take
+int row_tiles(int nc, bool f32, size_t rows) {
+  const int most = nc <= 4 ? 4 : (f32 ? 1 : 2);
+  return rows > 32 && most == 4 ? 4 : (rows > 16 && most >= 2 ? 2 : 1);
 }
 
 struct Plan {
   bool joined;
-  int nc, prt, srt;      // dims, row tiles of prefix and suffix workgroups
+  int nc, rt;  // dims and row tiles of a workgroup
   int pchunk, schunk, npp, nsp;
-  size_t rows, po_bytes, pml_bytes;
+  size_t prefix_wgs, wgs, rows, po_bytes, pml_bytes;
 };
 
 Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_prefix_attention_params &p) {
   Plan w{};
   const int hd = (int)pg.head_dim, nkv = (int)pg.n_kv_heads, rep = (int)p.n_heads / nkv;
-  const int parts = pg.dtype == SYN_HIP_KV_F32 ? 2 : (pg.dtype == SYN_HIP_KV_F16 ? 2 : 3);
   w.nc = hd <= 64 ? 2 : (hd <= 128 ? 4 : 8);
   w.rows = (size_t)p.n_groups * p.group_size * p.n_heads;
-  w.prt = row_tiles(w.nc, parts, (int)p.group_size * rep);
-  w.srt = row_tiles(w.nc, parts, rep);
   const size_t step = kTile * kWaves, seqs = (size_t)p.n_groups * p.group_size;
   w.joined = (size_t)p.max_prefix + p.max_suffix <= 4 * step;
-  if (w.joined) return w;
-  // parts enough for two workgroups a CU
-  auto cut = [&](size_t items, size_t len, int *chunk, int *n) {
-    const size_t tiles = cdiv(len, step), want = std::max<size_t>(1, cdiv(512, items));
-    const size_t per = std::max<size_t>(1, cdiv(tiles, want));
-    *chunk = (int)(per * step);
-    *n = (int)cdiv(tiles, per);
+  w.rt = w.joined ? 1 : row_tiles(w.nc, pg.dtype == SYN_HIP_KV_F32,
+                                  p.max_prefix ? (size_t)p.group_size * rep : rep);
+  const size_t sblocks = cdiv(rep, 16 * w.rt), sunits = seqs * nkv;
+  if (w.joined) {
+    w.wgs = round_up(sunits, 8) * sblocks;
+    return w;
+  }
+  // parts of about equal work for kWant workgroups in all
+  const size_t pblocks = cdiv((size_t)p.group_size * rep, 16 * w.rt), punits = (size_t)p.n_groups * nkv;
+  const size_t psteps = cdiv(p.max_prefix, step), ssteps = cdiv(p.max_suffix, step);
+  const size_t total = punits * pblocks * psteps + sunits * sblocks * ssteps;
+  const size_t per = std::max<size_t>(1, cdiv(total, kWant));
+  auto cut = [&](size_t steps, int *chunk, int *n) {
+    const size_t k = cdiv(steps, per);  // as many parts, of equal length
+    const size_t each = k ? cdiv(steps, k) : 0;
+    *chunk = (int)(each * step);
+    *n = each ? (int)cdiv(steps, each) : 0;
   };
-  const size_t pblocks = cdiv((size_t)p.group_size * rep, 16 * w.prt);
-  cut(std::max<size_t>(1, p.n_groups * nkv * pblocks), p.max_prefix, &w.pchunk, &w.npp);
-  cut(std::max<size_t>(1, seqs * nkv * cdiv(rep, 16 * w.srt)), p.max_suffix, &w.schunk, &w.nsp);
+  cut(psteps, &w.pchunk, &w.npp);
+  cut(ssteps, &w.schunk, &w.nsp);
+  w.prefix_wgs = round_up(punits * w.npp, 8) * pblocks;
+  w.wgs = w.prefix_wgs + round_up(sunits * w.nsp, 8) * sblocks;
   const size_t n = w.rows * (size_t)(w.npp + w.nsp);
   w.po_bytes = round_up(n * hd * 4, 16);
   w.pml_bytes = round_up(n * 8, 16);
   return w;
 }
 
-template <class T, int NC, int RT, int WHAT>
-syn_status_t launch_one(const AttnArgs &a, const KvPool<T> &pool, hipStream_t s) {
-  const size_t members = WHAT == kPrefix ? a.group_size : 1;
-  const size_t blocks = cdiv(members * a.rep, RT * 16);
-  const size_t parts = WHAT == kPrefix ? a.npp : (WHAT == kSuffix ? a.nsp : 1);
-  const size_t units = round_up(a.n_seqs / members * parts * pool.nkv, 8);
-  if (units * blocks > 0x7fffffffu) {
-    set_error("prefix_attention: more workgroups than a launch takes");
-    return SYN_ERR_INVALID_ARG;
-  }
-  hipLaunchKernelGGL((k_attend<T, NC, RT, WHAT>), dim3((unsigned)(units * blocks)),
-                     dim3(64 * kWaves), 0, s, a, pool);
+template <class T, int NC, int RT, bool JOINED = false>
+syn_status_t launch_one(const Plan &w, const AttnArgs &a, const KvPool<T> &pool, hipStream_t s) {
+  hipLaunchKernelGGL((k_attend<T, NC, RT, JOINED>), dim3((unsigned)w.wgs), dim3(64 * kWaves), 0, s, a,
+                     pool);
   SYN_LAUNCH_CHECK();
   return SYN_OK;
 }
 
-template <class T, int NC, int WHAT>
-syn_status_t launch_rt(int rt, const AttnArgs &a, const KvPool<T> &pool, hipStream_t s) {
-  if constexpr (NC * (Frag<T>::kParts == 3 ? 3 : 2) <= 8)
-    if (rt == 4) return launch_one<T, NC, 4, WHAT>(a, pool, s);
-  if constexpr (NC <= 4)
-    if (rt >= 2) return launch_one<T, NC, 2, WHAT>(a, pool, s);
-  return launch_one<T, NC, 1, WHAT>(a, pool, s);
-}
-
 template <class T, int NC>
 syn_status_t launch_nc(const Plan &w, const AttnArgs &a, const KvPool<T> &pool, hipStream_t s) {
-  if (w.joined) return launch_rt<T, NC, kJoined>(w.srt, a, pool, s);
-  if (w.npp) SYN_TRY((launch_rt<T, NC, kPrefix>(w.prt, a, pool, s)));
-  if (w.nsp) SYN_TRY((launch_rt<T, NC, kSuffix>(w.srt, a, pool, s)));
-  hipLaunchKernelGGL(k_join_parts, dim3((unsigned)cdiv(w.rows, 4)), dim3(256), 0, s, a, pool.hd);
+  if (w.joined) return launch_one<T, NC, 1, true>(w, a, pool, s);
+  if (w.rt == 1) {
+    SYN_TRY((launch_one<T, NC, 1>(w, a, pool, s)));
+  } else if (w.rt == 2) {
+    if constexpr (NC <= 4 || sizeof(T) == 2) SYN_TRY((launch_one<T, NC, 2>(w, a, pool, s)));
+  } else {
+    if constexpr (NC <= 4) SYN_TRY((launch_one<T, NC, 4>(w, a, pool, s)));
+  }
+  hipLaunchKernelGGL(k_join_parts, dim3((unsigned)w.rows), dim3(256), 0, s, a, pool.hd);
   SYN_LAUNCH_CHECK();
   return SYN_OK;
 }
@@ -530,6 +643,10 @@ extern "C" syn_status_t syn_hip_prefix_attention(
     return SYN_ERR_NULL_PTR;
   const Plan w = make_plan(*pages, *p);
   const size_t need = w.po_bytes + w.pml_bytes;
+  if (w.wgs > 0x7fffffffu || w.rows > 0x7fffffffu) {
+    set_error("prefix_attention: more workgroups than a launch takes");
+    return SYN_ERR_INVALID_ARG;
+  }
   if (need && !d_workspace) return SYN_ERR_NULL_PTR;
   if (need && (!aligned16(d_workspace) || workspace_bytes < need)) {
     set_error("prefix_attention: workspace unaligned or too small");
@@ -558,6 +675,8 @@ extern "C" syn_status_t syn_hip_prefix_attention(
   a.schunk = w.schunk;
   a.npp = w.npp;
   a.nsp = w.nsp;
+  a.prefix_wgs = (int)w.prefix_wgs;
+  a.q16 = aligned16(d_q) && p->ldq % 4 == 0;
   a.po = static_cast<float *>(d_workspace);
   a.pml = reinterpret_cast<float *>(static_cast<uint8_t *>(d_workspace) + w.po_bytes);
   hipStream_t s = pick_stream(stream);
