@@ -28,6 +28,7 @@ namespace {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr int kWaves = 4;
+constexpr float kSlack = 8.0f;
 constexpr int kTile = 32;  // positions a wave takes at a time
 #ifndef KWANT
 #define KWANT 512
@@ -60,17 +61,22 @@ template <class T> struct Frag;
 template <> struct Frag<_Float16> {
   using V = f16x8;
   static constexpr int kParts = 2;
-  // A weight is at least 2^kBias where its score is the reference maximum, so
-  // that the second part of the small ones is still a normal f16.
+  // A weight is 2^kBias where its score is the reference maximum (and at most
+  // 2^(kBias + kSlack), within f16), so that the second part of small ones
+  // is still a normal f16.
   static constexpr float kBias = 6.0f;
   static __device__ __forceinline__ V load(const _Float16 *p) {
     return *reinterpret_cast<const V *>(p);
   }
+  // both parts cut toward zero: the second holds what the first leaves to
+  // within 2^-21 of x
   static __device__ __forceinline__ void split(const float *x, V *p) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      p[0][j] = (_Float16)x[j];
-      p[1][j] = (_Float16)__builtin_fmaf((float)p[0][j], -1.0f, x[j]);
+    for (int j = 0; j < 8; j += 2) {
+      const auto h = __builtin_amdgcn_cvt_pkrtz(x[j], x[j + 1]);
+      const auto r = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], -1.0f, x[j]),
+                                                __builtin_fmaf((float)h[1], -1.0f, x[j + 1]));
+      p[0][j] = h[0], p[0][j + 1] = h[1], p[1][j] = r[0], p[1][j + 1] = r[1];
     }
   }
   static __device__ __forceinline__ f32x4 mma(const V &a, const V *b, f32x4 c) {
@@ -87,12 +93,23 @@ template <> struct Frag<__bf16> {
     return *reinterpret_cast<const V *>(p);
   }
   static __device__ __forceinline__ void split(const float *x, V *p) {
+    // the upper 16 bits of x and of what is left, twice: 24 bits in three parts
+    uint32_t u[3][8];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-      p[0][j] = (__bf16)x[j];
-      const float r = x[j] - (float)p[0][j];
-      p[1][j] = (__bf16)r;
-      p[2][j] = (__bf16)(r - (float)p[1][j]);
+      float r = x[j];
+#pragma unroll
+      for (int k = 0; k < 3; k++) {
+        u[k][j] = __float_as_uint(r) & 0xffff0000u;
+        r -= __uint_as_float(u[k][j]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+      u32x4 w;
+#pragma unroll
+      for (int j = 0; j < 4; j++) w[j] = __builtin_amdgcn_perm(u[k][2 * j + 1], u[k][2 * j], 0x07060302u);
+      p[k] = __builtin_bit_cast(V, w);
     }
   }
   static __device__ __forceinline__ f32x4 mma(const V &a, const V *b, f32x4 c) {
@@ -130,14 +147,20 @@ template <> struct Frag<float> {
   }
 };
 
-// over the four groups of 16 lanes
+// over the four groups of 16 lanes: a swap of halves (of odd and even groups)
+// of x with itself leaves each lane its own value and its partner's
+template <class Op> __device__ __forceinline__ float over_groups(float x, Op op) {
+  const uint32_t u = __float_as_uint(x);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t v = __float_as_uint(op(__uint_as_float(a[0]), __uint_as_float(a[1])));
+  const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 __device__ __forceinline__ float groups_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+  return over_groups(x, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float groups_sum(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+  return over_groups(x, [](float a, float b) { return a + b; });
 }
 
 // Positions from .. to of a page table, dealt to the waves by tiles, the first
@@ -321,30 +344,36 @@ template <class T, int NC, int RT> struct Attend {
       for (int t = 0; t < ACT; t++) {
         float x[8];
 #pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = s[t][0][j] * unscale[t], x[j + 4] = s[t][1][j] * unscale[t];
+        for (int j = 0; j < 4; j++) x[j] = s[t][0][j], x[j + 4] = s[t][1][j];
         if (!whole)
 #pragma unroll
           for (int j = 0; j < 8; j++) x[j] = there >> j & 1 ? x[j] : kNegInf;
-        float top = x[0];
+        float top = fmaxf(x[0], x[1]);
 #pragma unroll
-        for (int j = 1; j < 8; j++) top = fmaxf(top, x[j]);
-        top = fmaxf(groups_max(top), m[t]);
-        const float ref = top == kNegInf ? 0.0f : top;
-        const float back = __builtin_amdgcn_exp2f(m[t] - ref);
-        m[t] = top;
-        l[t] *= back;
+        for (int j = 2; j < 8; j += 2) top = fmaxf(fmaxf(x[j], x[j + 1]), top);
+        top = groups_max(top) * unscale[t];
+        // weights are relative to m, a maximum of earlier: the accumulators are
+        // rescaled only when a score is 2^kSlack times above it
+        if (__any(top > m[t] + kSlack)) {
+          const float up = fmaxf(m[t], top);
+          const float back = __builtin_amdgcn_exp2f(m[t] - (up == kNegInf ? 0.0f : up));
+          m[t] = up;
+          l[t] *= back;
+#pragma unroll
+          for (int d = 0; d < DT; d++) o[t][d] *= back;
+        }
+        const float ref = F::kBias - (m[t] == kNegInf ? 0.0f : m[t]);
+        float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-          x[j] = __builtin_amdgcn_exp2f(x[j] - ref + F::kBias);
-          l[t] += x[j];
+          x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], unscale[t], ref));
+          sum[j & 1] += x[j];
         }
+        l[t] += sum[0] + sum[1];
         V p[F::kParts];
         F::split(x, p);
 #pragma unroll
-        for (int d = 0; d < DT; d++) {
-          o[t][d] *= back;
-          o[t][d] = F::mma(vf[d], p, o[t][d]);
-        }
+        for (int d = 0; d < DT; d++) o[t][d] = F::mma(vf[d], p, o[t][d]);
       }
       if (k1 >= to) break;
       const bool next_v = pool.has(page_v);
