@@ -20,6 +20,7 @@
 #include <cmath>
 
 #include "kv_pages.hpp"
+#include "lds_dma.hpp"
 
 namespace syn {
 
@@ -46,8 +47,9 @@ struct AttnArgs {
   // the longest prefix and suffix; parts of query row (sequence, head) are
   // po[(sequence * nh + head) * (npp + nsp) + part][hd], pml[..][2] (max, sum)
   int pchunk, schunk, npp, nsp, prefix_wgs;
+  int prw, srw;  // tiles of 16 rows of a prefix and of a suffix workgroup: 1, 2 or 4
   float *po, *pml;
-  bool q16;  // rows of queries are 16-byte aligned
+  bool joined, q16;  // rows of queries are 16-byte aligned
 };
 
 // ---------------------------------------------------------------- products
@@ -170,277 +172,337 @@ struct Run {
   int from, to, first;
 };
 
-// RT: tiles of 16 query rows; NC: 32 dims each (hd <= 32 NC)
-template <class T, int NC, int RT> struct Attend {
+// One wave's part of the work: 16 query rows of a kv head.
+template <class T, int NC> struct Rows {
   using F = Frag<T>;
   using V = typename F::V;
-  static constexpr int DT = 2 * NC;
-  static constexpr int kLd = 32 * NC + 4;  // f32 rows on different banks
-  static constexpr size_t kQueryBytes = (size_t)RT * NC * F::kParts * 64 * sizeof(V);
-  static constexpr size_t kJoinBytes = (size_t)kWaves * 16 * kLd * 4;
-  static constexpr size_t kLdsBytes = kQueryBytes > kJoinBytes ? kQueryBytes : kJoinBytes;
-  // the queries' parts stay in LDS where registers would not hold them
-  static constexpr bool kKeep = RT * NC * F::kParts * sizeof(V) <= 64 * 4;
-  V q[kKeep ? RT : 1][NC][F::kParts], kf[2][NC], vf[DT];
-  const V *qs;  // [RT][NC][parts][64 lanes]
-  f32x4 o[RT][DT];
-  float m[RT], l[RT], unscale[RT];
-  int page_k, page_v;  // of the tile whose K and V are loaded next
+  static constexpr int DT = 2 * NC;           // tiles of 16 dims (hd <= 32 NC)
+  static constexpr int kFrags = 4 * NC;       // operand fragments of a tile of positions: K, then V
+  static constexpr int kLoads = kFrags * (int)sizeof(V) / 16;  // 1 KiB direct loads of a tile
+  static constexpr int kTileBytes = kLoads * 1024;
+  // tiles that the ring in LDS holds: 32 to 64 KiB, 128 where a tile has 64
+  static constexpr int kRing = kTileBytes <= 16384 ? 4 : 2;
+  static constexpr int kLd = 32 * NC + 4;     // f32 rows on different banks
+  static constexpr int kJoinBytes = kWaves * 16 * kLd * 4;
+  static constexpr int kLdsBytes = kRing * kTileBytes > kJoinBytes ? kRing * kTileBytes : kJoinBytes;
+  V q[NC][F::kParts];
+  f32x4 o[DT];
+  float m, l, unscale;
 
   // The rows' queries times scale, each row for an f16 pool times the power of
   // two that puts its largest element into [2^11, 2^12): both parts of every
-  // element that matters are normal.  Wave t splits tile t for all.
-  __device__ __forceinline__ void load_queries(const AttnArgs &a, int hd, int seq0, int head, int row0,
-                                               int rows, uint8_t *lds, float *scales) {
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, t = threadIdx.x >> 6;
-    V *to = reinterpret_cast<V *>(lds);
-    qs = to;
-    if (t < RT) {
-      const bool on = t * 16 + n < rows;
-      const int r = row0 + min(t * 16 + n, rows - 1), member = r / a.rep;
-      const float *src = a.q + (size_t)(seq0 + member) * a.ldq +
-                         (size_t)(head * a.rep + (r - member * a.rep)) * hd;
-      float x[NC][8], top = 0.0f;
-      if (a.q16) {
+  // element that matters are normal.  Rows past the last repeat it.
+  __device__ __forceinline__ void load_queries(const AttnArgs &a, int hd, int seq0, int head, int row,
+                                               int last) {
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int r = min(row + n, last), member = r / a.rep;
+    const float *src = a.q + (size_t)(seq0 + member) * a.ldq +
+                       (size_t)(head * a.rep + (r - member * a.rep)) * hd;
+    float x[NC][8], top = 0.0f;
+    if (a.q16) {
 #pragma unroll
-        for (int c = 0; c < NC; c++) {
-          const f32x4 *p = reinterpret_cast<const f32x4 *>(src + min((c * 4 + g) * 8, hd - 8));
-          const f32x4 u = p[0], v = p[1];
+      for (int c = 0; c < NC; c++) {
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(src + min((c * 4 + g) * 8, hd - 8));
+        const f32x4 u = p[0], v = p[1];
 #pragma unroll
-          for (int j = 0; j < 4; j++) x[c][j] = u[j], x[c][j + 4] = v[j];
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-          for (int j = 0; j < 8; j++) x[c][j] = src[min((c * 4 + g) * 8, hd - 8) + j];
+        for (int j = 0; j < 4; j++) x[c][j] = u[j], x[c][j + 4] = v[j];
       }
+    } else {
 #pragma unroll
       for (int c = 0; c < NC; c++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          x[c][j] = on && (c * 4 + g) * 8 < hd ? x[c][j] * a.scale : 0.0f;
-          top = fmaxf(top, fabsf(x[c][j]));
-        }
-      int e = 0;
-      if constexpr (F::kParts == 2) {
-        top = groups_max(top);
-        if (top > 0.0f && top < __builtin_huge_valf()) e = 11 - ilogbf(top);
-        e = min(max(e, -120), 120);  // a power of two within f32's own range either way
+        for (int j = 0; j < 8; j++) x[c][j] = src[min((c * 4 + g) * 8, hd - 8) + j];
+    }
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        x[c][j] = (c * 4 + g) * 8 < hd ? x[c][j] * a.scale : 0.0f;
+        top = fmaxf(top, fabsf(x[c][j]));
       }
+    unscale = 1.0f;
+    if constexpr (F::kParts == 2) {
+      top = groups_max(top);
+      int e = top > 0.0f && top < __builtin_huge_valf() ? 11 - ilogbf(top) : 0;
+      e = min(max(e, -120), 120);  // a power of two within f32's own range either way
       const float up = __builtin_ldexpf(1.0f, e);
-      if (g == 0) scales[t * 16 + n] = __builtin_ldexpf(1.0f, -e);
+      unscale = __builtin_ldexpf(1.0f, -e);
 #pragma unroll
-      for (int c = 0; c < NC; c++) {
-        if constexpr (F::kParts == 2)
+      for (int c = 0; c < NC; c++)
 #pragma unroll
-          for (int j = 0; j < 8; j++) x[c][j] *= up;
-        V part[F::kParts];
-        F::split(x[c], part);
-#pragma unroll
-        for (int k = 0; k < F::kParts; k++) to[((t * NC + c) * F::kParts + k) * 64 + lane] = part[k];
-      }
+        for (int j = 0; j < 8; j++) x[c][j] *= up;
     }
-    __syncthreads();
 #pragma unroll
-    for (int u = 0; u < RT; u++) {
-      if constexpr (kKeep)
+    for (int c = 0; c < NC; c++) F::split(x[c], q[c]);
+    m = kNegInf;
+    l = 0.0f;
 #pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-          for (int k = 0; k < F::kParts; k++) q[u][c][k] = qs[((u * NC + c) * F::kParts + k) * 64 + lane];
-      unscale[u] = scales[u * 16 + n];
-      m[u] = kNegInf;
-      l[u] = 0.0f;
-#pragma unroll
-      for (int d = 0; d < DT; d++) o[u][d] = f32x4{0, 0, 0, 0};
-    }
+    for (int d = 0; d < DT; d++) o[d] = f32x4{0, 0, 0, 0};
   }
 
-  // Lane (g, n) reads K of the group of 8 positions n / 4 of a tile and V of
-  // group g.  Positions past the end are read at the last group there is.
-  __device__ __forceinline__ int spot(int k0, int group, int to) { return min(k0 + 8 * group, (to - 1) & ~7); }
-  __device__ __forceinline__ void load_pages(const KvPool<T> &pool, const Run &r, int k0) {
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    page_k = r.table[spot(k0, n >> 2, r.to) >> pool.ps_shift];
-    page_v = r.table[spot(k0, g, r.to) >> pool.ps_shift];
+  // ---- a tile's operands: lane (g, n) has K of the position group n / 4 and
+  // V of group g, of the four groups of 8 positions.  Positions past the end
+  // are read at the last group there is.
+  struct Where {
+    int p0, p1, p2, p3;  // pages of the groups
+    __device__ __forceinline__ int of(int group) const {
+      const int a = p0, b = p1, c = p2, d = p3;  // values, not places: kept in registers
+      const int lo = group & 1 ? b : a, hi = group & 1 ? d : c;
+      return group & 2 ? hi : lo;
+    }
+  };
+  static __device__ __forceinline__ int spot(int k0, int group, int to) {
+    return min(k0 + 8 * group, (to - 1) & ~7);
   }
-  __device__ __forceinline__ void load_k(const KvPool<T> &pool, int head, const Run &r, int k0) {
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  // by scalar loads (k0 is the same for the whole wave): they do not queue
+  // with the K and V in flight
+  static __device__ __forceinline__ Where look_up(const KvPool<T> &pool, const Run &r, int k0) {
+    const auto *t = (const __attribute__((address_space(4))) int32_t *)(uintptr_t)r.table;
+    return Where{t[spot(k0, 0, r.to) >> pool.ps_shift], t[spot(k0, 1, r.to) >> pool.ps_shift],
+                 t[spot(k0, 2, r.to) >> pool.ps_shift], t[spot(k0, 3, r.to) >> pool.ps_shift]};
+  }
+  // which of the groups' pages are pages, a bit each
+  static __device__ __forceinline__ uint32_t found(const KvPool<T> &pool, const Where &w) {
+    return (pool.has(w.p0) ? 1u : 0u) | (pool.has(w.p1) ? 2u : 0u) | (pool.has(w.p2) ? 4u : 0u) |
+           (pool.has(w.p3) ? 8u : 0u);
+  }
+  static __device__ __forceinline__ const T *k_of(const KvPool<T> &pool, int head, const Run &r, int k0,
+                                                  const Where &w) {
+    const int n = threadIdx.x & 15, page = w.of(n >> 2);
     const int slot = (spot(k0, n >> 2, r.to) & (pool.ps - 1)) + (n & 3);
-    const T *kp = pool.k + pool.base(pool.has(page_k) ? page_k : 0, head) + (size_t)slot * 8;
+    return pool.k + pool.base(pool.has(page) ? page : 0, head) + (size_t)slot * 8;
+  }
+  static __device__ __forceinline__ const T *v_of(const KvPool<T> &pool, int head, const Run &r, int k0,
+                                                  const Where &w) {
+    const int g = (threadIdx.x & 63) >> 4, page = w.of(g);
+    const int group = (spot(k0, g, r.to) & (pool.ps - 1)) >> 3;
+    return pool.v + pool.base(pool.has(page) ? page : 0, head) + (size_t)group * pool.hd * 8;
+  }
+  // element offset of fragment f: K of half f % 2 at dims 32 (f / 2), then V
+  // of 16 dims
+  static __device__ __forceinline__ size_t k_off(const KvPool<T> &pool, int f) {
+    const int g = (threadIdx.x & 63) >> 4;
+    return (size_t)min((f >> 1) * 4 + g, (pool.hd >> 3) - 1) * pool.ps * 8 + (f & 1) * 32;
+  }
+  static __device__ __forceinline__ size_t v_off(const KvPool<T> &pool, int d) {
+    return (size_t)min(d * 16 + (int)(threadIdx.x & 15), pool.hd - 1) * 8;
+  }
+  // the positions 8g .. 8g+7 whose weights this lane holds, a bit each
+  static __device__ __forceinline__ uint32_t which(int k0, int to, uint32_t ok) {
+    const int g = (threadIdx.x & 63) >> 4, left = ok >> g & 1 ? to - (k0 + 8 * g) : 0;
+    return left >= 8 ? 0xff : (left <= 0 ? 0 : (1u << left) - 1);
+  }
+
+  // ---- the two products of a tile
+  template <class K> __device__ __forceinline__ void scores(K k, f32x4 *s) const {
+    s[0] = s[1] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int c = 0; c < NC; c++) {
-      const size_t at = (size_t)min(c * 4 + g, (pool.hd >> 3) - 1) * pool.ps * 8;
-      kf[0][c] = F::load(kp + at);
-      kf[1][c] = F::load(kp + at + 32);
+      s[0] = F::mma(k(2 * c), q[c], s[0]);
+      s[1] = F::mma(k(2 * c + 1), q[c], s[1]);
     }
+    // Read the sums before the next branch: where a conditional region lies
+    // between, the compiler pads the matrix instruction's latency on the
+    // longer way only.
+    asm volatile("" : "+v"(s[0]), "+v"(s[1]));
   }
-  __device__ __forceinline__ void load_v(const KvPool<T> &pool, int head, const Run &r, int k0) {
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int group = (spot(k0, g, r.to) & (pool.ps - 1)) >> 3;
-    const T *vp = pool.v + pool.base(pool.has(page_v) ? page_v : 0, head) + (size_t)group * pool.hd * 8;
+  template <class G> __device__ __forceinline__ void weigh(const f32x4 *s, bool whole, uint32_t there, G v) {
+    float x[8];
 #pragma unroll
-    for (int d = 0; d < DT; d++) vf[d] = F::load(vp + (size_t)min(d * 16 + n, pool.hd - 1) * 8);
-  }
-
-  // The wave's tiles of a run.  One set of registers: the next tile's K is
-  // requested when this one's scores are formed, its V when this one's product
-  // is, its pages a tile ahead of both.
-  template <int ACT>  // tiles of query rows in use
-  __device__ __forceinline__ void run_tiles(const KvPool<T> &pool, int head, const Run &r) {
-    const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
-    constexpr int kStep = kTile * kWaves;
-    const int to = r.to;
-    int k0 = r.from + ((wave - r.first) & (kWaves - 1)) * kTile;
-    if (k0 >= to) return;
-    load_pages(pool, r, k0);
-    bool has_k = pool.has(page_k), has_v = pool.has(page_v);
-    load_k(pool, head, r, k0);
-    load_v(pool, head, r, k0);
-    load_pages(pool, r, k0 + kStep);
-    for (;;) {
-      const int k1 = k0 + kStep;
-      const bool whole = __all(k0 + kTile <= to && has_k && has_v);
-      uint32_t there = 0xff;  // of the positions 8g .. 8g+7 whose weights this lane holds
-      if (!whole) {
-        const int left = has_v ? to - (k0 + 8 * g) : 0;
-        there = left >= 8 ? 0xff : (left <= 0 ? 0 : (1u << left) - 1);
-      }
-      f32x4 s[ACT][2];
+    for (int j = 0; j < 4; j++) x[j] = s[0][j], x[j + 4] = s[1][j];
+    if (!whole)
 #pragma unroll
-      for (int t = 0; t < ACT; t++) {
-        s[t][0] = s[t][1] = f32x4{0, 0, 0, 0};
+      for (int j = 0; j < 8; j++) x[j] = there >> j & 1 ? x[j] : kNegInf;
+    float top = fmaxf(x[0], x[1]);
 #pragma unroll
-        for (int c = 0; c < NC; c++) {
-          if constexpr (kKeep) {
-            s[t][0] = F::mma(kf[0][c], q[t][c], s[t][0]);
-            s[t][1] = F::mma(kf[1][c], q[t][c], s[t][1]);
-          } else {
+    for (int j = 2; j < 8; j += 2) top = fmaxf(fmaxf(x[j], x[j + 1]), top);
+    top = groups_max(top) * unscale;
+    // weights are relative to m, a maximum of earlier: the accumulators are
+    // rescaled only when a score is 2^kSlack times above it
+    if (__any(top > m + kSlack)) {
+      const float up = fmaxf(m, top);
+      const float back = __builtin_amdgcn_exp2f(m - (up == kNegInf ? 0.0f : up));
+      m = up;
+      l *= back;
 #pragma unroll
-            for (int k = 0; k < F::kParts; k++) q[0][c][k] = qs[((t * NC + c) * F::kParts + k) * 64 + lane];
-            s[t][0] = F::mma(kf[0][c], q[0][c], s[t][0]);
-            s[t][1] = F::mma(kf[1][c], q[0][c], s[t][1]);
-          }
-        }
-      }
-      // Read the sums before the next branch: where a conditional region lies
-      // between, the compiler pads the matrix instruction's latency on the
-      // longer way only.
+      for (int d = 0; d < DT; d++) o[d] *= back;
+    }
+    const float ref = F::kBias - (m == kNegInf ? 0.0f : m);
+    float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-      for (int t = 0; t < ACT; t++) asm volatile("" : "+v"(s[t][0]), "+v"(s[t][1]));
-      if (k1 < to) {
-        has_k = pool.has(page_k);
-        load_k(pool, head, r, k1);
-      }
+    for (int j = 0; j < 8; j++) {
+      x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], unscale, ref));
+      sum[j & 1] += x[j];
+    }
+    l += sum[0] + sum[1];
+    V p[F::kParts];
+    F::split(x, p);
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+      V f = v(d);
       if (!whole) {  // what is not there may hold anything: 0 times NaN is NaN
 #pragma unroll
-        for (int d = 0; d < DT; d++)
-#pragma unroll
-          for (int j = 0; j < 8; j++)
-            if (!(there >> j & 1)) F::clear(vf[d], j);
+        for (int j = 0; j < 8; j++)
+          if (!(there >> j & 1)) F::clear(f, j);
       }
+      o[d] = F::mma(f, p, o[d]);
+    }
+  }
+
+  // ---- 16 rows in all: the waves take the tiles of a run in turn, K and V in
+  // registers.  One set of them: the next tile's K is requested when this
+  // one's scores are formed, its V when this one's product is.
+  __device__ __forceinline__ void run_alone(const KvPool<T> &pool, int head, const Run &r) {
+    constexpr int kStep = kTile * kWaves;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int k0 = r.from + ((wave - r.first) & (kWaves - 1)) * kTile;
+    if (k0 >= r.to) return;
+    V kf[2 * NC], vf[DT];
+    Where w = look_up(pool, r, k0);
+    uint32_t ok = found(pool, w);
+    {
+      const T *k = k_of(pool, head, r, k0, w), *v = v_of(pool, head, r, k0, w);
 #pragma unroll
-      for (int t = 0; t < ACT; t++) {
-        float x[8];
+      for (int f = 0; f < 2 * NC; f++) kf[f] = F::load(k + k_off(pool, f));
 #pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = s[t][0][j], x[j + 4] = s[t][1][j];
-        if (!whole)
+      for (int d = 0; d < DT; d++) vf[d] = F::load(v + v_off(pool, d));
+    }
+    w = look_up(pool, r, k0 + kStep);
+    for (;;) {
+      const int k1 = k0 + kStep;
+      const bool whole = k0 + kTile <= r.to && ok == 15;
+      const uint32_t there = which(k0, r.to, ok);
+      f32x4 s[2];
+      scores([&](int f) { return kf[f]; }, s);
+      if (k1 < r.to) {
+        const T *k = k_of(pool, head, r, k1, w);
 #pragma unroll
-          for (int j = 0; j < 8; j++) x[j] = there >> j & 1 ? x[j] : kNegInf;
-        float top = fmaxf(x[0], x[1]);
-#pragma unroll
-        for (int j = 2; j < 8; j += 2) top = fmaxf(fmaxf(x[j], x[j + 1]), top);
-        top = groups_max(top) * unscale[t];
-        // weights are relative to m, a maximum of earlier: the accumulators are
-        // rescaled only when a score is 2^kSlack times above it
-        if (__any(top > m[t] + kSlack)) {
-          const float up = fmaxf(m[t], top);
-          const float back = __builtin_amdgcn_exp2f(m[t] - (up == kNegInf ? 0.0f : up));
-          m[t] = up;
-          l[t] *= back;
-#pragma unroll
-          for (int d = 0; d < DT; d++) o[t][d] *= back;
-        }
-        const float ref = F::kBias - (m[t] == kNegInf ? 0.0f : m[t]);
-        float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], unscale[t], ref));
-          sum[j & 1] += x[j];
-        }
-        l[t] += sum[0] + sum[1];
-        V p[F::kParts];
-        F::split(x, p);
-#pragma unroll
-        for (int d = 0; d < DT; d++) o[t][d] = F::mma(vf[d], p, o[t][d]);
+        for (int f = 0; f < 2 * NC; f++) kf[f] = F::load(k + k_off(pool, f));
       }
-      if (k1 >= to) break;
-      const bool next_v = pool.has(page_v);
-      const int pv = page_v;
-      load_pages(pool, r, k1 + kStep);
-      const int ahead = page_v;
-      page_v = pv;
-      load_v(pool, head, r, k1);
-      page_v = ahead;
-      has_v = next_v;
+      weigh(s, whole, there, [&](int d) { return vf[d]; });
+      if (k1 >= r.to) break;
+      const T *v = v_of(pool, head, r, k1, w);
+#pragma unroll
+      for (int d = 0; d < DT; d++) vf[d] = F::load(v + v_off(pool, d));
+      ok = found(pool, w);
+      w = look_up(pool, r, k1 + kStep);
       k0 = k1;
     }
   }
 
-  __device__ __forceinline__ void run(const KvPool<T> &pool, int head, int rows, const Run &r) {
-    if (RT == 1 || rows <= 16)
-      run_tiles<1>(pool, head, r);
-    else if (RT == 2 || rows <= 32)
-      run_tiles<RT < 2 ? RT : 2>(pool, head, r);
-    else
-      run_tiles<RT>(pool, head, r);
+  // ---- 16 rows to each of kWaves / KW waves: every wave reads every tile (KW
+  // 1) or every other (KW 2), so the tiles go through a ring in LDS, in
+  // fragment order, by direct loads that run kRing / KW - 1 steps ahead.
+  __device__ __forceinline__ void issue(const KvPool<T> &pool, int head, const Run &r, int k0, uint32_t lds,
+                                        const Where &w) {
+    constexpr int kHalves = (int)sizeof(V) / 16, kMine = kLoads / kWaves;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const T *k = k_of(pool, head, r, k0, w), *v = v_of(pool, head, r, k0, w);
+#pragma unroll
+    for (int i = 0; i < kMine; i++) {
+      const int b = i * kWaves + wave, f = b / kHalves;
+      const T *src = i < kMine / 2 ? k + k_off(pool, f) : v + v_off(pool, f - 2 * NC);
+      kr_dma(src + (b % kHalves) * 4, lds + b * 1024);
+    }
+  }
+  template <int KW>
+  __device__ __forceinline__ void run_shared(const KvPool<T> &pool, int head, const Run &r, uint8_t *ring) {
+    constexpr int S = kRing / KW, kAhead = S - 1, kStep = KW * kTile, kMine = KW * kLoads / kWaves;
+    static_assert(kLoads % (2 * kWaves) == 0 && 8 * kAhead < 32, "K and V in whole shares");
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr_of(ring));
+    const int n = (r.to - r.from + kStep - 1) / kStep;
+    const int mine = KW == 1 ? 0 : wave / (kWaves / KW);  // tile of a step
+    // found() of the tiles in flight: 4 bits a tile, 8 a step, this step's lowest
+    uint32_t ok = 0;
+#pragma unroll
+    for (int i = 0; i < kAhead; i++)
+      if (i < n)
+#pragma unroll
+        for (int t = 0; t < KW; t++) {
+          const int kt = r.from + i * kStep + t * kTile;
+          const Where w = look_up(pool, r, kt);
+          ok |= found(pool, w) << (8 * i + 4 * t);
+          issue(pool, head, r, kt, base + (i * KW + t) * kTileBytes, w);
+        }
+    int get = 0, put = kAhead;  // places in the ring
+    for (int i = 0; i < n; i++) {
+      const int k0 = r.from + i * kStep, k2 = k0 + kAhead * kStep;
+      const Where w0 = look_up(pool, r, k2), w1 = KW == 2 ? look_up(pool, r, k2 + kTile) : w0;
+      // step i has landed, and every wave is done with step i - 1
+      if (i + kAhead <= n)
+        kr_publish<(kAhead - 1) * kMine>();
+      else
+        kr_publish<0>();
+      if (i + kAhead < n) {
+        issue(pool, head, r, k2, base + put * KW * kTileBytes, w0);
+        if (KW == 2) issue(pool, head, r, k2 + kTile, base + (put * KW + 1) * kTileBytes, w1);
+        ok |= (found(pool, w0) | (KW == 2 ? found(pool, w1) << 4 : 0)) << (8 * kAhead);
+      }
+      const int kt = k0 + mine * kTile;
+      if (KW == 1 || kt < r.to) {
+        const uint8_t *f = ring + (get * KW + mine) * kTileBytes;
+        auto frag = [&](int j) {
+          if constexpr (sizeof(V) == 16) {
+            return reinterpret_cast<const V *>(f)[j * 64 + lane];
+          } else {  // two halves of 16 bytes a lane
+            const f32x4 *h = reinterpret_cast<const f32x4 *>(f) + j * 128 + lane;
+            return V{h[0], h[64]};
+          }
+        };
+        const uint32_t here = ok >> (4 * mine) & 15;
+        const bool whole = kt + kTile <= r.to && here == 15;
+        const uint32_t there = which(kt, r.to, here);
+        f32x4 s[2];
+        scores(frag, s);
+        weigh(s, whole, there, [&](int d) { return frag(2 * NC + d); });
+      }
+      ok >>= 8;
+      get = get + 1 == S ? 0 : get + 1;
+      put = put + 1 == S ? 0 : put + 1;
+    }
   }
 
-  // The four waves' results joined, in the order of the waves; a row's goes to
-  // the output, or to its part of the workspace.
+  // The results of the waves that share rows joined, in the order of the
+  // waves; a row's goes to the output, or to its part of the workspace.  RW
+  // tiles of rows: wave w has tile w % RW.
   __device__ __forceinline__ void finish(const AttnArgs &a, int hd, int seq0, int head, int row0, int rows,
-                                         int part, float *buf, float *ml) {
+                                         int RW, int part, float *buf, float *ml) {
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4, wave = tid >> 6;
     constexpr int kCols = 8 * NC;  // of four dims
+    const float sum = groups_sum(l);
+    __syncthreads();
+    if (g == 0) ml[(wave * 16 + n) * 2] = m, ml[(wave * 16 + n) * 2 + 1] = sum;
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
-      if (t * 16 >= rows) break;
-      const float sum = groups_sum(l[t]);
-      __syncthreads();
-      if (g == 0) ml[(wave * 16 + n) * 2] = m[t], ml[(wave * 16 + n) * 2 + 1] = sum;
+    for (int d = 0; d < DT; d++)
+      *reinterpret_cast<f32x4 *>(buf + (wave * 16 + n) * kLd + d * 16 + g * 4) = o[d];
+    __syncthreads();
+    for (int i = tid; i < rows * kCols; i += 64 * kWaves) {
+      const int r = i / kCols, c = i % kCols;
+      if (4 * c >= hd) continue;
+      float ls = 0.0f, mx = kNegInf;
+      f32x4 x{0, 0, 0, 0};
+      for (int w = r; w < kWaves * 16; w += RW * 16) mx = fmaxf(mx, ml[w * 2]);
+      for (int w = r; w < kWaves * 16; w += RW * 16) {
+        const float mw = ml[w * 2];
+        // (a wave with no position has sums of 0, or of NaN if its scores were)
+        const float f = mw == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(mw - mx);
+        const f32x4 y = *reinterpret_cast<const f32x4 *>(buf + w * kLd + 4 * c);
+        ls = __builtin_fmaf(ml[w * 2 + 1], f, ls);
 #pragma unroll
-      for (int d = 0; d < DT; d++)
-        *reinterpret_cast<f32x4 *>(buf + (wave * 16 + n) * kLd + d * 16 + g * 4) = o[t][d];
-      __syncthreads();
+        for (int k = 0; k < 4; k++) x[k] = __builtin_fmaf(y[k], f, x[k]);
+      }
+      const int row = row0 + r, member = row / a.rep;
+      const size_t qh = (size_t)head * a.rep + (row - member * a.rep), seq = seq0 + member;
+      if (part < 0) {
+        float *out = a.out + seq * a.ldo + qh * hd + 4 * c;
 #pragma unroll
-      for (int i = tid; i < 16 * kCols; i += 64 * kWaves) {
-        const int r = i / kCols, c = i % kCols;
-        if (t * 16 + r >= rows || 4 * c >= hd) continue;
-        float mw[kWaves], ls = 0.0f, mx = kNegInf;
-        f32x4 x{0, 0, 0, 0};
-#pragma unroll
-        for (int w = 0; w < kWaves; w++) mx = fmaxf(mx, mw[w] = ml[(w * 16 + r) * 2]);
-#pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-          // (a wave with no position has sums of 0, or of NaN if its scores were)
-          const float f = mw[w] == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(mw[w] - mx);
-          const f32x4 y = *reinterpret_cast<const f32x4 *>(buf + (w * 16 + r) * kLd + 4 * c);
-          ls = __builtin_fmaf(ml[(w * 16 + r) * 2 + 1], f, ls);
-#pragma unroll
-          for (int k = 0; k < 4; k++) x[k] = __builtin_fmaf(y[k], f, x[k]);
-        }
-        const int row = row0 + t * 16 + r, member = row / a.rep;
-        const size_t qh = (size_t)head * a.rep + (row - member * a.rep), seq = seq0 + member;
-        if (part < 0) {
-          float *out = a.out + seq * a.ldo + qh * hd + 4 * c;
-#pragma unroll
-          for (int k = 0; k < 4; k++) out[k] = ls == 0.0f ? 0.0f : x[k] / ls;
-        } else {
-          const size_t at = (seq * a.nh + qh) * (a.npp + a.nsp) + part;
-          *reinterpret_cast<f32x4 *>(a.po + at * hd + 4 * c) = x;
-          if (c == 0) a.pml[at * 2] = mx, a.pml[at * 2 + 1] = ls;
-        }
+        for (int k = 0; k < 4; k++) out[k] = ls == 0.0f ? 0.0f : x[k] / ls;
+      } else {
+        const size_t at = (seq * a.nh + qh) * (a.npp + a.nsp) + part;
+        *reinterpret_cast<f32x4 *>(a.po + at * hd + 4 * c) = x;
+        if (c == 0) a.pml[at * 2] = mx, a.pml[at * 2 + 1] = ls;
       }
     }
   }
@@ -450,42 +512,40 @@ __device__ __forceinline__ int clamped(const int32_t *len, int i, int most) {
   return most ? max(0, min(len[i], most)) : 0;
 }
 
-// JOINED: a workgroup has both runs of a sequence's rows whole.  Else the
+// Joined: a workgroup has both runs of a sequence's rows whole.  Else the
 // first workgroups have the parts of the prefixes, the others those of the
 // suffixes.
-template <class T, int NC, int RT, bool JOINED>
-__global__ void __launch_bounds__(64 * kWaves) k_attend(AttnArgs a, KvPool<T> pool) {
-  using W = Attend<T, NC, RT>;
+template <class T, int NC>
+__global__ void __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) k_attend(AttnArgs a, KvPool<T> pool) {
+  using W = Rows<T, NC>;
   __shared__ __align__(16) uint8_t lds[W::kLdsBytes];
-  __shared__ float ml[kWaves * 16 * 2], scales[RT * 16];
-  const bool prefix = !JOINED && (int)blockIdx.x < a.prefix_wgs;
-  const int i = JOINED || prefix ? blockIdx.x : blockIdx.x - a.prefix_wgs;
+  __shared__ float ml[kWaves * 16 * 2];
+  const bool prefix = (int)blockIdx.x < a.prefix_wgs;
+  const int i = prefix ? blockIdx.x : blockIdx.x - a.prefix_wgs;
   const int members = prefix ? a.group_size : 1;  // sequences whose rows go together
-  const int all = members * a.rep, blocks = (all + RT * 16 - 1) / (RT * 16);
-  const int parts = JOINED ? 1 : (prefix ? a.npp : a.nsp);
+  const int RW = prefix ? a.prw : a.srw;
+  const int all = members * a.rep, blocks = (all + RW * 16 - 1) / (RW * 16);
+  const int parts = a.joined ? 1 : (prefix ? a.npp : a.nsp);
   // workgroup i runs on XCD i % 8: the blocks of rows that read the same
   // positions come 8 apart and share that XCD's L2
   const int j = i >> 3, unit = (j / blocks) * 8 + (i & 7), block = j % blocks;
   const int head = unit % pool.nkv, u = unit / pool.nkv;
   const int part = u % parts, owner = u / parts;  // group or sequence
   if (owner * members >= a.n_seqs) return;
-  const int seq0 = owner * members, row0 = block * RT * 16, rows = min(RT * 16, all - row0);
+  const int seq0 = owner * members, row0 = block * RW * 16, rows = min(RW * 16, all - row0);
   const int group = prefix ? owner : owner / a.group_size;
-  const int32_t *pt = a.ptable + (size_t)group * a.ld_ptable;
-  const int32_t *st = a.table + (size_t)seq0 * a.ld_table;
-  W w;
-  if (JOINED) {
-    const int plen = clamped(a.plen, group, a.max_prefix), slen = clamped(a.slen, seq0, a.max_suffix);
-    w.load_queries(a, pool.hd, seq0, head, row0, rows, lds, scales);
-    w.run(pool, head, rows, Run{pt, 0, plen, 0});
-    w.run(pool, head, rows, Run{st, 0, slen, (plen + kTile - 1) / kTile});
-    w.finish(a, pool.hd, seq0, head, row0, rows, -1, reinterpret_cast<float *>(lds), ml);
-  } else {
-    const int len = prefix ? clamped(a.plen, group, a.max_prefix) : clamped(a.slen, seq0, a.max_suffix);
-    const int chunk = prefix ? a.pchunk : a.schunk, from = part * chunk, at = prefix ? part : a.npp + part;
-    if (from >= len) {  // nothing here: no rows to write, a sum of 0
-      for (int r = threadIdx.x; r < rows; r += 64 * kWaves) {
-        const int row = row0 + r, member = row / a.rep;
+  const int plen = prefix || a.joined ? clamped(a.plen, group, a.max_prefix) : 0;
+  const int slen = prefix ? 0 : clamped(a.slen, seq0, a.max_suffix);
+  Run r{prefix ? a.ptable + (size_t)group * a.ld_ptable : a.table + (size_t)seq0 * a.ld_table, 0, slen, 0};
+  int at = -1;
+  if (!a.joined) {
+    const int len = prefix ? plen : slen, chunk = prefix ? a.pchunk : a.schunk;
+    r.from = part * chunk;
+    r.to = min(r.from + chunk, len);
+    at = prefix ? part : a.npp + part;
+    if (r.from >= len) {  // nothing here: no rows to write, a sum of 0
+      for (int k = threadIdx.x; k < rows; k += 64 * kWaves) {
+        const int row = row0 + k, member = row / a.rep;
         const size_t p = ((size_t)(seq0 + member) * a.nh + (size_t)head * a.rep + (row - member * a.rep)) *
                              (a.npp + a.nsp) + at;
         a.pml[p * 2] = kNegInf;
@@ -493,10 +553,24 @@ __global__ void __launch_bounds__(64 * kWaves) k_attend(AttnArgs a, KvPool<T> po
       }
       return;
     }
-    w.load_queries(a, pool.hd, seq0, head, row0, rows, lds, scales);
-    w.run(pool, head, rows, Run{prefix ? pt : st, from, min(from + chunk, len), 0});
-    w.finish(a, pool.hd, seq0, head, row0, rows, at, reinterpret_cast<float *>(lds), ml);
   }
+  W w;
+  const int tile = (int)(threadIdx.x >> 6) & (RW - 1);
+  w.load_queries(a, pool.hd, seq0, head, row0 + tile * 16, row0 + rows - 1);
+  if (RW == 1) {
+    // joined: the prefix first, its next tile's wave begins the suffix
+    for (int k = a.joined ? 0 : 1; k < 2; k++) {
+      Run x = r;
+      if (k == 0) x = Run{a.ptable + (size_t)group * a.ld_ptable, 0, plen, 0};
+      if (k == 1 && a.joined) x.first = (plen + kTile - 1) / kTile;
+      w.run_alone(pool, head, x);
+    }
+  } else if (RW == 4) {
+    w.template run_shared<1>(pool, head, r, lds);
+  } else {
+    if constexpr (W::kRing == 4) w.template run_shared<2>(pool, head, r, lds);
+  }
+  w.finish(a, pool.hd, seq0, head, row0, rows, RW, at, reinterpret_cast<float *>(lds), ml);
 }
 
 // One workgroup a query row: the factors of 64 parts at a time by lanes, the
@@ -573,16 +647,9 @@ syn_status_t check_attention(const syn_hip_kv_pages *pages,
   return SYN_OK;
 }
 
-// tiles of 16 query rows that a workgroup holds, as many as there are up to
-// what the registers take
-int row_tiles(int nc, bool f32, size_t rows) {
-  const int most = nc <= 4 ? 4 : (f32 ? 1 : 2);
-  return rows > 32 && most == 4 ? 4 : (rows > 16 && most >= 2 ? 2 : 1);
-}
-
 struct Plan {
   bool joined;
-  int nc, rt;  // dims and row tiles of a workgroup
+  int nc, prw, srw;
   int pchunk, schunk, npp, nsp;
   size_t prefix_wgs, wgs, rows, po_bytes, pml_bytes;
 };
@@ -592,17 +659,20 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_prefix_attention_params
   const int hd = (int)pg.head_dim, nkv = (int)pg.n_kv_heads, rep = (int)p.n_heads / nkv;
   w.nc = hd <= 64 ? 2 : (hd <= 128 ? 4 : 8);
   w.rows = (size_t)p.n_groups * p.group_size * p.n_heads;
+  // two tiles of rows need a ring of four tiles of positions
+  const bool small = w.nc * (pg.dtype == SYN_HIP_KV_F32 ? 2 : 1) <= 4;
+  auto tiles = [&](size_t rows) { return rows <= 16 ? 1 : (rows <= 32 && small ? 2 : 4); };
   const size_t step = kTile * kWaves, seqs = (size_t)p.n_groups * p.group_size;
   w.joined = (size_t)p.max_prefix + p.max_suffix <= 4 * step;
-  w.rt = w.joined ? 1 : row_tiles(w.nc, pg.dtype == SYN_HIP_KV_F32,
-                                  p.max_prefix ? (size_t)p.group_size * rep : rep);
-  const size_t sblocks = cdiv(rep, 16 * w.rt), sunits = seqs * nkv;
+  w.prw = tiles((size_t)p.group_size * rep);
+  w.srw = w.joined ? 1 : tiles(rep);
+  const size_t sblocks = cdiv(rep, 16 * w.srw), sunits = seqs * nkv;
   if (w.joined) {
     w.wgs = round_up(sunits, 8) * sblocks;
     return w;
   }
   // parts of about equal work for kWant workgroups in all
-  const size_t pblocks = cdiv((size_t)p.group_size * rep, 16 * w.rt), punits = (size_t)p.n_groups * nkv;
+  const size_t pblocks = cdiv((size_t)p.group_size * rep, 16 * w.prw), punits = (size_t)p.n_groups * nkv;
   const size_t psteps = cdiv(p.max_prefix, step), ssteps = cdiv(p.max_suffix, step);
   const size_t total = punits * pblocks * psteps + sunits * sblocks * ssteps;
   const size_t per = std::max<size_t>(1, cdiv(total, kWant));
@@ -622,24 +692,11 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_prefix_attention_params
   return w;
 }
 
-template <class T, int NC, int RT, bool JOINED = false>
-syn_status_t launch_one(const Plan &w, const AttnArgs &a, const KvPool<T> &pool, hipStream_t s) {
-  hipLaunchKernelGGL((k_attend<T, NC, RT, JOINED>), dim3((unsigned)w.wgs), dim3(64 * kWaves), 0, s, a,
-                     pool);
-  SYN_LAUNCH_CHECK();
-  return SYN_OK;
-}
-
 template <class T, int NC>
-syn_status_t launch_nc(const Plan &w, const AttnArgs &a, const KvPool<T> &pool, hipStream_t s) {
-  if (w.joined) return launch_one<T, NC, 1, true>(w, a, pool, s);
-  if (w.rt == 1) {
-    SYN_TRY((launch_one<T, NC, 1>(w, a, pool, s)));
-  } else if (w.rt == 2) {
-    if constexpr (NC <= 4 || sizeof(T) == 2) SYN_TRY((launch_one<T, NC, 2>(w, a, pool, s)));
-  } else {
-    if constexpr (NC <= 4) SYN_TRY((launch_one<T, NC, 4>(w, a, pool, s)));
-  }
+syn_status_t launch(const Plan &w, const AttnArgs &a, const KvPool<T> &pool, hipStream_t s) {
+  hipLaunchKernelGGL((k_attend<T, NC>), dim3((unsigned)w.wgs), dim3(64 * kWaves), 0, s, a, pool);
+  SYN_LAUNCH_CHECK();
+  if (w.joined) return SYN_OK;
   hipLaunchKernelGGL(k_join_parts, dim3((unsigned)w.rows), dim3(256), 0, s, a, pool.hd);
   SYN_LAUNCH_CHECK();
   return SYN_OK;
@@ -705,6 +762,9 @@ extern "C" syn_status_t syn_hip_prefix_attention(
   a.npp = w.npp;
   a.nsp = w.nsp;
   a.prefix_wgs = (int)w.prefix_wgs;
+  a.prw = w.prw;
+  a.srw = w.srw;
+  a.joined = w.joined;
   a.q16 = aligned16(d_q) && p->ldq % 4 == 0;
   a.po = static_cast<float *>(d_workspace);
   a.pml = reinterpret_cast<float *>(static_cast<uint8_t *>(d_workspace) + w.po_bytes);
@@ -712,8 +772,8 @@ extern "C" syn_status_t syn_hip_prefix_attention(
   return kv_dispatch(pages->dtype, [&](auto t) -> syn_status_t {
     using T = decltype(t);
     const KvPool<T> pool = kv_pool<T>(*pages, p->layer);
-    if (w.nc == 2) return launch_nc<T, 2>(w, a, pool, s);
-    if (w.nc == 4) return launch_nc<T, 4>(w, a, pool, s);
-    return launch_nc<T, 8>(w, a, pool, s);
+    if (w.nc == 2) return launch<T, 2>(w, a, pool, s);
+    if (w.nc == 4) return launch<T, 4>(w, a, pool, s);
+    return launch<T, 8>(w, a, pool, s);
   });
 }
