@@ -629,8 +629,8 @@ syn_status_t syn_hip_hlm_destroy(syn_hip_hlm_t *m);
 /* A pool of pages, each page_size positions of every kv head:
  *   k [n_layers][n_pages][n_kv_heads][head_dim / 8][page_size][8]
  *   v [n_layers][n_pages][n_kv_heads][page_size / 8][head_dim][8]
- * page_size: a power of two, 8 to 1024; head_dim: a multiple of 8 up to 256;
- * k and v 16-byte aligned.  A sequence's positions are found through its row
+ * page_size: a power of two, 8 to 1024; head_dim: a multiple of 8 up to 256; a
+ * page below 2 GiB; k and v 16-byte aligned.  A sequence's positions are found through its row
  * of a page table: position i in page table[i / page_size], slot
  * i % page_size.  Entries outside [0, n_pages) name no page. */
 typedef struct {

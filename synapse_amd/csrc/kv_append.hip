@@ -143,6 +143,11 @@ syn_status_t check_pages(const syn_hip_kv_pages *p, const char *who) {
     set_error(std::string(who) + ": pages, layers and kv heads must be at least 1");
     return SYN_ERR_INVALID_ARG;
   }
+  // (kernels step through a page's bytes in 32 bits; from page to page in 64)
+  if (kv_page_elems(*p) * kv_elem_bytes(p->dtype) > 0x7fffffffu) {
+    set_error(std::string(who) + ": pages of at most 2^31 - 1 bytes");
+    return SYN_ERR_INVALID_ARG;
+  }
   if (!p->k || !p->v) return SYN_ERR_NULL_PTR;
   if (!aligned16(p->k) || !aligned16(p->v)) {
     set_error(std::string(who) + ": page pools must be 16-byte aligned");

@@ -172,6 +172,12 @@ struct Run {
   int from, to, first;
 };
 
+// A kv head's K and V of page 0, and the bytes from page to page.
+struct HeadBase {
+  const uint8_t *k, *v;
+  uint32_t page_bytes;
+};
+
 // One wave's part of the work: 16 query rows of a kv head.
 template <class T, int NC> struct Rows {
   using F = Frag<T>;
@@ -242,7 +248,9 @@ template <class T, int NC> struct Rows {
 
   // ---- a tile's operands: lane (g, n) has K of the position group n / 4 and
   // V of group g, of the four groups of 8 positions.  Positions past the end
-  // are read at the last group there is.
+  // are read at the last group there is.  Pages are looked up by scalar loads
+  // (k0 is the same for the whole wave), which do not queue with the K and V
+  // in flight; WIDE: a page holds whole tiles, so one serves all groups.
   struct Where {
     int p0, p1, p2, p3;  // pages of the groups
     __device__ __forceinline__ int of(int group) const {
@@ -254,38 +262,55 @@ template <class T, int NC> struct Rows {
   static __device__ __forceinline__ int spot(int k0, int group, int to) {
     return min(k0 + 8 * group, (to - 1) & ~7);
   }
-  // by scalar loads (k0 is the same for the whole wave): they do not queue
-  // with the K and V in flight
+  template <bool WIDE>
   static __device__ __forceinline__ Where look_up(const KvPool<T> &pool, const Run &r, int k0) {
     const auto *t = (const __attribute__((address_space(4))) int32_t *)(uintptr_t)r.table;
-    return Where{t[spot(k0, 0, r.to) >> pool.ps_shift], t[spot(k0, 1, r.to) >> pool.ps_shift],
-                 t[spot(k0, 2, r.to) >> pool.ps_shift], t[spot(k0, 3, r.to) >> pool.ps_shift]};
+    const int p = t[(uint32_t)spot(k0, 0, r.to) >> pool.ps_shift];
+    if (WIDE) return Where{p, p, p, p};
+    return Where{p, t[(uint32_t)spot(k0, 1, r.to) >> pool.ps_shift],
+                 t[(uint32_t)spot(k0, 2, r.to) >> pool.ps_shift],
+                 t[(uint32_t)spot(k0, 3, r.to) >> pool.ps_shift]};
   }
   // which of the groups' pages are pages, a bit each
+  template <bool WIDE>
   static __device__ __forceinline__ uint32_t found(const KvPool<T> &pool, const Where &w) {
+    if (WIDE) return pool.has(w.p0) ? 15u : 0u;
     return (pool.has(w.p0) ? 1u : 0u) | (pool.has(w.p1) ? 2u : 0u) | (pool.has(w.p2) ? 4u : 0u) |
            (pool.has(w.p3) ? 8u : 0u);
   }
-  static __device__ __forceinline__ const T *k_of(const KvPool<T> &pool, int head, const Run &r, int k0,
-                                                  const Where &w) {
-    const int n = threadIdx.x & 15, page = w.of(n >> 2);
-    const int slot = (spot(k0, n >> 2, r.to) & (pool.ps - 1)) + (n & 3);
-    return pool.k + pool.base(pool.has(page) ? page : 0, head) + (size_t)slot * 8;
+  // The addresses of a tile: K at k + koff (dims of a fragment) and V at v +
+  // voff; a tile that one page holds whole has wave-uniform k and v.
+  struct Tile {
+    const uint8_t *k, *v;
+  };
+  template <bool WIDE>
+  static __device__ __forceinline__ Tile tile_of(const KvPool<T> &pool, const HeadBase &hb, const Run &r,
+                                                 int k0, const Where &w) {
+    if (WIDE && k0 + kTile <= r.to) {
+      const uint64_t page = (uint64_t)(uint32_t)(pool.has(w.p0) ? w.p0 : 0) * hb.page_bytes;
+      const uint32_t slot = k0 & (pool.ps - 1);
+      return Tile{hb.k + page + slot * (8 * (uint32_t)sizeof(T)),
+                  hb.v + page + (slot >> 3) * (uint32_t)(pool.hd * 8 * (int)sizeof(T))};
+    }
+    // the offsets below are those of group n / 4 (K) and g (V) of a whole tile
+    const int n4 = (threadIdx.x & 15) >> 2, g = (threadIdx.x & 63) >> 4;
+    const int pk = w.of(n4), pv = w.of(g);
+    const int sk = (spot(k0, n4, r.to) & (pool.ps - 1)) - 8 * n4;
+    const int sv = ((spot(k0, g, r.to) & (pool.ps - 1)) >> 3) - g;
+    return Tile{hb.k + (uint64_t)(uint32_t)(pool.has(pk) ? pk : 0) * hb.page_bytes +
+                    (int64_t)(sk * 8 * (int)sizeof(T)),
+                hb.v + (uint64_t)(uint32_t)(pool.has(pv) ? pv : 0) * hb.page_bytes +
+                    (int64_t)(sv * (pool.hd * 8 * (int)sizeof(T)))};
   }
-  static __device__ __forceinline__ const T *v_of(const KvPool<T> &pool, int head, const Run &r, int k0,
-                                                  const Where &w) {
-    const int g = (threadIdx.x & 63) >> 4, page = w.of(g);
-    const int group = (spot(k0, g, r.to) & (pool.ps - 1)) >> 3;
-    return pool.v + pool.base(pool.has(page) ? page : 0, head) + (size_t)group * pool.hd * 8;
+  // bytes to fragment f: K of half f % 2 at dims 32 (f / 2); V of dims 16 f
+  static __device__ __forceinline__ uint32_t koff(const KvPool<T> &pool, int f) {
+    const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+    return (uint32_t)((min((f >> 1) * 4 + g, (pool.hd >> 3) - 1) * pool.ps + 8 * (n >> 2) + (n & 3) +
+                       (f & 1) * 4) * 8 * (int)sizeof(T));
   }
-  // element offset of fragment f: K of half f % 2 at dims 32 (f / 2), then V
-  // of 16 dims
-  static __device__ __forceinline__ size_t k_off(const KvPool<T> &pool, int f) {
-    const int g = (threadIdx.x & 63) >> 4;
-    return (size_t)min((f >> 1) * 4 + g, (pool.hd >> 3) - 1) * pool.ps * 8 + (f & 1) * 32;
-  }
-  static __device__ __forceinline__ size_t v_off(const KvPool<T> &pool, int d) {
-    return (size_t)min(d * 16 + (int)(threadIdx.x & 15), pool.hd - 1) * 8;
+  static __device__ __forceinline__ uint32_t voff(const KvPool<T> &pool, int f) {
+    const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+    return (uint32_t)((g * pool.hd + min(f * 16 + n, pool.hd - 1)) * 8 * (int)sizeof(T));
   }
   // the positions 8g .. 8g+7 whose weights this lane holds, a bit each
   static __device__ __forceinline__ uint32_t which(int k0, int to, uint32_t ok) {
@@ -294,25 +319,32 @@ template <class T, int NC> struct Rows {
   }
 
   // ---- the two products of a tile
-  template <class K> __device__ __forceinline__ void scores(K k, f32x4 *s) const {
+  __device__ __forceinline__ void scores(const V *k, f32x4 *s) const {
     s[0] = s[1] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int c = 0; c < NC; c++) {
-      s[0] = F::mma(k(2 * c), q[c], s[0]);
-      s[1] = F::mma(k(2 * c + 1), q[c], s[1]);
+      s[0] = F::mma(k[2 * c], q[c], s[0]);
+      s[1] = F::mma(k[2 * c + 1], q[c], s[1]);
     }
     // Read the sums before the next branch: where a conditional region lies
     // between, the compiler pads the matrix instruction's latency on the
     // longer way only.
     asm volatile("" : "+v"(s[0]), "+v"(s[1]));
   }
-  template <class G> __device__ __forceinline__ void weigh(const f32x4 *s, bool whole, uint32_t there, G v) {
+  __device__ __forceinline__ void weigh(const f32x4 *s, V *v, int k0, int to, uint32_t ok) {
     float x[8];
 #pragma unroll
     for (int j = 0; j < 4; j++) x[j] = s[0][j], x[j + 4] = s[1][j];
-    if (!whole)
+    if (k0 + kTile > to || ok != 15) {
+      const uint32_t there = which(k0, to, ok);
 #pragma unroll
-      for (int j = 0; j < 8; j++) x[j] = there >> j & 1 ? x[j] : kNegInf;
+      for (int j = 0; j < 8; j++) {
+        x[j] = there >> j & 1 ? x[j] : kNegInf;
+#pragma unroll
+        for (int d = 0; d < DT; d++)  // what is not there may hold anything: 0 times NaN is NaN
+          if (!(there >> j & 1)) F::clear(v[d], j);
+      }
+    }
     float top = fmaxf(x[0], x[1]);
 #pragma unroll
     for (int j = 2; j < 8; j += 2) top = fmaxf(fmaxf(x[j], x[j + 1]), top);
@@ -328,64 +360,54 @@ template <class T, int NC> struct Rows {
       for (int d = 0; d < DT; d++) o[d] *= back;
     }
     const float ref = F::kBias - (m == kNegInf ? 0.0f : m);
-    float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], unscale, ref));
-      sum[j & 1] += x[j];
-    }
-    l += sum[0] + sum[1];
+    for (int j = 0; j < 8; j++) x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], unscale, ref));
+    l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
     V p[F::kParts];
     F::split(x, p);
 #pragma unroll
-    for (int d = 0; d < DT; d++) {
-      V f = v(d);
-      if (!whole) {  // what is not there may hold anything: 0 times NaN is NaN
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-          if (!(there >> j & 1)) F::clear(f, j);
-      }
-      o[d] = F::mma(f, p, o[d]);
-    }
+    for (int d = 0; d < DT; d++) o[d] = F::mma(v[d], p, o[d]);
   }
 
   // ---- 16 rows in all: the waves take the tiles of a run in turn, K and V in
   // registers.  One set of them: the next tile's K is requested when this
   // one's scores are formed, its V when this one's product is.
-  __device__ __forceinline__ void run_alone(const KvPool<T> &pool, int head, const Run &r) {
+  template <bool WIDE>
+  __device__ __forceinline__ void run_alone(const KvPool<T> &pool, const HeadBase &hb, const Run &r) {
     constexpr int kStep = kTile * kWaves;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int k0 = r.from + ((wave - r.first) & (kWaves - 1)) * kTile;
     if (k0 >= r.to) return;
+    uint32_t ko[2 * NC], vo[DT];
+#pragma unroll
+    for (int f = 0; f < 2 * NC; f++) ko[f] = koff(pool, f), vo[f] = voff(pool, f);
     V kf[2 * NC], vf[DT];
-    Where w = look_up(pool, r, k0);
-    uint32_t ok = found(pool, w);
+    Where w = look_up<WIDE>(pool, r, k0);
+    uint32_t ok = found<WIDE>(pool, w);
     {
-      const T *k = k_of(pool, head, r, k0, w), *v = v_of(pool, head, r, k0, w);
+      const Tile t = tile_of<WIDE>(pool, hb, r, k0, w);
 #pragma unroll
-      for (int f = 0; f < 2 * NC; f++) kf[f] = F::load(k + k_off(pool, f));
+      for (int f = 0; f < 2 * NC; f++) kf[f] = F::load(reinterpret_cast<const T *>(t.k + ko[f]));
 #pragma unroll
-      for (int d = 0; d < DT; d++) vf[d] = F::load(v + v_off(pool, d));
+      for (int d = 0; d < DT; d++) vf[d] = F::load(reinterpret_cast<const T *>(t.v + vo[d]));
     }
-    w = look_up(pool, r, k0 + kStep);
+    w = look_up<WIDE>(pool, r, k0 + kStep);
     for (;;) {
       const int k1 = k0 + kStep;
-      const bool whole = k0 + kTile <= r.to && ok == 15;
-      const uint32_t there = which(k0, r.to, ok);
       f32x4 s[2];
-      scores([&](int f) { return kf[f]; }, s);
+      scores(kf, s);
+      Tile t;
       if (k1 < r.to) {
-        const T *k = k_of(pool, head, r, k1, w);
+        t = tile_of<WIDE>(pool, hb, r, k1, w);
 #pragma unroll
-        for (int f = 0; f < 2 * NC; f++) kf[f] = F::load(k + k_off(pool, f));
+        for (int f = 0; f < 2 * NC; f++) kf[f] = F::load(reinterpret_cast<const T *>(t.k + ko[f]));
       }
-      weigh(s, whole, there, [&](int d) { return vf[d]; });
+      weigh(s, vf, k0, r.to, ok);
       if (k1 >= r.to) break;
-      const T *v = v_of(pool, head, r, k1, w);
 #pragma unroll
-      for (int d = 0; d < DT; d++) vf[d] = F::load(v + v_off(pool, d));
-      ok = found(pool, w);
-      w = look_up(pool, r, k1 + kStep);
+      for (int d = 0; d < DT; d++) vf[d] = F::load(reinterpret_cast<const T *>(t.v + vo[d]));
+      ok = found<WIDE>(pool, w);
+      w = look_up<WIDE>(pool, r, k1 + kStep);
       k0 = k1;
     }
   }
@@ -393,27 +415,32 @@ template <class T, int NC> struct Rows {
   // ---- 16 rows to each of kWaves / KW waves: every wave reads every tile (KW
   // 1) or every other (KW 2), so the tiles go through a ring in LDS, in
   // fragment order, by direct loads that run kRing / KW - 1 steps ahead.
-  __device__ __forceinline__ void issue(const KvPool<T> &pool, int head, const Run &r, int k0, uint32_t lds,
-                                        const Where &w) {
-    constexpr int kHalves = (int)sizeof(V) / 16, kMine = kLoads / kWaves;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const T *k = k_of(pool, head, r, k0, w), *v = v_of(pool, head, r, k0, w);
+  static constexpr int kHalves = (int)sizeof(V) / 16;  // 16-byte loads of a fragment
+  static constexpr int kShare = kLoads / kWaves;       // direct loads of a tile by one wave: K, then V
+  template <bool WIDE>
+  __device__ __forceinline__ void issue(const KvPool<T> &pool, const HeadBase &hb, const Run &r, int k0,
+                                        uint32_t lds, const Where &w, const uint32_t *off) {
+    const Tile t = tile_of<WIDE>(pool, hb, r, k0, w);
 #pragma unroll
-    for (int i = 0; i < kMine; i++) {
-      const int b = i * kWaves + wave, f = b / kHalves;
-      const T *src = i < kMine / 2 ? k + k_off(pool, f) : v + v_off(pool, f - 2 * NC);
-      kr_dma(src + (b % kHalves) * 4, lds + b * 1024);
-    }
+    for (int i = 0; i < kShare; i++)
+      kr_dma((i < kShare / 2 ? t.k : t.v) + off[i], lds + i * kWaves * 1024);
   }
-  template <int KW>
-  __device__ __forceinline__ void run_shared(const KvPool<T> &pool, int head, const Run &r, uint8_t *ring) {
-    constexpr int S = kRing / KW, kAhead = S - 1, kStep = KW * kTile, kMine = KW * kLoads / kWaves;
+  template <bool WIDE, int KW>
+  __device__ __forceinline__ void run_shared(const KvPool<T> &pool, const HeadBase &hb, const Run &r,
+                                             uint8_t *ring) {
+    constexpr int S = kRing / KW, kAhead = S - 1, kStep = KW * kTile;
     static_assert(kLoads % (2 * kWaves) == 0 && 8 * kAhead < 32, "K and V in whole shares");
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr_of(ring));
     const int n = (r.to - r.from + kStep - 1) / kStep;
     const int mine = KW == 1 ? 0 : wave / (kWaves / KW);  // tile of a step
+    uint32_t off[kShare];
+#pragma unroll
+    for (int i = 0; i < kShare; i++) {
+      const int b = i * kWaves + wave, f = b / kHalves;
+      off[i] = (i < kShare / 2 ? koff(pool, f) : voff(pool, f - 2 * NC)) + (b % kHalves) * 16;
+    }
     // found() of the tiles in flight: 4 bits a tile, 8 a step, this step's lowest
     uint32_t ok = 0;
 #pragma unroll
@@ -422,26 +449,24 @@ template <class T, int NC> struct Rows {
 #pragma unroll
         for (int t = 0; t < KW; t++) {
           const int kt = r.from + i * kStep + t * kTile;
-          const Where w = look_up(pool, r, kt);
-          ok |= found(pool, w) << (8 * i + 4 * t);
-          issue(pool, head, r, kt, base + (i * KW + t) * kTileBytes, w);
+          const Where w = look_up<WIDE>(pool, r, kt);
+          ok |= found<WIDE>(pool, w) << (8 * i + 4 * t);
+          issue<WIDE>(pool, hb, r, kt, base + (i * KW + t) * kTileBytes + wave * 1024, w, off);
         }
     int get = 0, put = kAhead;  // places in the ring
     for (int i = 0; i < n; i++) {
       const int k0 = r.from + i * kStep, k2 = k0 + kAhead * kStep;
-      const Where w0 = look_up(pool, r, k2), w1 = KW == 2 ? look_up(pool, r, k2 + kTile) : w0;
+      const Where w0 = look_up<WIDE>(pool, r, k2), w1 = KW == 2 ? look_up<WIDE>(pool, r, k2 + kTile) : w0;
       // step i has landed, and every wave is done with step i - 1
       if (i + kAhead <= n)
-        kr_publish<(kAhead - 1) * kMine>();
+        kr_publish<(kAhead - 1) * KW * kShare>();
       else
         kr_publish<0>();
-      if (i + kAhead < n) {
-        issue(pool, head, r, k2, base + put * KW * kTileBytes, w0);
-        if (KW == 2) issue(pool, head, r, k2 + kTile, base + (put * KW + 1) * kTileBytes, w1);
-        ok |= (found(pool, w0) | (KW == 2 ? found(pool, w1) << 4 : 0)) << (8 * kAhead);
-      }
       const int kt = k0 + mine * kTile;
-      if (KW == 1 || kt < r.to) {
+      const uint32_t here = ok >> (4 * mine) & 15;
+      const bool on = KW == 1 || kt < r.to;
+      V kf[2 * NC], vf[DT];
+      if (on) {
         const uint8_t *f = ring + (get * KW + mine) * kTileBytes;
         auto frag = [&](int j) {
           if constexpr (sizeof(V) == 16) {
@@ -451,14 +476,25 @@ template <class T, int NC> struct Rows {
             return V{h[0], h[64]};
           }
         };
-        const uint32_t here = ok >> (4 * mine) & 15;
-        const bool whole = kt + kTile <= r.to && here == 15;
-        const uint32_t there = which(kt, r.to, here);
-        f32x4 s[2];
-        scores(frag, s);
-        weigh(s, whole, there, [&](int d) { return frag(2 * NC + d); });
+#pragma unroll
+        for (int j = 0; j < 2 * NC; j++) kf[j] = frag(j);
+#pragma unroll
+        for (int j = 0; j < DT; j++) vf[j] = frag(2 * NC + j);
+        // all of the tile is asked for before the first product waits
+        __builtin_amdgcn_sched_barrier(0);
       }
       ok >>= 8;
+      if (i + kAhead < n) {
+        issue<WIDE>(pool, hb, r, k2, base + put * KW * kTileBytes + wave * 1024, w0, off);
+        if (KW == 2)
+          issue<WIDE>(pool, hb, r, k2 + kTile, base + (put * KW + 1) * kTileBytes + wave * 1024, w1, off);
+        ok |= (found<WIDE>(pool, w0) | (KW == 2 ? found<WIDE>(pool, w1) << 4 : 0)) << (8 * (kAhead - 1));
+      }
+      if (on) {
+        f32x4 s[2];
+        scores(kf, s);
+        weigh(s, vf, kt, r.to, here);
+      }
       get = get + 1 == S ? 0 : get + 1;
       put = put + 1 == S ? 0 : put + 1;
     }
@@ -516,7 +552,7 @@ __device__ __forceinline__ int clamped(const int32_t *len, int i, int most) {
 // first workgroups have the parts of the prefixes, the others those of the
 // suffixes.
 template <class T, int NC>
-__global__ void __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) k_attend(AttnArgs a, KvPool<T> pool) {
+__global__ void __launch_bounds__(64 * kWaves, NC * sizeof(T) <= 8 ? 2 : 1) k_attend(AttnArgs a, KvPool<T> pool) {
   using W = Rows<T, NC>;
   __shared__ __align__(16) uint8_t lds[W::kLdsBytes];
   __shared__ float ml[kWaves * 16 * 2];
@@ -557,18 +593,32 @@ __global__ void __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) k_attend(AttnArg
   W w;
   const int tile = (int)(threadIdx.x >> 6) & (RW - 1);
   w.load_queries(a, pool.hd, seq0, head, row0 + tile * 16, row0 + rows - 1);
+  const size_t head_bytes = (size_t)pool.hd * pool.ps * sizeof(T);
+  const HeadBase hb{reinterpret_cast<const uint8_t *>(pool.k) + head * head_bytes,
+                    reinterpret_cast<const uint8_t *>(pool.v) + head * head_bytes,
+                    (uint32_t)(pool.nkv * head_bytes)};
+  const bool wide = pool.ps >= kTile;
   if (RW == 1) {
     // joined: the prefix first, its next tile's wave begins the suffix
     for (int k = a.joined ? 0 : 1; k < 2; k++) {
       Run x = r;
       if (k == 0) x = Run{a.ptable + (size_t)group * a.ld_ptable, 0, plen, 0};
       if (k == 1 && a.joined) x.first = (plen + kTile - 1) / kTile;
-      w.run_alone(pool, head, x);
+      if (wide)
+        w.template run_alone<true>(pool, hb, x);
+      else
+        w.template run_alone<false>(pool, hb, x);
     }
   } else if (RW == 4) {
-    w.template run_shared<1>(pool, head, r, lds);
-  } else {
-    if constexpr (W::kRing == 4) w.template run_shared<2>(pool, head, r, lds);
+    if (wide)
+      w.template run_shared<true, 1>(pool, hb, r, lds);
+    else
+      w.template run_shared<false, 1>(pool, hb, r, lds);
+  } else if constexpr (W::kRing == 4) {
+    if (wide)
+      w.template run_shared<true, 2>(pool, hb, r, lds);
+    else
+      w.template run_shared<false, 2>(pool, hb, r, lds);
   }
   w.finish(a, pool.hd, seq0, head, row0, rows, RW, at, reinterpret_cast<float *>(lds), ml);
 }

@@ -21,7 +21,8 @@ BAD_PAGES = [(dict(dtype=3), ARG), (dict(dtype=-1), ARG), (dict(page_size=4), AR
              (dict(page_size=24), ARG), (dict(page_size=2048), ARG), (dict(page_size=0), ARG),
              (dict(head_dim=0), ARG), (dict(head_dim=60), ARG), (dict(head_dim=264), ARG),
              (dict(n_kv_heads=0), ARG), (dict(n_pages=0), ARG), (dict(n_layers=0), ARG),
-             (dict(n_pages=1 << 31), ARG), (dict(k=None), NULL), (dict(v=None), NULL),
+             (dict(n_pages=1 << 31), ARG),
+             (dict(page_size=1024, head_dim=256, n_kv_heads=4096), ARG), (dict(k=None), NULL), (dict(v=None), NULL),
              (dict(k=FAKE + 4), ARG), (dict(v=FAKE + 8), ARG)]
 
 
