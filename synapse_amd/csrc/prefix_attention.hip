@@ -31,10 +31,6 @@ constexpr float kNegInf = -__builtin_huge_valf();
 constexpr int kWaves = 4;
 constexpr float kSlack = 8.0f;
 constexpr int kTile = 32;  // positions a wave takes at a time
-#ifndef KWANT
-#define KWANT 512
-#endif
-constexpr size_t kWant = KWANT;
 
 struct AttnArgs {
   const float *q;
@@ -178,8 +174,8 @@ struct HeadBase {
   uint32_t page_bytes;
 };
 
-// One wave's part of the work: 16 query rows of a kv head.
-template <class T, int NC> struct Rows {
+// One wave's part of the work: 16 query rows of a kv head.  FULL: hd is 32 NC.
+template <class T, int NC, bool FULL> struct Rows {
   using F = Frag<T>;
   using V = typename F::V;
   static constexpr int DT = 2 * NC;           // tiles of 16 dims (hd <= 32 NC)
@@ -305,12 +301,14 @@ template <class T, int NC> struct Rows {
   // bytes to fragment f: K of half f % 2 at dims 32 (f / 2); V of dims 16 f
   static __device__ __forceinline__ uint32_t koff(const KvPool<T> &pool, int f) {
     const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
-    return (uint32_t)((min((f >> 1) * 4 + g, (pool.hd >> 3) - 1) * pool.ps + 8 * (n >> 2) + (n & 3) +
+    const int d8 = FULL ? (f >> 1) * 4 + g : min((f >> 1) * 4 + g, (pool.hd >> 3) - 1);
+    return (uint32_t)((d8 * pool.ps + 8 * (n >> 2) + (n & 3) +
                        (f & 1) * 4) * 8 * (int)sizeof(T));
   }
   static __device__ __forceinline__ uint32_t voff(const KvPool<T> &pool, int f) {
     const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
-    return (uint32_t)((g * pool.hd + min(f * 16 + n, pool.hd - 1)) * 8 * (int)sizeof(T));
+    const int d = FULL ? f * 16 + n : min(f * 16 + n, pool.hd - 1);
+    return (uint32_t)((g * (FULL ? 32 * NC : pool.hd) + d) * 8 * (int)sizeof(T));
   }
   // the positions 8g .. 8g+7 whose weights this lane holds, a bit each
   static __device__ __forceinline__ uint32_t which(int k0, int to, uint32_t ok) {
@@ -378,18 +376,38 @@ template <class T, int NC> struct Rows {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int k0 = r.from + ((wave - r.first) & (kWaves - 1)) * kTile;
     if (k0 >= r.to) return;
-    uint32_t ko[2 * NC], vo[DT];
+    // (FULL: the fragments' offsets are even steps from the first)
+    const uint32_t k_first = koff(pool, 0), v_first = voff(pool, 0);
+    const uint32_t k_step = 32 * (uint32_t)(pool.ps * (int)sizeof(T));
+    uint32_t ko[FULL ? 1 : 2 * NC], vo[FULL ? 1 : DT];
+    if constexpr (!FULL)
 #pragma unroll
-    for (int f = 0; f < 2 * NC; f++) ko[f] = koff(pool, f), vo[f] = voff(pool, f);
+      for (int f = 0; f < 2 * NC; f++) ko[f] = koff(pool, f), vo[f] = voff(pool, f);
+    auto k_load = [&](const uint8_t *k, int f) {
+      const uint8_t *at;
+      if constexpr (FULL)
+        at = k + k_first + (f >> 1) * k_step + (f & 1) * (32 * (int)sizeof(T));
+      else
+        at = k + ko[f];
+      return F::load(reinterpret_cast<const T *>(at));
+    };
+    auto v_load = [&](const uint8_t *v, int d) {
+      const uint8_t *at;
+      if constexpr (FULL)
+        at = v + v_first + d * (128 * (int)sizeof(T));
+      else
+        at = v + vo[d];
+      return F::load(reinterpret_cast<const T *>(at));
+    };
     V kf[2 * NC], vf[DT];
     Where w = look_up<WIDE>(pool, r, k0);
     uint32_t ok = found<WIDE>(pool, w);
     {
       const Tile t = tile_of<WIDE>(pool, hb, r, k0, w);
 #pragma unroll
-      for (int f = 0; f < 2 * NC; f++) kf[f] = F::load(reinterpret_cast<const T *>(t.k + ko[f]));
+      for (int f = 0; f < 2 * NC; f++) kf[f] = k_load(t.k, f);
 #pragma unroll
-      for (int d = 0; d < DT; d++) vf[d] = F::load(reinterpret_cast<const T *>(t.v + vo[d]));
+      for (int d = 0; d < DT; d++) vf[d] = v_load(t.v, d);
     }
     w = look_up<WIDE>(pool, r, k0 + kStep);
     for (;;) {
@@ -400,12 +418,12 @@ template <class T, int NC> struct Rows {
       if (k1 < r.to) {
         t = tile_of<WIDE>(pool, hb, r, k1, w);
 #pragma unroll
-        for (int f = 0; f < 2 * NC; f++) kf[f] = F::load(reinterpret_cast<const T *>(t.k + ko[f]));
+        for (int f = 0; f < 2 * NC; f++) kf[f] = k_load(t.k, f);
       }
       weigh(s, vf, k0, r.to, ok);
       if (k1 >= r.to) break;
 #pragma unroll
-      for (int d = 0; d < DT; d++) vf[d] = F::load(reinterpret_cast<const T *>(t.v + vo[d]));
+      for (int d = 0; d < DT; d++) vf[d] = v_load(t.v, d);
       ok = found<WIDE>(pool, w);
       w = look_up<WIDE>(pool, r, k1 + kStep);
       k0 = k1;
@@ -418,31 +436,37 @@ template <class T, int NC> struct Rows {
   static constexpr int kHalves = (int)sizeof(V) / 16;  // 16-byte loads of a fragment
   static constexpr int kShare = kLoads / kWaves;       // direct loads of a tile by one wave: K, then V
   template <bool WIDE>
-  __device__ __forceinline__ void issue(const KvPool<T> &pool, const HeadBase &hb, const Run &r, int k0,
+  static __device__ __forceinline__ void issue(const KvPool<T> &pool, const HeadBase &hb, const Run &r, int k0,
                                         uint32_t lds, const Where &w, const uint32_t *off) {
     const Tile t = tile_of<WIDE>(pool, hb, r, k0, w);
 #pragma unroll
     for (int i = 0; i < kShare; i++)
       kr_dma((i < kShare / 2 ? t.k : t.v) + off[i], lds + i * kWaves * 1024);
   }
-  template <bool WIDE, int KW>
-  __device__ __forceinline__ void run_shared(const KvPool<T> &pool, const HeadBase &hb, const Run &r,
-                                             uint8_t *ring) {
-    constexpr int S = kRing / KW, kAhead = S - 1, kStep = KW * kTile;
-    static_assert(kLoads % (2 * kWaves) == 0 && 8 * kAhead < 32, "K and V in whole shares");
-    const int lane = threadIdx.x & 63;
+  // the direct loads of a wave's share of a tile
+  static __device__ __forceinline__ void share(const KvPool<T> &pool, uint32_t *off) {
+    static_assert(kLoads % (2 * kWaves) == 0, "K and V in whole shares");
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr_of(ring));
-    const int n = (r.to - r.from + kStep - 1) / kStep;
-    const int mine = KW == 1 ? 0 : wave / (kWaves / KW);  // tile of a step
-    uint32_t off[kShare];
 #pragma unroll
     for (int i = 0; i < kShare; i++) {
       const int b = i * kWaves + wave, f = b / kHalves;
       off[i] = (i < kShare / 2 ? koff(pool, f) : voff(pool, f - 2 * NC)) + (b % kHalves) * 16;
     }
-    // found() of the tiles in flight: 4 bits a tile, 8 a step, this step's lowest
-    uint32_t ok = 0;
+  }
+  static __device__ __forceinline__ uint32_t ring_base(uint8_t *ring) {
+    return __builtin_amdgcn_readfirstlane(lds_addr_of(ring) + (threadIdx.x >> 6) * 1024);
+  }
+  // the first steps' loads; returns found() of their tiles: 4 bits a tile, 8 a
+  // step, the first lowest
+  template <bool WIDE, int KW>
+  static __device__ __forceinline__ uint32_t start_shared(const KvPool<T> &pool, const HeadBase &hb,
+                                                          const Run &r, uint8_t *ring) {
+    constexpr int S = kRing / KW, kAhead = S - 1, kStep = KW * kTile;
+    static_assert(8 * kAhead < 32, "found() of a ring in a word");
+    const int n = (r.to - r.from + kStep - 1) / kStep;
+    const uint32_t base = ring_base(ring);
+    uint32_t off[kShare], ok = 0;
+    share(pool, off);
 #pragma unroll
     for (int i = 0; i < kAhead; i++)
       if (i < n)
@@ -451,8 +475,21 @@ template <class T, int NC> struct Rows {
           const int kt = r.from + i * kStep + t * kTile;
           const Where w = look_up<WIDE>(pool, r, kt);
           ok |= found<WIDE>(pool, w) << (8 * i + 4 * t);
-          issue<WIDE>(pool, hb, r, kt, base + (i * KW + t) * kTileBytes + wave * 1024, w, off);
+          issue<WIDE>(pool, hb, r, kt, base + (i * KW + t) * kTileBytes, w, off);
         }
+    return ok;
+  }
+  template <bool WIDE, int KW>
+  __device__ __forceinline__ void run_shared(const KvPool<T> &pool, const HeadBase &hb, const Run &r,
+                                             uint8_t *ring, uint32_t ok) {
+    constexpr int S = kRing / KW, kAhead = S - 1, kStep = KW * kTile;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t base = ring_base(ring);
+    const int n = (r.to - r.from + kStep - 1) / kStep;
+    const int mine = KW == 1 ? 0 : wave / (kWaves / KW);  // tile of a step
+    uint32_t off[kShare];
+    share(pool, off);
     int get = 0, put = kAhead;  // places in the ring
     for (int i = 0; i < n; i++) {
       const int k0 = r.from + i * kStep, k2 = k0 + kAhead * kStep;
@@ -485,9 +522,9 @@ template <class T, int NC> struct Rows {
       }
       ok >>= 8;
       if (i + kAhead < n) {
-        issue<WIDE>(pool, hb, r, k2, base + put * KW * kTileBytes + wave * 1024, w0, off);
+        issue<WIDE>(pool, hb, r, k2, base + put * KW * kTileBytes, w0, off);
         if (KW == 2)
-          issue<WIDE>(pool, hb, r, k2 + kTile, base + (put * KW + 1) * kTileBytes + wave * 1024, w1, off);
+          issue<WIDE>(pool, hb, r, k2 + kTile, base + (put * KW + 1) * kTileBytes, w1, off);
         ok |= (found<WIDE>(pool, w0) | (KW == 2 ? found<WIDE>(pool, w1) << 4 : 0)) << (8 * (kAhead - 1));
       }
       if (on) {
@@ -548,12 +585,15 @@ __device__ __forceinline__ int clamped(const int32_t *len, int i, int most) {
   return most ? max(0, min(len[i], most)) : 0;
 }
 
+// workgroups of a CU that share its registers
+template <class T, int NC> constexpr int kResident = NC * sizeof(T) <= 8 ? 2 : 1;
+
 // Joined: a workgroup has both runs of a sequence's rows whole.  Else the
 // first workgroups have the parts of the prefixes, the others those of the
 // suffixes.
-template <class T, int NC>
-__global__ void __launch_bounds__(64 * kWaves, NC * sizeof(T) <= 8 ? 2 : 1) k_attend(AttnArgs a, KvPool<T> pool) {
-  using W = Rows<T, NC>;
+template <class T, int NC, bool FULL>
+__global__ void __launch_bounds__(64 * kWaves, (kResident<T, NC>)) k_attend(AttnArgs a, KvPool<T> pool) {
+  using W = Rows<T, NC, FULL>;
   __shared__ __align__(16) uint8_t lds[W::kLdsBytes];
   __shared__ float ml[kWaves * 16 * 2];
   const bool prefix = (int)blockIdx.x < a.prefix_wgs;
@@ -590,14 +630,22 @@ __global__ void __launch_bounds__(64 * kWaves, NC * sizeof(T) <= 8 ? 2 : 1) k_at
       return;
     }
   }
-  W w;
-  const int tile = (int)(threadIdx.x >> 6) & (RW - 1);
-  w.load_queries(a, pool.hd, seq0, head, row0 + tile * 16, row0 + rows - 1);
   const size_t head_bytes = (size_t)pool.hd * pool.ps * sizeof(T);
   const HeadBase hb{reinterpret_cast<const uint8_t *>(pool.k) + head * head_bytes,
                     reinterpret_cast<const uint8_t *>(pool.v) + head * head_bytes,
                     (uint32_t)(pool.nkv * head_bytes)};
   const bool wide = pool.ps >= kTile;
+  uint32_t ok = 0;
+  if (RW == 4)
+    ok = wide ? W::template start_shared<true, 1>(pool, hb, r, lds)
+              : W::template start_shared<false, 1>(pool, hb, r, lds);
+  if constexpr (W::kRing == 4)
+    if (RW == 2)
+      ok = wide ? W::template start_shared<true, 2>(pool, hb, r, lds)
+                : W::template start_shared<false, 2>(pool, hb, r, lds);
+  W w;
+  const int tile = (int)(threadIdx.x >> 6) & (RW - 1);
+  w.load_queries(a, pool.hd, seq0, head, row0 + tile * 16, row0 + rows - 1);
   if (RW == 1) {
     // joined: the prefix first, its next tile's wave begins the suffix
     for (int k = a.joined ? 0 : 1; k < 2; k++) {
@@ -611,49 +659,53 @@ __global__ void __launch_bounds__(64 * kWaves, NC * sizeof(T) <= 8 ? 2 : 1) k_at
     }
   } else if (RW == 4) {
     if (wide)
-      w.template run_shared<true, 1>(pool, hb, r, lds);
+      w.template run_shared<true, 1>(pool, hb, r, lds, ok);
     else
-      w.template run_shared<false, 1>(pool, hb, r, lds);
+      w.template run_shared<false, 1>(pool, hb, r, lds, ok);
   } else if constexpr (W::kRing == 4) {
     if (wide)
-      w.template run_shared<true, 2>(pool, hb, r, lds);
+      w.template run_shared<true, 2>(pool, hb, r, lds, ok);
     else
-      w.template run_shared<false, 2>(pool, hb, r, lds);
+      w.template run_shared<false, 2>(pool, hb, r, lds, ok);
   }
   w.finish(a, pool.hd, seq0, head, row0, rows, RW, at, reinterpret_cast<float *>(lds), ml);
 }
 
-// One workgroup a query row: the factors of 64 parts at a time by lanes, the
-// parts' rows four to a step over the waves (all loads of a step in flight),
-// the waves' sums joined in order.
+// One workgroup a query row: wave w takes parts w, w + 4, ..., eight in flight
+// and the first eight before their weights are known; the waves' sums are
+// joined in order.
 __global__ void __launch_bounds__(256) k_join_parts(AttnArgs a, int hd) {
   __shared__ float xs[3][kKvMaxHeadDim];
+  constexpr int kU = 8;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const size_t row = blockIdx.x;
   const int n = a.npp + a.nsp;
   const float *ml = a.pml + row * n * 2, *po = a.po + row * n * hd;
+  const int d0 = min(4 * lane, hd - 4);
+  f32x4 x{0, 0, 0, 0}, y[kU];
+  auto ask = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < kU; u++)
+      y[u] = *reinterpret_cast<const f32x4 *>(po + (size_t)min(i0 + 4 * u, n - 1) * hd + d0);
+  };
+  ask(wave);
   float top = kNegInf;
   for (int i = lane; i < n; i += 64) top = fmaxf(top, ml[2 * i]);
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  f32x4 x{0, 0, 0, 0};
-  const int d0 = min(4 * lane, hd - 4);
   float l = 0.0f;
   for (int i0 = 0; i0 < n; i0 += 64) {
-    const int i = i0 + lane;
-    const float lp = i < n ? ml[2 * i + 1] : 0.0f;
+    const int i = min(i0 + lane, n - 1);
+    const float lp = i0 + lane < n ? ml[2 * i + 1] : 0.0f;
     const float f = lp == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml[2 * i] - top);
     l += lp * f;
     const int most = min(64, n - i0);
-    for (int k = 4 * wave; k < most; k += 16) {
-      f32x4 y[4];
+    for (int k = wave; k < most; k += 4 * kU) {
+      if (i0 + k != wave) ask(i0 + k);
 #pragma unroll
-      for (int u = 0; u < 4; u++)
-        y[u] = *reinterpret_cast<const f32x4 *>(po + (size_t)(i0 + min(k + u, most - 1)) * hd + d0);
-#pragma unroll
-      for (int u = 0; u < 4; u++) {
-        const float fu = __shfl(f, (k + u) & 63);
+      for (int u = 0; u < kU; u++) {
+        const float fu = __shfl(f, (k + 4 * u) & 63);
         // (a part with no position has left its row unwritten)
-        if (k + u < most && fu != 0.0f)
+        if (k + 4 * u < most && fu != 0.0f)
 #pragma unroll
           for (int c = 0; c < 4; c++) x[c] = __builtin_fmaf(y[u][c], fu, x[c]);
       }
@@ -721,11 +773,16 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_prefix_attention_params
     w.wgs = round_up(sunits, 8) * sblocks;
     return w;
   }
-  // parts of about equal work for kWant workgroups in all
+  // Parts of about equal work for as many workgroups as the chip holds at
+  // once: by LDS four a CU, two, or one.  (512 workgroups of 64 dims in 16 bits,
+  // 48 sequences of 1500 positions over a shared 8200: 45 us, 1024: 40; of 128
+  // dims, 64 sequences over four prefixes of 32768: 110 and 127.)
+  const int tile_bytes = w.nc * (pg.dtype == SYN_HIP_KV_F32 ? 8192 : 4096);
+  const size_t want = tile_bytes <= 8192 ? 1024 : (tile_bytes <= 16384 ? 512 : 256);
   const size_t pblocks = cdiv((size_t)p.group_size * rep, 16 * w.prw), punits = (size_t)p.n_groups * nkv;
   const size_t psteps = cdiv(p.max_prefix, step), ssteps = cdiv(p.max_suffix, step);
   const size_t total = punits * pblocks * psteps + sunits * sblocks * ssteps;
-  const size_t per = std::max<size_t>(1, cdiv(total, kWant));
+  const size_t per = std::max<size_t>(1, cdiv(total, want));
   auto cut = [&](size_t steps, int *chunk, int *n) {
     const size_t k = cdiv(steps, per);  // as many parts, of equal length
     const size_t each = k ? cdiv(steps, k) : 0;
@@ -744,7 +801,11 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_prefix_attention_params
 
 template <class T, int NC>
 syn_status_t launch(const Plan &w, const AttnArgs &a, const KvPool<T> &pool, hipStream_t s) {
-  hipLaunchKernelGGL((k_attend<T, NC>), dim3((unsigned)w.wgs), dim3(64 * kWaves), 0, s, a, pool);
+  const dim3 grid((unsigned)w.wgs), block(64 * kWaves);
+  if (pool.hd == 32 * NC)
+    hipLaunchKernelGGL((k_attend<T, NC, true>), grid, block, 0, s, a, pool);
+  else
+    hipLaunchKernelGGL((k_attend<T, NC, false>), grid, block, 0, s, a, pool);
   SYN_LAUNCH_CHECK();
   if (w.joined) return SYN_OK;
   hipLaunchKernelGGL(k_join_parts, dim3((unsigned)w.rows), dim3(256), 0, s, a, pool.hd);
