@@ -7,21 +7,24 @@ namespace syn {
 namespace {
 
 // ---------------------------------------------------------------- choice
-// The order of continuations: larger value first, then the lower index.
+// Value of (beam b, token t): score_b + logit_t - log sum exp(logits of b).
+// Rows are cut into chunks over the whole chip: a workgroup reads its chunk
+// once into registers, forms max and sum of exp, and keeps the n_select best
+// logits (the order within a beam is that of its logits); one workgroup a
+// group then joins the sums and chooses among the chunks' candidates by their
+// values in f64.  The selection itself never sorts: if G >= n groups of values
+// are formed, n values at least are not below the least of the groups' maxima,
+// and few are; those go to LDS, where each counts the ones before it.
+//
+// Equal values go to the lower (beam, token).  A value of -inf is a candidate
+// only when a group has fewer than n_select others, so the chunks leave those
+// out and the second kernel fills up with them in order.
 struct Cand {
-  float v;
-  int i;
+  float x;
+  int i;  // token
 };
-__device__ __forceinline__ bool before(float av, int ai, float bv, int bi) {
-  return av > bv || (av == bv && ai < bi);
-}
-
-// what the first kernel leaves of a row: its n_select best logits, largest
-// logit and log of the sum of exp(logit - largest)
-struct RowStat {
-  double logsum;
-  float top;
-  int pad;
+struct ChunkStat {
+  float top, sum;  // largest logit, sum of exp(logit - top)
 };
 
 struct SelectArgs {
@@ -30,133 +33,387 @@ struct SelectArgs {
   int32_t *parent, *finished_out;
   uint32_t *token;
   float *score;
-  Cand *cand;     // [rows][n_select]
-  RowStat *stat;  // [rows]
+  Cand *cand;       // [rows][chunks][n_select], best first, then places of -inf
+  ChunkStat *stat;  // [rows][chunks]
   size_t ld;
-  int vocab, n_beams, n_select, eos, pad;
+  int vocab, chunks, n_beams, n_select, eos, pad;
+  bool aligned;     // rows are 16-byte aligned
 };
 
-__device__ __forceinline__ float masked(float x) {
-  return x != x ? -__builtin_inff() : x;
+constexpr float kNone = -__builtin_huge_valf();
+
+__device__ __forceinline__ bool is_dead(const SelectArgs &a, size_t row) {
+  return !isfinite(a.scores[row]);
+}
+__device__ __forceinline__ bool is_done(const SelectArgs &a, size_t row) {
+  return a.finished && a.finished[row] != 0;
 }
 
-constexpr int kRowNT = 1024;
-__global__ void __launch_bounds__(kRowNT) k_beam_rows(SelectArgs a) {
-  __shared__ float rv[16];
-  __shared__ int ri[16];
-  __shared__ double rs[16];
-  const int row = blockIdx.x, tid = threadIdx.x, V = a.vocab;
-  Cand *out = a.cand + (size_t)row * a.n_select;
-  if (!isfinite(a.scores[row])) {  // no continuation: every one -inf
-    for (int i = tid; i < a.n_select; i += kRowNT)
-      out[i] = Cand{-__builtin_inff(), i < V ? i : -1};
-    if (tid == 0) a.stat[row] = RowStat{0.0, 0.0f, 0};
+// x of a partner lane: steps 1 to 32 together reach every lane of the wave, by
+// lane moves (no trip through LDS); what steps O, O / 2, ... have combined is
+// the same in all lanes that they connect
+template <int STEP> __device__ __forceinline__ uint32_t partner(uint32_t x) {
+  if constexpr (STEP == 32 || STEP == 16) {
+    const auto p = STEP == 32 ? __builtin_amdgcn_permlane32_swap(x, x, false, false)
+                              : __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return threadIdx.x & STEP ? p[0] : p[1];
+  } else {
+    // row_mirror, row_half_mirror, two quad permutations
+    constexpr int ctl = STEP == 8 ? 0x140 : (STEP == 4 ? 0x141 : (STEP == 2 ? 0x4e : 0xb1));
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctl, 0xf, 0xf, false);
+  }
+}
+template <int STEP> __device__ __forceinline__ float partner(float x) {
+  return __uint_as_float(partner<STEP>(__float_as_uint(x)));
+}
+template <int STEP> __device__ __forceinline__ double partner(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x);
+  const uint64_t lo = partner<STEP>((uint32_t)u), hi = partner<STEP>((uint32_t)(u >> 32));
+  return __longlong_as_double((long long)(hi << 32 | lo));
+}
+template <class F, class Op> __device__ __forceinline__ F over_wave(F x, Op op) {
+  x = op(x, partner<32>(x));
+  x = op(x, partner<16>(x));
+  x = op(x, partner<8>(x));
+  x = op(x, partner<4>(x));
+  x = op(x, partner<2>(x));
+  return op(x, partner<1>(x));
+}
+__device__ __forceinline__ float greater(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ double greater(double a, double b) { return fmax(a, b); }
+__device__ __forceinline__ float lesser(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ double lesser(double a, double b) { return fmin(a, b); }
+template <class F> __device__ __forceinline__ F wave_max(F x) {
+  return over_wave(x, [](F a, F b) { return greater(a, b); });
+}
+template <class F> __device__ __forceinline__ F wave_sum(F x) {
+  return over_wave(x, [](F a, F b) { return a + b; });
+}
+// The lanes in G groups (a power of two): the steps above G give every lane its
+// group's maximum, those below the least of them.
+template <class F> __device__ __forceinline__ F group_max(F x, int G) {
+  if (G <= 32) x = greater(x, partner<32>(x));
+  if (G <= 16) x = greater(x, partner<16>(x));
+  if (G <= 8) x = greater(x, partner<8>(x));
+  if (G <= 4) x = greater(x, partner<4>(x));
+  if (G <= 2) x = greater(x, partner<2>(x));
+  if (G <= 1) x = greater(x, partner<1>(x));
+  return x;
+}
+template <class F> __device__ __forceinline__ F least_group(F x, int G) {
+  if (G > 1) x = lesser(x, partner<1>(x));
+  if (G > 2) x = lesser(x, partner<2>(x));
+  if (G > 4) x = lesser(x, partner<4>(x));
+  if (G > 8) x = lesser(x, partner<8>(x));
+  if (G > 16) x = lesser(x, partner<16>(x));
+  if (G > 32) x = lesser(x, partner<32>(x));
+  return x;
+}
+
+// keys that order as (value descending, index ascending) when the larger is
+// first; no key is 0
+__device__ __forceinline__ uint64_t key_of(float x, int i) {
+  const uint32_t u = __float_as_uint(x);
+  return (uint64_t)(u >> 31 ? ~u : u | 0x80000000u) << 32 | (uint32_t)~i;
+}
+__device__ __forceinline__ Cand cand_of(uint64_t key) {
+  const uint32_t u = (uint32_t)(key >> 32);
+  return Cand{__uint_as_float(u >> 31 ? u & 0x7fffffffu : ~u), (int)~(uint32_t)key};
+}
+
+constexpr int kChunkNT = 256;
+constexpr int kWaveCap = 256;  // of a wave's candidates
+
+template <int PER>  // values a thread
+__global__ void __launch_bounds__(kChunkNT) k_beam_chunks(SelectArgs a) {
+  __shared__ __align__(16) uint64_t list[4][kWaveCap];
+  __shared__ float wtop[4], wsum[4], wgroup[4][64];
+  __shared__ int count[4], ri[4];
+  const int row = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const size_t at = (size_t)row * a.chunks + chunk;
+  Cand *out = a.cand + at * a.n_select;
+  if (is_dead(a, row) || is_done(a, row)) {
+    if (tid == 0) a.stat[at] = ChunkStat{kNone, 0.0f};
+    for (int i = tid; i < a.n_select; i += kChunkNT) out[i] = Cand{kNone, 0};
     return;
   }
-  if (a.finished && a.finished[row]) {
-    for (int i = tid; i < a.n_select; i += kRowNT) {
-      const int t = i == 0 ? a.pad : (i - 1 < a.pad ? i - 1 : i);
-      out[i] = Cand{i == 0 ? 0.0f : -__builtin_inff(), t < V ? t : -1};
+  // element e of thread t: t * 4 + e % 4 of every 1024
+  const int first = chunk * (kChunkNT * PER), left = min(a.vocab - first, kChunkNT * PER);
+  const float *x0 = a.logits + (size_t)row * a.ld + first;
+  float x[PER];
+  if (a.aligned && left == kChunkNT * PER) {
+#pragma unroll
+    for (int i = 0; i < PER; i += 4) {
+      const f32x4 v = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(x0 + i * kChunkNT + tid * 4));
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[i + j] = v[j];
     }
-    if (tid == 0) a.stat[row] = RowStat{0.0, 0.0f, 0};
-    return;
+  } else {  // (no load behind a branch: all are in flight together)
+#pragma unroll
+    for (int i = 0; i < PER; i++) x[i] = x0[min((i / 4 * kChunkNT + tid) * 4 + i % 4, left - 1)];
+#pragma unroll
+    for (int i = 0; i < PER; i++) x[i] = (i / 4 * kChunkNT + tid) * 4 + i % 4 < left ? x[i] : kNone;
   }
-  const float *x = a.logits + (size_t)row * a.ld;
-  float pv = __builtin_inff();
-  int pi = -1;
-  float top = 0.0f;
-  for (int r = 0; r < a.n_select; r++) {
-    float bv = -__builtin_inff();
-    int bi = 0x7fffffff;
-    for (int i = tid; i < V; i += kRowNT) {
-      const float v = masked(x[i]);
-      if (before(pv, pi, v, i) && before(v, i, bv, bi)) bv = v, bi = i;
-    }
-    for (int o = 32; o > 0; o >>= 1) {
-      const float v = __shfl_xor(bv, o);
-      const int i = __shfl_xor(bi, o);
-      if (before(v, i, bv, bi)) bv = v, bi = i;
-    }
-    if ((tid & 63) == 0) rv[tid >> 6] = bv, ri[tid >> 6] = bi;
-    __syncthreads();
-    bv = rv[0], bi = ri[0];
-    for (int w = 1; w < 16; w++)
-      if (before(rv[w], ri[w], bv, bi)) bv = rv[w], bi = ri[w];
-    __syncthreads();
-    if (r == 0) top = bv;
-    if (tid == 0) out[r] = Cand{bv, bi == 0x7fffffff ? -1 : bi};
-    pv = bv;
-    pi = bi;
+  float top = kNone, half = kNone;  // of all values; of the second half
+#pragma unroll
+  for (int i = 0; i < PER; i++) {
+    x[i] = fmaxf(x[i], kNone);  // NaN: -inf
+    if (i < PER / 2)
+      top = fmaxf(top, x[i]);
+    else
+      half = fmaxf(half, x[i]);
   }
-  double s = 0.0;
-  for (int i = tid; i < V; i += kRowNT) {
-    const float v = masked(x[i]);
-    s += v == top ? 1.0 : (double)expf(v - top);
-  }
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  if ((tid & 63) == 0) rs[tid >> 6] = s;
+  // Groups of threads, the same of every wave; above 64, two of each lane's
+  // values, both of which are not below the lesser.
+  const int n = a.n_select;
+  const int pow2 = n <= 1 ? 1 : 1 << (32 - __builtin_clz(n - 1)), G = min(pow2, 64);
+  wgroup[wave][lane] = group_max(pow2 > 64 ? fminf(top, half) : fmaxf(top, half), G);
+  top = wave_max(fmaxf(top, half));
+  if (lane == 0) wtop[wave] = top;
   __syncthreads();
-  if (tid == 0) {
-    s = 0.0;
-    for (int w = 0; w < 16; w++) s += rs[w];
-    a.stat[row] = RowStat{log(s), top, 0};
+  top = fmaxf(fmaxf(wtop[0], wtop[1]), fmaxf(wtop[2], wtop[3]));
+  const float tau = fmaxf(least_group(fmaxf(fmaxf(wgroup[0][lane], wgroup[1][lane]),
+                                            fmaxf(wgroup[2][lane], wgroup[3][lane])), G),
+                          -3.402823466e38f);  // finite: -inf is no candidate
+  float sum = 0.0f;
+  if (top == __builtin_huge_valf()) {
+#pragma unroll
+    for (int i = 0; i < PER; i++) sum += x[i] == top ? 1.0f : 0.0f;
+  } else if (top > kNone) {
+#pragma unroll
+    for (int i = 0; i < PER; i++) sum += __builtin_amdgcn_exp2f((x[i] - top) * 1.44269504088896340736f);
   }
+  sum = wave_sum(sum);
+  if (lane == 0) wsum[wave] = sum;
+  int held = 0;  // the same in every lane
+#pragma unroll
+  for (int i = 0; i < PER; i++) {
+    const bool in = x[i] >= tau;
+    const uint64_t who = __ballot(in);
+    if (!who) continue;
+    const int k = held + __popcll(who & ((1ull << lane) - 1));
+    if (in && k < kWaveCap) list[wave][k] = key_of(x[i], first + (i / 4 * kChunkNT + tid) * 4 + i % 4);
+    held += __popcll(who);
+  }
+  if (lane == 0) count[wave] = held;
+  if (lane < 8 && held + lane < kWaveCap) list[wave][held + lane] = 0;  // read in eights
+  __syncthreads();
+  const int K = count[0] + count[1] + count[2] + count[3];
+  const int most = max(max(count[0], count[1]), max(count[2], count[3]));
+  if (most <= kWaveCap) {
+    for (int k = lane; k < held; k += 64) {
+      const uint64_t key = list[wave][k];
+      int before = 0;
+      for (int w = 0; w < 4; w++)
+        for (int j = 0; j < count[w]; j += 8) {
+          uint64_t o[8];
+#pragma unroll
+          for (int u = 0; u < 8; u++) o[u] = list[w][j + u];
+#pragma unroll
+          for (int u = 0; u < 8; u++) before += o[u] > key;
+        }
+      if (before < n) out[before] = cand_of(key);
+    }
+    for (int i = K + tid; i < n; i += kChunkNT) out[i] = Cand{kNone, 0};
+  } else {
+    // many values alike: one after the other, each the first behind the last
+    float pv = __builtin_huge_valf();
+    int pi = -1;
+    for (int r = 0; r < n; r++) {
+      float bv = kNone;
+      int bi = 0x7fffffff;
+#pragma unroll
+      for (int i = 0; i < PER; i++) {
+        const int e = first + (i / 4 * kChunkNT + tid) * 4 + i % 4;
+        const bool behind = x[i] < pv || (x[i] == pv && e > pi);
+        if (behind && x[i] > kNone && (x[i] > bv || (x[i] == bv && e < bi))) bv = x[i], bi = e;
+      }
+      for (int o = 32; o > 0; o >>= 1) {
+        const float v = __shfl_xor(bv, o);
+        const int i = __shfl_xor(bi, o);
+        if (v > bv || (v == bv && i < bi)) bv = v, bi = i;
+      }
+      __syncthreads();
+      if (lane == 0) wtop[wave] = bv, ri[wave] = bi;
+      __syncthreads();
+      bv = wtop[0], bi = ri[0];
+      for (int w = 1; w < 4; w++)
+        if (wtop[w] > bv || (wtop[w] == bv && ri[w] < bi)) bv = wtop[w], bi = ri[w];
+      if (tid == 0) out[r] = Cand{bv, bi};
+      pv = bv;
+      pi = bi;
+    }
+  }
+  if (tid == 0) a.stat[at] = ChunkStat{top, (wsum[0] + wsum[1]) + (wsum[2] + wsum[3])};
 }
 
-// one workgroup a group: the n_select best of the rows' candidates
-__global__ void __launch_bounds__(256) k_beam_merge(SelectArgs a) {
-  __shared__ double val[kMaxBeams * kMaxSelect];
-  __shared__ double rv[4];
-  __shared__ int ri[4];
-  const int g = blockIdx.x, tid = threadIdx.x, W = a.n_beams, n = a.n_select;
-  const size_t row0 = (size_t)g * W;
-  const Cand *c = a.cand + row0 * n;
-  for (int j = tid; j < W * n; j += 256) {
-    const int b = j / n;
-    const RowStat st = a.stat[row0 + b];
-    const float sc = a.scores[row0 + b], x = c[j].v;
-    const double d = x == st.top ? 0.0 : (double)x - (double)st.top;
-    double v = (double)sc + (d - st.logsum);
-    if (x == -__builtin_inff()) v = -__builtin_inf();
-    if (c[j].i < 0) v = __builtin_nan("");
-    val[j] = v;
-  }
+constexpr int kMergeNT = 1024;
+constexpr int kMergeCap = 1024;
+
+// one workgroup a group
+__global__ void __launch_bounds__(kMergeNT) k_beam_merge(SelectArgs a) {
+  struct Pick {
+    double v;
+    int b, t;
+  };
+  __shared__ Pick list[kMergeCap];
+  __shared__ uint64_t keys[kMergeCap + 4], index[kMergeCap + 4];
+  __shared__ double logsum[kMaxBeams], wtau[16];
+  __shared__ float top[kMaxBeams], score[kMaxBeams];
+  __shared__ int state[kMaxBeams];  // 0 live, 1 finished, 2 without a continuation
   __shared__ int done[kMaxBeams];
-  for (int b = tid; b < W; b += 256) done[b] = a.finished ? a.finished[row0 + b] != 0 : 0;
-  __syncthreads();
-  // candidates of a row are in order already, so among equal values the lower
-  // j is the lower (beam, token)
-  double pv = __builtin_inf();
-  int pj = -1;
-  for (int r = 0; r < n; r++) {
-    double bv = -__builtin_inf();
-    int bj = 0x7fffffff;
-    for (int j = tid; j < W * n; j += 256) {
-      const double v = val[j];
-      if ((v < pv || (v == pv && j > pj)) && (v > bv || (v == bv && j < bj))) bv = v, bj = j;
+  __shared__ int count, chosen, rj[16];
+  const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int W = a.n_beams, n = a.n_select, C = a.chunks;
+  const size_t row0 = (size_t)g * W;
+  if (tid == 0) count = 0, chosen = 0;
+  const int L = W * C, T = L * n;  // lists, and places in them
+  const Cand *cand = a.cand + row0 * C * n;
+  // the thread's first candidates are asked for ahead of the sums
+  constexpr int kHeld = 4;
+  Cand mine[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; k++) mine[k] = cand[min(tid + k * kMergeNT, T - 1)];
+  for (int b = wave; b < W; b += kMergeNT / 64) {
+    const ChunkStat *st = a.stat + (row0 + b) * C;
+    const ChunkStat q0 = st[min(lane, C - 1)];
+    float m = q0.top;
+    for (int c = lane + 64; c < C; c += 64) m = fmaxf(m, st[c].top);
+    m = wave_max(m);
+    double s = 0.0;
+    for (int c = lane; c < C; c += 64) {
+      const ChunkStat q = c == lane ? q0 : st[c];
+      if (q.top > kNone) s += q.top == m ? (double)q.sum : (double)q.sum * exp((double)q.top - (double)m);
     }
-    for (int o = 32; o > 0; o >>= 1) {
-      const double v = __shfl_xor(bv, o);
-      const int j = __shfl_xor(bj, o);
-      if (v > bv || (v == bv && j < bj)) bv = v, bj = j;
+    s = wave_sum(s);
+    if (lane == 0) {
+      top[b] = m;
+      logsum[b] = s > 0.0 ? log(s) : 0.0;
+      score[b] = a.scores[row0 + b];
+      done[b] = is_done(a, row0 + b);
+      state[b] = is_dead(a, row0 + b) ? 2 : done[b];
     }
-    if ((tid & 63) == 0) rv[tid >> 6] = bv, ri[tid >> 6] = bj;
-    __syncthreads();
-    bv = rv[0], bj = ri[0];
-    for (int w = 1; w < 4; w++)
-      if (rv[w] > bv || (rv[w] == bv && ri[w] < bj)) bv = rv[w], bj = ri[w];
-    __syncthreads();
-    if (tid == 0) {
-      const int b = bj / n;
-      const size_t o = (size_t)g * n + r;
-      a.parent[o] = b;
-      a.token[o] = (uint32_t)c[bj].i;
-      a.score[o] = (float)bv;
-      if (a.finished_out) a.finished_out[o] = done[b] || c[bj].i == a.eos;
-    }
-    pv = bv;
-    pj = bj;
   }
+  __syncthreads();
+  const double none = -__builtin_huge_val();
+  auto value = [&](int b, float x) {  // of a live beam
+    const double d = x == top[b] ? 0.0 : (double)x - (double)top[b];
+    return x == kNone ? none : (double)score[b] + (d - logsum[b]);
+  };
+  // candidate j: the lists' places (those of beams that do not live are empty)
+  auto pick = [&](int j, const Cand &c) {
+    const int b = (int)((uint32_t)j / (uint32_t)n / (uint32_t)C);
+    return Pick{value(b, c.x), b, c.i};
+  };
+  auto ahead = [](const Pick &p, const Pick &q) {
+    return p.v > q.v || (p.v == q.v && (p.b < q.b || (p.b == q.b && p.t < q.t)));
+  };
+  // Lists are in order: if the D-th of a list is not below tau, D of it are
+  // not.  Of the lists of a wave in G groups, D G >= n, the least group maximum.
+  const int G = min(n <= 1 ? 1 : 1 << (32 - __builtin_clz(n - 1)), 1 << (31 - __builtin_clz(min(L, 64))));
+  const int D = (n + G - 1) / G;
+  double key = none;
+  for (int q = tid; q < L; q += kMergeNT) {
+    const int j = q * n + D - 1;
+    key = fmax(key, pick(j, cand[j]).v);
+  }
+  const double tau_w = least_group(group_max(key, G), G);
+  if (lane == 0) wtau[wave] = tau_w;
+  __syncthreads();
+  double tau = none;
+  for (int w = 0; w < kMergeNT / 64; w++) tau = fmax(tau, wtau[w]);
+  auto offer = [&](const Pick &p) {
+    if (p.v >= tau && p.v > none) {
+      const int k = atomicAdd(&count, 1);
+      if (k < kMergeCap) list[k] = p;
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < kHeld; k++)
+    if (tid + k * kMergeNT < T) offer(pick(tid + k * kMergeNT, mine[k]));
+  for (int j = tid + kHeld * kMergeNT; j < T; j += kMergeNT) offer(pick(j, cand[j]));
+  if (tid < W && state[tid] == 1) offer(Pick{(double)score[tid], tid, a.pad});
+  __syncthreads();
+  const int K = count;
+  auto emit = [&](int r, const Pick &p) {
+    const size_t o = (size_t)g * n + r;
+    a.parent[o] = p.b;
+    a.token[o] = (uint32_t)p.t;
+    a.score[o] = (float)p.v;
+    if (a.finished_out) a.finished_out[o] = done[p.b] || p.t == a.eos;
+  };
+  if (K <= kMergeCap) {
+    for (int k = tid; k < K + 4; k += kMergeNT) {
+      const Pick p = list[min(k, K - 1)];
+      const uint64_t u = (uint64_t)__double_as_longlong(p.v);
+      keys[k] = k < K ? (u >> 63 ? ~u : u | 1ull << 63) : 0;
+      index[k] = ~((uint64_t)p.b << 32 | (uint32_t)p.t);
+    }
+    __syncthreads();
+    for (int k = tid; k < K; k += kMergeNT) {
+      const uint64_t key = keys[k], mine_at = index[k];
+      int before = 0;
+      for (int j = 0; j < K; j += 4) {
+        uint64_t o[4], i[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) o[u] = keys[j + u], i[u] = index[j + u];
+#pragma unroll
+        for (int u = 0; u < 4; u++) before += (o[u] > key) | ((o[u] == key) & (i[u] > mine_at));
+      }
+      if (before < n) emit(before, list[k]);
+    }
+    if (tid == 0) chosen = min(K, n);
+  } else {
+    Pick last{__builtin_huge_val(), -1, -1};
+    for (int r = 0; r < n; r++) {
+      Pick p{none, 0x7fffffff, 0};
+      for (int j = tid; j < T + W; j += kMergeNT) {
+        Pick q{none, 0, 0};
+        if (j < T)
+          q = pick(j, cand[j]);
+        else if (state[j - T] == 1)
+          q = Pick{(double)score[j - T], j - T, a.pad};
+        if (q.v > none && ahead(last, q) && ahead(q, p)) p = q;
+      }
+      // the first of the wave, of the workgroup
+      for (int o = 32; o > 0; o >>= 1) {
+        const Pick q{__shfl_xor(p.v, o), __shfl_xor(p.b, o), __shfl_xor(p.t, o)};
+        if (ahead(q, p)) p = q;
+      }
+      __syncthreads();
+      if (lane == 0) list[wave] = p;
+      __syncthreads();
+      for (int w = 0; w < kMergeNT / 64; w++)
+        if (ahead(list[w], p)) p = list[w];
+      if (tid == 0) emit(r, p);
+      last = p;
+    }
+    if (tid == 0) chosen = n;
+  }
+  __syncthreads();
+  if (chosen >= n) return;
+  // Fewer than n_select: the rest are the first continuations of value -inf.
+  int have = chosen;
+  for (int b = 0; b < W && have < n; b++)
+    for (int t0 = 0; t0 < a.vocab && have < n; t0 += kMergeNT) {
+      const int t = t0 + tid;
+      bool in = false;
+      if (t < a.vocab)
+        in = state[b] == 2 || (state[b] == 1 ? t != a.pad
+                                             : value(b, fmaxf(a.logits[(row0 + b) * a.ld + t], kNone)) == none);
+      const uint64_t who = __ballot(in);
+      __syncthreads();
+      if (lane == 0) rj[wave] = __popcll(who);
+      __syncthreads();
+      int at = have, all = 0;
+      for (int w = 0; w < kMergeNT / 64; w++) {
+        at += w < wave ? rj[w] : 0;
+        all += rj[w];
+      }
+      at += __popcll(who & ((1ull << lane) - 1));
+      if (in && at < n) emit(at, Pick{none, b, t});
+      have += all;
+    }
 }
 
 syn_status_t check_select(const syn_hip_beam_select_params *p) {
@@ -165,9 +422,10 @@ syn_status_t check_select(const syn_hip_beam_select_params *p) {
     set_error("beam_select: 1 to 64 beams and 1 to 128 continuations");
     return SYN_ERR_INVALID_ARG;
   }
-  if (!p->vocab || p->vocab > 0x7fffff00u || (uint64_t)p->n_select > p->n_beams * (uint64_t)p->vocab ||
-      (uint64_t)p->n_groups * p->n_beams > 0x7fffffffu) {
-    set_error("beam_select: fewer continuations than n_select, or too many rows");
+  if (!p->vocab || p->vocab > 0x7ff00000u || (uint64_t)p->n_select > p->n_beams * (uint64_t)p->vocab ||
+      (uint64_t)p->n_groups * p->n_beams > 65535u ||
+      (uint64_t)p->n_beams * p->n_select * cdiv(p->vocab, 2048) > 0x7ffffff0u) {
+    set_error("beam_select: fewer continuations than n_select, or too many rows or candidates");
     return SYN_ERR_INVALID_ARG;
   }
   if (p->ld_logits < p->vocab) {
@@ -178,14 +436,18 @@ syn_status_t check_select(const syn_hip_beam_select_params *p) {
 }
 
 struct SelectSpace {
+  int per, chunks;
   size_t stat, cand, total;
 };
 SelectSpace select_space(const syn_hip_beam_select_params &p) {
   const size_t rows = (size_t)p.n_groups * p.n_beams;
   SelectSpace s;
+  // chunks of 8192 logits; of 2048 where those would not fill the chip
+  s.per = rows * cdiv(p.vocab, kChunkNT * 32) >= 256 ? 32 : 8;
+  s.chunks = (int)cdiv(p.vocab, (size_t)kChunkNT * s.per);
   s.stat = 0;
-  s.cand = round_up(rows * sizeof(RowStat), 16);
-  s.total = s.cand + round_up(rows * p.n_select * sizeof(Cand), 16);
+  s.cand = round_up(rows * s.chunks * sizeof(ChunkStat), 16);
+  s.total = s.cand + round_up(rows * s.chunks * p.n_select * sizeof(Cand), 16);
   return s;
 }
 
@@ -333,13 +595,17 @@ syn_status_t syn_hip_beam_select(const syn_hip_beam_select_params *p, const floa
   SYN_TRY(ensure_init());
   uint8_t *ws = static_cast<uint8_t *>(d_workspace);
   const SelectArgs a{d_logits, d_scores, d_finished, d_parent, d_finished_out, d_token, d_score,
-                     reinterpret_cast<Cand *>(ws + sp.cand),
-                     reinterpret_cast<RowStat *>(ws + sp.stat), p->ld_logits, (int)p->vocab,
-                     (int)p->n_beams, (int)p->n_select, p->eos, p->pad};
+                     reinterpret_cast<Cand *>(ws + sp.cand), reinterpret_cast<ChunkStat *>(ws),
+                     p->ld_logits, (int)p->vocab, sp.chunks, (int)p->n_beams, (int)p->n_select,
+                     p->eos, p->pad, aligned16(d_logits) && p->ld_logits % 4 == 0};
   hipStream_t s = pick_stream(stream);
-  hipLaunchKernelGGL(k_beam_rows, dim3(p->n_groups * p->n_beams), dim3(kRowNT), 0, s, a);
+  const dim3 grid((unsigned)sp.chunks, p->n_groups * p->n_beams);
+  if (sp.per == 32)
+    hipLaunchKernelGGL(k_beam_chunks<32>, grid, dim3(kChunkNT), 0, s, a);
+  else
+    hipLaunchKernelGGL(k_beam_chunks<8>, grid, dim3(kChunkNT), 0, s, a);
   SYN_LAUNCH_CHECK();
-  hipLaunchKernelGGL(k_beam_merge, dim3(p->n_groups), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(k_beam_merge, dim3(p->n_groups), dim3(kMergeNT), 0, s, a);
   SYN_LAUNCH_CHECK();
   return SYN_OK;
 }

@@ -137,7 +137,8 @@ def select(ptrs=None, ws=FAKE, ws_bytes=None, **kw):
 @pytest.mark.parametrize("kw,want", [
     (dict(n_beams=0), ARG), (dict(n_beams=65), ARG), (dict(n_select=0), ARG),
     (dict(n_select=129), ARG), (dict(vocab=0), ARG), (dict(vocab=1, ld_logits=1), ARG),
-    (dict(vocab=1 << 31, ld_logits=1 << 31), ARG), (dict(ld_logits=99), SHAPE),
+    (dict(vocab=1 << 31, ld_logits=1 << 31), ARG), (dict(n_groups=20000), ARG),
+    (dict(n_beams=64, n_select=128, vocab=1 << 30, ld_logits=1 << 30), ARG), (dict(ld_logits=99), SHAPE),
     (dict(pad=-1), ARG), (dict(pad=100), ARG), (dict(ptrs=dict(x=None)), NULL),
     (dict(ptrs=dict(s=None)), NULL), (dict(ptrs=dict(p=None)), NULL), (dict(ptrs=dict(t=None)), NULL),
     (dict(ptrs=dict(v=None)), NULL), (dict(ws=None), NULL), (dict(ws=FAKE + 4), ARG),

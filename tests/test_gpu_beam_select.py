@@ -201,3 +201,29 @@ def test_scores_and_flags_in_place_over_replays():
             assert np.array_equal(fin[r] != 0, f)
         c.scores, c.fin = new, fin
     g.close()
+
+
+@pytest.mark.parametrize("vocab", [2048, 8192, 30000])
+def test_more_equal_logits_than_a_list_holds(vocab):
+    """whole chunks of one value, and of a few values with the best repeated"""
+    c = Case(12, 2, 3, 7, vocab, finished=False)
+    c.x[0] = 0.5
+    c.x[1] = np.where(np.arange(vocab) % 3 == 0, 1.0, -1.0)
+    c.x[2, vocab // 2:] = -np.inf
+    c.x[3:] = np.round(c.x[3:] * 2)
+    c.scores[3:] = c.scores[3]
+    c.call()
+    R.sync()
+    c.check()
+
+
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 128])
+def test_few_words_left_by_a_mask(n):
+    """most logits are -inf, as a grammar leaves them"""
+    c = Case(13, 2, 4, n, 40000, finished=False)
+    keep = c.rng.random(c.x.shape) < 2e-3
+    c.x[~keep] = -np.inf
+    c.x[5] = -np.inf
+    c.call()
+    R.sync()
+    c.check()
