@@ -274,6 +274,11 @@ __global__ void __launch_bounds__(kMergeNT) k_beam_merge(SelectArgs a) {
   Cand mine[kHeld];
 #pragma unroll
   for (int k = 0; k < kHeld; k++) mine[k] = cand[min(tid + k * kMergeNT, T - 1)];
+  // Lists are in order: if the D-th of a list is not below tau, D of it are
+  // not.  Of the lists of a wave in G groups, D G >= n, the least group maximum.
+  const int G = min(n <= 1 ? 1 : 1 << (32 - __builtin_clz(n - 1)), 1 << (31 - __builtin_clz(min(L, 64))));
+  const int D = (n + G - 1) / G;
+  const Cand front = cand[min(tid, L - 1) * n + D - 1];
   for (int b = wave; b < W; b += kMergeNT / 64) {
     const ChunkStat *st = a.stat + (row0 + b) * C;
     const ChunkStat q0 = st[min(lane, C - 1)];
@@ -308,14 +313,10 @@ __global__ void __launch_bounds__(kMergeNT) k_beam_merge(SelectArgs a) {
   auto ahead = [](const Pick &p, const Pick &q) {
     return p.v > q.v || (p.v == q.v && (p.b < q.b || (p.b == q.b && p.t < q.t)));
   };
-  // Lists are in order: if the D-th of a list is not below tau, D of it are
-  // not.  Of the lists of a wave in G groups, D G >= n, the least group maximum.
-  const int G = min(n <= 1 ? 1 : 1 << (32 - __builtin_clz(n - 1)), 1 << (31 - __builtin_clz(min(L, 64))));
-  const int D = (n + G - 1) / G;
   double key = none;
   for (int q = tid; q < L; q += kMergeNT) {
     const int j = q * n + D - 1;
-    key = fmax(key, pick(j, cand[j]).v);
+    key = fmax(key, pick(j, q == tid ? front : cand[j]).v);
   }
   const double tau_w = least_group(group_max(key, G), G);
   if (lane == 0) wtau[wave] = tau_w;
