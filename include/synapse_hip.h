@@ -749,6 +749,27 @@ syn_status_t syn_hip_beam_reorder_pages(const syn_hip_kv_pages *pages, size_t n_
                                         const int32_t *d_len, int32_t *d_table, size_t ld_table,
                                         int32_t *d_spare, void *stream);
 
+/* Beam search with the K-quant decoder over the operators above: the prompt is
+ * prefilled once, then n_beams continuations are decoded as the rows of one
+ * batch, each step a replayed HIP graph with no host work (every 16 steps the
+ * host looks whether all beams have ended).  The n_beams continuations of at
+ * most max_new tokens come back best first, by score / length^length_penalty
+ * (0: the score): out_tokens [n_beams][max_new] (places behind the eos hold
+ * it), out_lengths and out_scores [n_beams] (nullable; length with the eos,
+ * score the sum of the tokens' log-probabilities).  A beam ends with `eos`
+ * (-1: none) and competes with its score from then on.  The keys and values of
+ * prompt and beams are kept in kv_dtype; n_prompt + max_new - 1 <= max_seq.
+ * Afterwards the model's own cache holds the prompt. */
+typedef struct {
+  uint32_t n_beams;
+  int32_t eos, kv_dtype; /* SYN_HIP_KV_* */
+  float length_penalty;
+} syn_hip_beam_search;
+syn_status_t syn_hip_klm_generate_beams(syn_hip_klm_t *m, const uint32_t *prompt, size_t n_prompt,
+                                        size_t max_new, const syn_hip_beam_search *p,
+                                        uint32_t *out_tokens, uint32_t *out_lengths,
+                                        float *out_scores);
+
 /* -- harness helpers (no reference counterpart) -- */
 /* Encode f32 [n,k] into Q8_0 / Q4_K / Q6_K block bytes.  The reference has no
  * encoder for these formats (only dequantizers); any encoding is valid since

@@ -1,5 +1,6 @@
 // Beam search's choice over beams and vocabulary, and the states that follow
 // it.
+#include "beam.hpp"
 #include "kv_pages.hpp"
 
 namespace syn {
@@ -524,32 +525,49 @@ __global__ void __launch_bounds__(256) k_copy_pages(PagesArgs a) {
   }
 }
 
-// grid (columns / 64, group), after the copies
-__global__ void __launch_bounds__(64) k_reorder_tables(PagesArgs a) {
+// grid (columns / 64, group), after the copies: the waves take the rows in
+// turn, all entries of a column are read before one is written
+__global__ void __launch_bounds__(256) k_reorder_tables(PagesArgs a) {
   __shared__ int32_t stage[kMaxBeams][64];
-  const int l = threadIdx.x, g = blockIdx.y, W = a.W;
+  const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, g = blockIdx.y, W = a.W;
   const size_t col = (size_t)blockIdx.x * 64 + l;
   size_t full;
   int rest;
   held(a, g, &full, &rest);
-  if (col > full || col >= a.ld_table) return;
+  if ((size_t)blockIdx.x * 64 > full) return;
   const int32_t *par = a.parent + (size_t)g * W;
-  int32_t *t = a.table + (size_t)g * W * a.ld_table + col;
-  if (col < full) {
-    for (int b = 0; b < W; b++) {
-      const int p = par[b];
-      stage[b][l] = t[((uint32_t)p < (uint32_t)W ? p : b) * a.ld_table];
-    }
-    for (int b = 0; b < W; b++) t[b * a.ld_table] = stage[b][l];
-  } else if (rest) {
-    for (int b = 0; b < W; b++) {
-      const int p = par[b];
-      if (p == b || (uint32_t)p >= (uint32_t)W) continue;
+  int32_t *t = a.table + (size_t)g * W * a.ld_table + col, *spare = a.spare + (size_t)g * W;
+  const bool gather = col < full;
+#pragma unroll 4
+  for (int b = wave; b < W; b += 4) {
+    const int p = par[b];
+    if (gather) stage[b][l] = t[((uint32_t)p < (uint32_t)W ? p : b) * a.ld_table];
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int b = wave; b < W; b += 4) {
+    const int p = par[b];
+    if (gather) {
+      t[b * a.ld_table] = stage[b][l];
+    } else if (col == full && col < a.ld_table && rest && p != b && (uint32_t)p < (uint32_t)W) {
       const int32_t mine = t[b * a.ld_table];
-      t[b * a.ld_table] = a.spare[(size_t)g * W + b];
-      a.spare[(size_t)g * W + b] = mine;
+      t[b * a.ld_table] = spare[b];
+      spare[b] = mine;
     }
   }
+}
+
+__global__ void __launch_bounds__(64)
+    k_beam_advance(BeamCounters c, int n_beams, const uint32_t *token, uint32_t *history, size_t ld) {
+  const int b = threadIdx.x, step = *c.step;
+  __syncthreads();
+  if (b < n_beams) {
+    history[b * ld + step] = token[b];
+    c.pos[b]++;
+    c.index[b]++;
+    c.len[b]++;
+  }
+  if (b == 0) *c.step = step + 1;
 }
 
 syn_status_t check_beams(size_t n_groups, size_t n_beams, const char *who) {
@@ -561,6 +579,13 @@ syn_status_t check_beams(size_t n_groups, size_t n_beams, const char *who) {
 }
 
 }  // namespace
+
+syn_status_t launch_beam_advance(const BeamCounters &c, int n_beams, const uint32_t *token,
+                                 uint32_t *history, size_t ld_history, hipStream_t s) {
+  hipLaunchKernelGGL(k_beam_advance, dim3(1), dim3(64), 0, s, c, n_beams, token, history, ld_history);
+  SYN_LAUNCH_CHECK();
+  return SYN_OK;
+}
 
 }  // namespace syn
 
@@ -675,7 +700,7 @@ syn_status_t syn_hip_beam_reorder_pages(const syn_hip_kv_pages *pages, size_t n_
                      dim3(256), 0, s, a);
   SYN_LAUNCH_CHECK();
   hipLaunchKernelGGL(k_reorder_tables, dim3((unsigned)cdiv(ld_table, 64), (unsigned)n_groups),
-                     dim3(64), 0, s, a);
+                     dim3(256), 0, s, a);
   SYN_LAUNCH_CHECK();
   return SYN_OK;
 }

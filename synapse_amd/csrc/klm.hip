@@ -6,17 +6,43 @@
 // driver; activations stay f32 between layers (no activation quantization
 // on this path, as in the reference).
 #include <algorithm>
+#include <cmath>
 #include <cstring>
+#include <memory>
 #include <string>
 #include <thread>
 #include <vector>
 
+#include "beam.hpp"
 #include "decode_fused.hpp"
 #include "klm_fused.hpp"
+#include "kv_pages.hpp"
 #include "kquant.hpp"
 #include "layer_ops.hpp"
 
 using namespace syn;
+
+// What a beam search of one shape keeps on the device: pages for the prompt and
+// for each beam's tokens (and its spare), tables, counters, per-beam rows, and
+// the captured step.
+struct BeamSpace {
+  size_t n_prompt = 0, max_new = 0, W = 0;
+  int32_t eos = -1, dtype = SYN_HIP_KV_F32;
+  syn_hip_kv_pages pages{};
+  size_t prefix_cols = 0, cols = 0;
+  DevBuf k, v, ptable, plen, table, spare, count, iota, zeros;
+  DevBuf logits, scores, finished, parent, token, history, attn_ws, select_ws;
+  size_t attn_bytes = 0, select_bytes = 0;
+  BeamCounters counters{};
+  syn_hip_beam_select_params select{};
+  hipGraphExec_t graph = nullptr;
+  ~BeamSpace() {
+    if (graph) (void)hipGraphExecDestroy(graph);
+  }
+  bool is(size_t np, size_t mn, size_t w, const syn_hip_beam_search &p) const {
+    return n_prompt == np && max_new == mn && W == w && eos == p.eos && dtype == p.kv_dtype;
+  }
+};
 
 struct syn_hip_klm_s {
   syn_hip_klm_config c{};
@@ -46,6 +72,7 @@ struct syn_hip_klm_s {
   bool fused_ok = false;
   KqfPlan fp_qkv, fp_o, fp_gu, fp_down, fp_lm;
   DevBuf f_r, f_qkv, f_ao, f_aml, f_pv, f_pi, f_pv2;
+  std::unique_ptr<BeamSpace> beams;  // of the last beam search
 
   ~syn_hip_klm_s() {
     if (graph) (void)hipGraphExecDestroy(graph);
@@ -146,8 +173,10 @@ struct syn_hip_klm_s {
     return SYN_OK;
   }
 
-  // cache_off (prefill only): cache row of the first of `rows` tokens
-  syn_status_t layer(size_t l, int rows, bool prefill, hipStream_t s, int cache_off = 0) {
+  // cache_off (prefill only): cache row of the first of `rows` tokens; with
+  // `prompt` set, the rows' keys and values go to its pages too
+  syn_status_t layer(size_t l, int rows, bool prefill, hipStream_t s, int cache_off = 0,
+                     BeamSpace *prompt = nullptr) {
     Layer &Ly = layers[l];
     const float eps = c.base.eps;
     const int nh = (int)c.base.n_heads, nkv = (int)c.base.n_kv_heads;
@@ -157,6 +186,14 @@ struct syn_hip_klm_s {
                                  attn_nw.as<float>() + l * h, eps, rows, (int)h, nullptr, 0,
                                  nullptr, normed.as<float>(), s));
     SYN_TRY(Ly.qkv.gemv(rows, normed.as<float>(), h, qkv.as<float>(), n_qkv, s));
+    if (prompt) {
+      const syn_hip_kv_append_params p = append_params(l, 0, 1, prompt->prefix_cols);
+      const float *k = qkv.as<float>() + qd;
+      SYN_TRY(syn_hip_kv_append(&prompt->pages, &p, rows, nullptr, k, k + kvd, nullptr, kn,
+                                rope_cos.as<float>(), rope_sin.as<float>(), prompt->iota.as<int32_t>(),
+                                prompt->zeros.as<int32_t>(), prompt->iota.as<int32_t>(),
+                                prompt->ptable.as<int32_t>(), nullptr, s));
+    }
     if (!prefill && fused_attention_fits((int)hd, (int)S)) {
       // one kernel per query head: head norms, RoPE, KV append and attention
       RowSrc src;
@@ -385,9 +422,9 @@ struct syn_hip_klm_s {
 
   // the layers of CausalLM::forward_prefill (causal_lm.rs:195-224) over n
   // tokens whose ids are on the device, appended at cache rows cache_off ..
-  syn_status_t prefill_rows(const uint32_t *d_ids, int n, int cache_off) {
+  syn_status_t prefill_rows(const uint32_t *d_ids, int n, int cache_off, BeamSpace *prompt = nullptr) {
     SYN_TRY(launch_embed(embed.as<float>(), d_ids, n, (int)h, (int)vocab, x.as<float>(), stream));
-    for (size_t l = 0; l < L; l++) SYN_TRY(layer(l, n, true, stream, cache_off));
+    for (size_t l = 0; l < L; l++) SYN_TRY(layer(l, n, true, stream, cache_off, prompt));
     return SYN_OK;
   }
 
@@ -422,6 +459,258 @@ struct syn_hip_klm_s {
     StepState cur;
     SYN_TRY(get_state(&cur));
     if (new_len < (size_t)cur.pos) SYN_TRY(set_state((int)new_len, cur.token, cur.step));
+    return SYN_OK;
+  }
+
+  // ---- beam search: the prompt is prefilled as ever and its keys and values
+  // stored once; the beams' tokens are decoded as rows of one batch over it.
+  syn_hip_kv_append_params append_params(size_t l, size_t n_heads, size_t n_seqs, size_t cols) const {
+    syn_hip_kv_append_params p{};
+    p.layer = (uint32_t)l;
+    p.n_heads = (uint32_t)n_heads;
+    p.n_seqs = (uint32_t)n_seqs;
+    p.rotary_dim = (uint32_t)hd;
+    p.n_positions = (uint32_t)S;
+    p.eps = c.base.eps;
+    p.ldq = p.ldk = p.ldv = n_qkv;
+    p.ldo = qd;
+    p.ld_table = cols;
+    return p;
+  }
+  syn_hip_prefix_attention_params attend_params(const BeamSpace &b, size_t l) const {
+    syn_hip_prefix_attention_params p{};
+    p.layer = (uint32_t)l;
+    p.n_heads = c.base.n_heads;
+    p.n_groups = 1;
+    p.group_size = (uint32_t)b.W;
+    p.max_prefix = (uint32_t)b.n_prompt;
+    p.max_suffix = (uint32_t)(b.max_new - 1);
+    p.ldq = p.ldo = qd;
+    p.ld_prefix_table = b.prefix_cols;
+    p.ld_table = b.cols;
+    return p;
+  }
+
+  syn_status_t make_beams(size_t n_prompt, size_t max_new, size_t W, const syn_hip_beam_search &bs) {
+    if (beams && beams->is(n_prompt, max_new, W, bs)) return SYN_OK;
+    SYN_HIP(hipStreamSynchronize(stream));
+    beams.reset();
+    auto b = std::make_unique<BeamSpace>();
+    constexpr size_t kPage = 16;  // positions; a step copies half of one a beam at most on average
+    b->n_prompt = n_prompt;
+    b->max_new = max_new;
+    b->W = W;
+    b->eos = bs.eos;
+    b->dtype = bs.kv_dtype;
+    b->prefix_cols = cdiv(n_prompt, kPage);
+    b->cols = std::max<size_t>(1, cdiv(max_new - 1, kPage));
+    syn_hip_kv_pages &pg = b->pages;
+    pg.dtype = bs.kv_dtype;
+    pg.page_size = kPage;
+    pg.n_pages = (uint32_t)(b->prefix_cols + W * (b->cols + 1));
+    pg.n_layers = (uint32_t)L;
+    pg.n_kv_heads = c.base.n_kv_heads;
+    pg.head_dim = (uint32_t)hd;
+    SYN_TRY(b->k.alloc(kv_pool_bytes(pg)));
+    SYN_TRY(b->v.alloc(kv_pool_bytes(pg)));
+    pg.k = b->k.p;
+    pg.v = b->v.p;
+    SYN_TRY(check_pages(&pg, "klm_generate_beams"));
+    SYN_TRY(b->ptable.alloc(b->prefix_cols * 4));
+    SYN_TRY(b->plen.alloc(4));
+    SYN_TRY(b->table.alloc(W * b->cols * 4));
+    SYN_TRY(b->spare.alloc(W * 4));
+    SYN_TRY(b->count.alloc((3 * W + 1) * 4));
+    SYN_TRY(b->iota.alloc(n_prompt * 4));
+    SYN_TRY(b->zeros.alloc(n_prompt * 4));
+    SYN_TRY(b->logits.alloc(W * round_up(vocab, 4) * 4));
+    SYN_TRY(b->scores.alloc(W * 4));
+    SYN_TRY(b->finished.alloc(W * 4));
+    SYN_TRY(b->parent.alloc(W * 4));
+    SYN_TRY(b->token.alloc(W * 4));
+    SYN_TRY(b->history.alloc(W * max_new * 4));
+    b->counters.pos = b->count.as<int32_t>();
+    b->counters.index = b->counters.pos + W;
+    b->counters.len = b->counters.index + W;
+    b->counters.step = b->counters.len + W;
+    const syn_hip_prefix_attention_params ap = attend_params(*b, 0);
+    SYN_TRY(syn_hip_prefix_attention_workspace(&pg, &ap, &b->attn_bytes));
+    SYN_TRY(b->attn_ws.alloc(b->attn_bytes));
+    syn_hip_beam_select_params &sp = b->select;
+    sp.n_groups = 1;
+    sp.n_beams = sp.n_select = (uint32_t)W;
+    sp.eos = bs.eos;
+    sp.pad = std::max(bs.eos, 0);
+    sp.vocab = vocab;
+    sp.ld_logits = round_up(vocab, 4);  // 16-byte rows
+    syn_hip_beam_select_params first = sp;  // the prompt's: one row
+    first.n_beams = 1;
+    size_t first_bytes = 0;
+    SYN_TRY(syn_hip_beam_select_workspace(&sp, &b->select_bytes));
+    SYN_TRY(syn_hip_beam_select_workspace(&first, &first_bytes));
+    b->select_bytes = std::max(b->select_bytes, first_bytes);
+    SYN_TRY(b->select_ws.alloc(b->select_bytes));
+    SYN_TRY(lm_head.prepare(W));
+    beams = std::move(b);
+    return SYN_OK;
+  }
+
+  // the state at the beginning: every page the row's own
+  syn_status_t reset_beams(BeamSpace &b) {
+    std::vector<int32_t> t(std::max({b.prefix_cols, b.W * (b.cols + 1), b.n_prompt, 3 * b.W + 1}));
+    auto put = [&](DevBuf &d, size_t n, int32_t first, int32_t by) -> syn_status_t {
+      for (size_t i = 0; i < n; i++) t[i] = first + by * (int32_t)i;
+      SYN_HIP(hipMemcpyAsync(d.p, t.data(), n * 4, hipMemcpyHostToDevice, stream));
+      SYN_HIP(hipStreamSynchronize(stream));
+      return SYN_OK;
+    };
+    const int32_t own = (int32_t)b.prefix_cols, n_own = (int32_t)(b.W * b.cols);
+    SYN_TRY(put(b.ptable, b.prefix_cols, 0, 1));
+    SYN_TRY(put(b.plen, 1, (int32_t)b.n_prompt, 0));
+    SYN_TRY(put(b.table, b.W * b.cols, own, 1));
+    SYN_TRY(put(b.spare, b.W, own + n_own, 1));
+    SYN_TRY(put(b.iota, b.n_prompt, 0, 1));
+    SYN_TRY(put(b.zeros, b.n_prompt, 0, 0));
+    SYN_TRY(put(b.finished, b.W, 0, 0));
+    SYN_TRY(put(b.scores, b.W, 0, 0));  // (0.0f)
+    // so that the first advance leaves the first decoded token's place
+    for (size_t i = 0; i < b.W; i++) {
+      t[i] = (int32_t)b.n_prompt - 1;
+      t[b.W + i] = -1;
+      t[2 * b.W + i] = 0;
+    }
+    t[3 * b.W] = 0;
+    SYN_HIP(hipMemcpyAsync(b.count.p, t.data(), (3 * b.W + 1) * 4, hipMemcpyHostToDevice, stream));
+    SYN_HIP(hipStreamSynchronize(stream));
+    return SYN_OK;
+  }
+
+  syn_status_t beam_layer(BeamSpace &b, size_t l, hipStream_t s) {
+    Layer &Ly = layers[l];
+    const int W = (int)b.W;
+    const float eps = c.base.eps;
+    SYN_TRY(launch_rmsnorm_quant(x.as<float>(), l == 0 ? nullptr : down.as<float>(),
+                                 attn_nw.as<float>() + l * h, eps, W, (int)h, nullptr, 0, nullptr,
+                                 normed.as<float>(), s));
+    SYN_TRY(Ly.qkv.gemv(W, normed.as<float>(), h, qkv.as<float>(), n_qkv, s));
+    const syn_hip_kv_append_params ap = append_params(l, c.base.n_heads, b.W, b.cols);
+    const float *q = qkv.as<float>();
+    SYN_TRY(syn_hip_kv_append(&b.pages, &ap, b.W, q, q + qd, q + qd + kvd,
+                              c.qk_norm ? q_nw.as<float>() + l * hd : nullptr,
+                              c.qk_norm ? k_nw.as<float>() + l * hd : nullptr, rope_cos.as<float>(),
+                              rope_sin.as<float>(), b.counters.pos, nullptr, b.counters.index,
+                              b.table.as<int32_t>(), qrot.as<float>(), s));
+    const syn_hip_prefix_attention_params tp = attend_params(b, l);
+    SYN_TRY(syn_hip_prefix_attention(&b.pages, &tp, qrot.as<float>(), b.ptable.as<int32_t>(),
+                                     b.plen.as<int32_t>(), b.table.as<int32_t>(), b.counters.len,
+                                     attn.as<float>(), b.attn_ws.p, b.attn_bytes, s));
+    SYN_TRY(Ly.o.gemv(W, attn.as<float>(), qd, o.as<float>(), h, s));
+    SYN_TRY(launch_rmsnorm_quant(x.as<float>(), o.as<float>(), ffn_nw.as<float>() + l * h, eps, W,
+                                 (int)h, nullptr, 0, nullptr, normed.as<float>(), s));
+    SYN_TRY(Ly.gu.gemv(W, normed.as<float>(), h, gu.as<float>(), 2 * inter, s));
+    SYN_TRY(launch_swiglu_f32(gu.as<float>(), (int)(2 * inter), W, (int)inter, hbuf.as<float>(),
+                              (int)inter, s));
+    return Ly.down.gemv(W, hbuf.as<float>(), inter, down.as<float>(), h, s);
+  }
+
+  // one token for every beam, then the choice and what follows it
+  syn_status_t beam_step(BeamSpace &b, hipStream_t s) {
+    const int W = (int)b.W;
+    SYN_TRY(launch_embed(embed.as<float>(), b.token.as<uint32_t>(), W, (int)h, (int)vocab,
+                         x.as<float>(), s));
+    for (size_t l = 0; l < L; l++) SYN_TRY(beam_layer(b, l, s));
+    SYN_TRY(launch_rmsnorm_quant(x.as<float>(), down.as<float>(), final_nw.as<float>(), c.base.eps, W,
+                                 (int)h, nullptr, 0, nullptr, normed.as<float>(), s));
+    SYN_TRY(lm_head.gemv(W, normed.as<float>(), h, b.logits.as<float>(), b.select.ld_logits, s));
+    SYN_TRY(syn_hip_beam_select(&b.select, b.logits.as<float>(), b.scores.as<float>(),
+                                b.finished.as<int32_t>(), b.parent.as<int32_t>(),
+                                b.token.as<uint32_t>(), b.scores.as<float>(),
+                                b.finished.as<int32_t>(), b.select_ws.p, b.select_bytes, s));
+    SYN_TRY(syn_hip_beam_reorder_pages(&b.pages, 1, b.W, b.parent.as<int32_t>(), b.counters.len,
+                                       b.table.as<int32_t>(), b.cols, b.spare.as<int32_t>(), s));
+    SYN_TRY(syn_hip_beam_reorder_rows(1, b.W, b.parent.as<int32_t>(), b.history.p, b.max_new * 4,
+                                      b.max_new * 4, 1, 0, s));
+    return launch_beam_advance(b.counters, W, b.token.as<uint32_t>(), b.history.as<uint32_t>(),
+                               b.max_new, s);
+  }
+
+  syn_status_t generate_beams(const uint32_t *prompt, size_t n_prompt, size_t max_new,
+                              const syn_hip_beam_search &bs, uint32_t *out_tokens,
+                              uint32_t *out_lengths, float *out_scores) {
+    const size_t W = bs.n_beams;
+    SYN_TRY(make_beams(n_prompt, max_new, W, bs));
+    BeamSpace &b = *beams;
+    SYN_TRY(reset_beams(b));
+    if (use_graph && !b.graph && max_new > 1) {
+      hipGraph_t g;
+      SYN_HIP(hipStreamBeginCapture(stream, hipStreamCaptureModeThreadLocal));
+      const syn_status_t st_ = beam_step(b, stream);
+      hipError_t e = hipStreamEndCapture(stream, &g);
+      if (st_ != SYN_OK) {
+        if (e == hipSuccess) (void)hipGraphDestroy(g);
+        return st_;
+      }
+      if (e != hipSuccess) return hip_fail(e, "hipStreamEndCapture", __FILE__, __LINE__);
+      e = hipGraphInstantiate(&b.graph, g, nullptr, nullptr, 0);
+      (void)hipGraphDestroy(g);
+      if (e != hipSuccess) {
+        b.graph = nullptr;
+        return hip_fail(e, "hipGraphInstantiate", __FILE__, __LINE__);
+      }
+    }
+    // the prompt, and its continuations as the first choice of a single beam
+    // (scores and flags in place: one group's are read before they are written)
+    hp.known = false;
+    SYN_HIP(hipMemcpyAsync(ids.p, prompt, n_prompt * 4, hipMemcpyHostToDevice, stream));
+    SYN_TRY(set_state(0, 0, 0));
+    SYN_TRY(prefill_rows(ids.as<uint32_t>(), (int)n_prompt, 0, &b));
+    SYN_TRY(head((int)n_prompt - 1, (int)n_prompt, stream));
+    syn_hip_beam_select_params first = b.select;
+    first.n_beams = 1;
+    SYN_TRY(syn_hip_beam_select(&first, logits.as<float>(), b.scores.as<float>(),
+                                b.finished.as<int32_t>(), b.parent.as<int32_t>(),
+                                b.token.as<uint32_t>(), b.scores.as<float>(),
+                                b.finished.as<int32_t>(), b.select_ws.p, b.select_bytes, stream));
+    SYN_TRY(launch_beam_advance(b.counters, (int)W, b.token.as<uint32_t>(), b.history.as<uint32_t>(),
+                                max_new, stream));
+    std::vector<int32_t> fin(W, 0);
+    size_t done = 1;
+    for (; done < max_new; done++) {
+      if (use_graph)
+        SYN_HIP(hipGraphLaunch(b.graph, stream));
+      else
+        SYN_TRY(beam_step(b, stream));
+      if (bs.eos >= 0 && done % 16 == 0) {  // nothing left to decode?
+        SYN_HIP(hipMemcpyAsync(fin.data(), b.finished.p, W * 4, hipMemcpyDeviceToHost, stream));
+        SYN_HIP(hipStreamSynchronize(stream));
+        if (std::all_of(fin.begin(), fin.end(), [](int32_t f) { return f != 0; })) {
+          done++;
+          break;
+        }
+      }
+    }
+    std::vector<uint32_t> hist(W * max_new);
+    std::vector<float> score(W);
+    SYN_HIP(hipMemcpyAsync(hist.data(), b.history.p, hist.size() * 4, hipMemcpyDeviceToHost, stream));
+    SYN_HIP(hipMemcpyAsync(score.data(), b.scores.p, W * 4, hipMemcpyDeviceToHost, stream));
+    SYN_HIP(hipStreamSynchronize(stream));
+    // best first, by score / length^penalty (a beam's length ends with its eos)
+    std::vector<size_t> len(W), order(W);
+    std::vector<double> rank(W);
+    for (size_t i = 0; i < W; i++) {
+      const uint32_t *t = hist.data() + i * max_new;
+      len[i] = bs.eos < 0 ? done : std::min<size_t>(done, std::find(t, t + done, (uint32_t)bs.eos) - t + 1);
+      rank[i] = (double)score[i] / std::pow((double)len[i], (double)bs.length_penalty);
+      order[i] = i;
+    }
+    std::stable_sort(order.begin(), order.end(), [&](size_t i, size_t j) { return rank[i] > rank[j]; });
+    for (size_t r = 0; r < W; r++) {
+      const size_t i = order[r];
+      for (size_t t = 0; t < max_new; t++)
+        out_tokens[r * max_new + t] = t < len[i] ? hist[i * max_new + t] : (uint32_t)b.select.pad;
+      if (out_lengths) out_lengths[r] = (uint32_t)len[i];
+      if (out_scores) out_scores[r] = score[i];
+    }
     return SYN_OK;
   }
 
@@ -717,6 +1006,41 @@ syn_status_t syn_hip_klm_generate_speculative(syn_hip_klm_t *m, const uint32_t *
                            m->stream));
   SYN_HIP(hipStreamSynchronize(m->stream));
   return SYN_OK;
+}
+
+syn_status_t syn_hip_klm_generate_beams(syn_hip_klm_t *m, const uint32_t *prompt, size_t n_prompt,
+                                        size_t max_new, const syn_hip_beam_search *p,
+                                        uint32_t *out_tokens, uint32_t *out_lengths,
+                                        float *out_scores) {
+  SYN_TRY(check_klm(m));
+  if (!prompt || !p || !out_tokens) return SYN_ERR_NULL_PTR;
+  if (max_new == 0) return SYN_OK;
+  if (n_prompt == 0 || n_prompt > m->S || max_new - 1 > m->S - n_prompt) {
+    set_error("beam search: prompt + generated tokens must be in [1, max_seq]");
+    return SYN_ERR_INVALID_ARG;
+  }
+  if (!p->n_beams || p->n_beams > kMaxBeams || p->n_beams > m->S || p->n_beams > m->vocab) {
+    set_error("beam search: 1 to 64 beams, at most max_seq and the vocabulary");
+    return SYN_ERR_INVALID_ARG;
+  }
+  if (p->eos >= 0 && (size_t)p->eos >= m->vocab) {
+    set_error("beam search: eos outside the vocabulary");
+    return SYN_ERR_INVALID_ARG;
+  }
+  if (p->kv_dtype != SYN_HIP_KV_F32 && p->kv_dtype != SYN_HIP_KV_F16 && p->kv_dtype != SYN_HIP_KV_BF16) {
+    set_error("beam search: unknown cache dtype");
+    return SYN_ERR_INVALID_ARG;
+  }
+  if (m->hd % 8 || m->hd > kKvMaxHeadDim) {
+    set_error("beam search: head_dim must be a multiple of 8 up to 256");
+    return SYN_ERR_INVALID_ARG;
+  }
+  try {
+    return m->generate_beams(prompt, n_prompt, max_new, *p, out_tokens, out_lengths, out_scores);
+  } catch (const std::bad_alloc &) {
+    set_error("beam search: host memory");
+    return SYN_ERR_OUT_OF_MEMORY;
+  }
 }
 
 syn_status_t syn_hip_klm_forward_one(syn_hip_klm_t *m, uint32_t token, float *host_logits) {

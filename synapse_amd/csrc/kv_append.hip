@@ -2,6 +2,8 @@
 // the way: y = x * gain / sqrt(mean x^2 + eps) per head, then each pair (a, b)
 // of the first rotary_dim dims turned by its position's angle, f32 throughout,
 // rounded once (to nearest even) where a 16-bit pool stores it.
+#include <algorithm>
+
 #include "kv_pages.hpp"
 
 namespace syn {
@@ -18,106 +20,206 @@ struct AppendArgs {
   size_t ldq, ldk, ldv, ldo, ld_table;
   int n_tokens, nh, n_seqs, rd, interleaved, n_pos;
   float eps;
+  bool vec_in, vec_out, vec_rot;  // 16-byte rows of q, k, v; of q_out; of the tables, half of rd
 };
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) k_kv_append(AppendArgs a, KvPool<T> pool) {
-  extern __shared__ float xs[];  // [kTok][hd + 4]
-  __shared__ float inv[kTok];
-  __shared__ int row_pos[kTok], row_page[kTok], row_slot[kTok], whole[kTok];
-  const int tid = threadIdx.x, hd = pool.hd, ldx = hd + 4;
-  const int t0 = blockIdx.x * kTok, head = blockIdx.y;
-  const int nt = min(kTok, a.n_tokens - t0);
-  const bool is_q = head < a.nh, is_k = !is_q && head < a.nh + pool.nkv;
-  const int h = is_q ? head : (is_k ? head - a.nh : head - a.nh - pool.nkv);
-  const float *src = is_q ? a.q : (is_k ? a.k : a.v);
-  const size_t lds = is_q ? a.ldq : (is_k ? a.ldk : a.ldv);
+// four consecutive floats
+__device__ __forceinline__ f32x4 load4(const float *p, bool vec) {
+  if (vec) return *reinterpret_cast<const f32x4 *>(p);
+  return f32x4{p[0], p[1], p[2], p[3]};
+}
+// sum over the 16 lanes of a token
+__device__ __forceinline__ float row_sum(float x) {
+  auto add = [&](int y) { x += __int_as_float(y); };
+  add(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xb1, 0xf, 0xf, false));   // lane ^ 1
+  add(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4e, 0xf, 0xf, false));   // lane ^ 2
+  add(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x141, 0xf, 0xf, false));  // 7 - lane
+  add(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x140, 0xf, 0xf, false));  // 15 - lane
+  return x;
+}
 
-  if (tid < kTok) {
-    int pos = -1, page = -1, slot = 0;
-    if (tid < nt) {
-      const int t = t0 + tid;
-      pos = a.pos[t];
-      if ((uint32_t)pos >= (uint32_t)a.n_pos) pos = -1;
-      const int seq = a.seq ? a.seq[t] : t, i = a.index[t];
-      const int col = i >> pool.ps_shift;
-      if (pos >= 0 && i >= 0 && (size_t)col < a.ld_table && (uint32_t)seq < (uint32_t)a.n_seqs) {
-        page = a.table[(size_t)seq * a.ld_table + col];
-        if (!pool.has(page)) page = -1;
-        slot = i & (pool.ps - 1);
+// A workgroup takes 16 tokens and every gridDim.y-th head (queries, keys, then
+// values): 16 threads a token, each four dims of every 64.  A thread's angles
+// are the same for all heads and stay in registers; the other half of a pair
+// comes from the token's row in LDS, which only its own wave writes.  The next
+// head is requested before this one is worked on.  Bound by its bytes: read
+// once, written once.  KD: 64 dims each (hd <= 64 KD).
+template <class T, int KD>
+__global__ void __launch_bounds__(kThreads) k_kv_append(AppendArgs a, KvPool<T> pool) {
+  __shared__ __align__(16) float xs[kTok][64 * KD + 4];
+  __shared__ int row_page[kTok], row_slot[kTok], whole[kTok];
+  const int tid = threadIdx.x, hd = pool.hd, t = tid >> 4, l = tid & 15;
+  const int t0 = blockIdx.x * kTok, nt = min(kTok, a.n_tokens - t0);
+  const int heads = a.nh + 2 * pool.nkv;
+  const size_t tok = t0 + min(t, nt - 1);  // (threads past the last repeat it and write nothing)
+
+  auto row_of = [&](int head) {
+    const bool is_q = head < a.nh, is_k = !is_q && head < a.nh + pool.nkv;
+    const float *src = is_q ? a.q : (is_k ? a.k : a.v);
+    const size_t ld = is_q ? a.ldq : (is_k ? a.ldk : a.ldv);
+    const int h = is_q ? head : (is_k ? head - a.nh : head - a.nh - pool.nkv);
+    return src + tok * ld + (size_t)h * hd;
+  };
+  f32x4 next[KD];
+  auto ask = [&](int head) {
+    const float *src = row_of(head);
+#pragma unroll
+    for (int k = 0; k < KD; k++) next[k] = load4(src + min(64 * k + 4 * l, hd - 4), a.vec_in);
+  };
+  ask(blockIdx.y);
+
+  // the token's place, and its angles
+  int pos = a.pos[tok], page = -1, slot = 0;
+  {
+    const int seq = a.seq ? a.seq[tok] : (int)tok, i = a.index[tok];
+    const bool known = (uint32_t)pos < (uint32_t)a.n_pos;
+    if (!known || t >= nt) pos = -1;
+    const int col = i >> pool.ps_shift;
+    if (pos >= 0 && i >= 0 && (size_t)col < a.ld_table && (uint32_t)seq < (uint32_t)a.n_seqs) {
+      page = a.table[(size_t)seq * a.ld_table + col];
+      if (!pool.has(page)) page = -1;
+      slot = i & (pool.ps - 1);
+    }
+    if (l == 0) row_page[t] = page, row_slot[t] = slot;
+  }
+  const int half = a.rd >> 1;
+  f32x4 c[KD], s[KD];  // of the thread's dims; s negative where the pair's first half is
+  const size_t at = (size_t)max(pos, 0) * half;
+#pragma unroll
+  for (int k = 0; k < KD; k++) {
+    c[k] = f32x4{1, 1, 1, 1};
+    s[k] = f32x4{0, 0, 0, 0};
+    const int d0 = 64 * k + 4 * l;
+    if (d0 >= a.rd) continue;
+    if (a.vec_rot && !a.interleaved) {
+      const int i = d0 < half ? d0 : d0 - half;
+      c[k] = load4(a.cs + at + i, true);
+      s[k] = load4(a.sn + at + i, true);
+      if (d0 < half) s[k] = -s[k];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int d = d0 + j;
+        if (d >= a.rd) break;
+        const bool lo = a.interleaved ? !(d & 1) : d < half;
+        const int i = a.interleaved ? d >> 1 : (lo ? d : d - half);
+        c[k][j] = a.cs[at + i];
+        s[k][j] = lo ? -a.sn[at + i] : a.sn[at + i];
       }
     }
-    row_pos[tid] = pos;
-    row_page[tid] = page;
-    row_slot[tid] = slot;
   }
-  for (int i = tid; i < nt * hd; i += kThreads) {
-    const int t = i / hd, d = i - t * hd;
-    xs[t * ldx + d] = src[(size_t)(t0 + t) * lds + (size_t)h * hd + d];
+  __syncthreads();
+  // 8 tokens that fill an aligned group of 8 positions are written together
+  if (tid < kTok) {
+    bool w = tid + 8 <= nt && row_page[tid] >= 0 && (row_slot[tid] & 7) == 0;
+    for (int j = 1; w && j < 8; j++)
+      w = row_page[tid + j] == row_page[tid] && row_slot[tid + j] == row_slot[tid] + j;
+    whole[tid] = w;
   }
   __syncthreads();
 
-  const float *gain = is_q ? a.qn : (is_k ? a.kn : nullptr);
-  if (gain) {
-    // 16 threads a token
-    const int t = tid >> 4, l = tid & 15;
-    float s = 0.0f;
-    if (t < nt)
-      for (int d = l; d < hd; d += 16) s = __builtin_fmaf(xs[t * ldx + d], xs[t * ldx + d], s);
-    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
-    if (l == 0) inv[t] = 1.0f / sqrtf(s / (float)hd + a.eps);
-    __syncthreads();
-    for (int i = tid; i < nt * hd; i += kThreads) {
-      const int tt = i / hd, d = i - tt * hd;
-      xs[tt * ldx + d] = xs[tt * ldx + d] * gain[d] * inv[tt];
-    }
-    __syncthreads();
-  }
-
-  const int half = a.rd >> 1;
-  auto turned = [&](int t, int d) {
-    const float x = xs[t * ldx + d];
-    if (d >= a.rd) return x;
-    const bool lo = a.interleaved ? !(d & 1) : d < half;
-    const int i = a.interleaved ? d >> 1 : (lo ? d : d - half);
-    const float y = xs[t * ldx + (a.interleaved ? d ^ 1 : (lo ? d + half : d - half))];
-    const size_t at = (size_t)row_pos[t] * half + i;
-    const float c = a.cs[at], s = a.sn[at];
-    return __builtin_fmaf(x, c, lo ? -(y * s) : y * s);
-  };
-
-  if (is_q) {
-    for (int i = tid; i < nt * hd; i += kThreads) {
-      const int t = i / hd, d = i - t * hd;
-      if (row_pos[t] >= 0) a.qo[(size_t)(t0 + t) * a.ldo + (size_t)h * hd + d] = turned(t, d);
-    }
-  } else if (is_k) {
-    const int n8 = hd >> 3;  // consecutive threads write consecutive positions
-    for (int i = tid; i < nt * n8; i += kThreads) {
-      const int t = i % nt, c = i / nt;
-      if (row_page[t] < 0) continue;
-      T *dst = pool.k + pool.base(row_page[t], h) + pool.k_at(row_slot[t], c * 8);
-      for (int j = 0; j < 8; j++) dst[j] = (T)turned(t, c * 8 + j);
-    }
-  } else {
-    // 8 tokens that fill an aligned group of 8 positions are written together
-    if (tid < kTok) {
-      bool w = tid + 8 <= nt && row_page[tid] >= 0 && (row_slot[tid] & 7) == 0;
-      for (int j = 1; w && j < 8; j++)
-        w = row_page[tid + j] == row_page[tid] && row_slot[tid + j] == row_slot[tid] + j;
-      whole[tid] = w;
-    }
-    __syncthreads();
-    for (int i = tid; i < nt * hd; i += kThreads) {
-      const int t = i / hd, d = i - t * hd;
-      if (row_page[t] < 0) continue;
-      T *dst = pool.v + pool.base(row_page[t], h) + pool.v_at(row_slot[t], d);
-      const int lead = t - (row_slot[t] & 7);
-      if (whole[t]) {
-        for (int j = 0; j < 8; j++) dst[j] = (T)xs[(t + j) * ldx + d];
-      } else if (lead < 0 || !whole[lead]) {
-        *dst = (T)xs[t * ldx + d];
+  for (int head = blockIdx.y; head < heads; head += gridDim.y) {
+    const bool is_q = head < a.nh, is_k = !is_q && head < a.nh + pool.nkv;
+    f32x4 x[KD];
+#pragma unroll
+    for (int k = 0; k < KD; k++) x[k] = next[k];
+    if (head + (int)gridDim.y < heads) ask(head + gridDim.y);
+    if (is_q || is_k) {
+      const float *gain = is_q ? a.qn : a.kn;
+      if (gain) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KD; k++)
+          if (64 * k + 4 * l < hd)
+#pragma unroll
+            for (int j = 0; j < 4; j++) sum = __builtin_fmaf(x[k][j], x[k][j], sum);
+        const float inv = 1.0f / sqrtf(row_sum(sum) / (float)hd + a.eps);
+#pragma unroll
+        for (int k = 0; k < KD; k++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) x[k][j] = x[k][j] * gain[min(64 * k + 4 * l, hd - 4) + j] * inv;
       }
+      if (a.rd) {
+        f32x4 y[KD];  // the pairs' other halves
+        if (a.interleaved) {
+#pragma unroll
+          for (int k = 0; k < KD; k++) y[k] = f32x4{x[k][1], x[k][0], x[k][3], x[k][2]};
+        } else {
+#pragma unroll
+          for (int k = 0; k < KD; k++) *reinterpret_cast<f32x4 *>(&xs[t][64 * k + 4 * l]) = x[k];
+          __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int k = 0; k < KD; k++) {
+            const int d0 = 64 * k + 4 * l;
+            if (a.vec_rot) {
+              const int d = d0 < half ? d0 + half : d0 - half;
+              y[k] = *reinterpret_cast<const f32x4 *>(&xs[t][d0 < a.rd ? d : 0]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; j++) {
+                const int d = d0 + j < half ? d0 + j + half : d0 + j - half;
+                y[k][j] = xs[t][d0 + j < a.rd ? d : 0];
+              }
+            }
+          }
+          __builtin_amdgcn_wave_barrier();  // (the next head's rows are written behind these reads)
+        }
+#pragma unroll
+        for (int k = 0; k < KD; k++)
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            if (64 * k + 4 * l + j < a.rd) x[k][j] = __builtin_fmaf(x[k][j], c[k][j], y[k][j] * s[k][j]);
+      }
+      if (is_q) {
+        float *dst = a.qo + tok * a.ldo + (size_t)head * hd;
+        if (pos >= 0)
+#pragma unroll
+          for (int k = 0; k < KD; k++) {
+            const int d = 64 * k + 4 * l;
+            if (d >= hd) continue;
+            if (a.vec_out)
+              *reinterpret_cast<f32x4 *>(dst + d) = x[k];
+            else
+#pragma unroll
+              for (int j = 0; j < 4; j++) dst[d + j] = x[k][j];
+          }
+      } else if (page >= 0) {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        T *dst = pool.k + pool.base(page, head - a.nh);
+#pragma unroll
+        for (int k = 0; k < KD; k++) {
+          const int d = 64 * k + 4 * l;
+          if (d >= hd) continue;
+          t4 v;
+#pragma unroll
+          for (int j = 0; j < 4; j++) v[j] = (T)x[k][j];
+          *reinterpret_cast<t4 *>(dst + pool.k_at(slot, d)) = v;
+        }
+      }
+    } else {
+      // V: positions of a dim are next to each other, so the tokens change
+      // places through LDS
+#pragma unroll
+      for (int k = 0; k < KD; k++) *reinterpret_cast<f32x4 *>(&xs[t][64 * k + 4 * l]) = x[k];
+      __syncthreads();
+      const int h = head - a.nh - pool.nkv;
+      typedef T t8 __attribute__((ext_vector_type(8)));
+      for (int d = tid & (64 * KD - 1); d < hd; d += 64 * KD)
+        for (int r = tid / (64 * KD); r < kTok; r += kThreads / (64 * KD)) {
+          if (row_page[r] < 0) continue;
+          T *dst = pool.v + pool.base(row_page[r], h) + pool.v_at(row_slot[r], d);
+          const int lead = r - (row_slot[r] & 7);
+          if (whole[r]) {
+            t8 v;
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = (T)xs[r + j][d];
+            *reinterpret_cast<t8 *>(dst) = v;
+          } else if (lead < 0 || !whole[lead]) {
+            *dst = (T)xs[r][d];
+          }
+        }
+      __syncthreads();
     }
   }
 }
@@ -191,16 +293,27 @@ extern "C" syn_status_t syn_hip_kv_append(
     return SYN_ERR_INVALID_ARG;
   }
   SYN_TRY(ensure_init());
-  const AppendArgs a{d_q,      d_k,    d_v,    d_q_norm, d_k_norm, d_cos,       d_sin,
-                     d_pos,    d_seq,  d_index, d_table, d_q_out,  p->ldq,      p->ldk,
-                     p->ldv,   p->ldo, p->ld_table, (int)n_tokens, (int)nh, (int)p->n_seqs,
-                     (int)p->rotary_dim, p->interleaved, (int)p->n_positions, p->eps};
-  const dim3 grid((unsigned)cdiv(n_tokens, kTok), (unsigned)(nh + 2 * nkv));
-  const size_t shm = kTok * (hd + 4) * sizeof(float);
+  AppendArgs a{d_q,      d_k,    d_v,    d_q_norm, d_k_norm, d_cos,       d_sin,
+               d_pos,    d_seq,  d_index, d_table, d_q_out,  p->ldq,      p->ldk,
+               p->ldv,   p->ldo, p->ld_table, (int)n_tokens, (int)nh, (int)p->n_seqs,
+               (int)p->rotary_dim, p->interleaved, (int)p->n_positions, p->eps};
+  a.vec_in = aligned16(d_k) && aligned16(d_v) && p->ldk % 4 == 0 && p->ldv % 4 == 0 &&
+             (!nh || (aligned16(d_q) && p->ldq % 4 == 0));
+  a.vec_out = aligned16(d_q_out) && p->ldo % 4 == 0;
+  a.vec_rot = aligned16(d_cos) && aligned16(d_sin) && p->rotary_dim % 8 == 0;
+  // enough workgroups to fill the chip several times over, then heads in turn
+  const size_t tiles = cdiv(n_tokens, kTok), heads = nh + 2 * nkv;
+  const dim3 grid((unsigned)tiles, (unsigned)std::min(heads, std::max<size_t>(1, cdiv(2048, tiles))));
   return kv_dispatch(pages->dtype, [&](auto t) -> syn_status_t {
     using T = decltype(t);
-    hipLaunchKernelGGL(k_kv_append<T>, grid, dim3(kThreads), shm, pick_stream(stream), a,
-                       kv_pool<T>(*pages, p->layer));
+    const KvPool<T> pool = kv_pool<T>(*pages, p->layer);
+    hipStream_t s = pick_stream(stream);
+    if (hd <= 64)
+      hipLaunchKernelGGL((k_kv_append<T, 1>), grid, dim3(kThreads), 0, s, a, pool);
+    else if (hd <= 128)
+      hipLaunchKernelGGL((k_kv_append<T, 2>), grid, dim3(kThreads), 0, s, a, pool);
+    else
+      hipLaunchKernelGGL((k_kv_append<T, 4>), grid, dim3(kThreads), 0, s, a, pool);
     SYN_LAUNCH_CHECK();
     return SYN_OK;
   });

@@ -97,6 +97,12 @@ class BeamSelect(C.Structure):
                 ("ld_logits", C.c_size_t)]
 
 
+class BeamSearch(C.Structure):
+    """syn_hip_beam_search"""
+    _fields_ = [("n_beams", C.c_uint32), ("eos", C.c_int32), ("kv_dtype", C.c_int32),
+                ("length_penalty", C.c_float)]
+
+
 SIGNATURES = {
     "syn_quantize_per_channel_int8": (ST, [P, SZ, SZ, P, P]),
     "syn_qgemm_int8": (ST, [SZ, SZ, SZ, P, SZ, P, SZ, P, SZ, P, P]),
@@ -157,6 +163,7 @@ SIGNATURES = {
     "syn_hip_qlm_set_options": (ST, [P, C.c_int, C.c_int]),
     "syn_hip_qlm_set_sampler": (ST, [P, C.POINTER(SamplerParams), C.c_uint64]),
     "syn_hip_sample": (ST, [P, SZ, P, SZ, C.POINTER(SamplerParams), C.c_float, P, P, P]),
+    "syn_hip_klm_generate_beams": (ST, [P, P, SZ, SZ, C.POINTER(BeamSearch), P, P, P]),
     "syn_hip_kv_append": (ST, [C.POINTER(KvPages), C.POINTER(KvAppend), SZ] + [P] * 13),
     "syn_hip_prefix_attention_workspace": (ST, [C.POINTER(KvPages), C.POINTER(PrefixAttention),
                                                 C.POINTER(SZ)]),
@@ -778,6 +785,18 @@ class KQuantCausalLM:
                                                      draft_layers, ptr(toks), ptr(margins)),
               "klm_generate_speculative")
         return toks, margins
+
+    def generate_beams(self, prompt, max_new: int, n_beams: int, eos: int = -1, kv_dtype: int = KV_F32,
+                       length_penalty: float = 0.0):
+        """Beam search: (tokens [n_beams, max_new], lengths, scores), best first."""
+        prompt = np.ascontiguousarray(prompt, np.uint32)
+        toks = np.zeros((n_beams, max_new), np.uint32)
+        lens, scores = np.zeros(n_beams, np.uint32), np.zeros(n_beams, np.float32)
+        p = BeamSearch(n_beams, eos, kv_dtype, length_penalty)
+        check(lib().syn_hip_klm_generate_beams(self.h, ptr(prompt), prompt.size, max_new, C.byref(p),
+                                               ptr(toks), ptr(lens), ptr(scores)),
+              "klm_generate_beams")
+        return toks, lens, scores
 
     def time(self, prompt, steps: int):
         prompt = np.ascontiguousarray(prompt, np.uint32)
