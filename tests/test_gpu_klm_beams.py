@@ -73,7 +73,7 @@ def search(o, prompt, max_new, W, eos):
             x = logp(o.prefill(np.concatenate([prompt, np.uint32(toks)])))
             cand += [(s + x[t], b, int(t)) for t in np.argsort(-x, kind="stable")[:W + 1]]
         cand.sort(key=lambda c: (-c[0], c[1], c[2]))
-        close = min([close] + [cand[i][0] - cand[i + 1][0] for i in range(W)])
+        close = min([close] + [cand[i][0] - cand[i + 1][0] for i in range(min(W, len(cand) - 1))])
         beams = [(s, beams[b][1] + [t], beams[b][2] or t == eos) for s, b, t in cand[:W]]
     return beams, close
 
@@ -250,3 +250,28 @@ def test_steps_by_hand(dtype):
             assert np.array_equal(token.download((rows,), np.int32)[s], t)
         scores = new
         mine = [mine[r // W * W + par[r]] for r in range(rows)]
+
+
+@pytest.mark.parametrize("W,plen,max_new,eos", [(4, 21, 20, -1), (3, 1, 18, 7), (6, 40, 12, -1), (2, 17, 30, 11)])
+def test_beam_search_over_the_decoders_own_logits(W, plen, max_new, eos):
+    """The same prefill, and the decoder's own single steps: both sides sum in
+    f32 in different orders (512 terms: 3e-5 relative, logits up to about ten),
+    so choices more than 1e-3 apart are the same."""
+    _, g = build()
+
+    class Own:
+        def prefill(self, ids):
+            lg = g.prefill(ids[:plen])
+            for t in ids[plen:]:
+                lg = g.forward_one(int(t))
+            return lg
+
+    prompt = O.token_ids(plen, 0x5EED0000 + 77 + plen, TINY["vocab"])
+    beams, close = search(Own(), prompt, max_new, W, eos)
+    toks, lens, scores = g.generate_beams(prompt, max_new, W, eos)
+    best = sorted(beams, key=lambda b: -b[0])
+    assert abs(best[0][0] - scores[0]) <= 1e-3 or close < 2e-3
+    if close >= 2e-3:
+        for r, (s, t, fin) in enumerate(best):
+            n = t.index(eos) + 1 if fin else len(t)
+            assert toks[r, :lens[r]].tolist() == t[:n] and abs(s - scores[r]) <= 1e-3
