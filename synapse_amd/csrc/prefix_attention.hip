@@ -503,21 +503,23 @@ template <class T, int NC, bool FULL> struct Rows {
       const uint32_t here = ok >> (4 * mine) & 15;
       const bool on = KW == 1 || kt < r.to;
       V kf[2 * NC], vf[DT];
+      const uint8_t *f = ring + (get * KW + mine) * kTileBytes;
+      auto frag = [&](int j) {
+        if constexpr (sizeof(V) == 16) {
+          return reinterpret_cast<const V *>(f)[j * 64 + lane];
+        } else {  // two halves of 16 bytes a lane
+          const f32x4 *h = reinterpret_cast<const f32x4 *>(f) + j * 128 + lane;
+          return V{h[0], h[64]};
+        }
+      };
       if (on) {
-        const uint8_t *f = ring + (get * KW + mine) * kTileBytes;
-        auto frag = [&](int j) {
-          if constexpr (sizeof(V) == 16) {
-            return reinterpret_cast<const V *>(f)[j * 64 + lane];
-          } else {  // two halves of 16 bytes a lane
-            const f32x4 *h = reinterpret_cast<const f32x4 *>(f) + j * 128 + lane;
-            return V{h[0], h[64]};
-          }
-        };
 #pragma unroll
         for (int j = 0; j < 2 * NC; j++) kf[j] = frag(j);
+        // all of the tile is asked for before the first product waits (V of an
+        // f32 pool after it: two workgroups a CU need the registers)
+        if constexpr (sizeof(V) == 16)
 #pragma unroll
-        for (int j = 0; j < DT; j++) vf[j] = frag(2 * NC + j);
-        // all of the tile is asked for before the first product waits
+          for (int j = 0; j < DT; j++) vf[j] = frag(2 * NC + j);
         __builtin_amdgcn_sched_barrier(0);
       }
       ok >>= 8;
@@ -530,6 +532,9 @@ template <class T, int NC, bool FULL> struct Rows {
       if (on) {
         f32x4 s[2];
         scores(kf, s);
+        if constexpr (sizeof(V) != 16)
+#pragma unroll
+          for (int j = 0; j < DT; j++) vf[j] = frag(2 * NC + j);
         weigh(s, vf, kt, r.to, here);
       }
       get = get + 1 == S ? 0 : get + 1;
@@ -586,13 +591,13 @@ __device__ __forceinline__ int clamped(const int32_t *len, int i, int most) {
 }
 
 // workgroups of a CU that share its registers
-template <class T, int NC> constexpr int kResident = NC * sizeof(T) <= 8 ? 2 : 1;
+template <class T, int NC, bool FULL> constexpr int kResident = NC == 8 || (NC * sizeof(T) == 16 && !FULL) ? 1 : 2;
 
 // Joined: a workgroup has both runs of a sequence's rows whole.  Else the
 // first workgroups have the parts of the prefixes, the others those of the
 // suffixes.
 template <class T, int NC, bool FULL>
-__global__ void __launch_bounds__(64 * kWaves, (kResident<T, NC>)) k_attend(AttnArgs a, KvPool<T> pool) {
+__global__ void __launch_bounds__(64 * kWaves, (kResident<T, NC, FULL>)) k_attend(AttnArgs a, KvPool<T> pool) {
   using W = Rows<T, NC, FULL>;
   __shared__ __align__(16) uint8_t lds[W::kLdsBytes];
   __shared__ float ml[kWaves * 16 * 2];
@@ -761,11 +766,19 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_prefix_attention_params
   const int hd = (int)pg.head_dim, nkv = (int)pg.n_kv_heads, rep = (int)p.n_heads / nkv;
   w.nc = hd <= 64 ? 2 : (hd <= 128 ? 4 : 8);
   w.rows = (size_t)p.n_groups * p.group_size * p.n_heads;
-  // two tiles of rows need a ring of four tiles of positions
+  // Two tiles of rows need a ring of four tiles of positions; where it holds
+  // two, their blocks read K and V once each, the second time from L2.
   const bool small = w.nc * (pg.dtype == SYN_HIP_KV_F32 ? 2 : 1) <= 4;
-  auto tiles = [&](size_t rows) { return rows <= 16 ? 1 : (rows <= 32 && small ? 2 : 4); };
+  auto tiles = [&](size_t rows) { return rows <= 16 ? 1 : (rows <= 32 ? (small ? 2 : 1) : 4); };
   const size_t step = kTile * kWaves, seqs = (size_t)p.n_groups * p.group_size;
-  w.joined = (size_t)p.max_prefix + p.max_suffix <= 4 * step;
+  // One launch, each sequence's rows whole, where a second launch would cost
+  // more than the prefix read again for every sequence (from L2): 24 heads of
+  // 128, 8 sequences, f16: 900 positions 11.2 us against 12.2 in parts, 1600
+  // 14.7 against 12.9; 128 sequences of 900, 32.6 against 31.0.  An f32 tile has
+  // twice the bytes and four times the matrix instructions' time: 500 positions
+  // 17.9 us, 900 in parts 12.8.
+  const size_t whole = pg.dtype == SYN_HIP_KV_F32 ? 2 : (seqs * nkv <= 512 ? 8 : 4);
+  w.joined = (size_t)p.max_prefix + p.max_suffix <= whole * step;
   w.prw = tiles((size_t)p.group_size * rep);
   w.srw = w.joined ? 1 : tiles(rep);
   const size_t sblocks = cdiv(rep, 16 * w.srw), sunits = seqs * nkv;
@@ -774,11 +787,10 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_prefix_attention_params
     return w;
   }
   // Parts of about equal work for as many workgroups as the chip holds at
-  // once: by LDS four a CU, two, or one.  (512 workgroups of 64 dims in 16 bits,
+  // once, four a CU, two, or one.  (512 workgroups of 64 dims in 16 bits,
   // 48 sequences of 1500 positions over a shared 8200: 45 us, 1024: 40; of 128
   // dims, 64 sequences over four prefixes of 32768: 110 and 127.)
-  const int tile_bytes = w.nc * (pg.dtype == SYN_HIP_KV_F32 ? 8192 : 4096);
-  const size_t want = tile_bytes <= 8192 ? 1024 : (tile_bytes <= 16384 ? 512 : 256);
+  const size_t want = w.nc == 8 ? 256 : (w.nc == 4 || pg.dtype == SYN_HIP_KV_F32 ? 512 : 1024);
   const size_t pblocks = cdiv((size_t)p.group_size * rep, 16 * w.prw), punits = (size_t)p.n_groups * nkv;
   const size_t psteps = cdiv(p.max_prefix, step), ssteps = cdiv(p.max_suffix, step);
   const size_t total = punits * pblocks * psteps + sunits * sblocks * ssteps;
