@@ -20,7 +20,7 @@ struct AppendArgs {
   size_t ldq, ldk, ldv, ldo, ld_table;
   int n_tokens, nh, n_seqs, rd, interleaved, n_pos;
   float eps;
-  bool vec_in, vec_out, vec_rot;  // 16-byte rows of q, k, v; of q_out; of the tables, half of rd
+  bool vec_in, vec_out, vec_rot, vec_gain;  // 16-byte rows of q, k, v; of q_out; of the tables (half of rd too); gains
 };
 
 // four consecutive floats
@@ -108,15 +108,17 @@ __global__ void __launch_bounds__(kThreads) k_kv_append(AppendArgs a, KvPool<T> 
       }
     }
   }
-  __syncthreads();
   // 8 tokens that fill an aligned group of 8 positions are written together
-  if (tid < kTok) {
+  const int last = blockIdx.y + (heads - 1 - (int)blockIdx.y) / (int)gridDim.y * (int)gridDim.y;
+  const bool has_v = last >= a.nh + pool.nkv;
+  if (has_v) __syncthreads();
+  if (has_v && tid < kTok) {
     bool w = tid + 8 <= nt && row_page[tid] >= 0 && (row_slot[tid] & 7) == 0;
     for (int j = 1; w && j < 8; j++)
       w = row_page[tid + j] == row_page[tid] && row_slot[tid + j] == row_slot[tid] + j;
     whole[tid] = w;
   }
-  __syncthreads();
+  if (has_v) __syncthreads();
 
   for (int head = blockIdx.y; head < heads; head += gridDim.y) {
     const bool is_q = head < a.nh, is_k = !is_q && head < a.nh + pool.nkv;
@@ -127,6 +129,9 @@ __global__ void __launch_bounds__(kThreads) k_kv_append(AppendArgs a, KvPool<T> 
     if (is_q || is_k) {
       const float *gain = is_q ? a.qn : a.kn;
       if (gain) {
+        f32x4 w[KD];
+#pragma unroll
+        for (int k = 0; k < KD; k++) w[k] = load4(gain + min(64 * k + 4 * l, hd - 4), a.vec_gain);
         float sum = 0.0f;
 #pragma unroll
         for (int k = 0; k < KD; k++)
@@ -137,7 +142,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_append(AppendArgs a, KvPool<T> 
 #pragma unroll
         for (int k = 0; k < KD; k++)
 #pragma unroll
-          for (int j = 0; j < 4; j++) x[k][j] = x[k][j] * gain[min(64 * k + 4 * l, hd - 4) + j] * inv;
+          for (int j = 0; j < 4; j++) x[k][j] = x[k][j] * w[k][j] * inv;
       }
       if (a.rd) {
         f32x4 y[KD];  // the pairs' other halves
@@ -301,9 +306,12 @@ extern "C" syn_status_t syn_hip_kv_append(
              (!nh || (aligned16(d_q) && p->ldq % 4 == 0));
   a.vec_out = aligned16(d_q_out) && p->ldo % 4 == 0;
   a.vec_rot = aligned16(d_cos) && aligned16(d_sin) && p->rotary_dim % 8 == 0;
-  // enough workgroups to fill the chip several times over, then heads in turn
+  a.vec_gain = aligned16(d_q_norm) && aligned16(d_k_norm);
+  // Workgroups enough to fill the chip, then heads in turn, whose angles are
+  // there already (8192 tokens of 48 heads: 97 us with 1024 workgroups, 95 with
+  // 2048, 107 with 512 and 4096; 517: 9.9, 11.3, 10.3, 11.2).
   const size_t tiles = cdiv(n_tokens, kTok), heads = nh + 2 * nkv;
-  const dim3 grid((unsigned)tiles, (unsigned)std::min(heads, std::max<size_t>(1, cdiv(2048, tiles))));
+  const dim3 grid((unsigned)tiles, (unsigned)std::min(heads, std::max<size_t>(1, cdiv(1024, tiles))));
   return kv_dispatch(pages->dtype, [&](auto t) -> syn_status_t {
     using T = decltype(t);
     const KvPool<T> pool = kv_pool<T>(*pages, p->layer);

@@ -587,7 +587,8 @@ template <class T, int NC, bool FULL> struct Rows {
 };
 
 __device__ __forceinline__ int clamped(const int32_t *len, int i, int most) {
-  return most ? max(0, min(len[i], most)) : 0;
+  const auto *t = (const __attribute__((address_space(4))) int32_t *)(uintptr_t)len;  // a scalar load
+  return most ? max(0, min(t[i], most)) : 0;
 }
 
 // workgroups of a CU that share its registers
@@ -676,24 +677,25 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, NC, FULL>)) k_atten
   w.finish(a, pool.hd, seq0, head, row0, rows, RW, at, reinterpret_cast<float *>(lds), ml);
 }
 
-// One workgroup a query row: wave w takes parts w, w + 4, ..., eight in flight
-// and the first eight before their weights are known; the waves' sums are
-// joined in order.
+// One workgroup a query row: its lanes hold four dims of several parts at
+// once (LANES to a part), the first of them asked for before their weights
+// are known; the sums are joined in a fixed order.
+template <int LANES>
 __global__ void __launch_bounds__(256) k_join_parts(AttnArgs a, int hd) {
-  __shared__ float xs[3][kKvMaxHeadDim];
-  constexpr int kU = 8;
+  __shared__ float xs[4][4 * LANES];
+  constexpr int kSub = 64 / LANES, kU = 4, kStep = 4 * kSub;  // parts of a wave, and of all four, at once
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int sub = wave * kSub + lane / LANES, c4 = 4 * (lane % LANES);
   const size_t row = blockIdx.x;
   const int n = a.npp + a.nsp;
-  const float *ml = a.pml + row * n * 2, *po = a.po + row * n * hd;
-  const int d0 = min(4 * lane, hd - 4);
+  const float *ml = a.pml + row * n * 2, *po = a.po + row * n * hd + min(c4, hd - 4);
   f32x4 x{0, 0, 0, 0}, y[kU];
   auto ask = [&](int i0) {
 #pragma unroll
     for (int u = 0; u < kU; u++)
-      y[u] = *reinterpret_cast<const f32x4 *>(po + (size_t)min(i0 + 4 * u, n - 1) * hd + d0);
+      y[u] = *reinterpret_cast<const f32x4 *>(po + (size_t)min(i0 + u * kStep + sub, n - 1) * hd);
   };
-  ask(wave);
+  ask(0);
   float top = kNegInf;
   for (int i = lane; i < n; i += 64) top = fmaxf(top, ml[2 * i]);
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
@@ -704,29 +706,30 @@ __global__ void __launch_bounds__(256) k_join_parts(AttnArgs a, int hd) {
     const float f = lp == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml[2 * i] - top);
     l += lp * f;
     const int most = min(64, n - i0);
-    for (int k = wave; k < most; k += 4 * kU) {
-      if (i0 + k != wave) ask(i0 + k);
+    for (int k = 0; k < most; k += kU * kStep) {
+      if (i0 + k) ask(i0 + k);
 #pragma unroll
       for (int u = 0; u < kU; u++) {
-        const float fu = __shfl(f, (k + 4 * u) & 63);
+        const int at = k + u * kStep + sub;
+        const float fu = __shfl(f, at & 63);
         // (a part with no position has left its row unwritten)
-        if (k + 4 * u < most && fu != 0.0f)
+        if (at < most && fu != 0.0f)
 #pragma unroll
           for (int c = 0; c < 4; c++) x[c] = __builtin_fmaf(y[u][c], fu, x[c]);
       }
     }
   }
   for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
-  if (wave > 0 && 4 * lane < hd) *reinterpret_cast<f32x4 *>(&xs[wave - 1][4 * lane]) = x;
-  __syncthreads();
-  if (wave == 0 && 4 * lane < hd) {
-    const size_t seq = row / a.nh, head = row - seq * a.nh;
-    float *out = a.out + seq * a.ldo + head * hd + 4 * lane;
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-      const float v = x[c] + xs[0][4 * lane + c] + xs[1][4 * lane + c] + xs[2][4 * lane + c];
-      out[c] = l == 0.0f ? 0.0f : v / l;
-    }
+  for (int o = LANES; o < 64; o *= 2)
+#pragma unroll
+    for (int c = 0; c < 4; c++) x[c] += __shfl_xor(x[c], o);
+  if (lane < LANES) *reinterpret_cast<f32x4 *>(&xs[wave][c4]) = x;
+  __syncthreads();
+  if (tid < hd) {
+    const size_t seq = row / a.nh, head = row - seq * a.nh;
+    const float v = (xs[0][tid] + xs[1][tid]) + (xs[2][tid] + xs[3][tid]);
+    a.out[seq * a.ldo + head * hd + tid] = l == 0.0f ? 0.0f : v / l;
   }
 }
 
@@ -820,7 +823,13 @@ syn_status_t launch(const Plan &w, const AttnArgs &a, const KvPool<T> &pool, hip
     hipLaunchKernelGGL((k_attend<T, NC, false>), grid, block, 0, s, a, pool);
   SYN_LAUNCH_CHECK();
   if (w.joined) return SYN_OK;
-  hipLaunchKernelGGL(k_join_parts, dim3((unsigned)w.rows), dim3(256), 0, s, a, pool.hd);
+  const dim3 rows((unsigned)w.rows);
+  if (NC == 2)
+    hipLaunchKernelGGL(k_join_parts<16>, rows, dim3(256), 0, s, a, pool.hd);
+  else if (NC == 4)
+    hipLaunchKernelGGL(k_join_parts<32>, rows, dim3(256), 0, s, a, pool.hd);
+  else
+    hipLaunchKernelGGL(k_join_parts<64>, rows, dim3(256), 0, s, a, pool.hd);
   SYN_LAUNCH_CHECK();
   return SYN_OK;
 }
