@@ -700,7 +700,9 @@ struct syn_hip_klm_s {
     for (size_t i = 0; i < W; i++) {
       const uint32_t *t = hist.data() + i * max_new;
       len[i] = bs.eos < 0 ? done : std::min<size_t>(done, std::find(t, t + done, (uint32_t)bs.eos) - t + 1);
-      rank[i] = (double)score[i] / std::pow((double)len[i], (double)bs.length_penalty);
+      const double by = std::pow((double)len[i], (double)bs.length_penalty);
+      rank[i] = std::isfinite(score[i]) ? (double)score[i] / by : (double)score[i];  // (no -inf / inf)
+      if (std::isnan(rank[i])) rank[i] = 0.0;                                       // 0 / 0
       order[i] = i;
     }
     std::stable_sort(order.begin(), order.end(), [&](size_t i, size_t j) { return rank[i] > rank[j]; });
@@ -826,6 +828,7 @@ syn_status_t syn_hip_klm_create(const syn_hip_klm_config *cfg, syn_hip_klm_t **o
 
 syn_status_t syn_hip_klm_set_embed(syn_hip_klm_t *m, const float *embed) {
   if (!m || !embed) return SYN_ERR_NULL_PTR;
+  m->beams.reset();  // its captured step holds the buffers' addresses
   SYN_TRY(m->embed.alloc(m->vocab * m->h * 4));
   SYN_HIP(hipMemcpy(m->embed.p, embed, m->vocab * m->h * 4, hipMemcpyHostToDevice));
   m->have_embed = true;
@@ -836,11 +839,13 @@ syn_status_t syn_hip_klm_set_proj(syn_hip_klm_t *m, uint32_t layer, int proj,
                                   const uint8_t *gguf_bytes) {
   if (!m || !gguf_bytes) return SYN_ERR_NULL_PTR;
   if (layer >= m->L || proj < 0 || proj > 6) return SYN_ERR_INVALID_ARG;
+  m->beams.reset();
   return m->set_proj(layer, proj, gguf_bytes);
 }
 
 syn_status_t syn_hip_klm_set_lm_head(syn_hip_klm_t *m, const uint8_t *gguf_bytes) {
   if (!m || !gguf_bytes) return SYN_ERR_NULL_PTR;
+  m->beams.reset();
   SYN_TRY(m->lm_head.upload(m->c.fmt_lm_head, gguf_bytes, m->vocab, m->h));
   m->have_lm = true;
   return SYN_OK;
@@ -1029,6 +1034,10 @@ syn_status_t syn_hip_klm_generate_beams(syn_hip_klm_t *m, const uint32_t *prompt
   }
   if (p->kv_dtype != SYN_HIP_KV_F32 && p->kv_dtype != SYN_HIP_KV_F16 && p->kv_dtype != SYN_HIP_KV_BF16) {
     set_error("beam search: unknown cache dtype");
+    return SYN_ERR_INVALID_ARG;
+  }
+  if (!std::isfinite(p->length_penalty)) {
+    set_error("beam search: length_penalty is not finite");
     return SYN_ERR_INVALID_ARG;
   }
   if (m->hd % 8 || m->hd > kKvMaxHeadDim) {

@@ -140,14 +140,38 @@ def test_length_penalty_orders_the_beams():
         assert (np.diff(rank) <= 1e-12).all()
 
 
+def test_extreme_length_penalties_keep_an_order():
+    _, g = build()
+    prompt = O.token_ids(12, 9, TINY["vocab"])
+    plain = g.generate_beams(prompt, 15, 5, eos=3)
+    for alpha in (-3e38, 3e38):
+        toks, lens, scores = g.generate_beams(prompt, 15, 5, eos=3, length_penalty=alpha)
+        assert sorted(scores.tolist()) == sorted(plain[2].tolist())
+
+
+def test_weights_set_again_between_searches():
+    """the captured step does not outlive the buffers that it reads"""
+    _, g = build()
+    _, want = build(head_std=0.3)
+    prompt = O.token_ids(20, 4, TINY["vocab"])
+    g.generate_beams(prompt, 9, 4)
+    n = TINY["vocab"] * TINY["hidden"]
+    w = O.normal(n, 0x5EED0000 + 1 + 8 * TINY["n_layers"], 0.3).reshape(TINY["vocab"], TINY["hidden"])
+    g.set_lm_head(hip.kquant_encode(hip.FMT_Q6_K, w))
+    g.finalize()
+    for a, b in zip(g.generate_beams(prompt, 9, 4), want.generate_beams(prompt, 9, 4)):
+        assert np.array_equal(a, b)
+
+
 @pytest.mark.parametrize("kw", [dict(n_beams=0), dict(n_beams=65), dict(eos=301), dict(kv_dtype=3),
-                                dict(max_new=90), dict(plen=0), dict(plen=97)])
+                                dict(max_new=90), dict(plen=0), dict(plen=97),
+                                dict(penalty=float("nan")), dict(penalty=float("inf"))])
 def test_refusals(kw):
     _, g = build()
-    d = dict(n_beams=4, eos=-1, kv_dtype=0, max_new=8, plen=10)
+    d = dict(n_beams=4, eos=-1, kv_dtype=0, max_new=8, plen=10, penalty=0.0)
     d.update(kw)
     prompt = np.zeros(max(d["plen"], 1), np.uint32)
-    p = hip.BeamSearch(d["n_beams"], d["eos"], d["kv_dtype"], 0.0)
+    p = hip.BeamSearch(d["n_beams"], d["eos"], d["kv_dtype"], d["penalty"])
     out = np.zeros((65, 96), np.uint32)
     assert hip.lib().syn_hip_klm_generate_beams(g.h, hip.ptr(prompt), d["plen"], d["max_new"],
                                                 C.byref(p), hip.ptr(out), None, None) == 2
