@@ -653,7 +653,7 @@ typedef struct {
  * d_index[t].  A token with d_pos outside [0, n_positions) is skipped
  * altogether; one whose d_index is negative or past the table, or whose page
  * is outside the pool, is rotated but not stored (padding).  Tokens stored at
- * the same place leave either's values there.  n_heads = 0: no queries (d_q
+ * the same place leave either's values there.  At most 2^28 - 16 tokens.  n_heads = 0: no queries (d_q
  * and d_q_out unused).  d_q_out may be d_q with ldo == ldq. */
 typedef struct {
   uint32_t layer, n_heads, n_seqs, rotary_dim;
@@ -682,7 +682,11 @@ syn_status_t syn_hip_kv_append(const syn_hip_kv_pages *pages, const syn_hip_kv_a
  * widths decide the split of the work, so a captured call keeps them);
  * a negative length is 0.  Positions in pages outside the pool are left out;
  * a sequence with no position gives zeros.  Scores, softmax and sums are f32;
- * 16-bit pools are read as stored.  The workspace holds the parts of a split
+ * 16-bit pools are read as stored.  d_q and the keys and values of the
+ * positions that count are finite (an infinity among them may give NaN where
+ * the formula has a limit); what lies behind a length or in slots that no
+ * length reaches may hold anything.  d_out is apart from d_q.  At most 65535
+ * sequences, and sequences * n_heads below 2^24.  The workspace holds the parts of a split
  * prefix or suffix (size from syn_hip_prefix_attention_workspace, which may
  * be 0; 16-byte aligned). */
 typedef struct {
@@ -714,7 +718,9 @@ syn_status_t syn_hip_prefix_attention(const syn_hip_kv_pages *pages,
  * (nullable) whether the parent was finished or the token is eos (-1: none).
  * 1 <= n_beams <= 64, 1 <= n_select <= 128, n_select <= n_beams * vocab;
  * d_score may be d_scores and d_finished_out d_finished when n_select ==
- * n_beams.  The workspace (16-byte aligned) is needed by every call. */
+ * n_beams.  n_groups * n_beams is at most 65535, and n_beams * n_select *
+ * ceil(vocab / 2048) below 2^31.  The workspace (16-byte aligned) is needed by
+ * every call. */
 typedef struct {
   uint32_t n_groups, n_beams, n_select;
   int32_t eos, pad;
@@ -730,7 +736,10 @@ syn_status_t syn_hip_beam_select(const syn_hip_beam_select_params *p, const floa
 /* States follow the chosen beams, in place: in each of n_buffers buffers
  * (buffer_stride bytes apart), row g * n_beams + b becomes what row
  * g * n_beams + d_parent[g * n_beams + b] was.  row_bytes of every row_stride
- * bytes are moved; a parent outside [0, n_beams) leaves its row as it is. */
+ * bytes are moved; a parent outside [0, n_beams) leaves its row as it is.
+ * 1 <= n_beams <= 64, n_groups * n_beams and n_buffers at most 65535; a row
+ * has fewer than 2^32 units of the 16, 4 or 1 bytes that d_rows, row_bytes and
+ * the strides are multiples of. */
 syn_status_t syn_hip_beam_reorder_rows(size_t n_groups, size_t n_beams, const int32_t *d_parent,
                                        void *d_rows, size_t row_bytes, size_t row_stride,
                                        size_t n_buffers, size_t buffer_stride, void *stream);
@@ -740,7 +749,10 @@ syn_status_t syn_hip_beam_reorder_rows(size_t n_groups, size_t n_beams, const in
  * A row takes its parent's entries for the pages that are full; the page that
  * is not is copied (positions up to the next multiple of 8) into the page
  * d_spare[row], which becomes the row's, and the row's own old one becomes its
- * spare.  The entries after it stay the row's.  So if every entry from column
+ * spare (nothing is copied from or into a page outside the pool, but the
+ * entries change places all the same).  A parent outside [0, n_beams) leaves
+ * its row as it is; the limits are those of the rows.  The entries after it
+ * stay the row's.  So if every entry from column
  * d_len[g] / page_size on and every spare name distinct pages that nothing
  * else refers to, that stays so, with no allocator and no count of references:
  * pages are filled by one row at a time and never written again once full. */

@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kMergeNT) k_beam_merge(SelectArgs a) {
   };
   if (K <= kMergeCap) {
     for (int k = tid; k < K + 4; k += kMergeNT) {
-      const Pick p = list[min(k, K - 1)];
+      const Pick p = list[max(min(k, K - 1), 0)];
       const uint64_t u = (uint64_t)__double_as_longlong(p.v);
       keys[k] = k < K ? (u >> 63 ? ~u : u | 1ull << 63) : 0;
       index[k] = ~((uint64_t)p.b << 32 | (uint32_t)p.t);
@@ -645,20 +645,20 @@ syn_status_t syn_hip_beam_reorder_rows(size_t n_groups, size_t n_beams, const in
     set_error("beam_reorder_rows: rows or buffers overlap");
     return SYN_ERR_SHAPE_MISMATCH;
   }
-  if (n_buffers > 65535u || row_bytes > (size_t)1 << 36) {
-    set_error("beam_reorder_rows: at most 65535 buffers of rows up to 64 GiB");
+  if (n_buffers > 65535u) {
+    set_error("beam_reorder_rows: at most 65535 buffers");
     return SYN_ERR_INVALID_ARG;
   }
   if (!n_groups || !row_bytes || !n_buffers) return SYN_OK;
   if (!d_parent || !d_rows) return SYN_ERR_NULL_PTR;
-  SYN_TRY(ensure_init());
   const size_t all = reinterpret_cast<uintptr_t>(d_rows) | row_bytes | row_stride |
                      (n_buffers > 1 ? buffer_stride : 0);
   const size_t unit = all % 16 == 0 ? 16 : (all % 4 == 0 ? 4 : 1), units = row_bytes / unit;
-  if (cdiv(units, 64) > 0x7fffffffu) {
+  if (cdiv(units, 64) > kMaxThreads / 64) {
     set_error("beam_reorder_rows: rows too long for their alignment");
     return SYN_ERR_INVALID_ARG;
   }
+  SYN_TRY(ensure_init());
   const dim3 grid((unsigned)cdiv(units, 64), (unsigned)n_groups, (unsigned)n_buffers);
   const size_t shm = n_beams * 64 * unit;
   hipStream_t s = pick_stream(stream);
@@ -682,7 +682,8 @@ syn_status_t syn_hip_beam_reorder_pages(const syn_hip_kv_pages *pages, size_t n_
                                         int32_t *d_spare, void *stream) {
   SYN_TRY(check_pages(pages, "beam_reorder_pages"));
   SYN_TRY(check_beams(n_groups, n_beams, "beam_reorder_pages"));
-  if ((uint64_t)pages->n_layers * pages->n_kv_heads > 0x7fffffffu || ld_table > 0x7fffffffu) {
+  if ((uint64_t)pages->n_layers * pages->n_kv_heads > kMaxThreads / 256 ||
+      cdiv(ld_table, 64) > kMaxThreads / 256) {
     set_error("beam_reorder_pages: too many layers, heads or table columns");
     return SYN_ERR_INVALID_ARG;
   }

@@ -280,7 +280,7 @@ extern "C" syn_status_t syn_hip_kv_append(
     set_error("kv_append: layer outside the pool, or rotary_dim not even and at most head_dim");
     return SYN_ERR_INVALID_ARG;
   }
-  if (n_tokens > 0x7fffffffu || p->n_seqs > 0x7fffffffu || p->n_positions > 0x7fffffffu ||
+  if (cdiv(n_tokens, kTok) > kMaxThreads / kThreads || p->n_seqs > 0x7fffffffu || p->n_positions > 0x7fffffffu ||
       nh + 2 * nkv > 65535u) {
     set_error("kv_append: too many tokens, sequences, positions or heads");
     return SYN_ERR_INVALID_ARG;

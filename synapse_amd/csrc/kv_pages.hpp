@@ -33,6 +33,7 @@ template <class T> struct KvPool {
 
 constexpr uint32_t kKvMaxHeadDim = 256;
 constexpr uint32_t kKvMaxPage = 1024;
+constexpr size_t kMaxThreads = 0xffffffffu;  // of a launch, in one dimension
 constexpr uint32_t kMaxBeams = 64;
 constexpr uint32_t kMaxSelect = 128;
 

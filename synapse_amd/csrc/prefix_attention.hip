@@ -734,29 +734,6 @@ __global__ void __launch_bounds__(256) k_join_parts(AttnArgs a, int hd) {
 }
 
 // ---------------------------------------------------------------- host
-syn_status_t check_attention(const syn_hip_kv_pages *pages,
-                             const syn_hip_prefix_attention_params *p) {
-  if (!p) return SYN_ERR_NULL_PTR;
-  SYN_TRY(check_pages(pages, "prefix_attention"));
-  const size_t hd = pages->head_dim, rows = (size_t)p->n_groups * p->group_size;
-  if (p->layer >= pages->n_layers || !p->n_heads || p->n_heads % pages->n_kv_heads ||
-      p->n_heads > 65535u) {
-    set_error("prefix_attention: layer outside the pool, or n_heads no multiple of n_kv_heads");
-    return SYN_ERR_INVALID_ARG;
-  }
-  if (rows > 65535u || p->max_prefix > 0x7fffff00u || p->max_suffix > 0x7fffff00u) {
-    set_error("prefix_attention: more than 65535 sequences or 2^31 positions");
-    return SYN_ERR_INVALID_ARG;
-  }
-  if (p->ldq < p->n_heads * hd || p->ldo < p->n_heads * hd ||
-      p->ld_prefix_table < cdiv(p->max_prefix, pages->page_size) ||
-      p->ld_table < cdiv(p->max_suffix, pages->page_size)) {
-    set_error("prefix_attention: rows or page tables shorter than the heads or the lengths");
-    return SYN_ERR_SHAPE_MISMATCH;
-  }
-  return SYN_OK;
-}
-
 struct Plan {
   bool joined;
   int nc, prw, srw;
@@ -814,6 +791,34 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_prefix_attention_params
   return w;
 }
 
+syn_status_t check_attention(const syn_hip_kv_pages *pages,
+                             const syn_hip_prefix_attention_params *p) {
+  if (!p) return SYN_ERR_NULL_PTR;
+  SYN_TRY(check_pages(pages, "prefix_attention"));
+  const size_t hd = pages->head_dim, rows = (size_t)p->n_groups * p->group_size;
+  if (p->layer >= pages->n_layers || !p->n_heads || p->n_heads % pages->n_kv_heads ||
+      p->n_heads > 65535u) {
+    set_error("prefix_attention: layer outside the pool, or n_heads no multiple of n_kv_heads");
+    return SYN_ERR_INVALID_ARG;
+  }
+  if (rows > 65535u || p->max_prefix > 0x7fffff00u || p->max_suffix > 0x7fffff00u) {
+    set_error("prefix_attention: more than 65535 sequences or 2^31 positions");
+    return SYN_ERR_INVALID_ARG;
+  }
+  if (p->ldq < p->n_heads * hd || p->ldo < p->n_heads * hd ||
+      p->ld_prefix_table < cdiv(p->max_prefix, pages->page_size) ||
+      p->ld_table < cdiv(p->max_suffix, pages->page_size)) {
+    set_error("prefix_attention: rows or page tables shorter than the heads or the lengths");
+    return SYN_ERR_SHAPE_MISMATCH;
+  }
+  const Plan w = make_plan(*pages, *p);
+  if (w.wgs > kMaxThreads / (64 * kWaves) || w.rows > kMaxThreads / 256) {
+    set_error("prefix_attention: more workgroups than a launch takes");
+    return SYN_ERR_INVALID_ARG;
+  }
+  return SYN_OK;
+}
+
 template <class T, int NC>
 syn_status_t launch(const Plan &w, const AttnArgs &a, const KvPool<T> &pool, hipStream_t s) {
   const dim3 grid((unsigned)w.wgs), block(64 * kWaves);
@@ -861,10 +866,6 @@ extern "C" syn_status_t syn_hip_prefix_attention(
     return SYN_ERR_NULL_PTR;
   const Plan w = make_plan(*pages, *p);
   const size_t need = w.po_bytes + w.pml_bytes;
-  if (w.wgs > 0x7fffffffu || w.rows > 0x7fffffffu) {
-    set_error("prefix_attention: more workgroups than a launch takes");
-    return SYN_ERR_INVALID_ARG;
-  }
   if (need && !d_workspace) return SYN_ERR_NULL_PTR;
   if (need && (!aligned16(d_workspace) || workspace_bytes < need)) {
     set_error("prefix_attention: workspace unaligned or too small");

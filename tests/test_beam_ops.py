@@ -48,7 +48,7 @@ def test_append_refuses_pages(kw, want):
     (dict(layer=2), ARG), (dict(rotary_dim=63), ARG), (dict(rotary_dim=66), ARG),
     (dict(ldq=255), SHAPE), (dict(ldo=255), SHAPE), (dict(ldk=127), SHAPE), (dict(ldv=127), SHAPE),
     (dict(n_heads=70000, ldq=1 << 30, ldo=1 << 30), ARG), (dict(n_seqs=1 << 31), ARG),
-    (dict(n_positions=1 << 31), ARG), (dict(n=1 << 31), ARG),
+    (dict(n_positions=1 << 31), ARG), (dict(n=1 << 31), ARG), (dict(n=(1 << 28) - 15), ARG),
     (dict(ptrs=dict(k=None)), NULL), (dict(ptrs=dict(v=None)), NULL), (dict(ptrs=dict(q=None)), NULL),
     (dict(ptrs=dict(out=None)), NULL), (dict(ptrs=dict(cos=None)), NULL),
     (dict(ptrs=dict(sin=None)), NULL), (dict(ptrs=dict(pos=None)), NULL),
@@ -93,6 +93,9 @@ def test_attention_refuses_pages(kw, want):
     (dict(ldo=255), SHAPE), (dict(ld_prefix_table=2), SHAPE), (dict(ld_table=1), SHAPE),
     (dict(n_groups=70000, group_size=1), ARG), (dict(max_prefix=0xffffffff), ARG),
     (dict(max_suffix=0xffffffff), ARG), (dict(ptrs=dict(q=None)), NULL),
+    # more threads than a launch holds: rows of the join, blocks of the attention
+    (dict(n_groups=65535, group_size=1, n_heads=258, ldq=1 << 16, ldo=1 << 16), ARG),
+    (dict(n_groups=1, group_size=65535, n_heads=512, ldq=1 << 16, ldo=1 << 16), ARG),
     (dict(ptrs=dict(out=None)), NULL), (dict(ptrs=dict(pt=None)), NULL),
     (dict(ptrs=dict(pl=None)), NULL), (dict(ptrs=dict(t=None)), NULL),
     (dict(ptrs=dict(l=None)), NULL), (dict(n_groups=0), OK), (dict(group_size=0), OK)])
@@ -157,6 +160,7 @@ def test_select_null_struct():
     ((40000, 2, FAKE, FAKE, 64, 64, 1, 0), ARG), ((2, 4, FAKE, FAKE, 64, 60, 1, 0), SHAPE),
     ((2, 4, FAKE, FAKE, 64, 64, 2, 511), SHAPE), ((2, 4, FAKE, FAKE, 64, 64, 70000, 512), ARG),
     ((2, 4, None, FAKE, 64, 64, 1, 0), NULL), ((2, 4, FAKE, None, 64, 64, 1, 0), NULL),
+    ((1, 2, FAKE, FAKE, 1 << 36, 1 << 36, 1, 0), ARG), ((1, 2, FAKE, FAKE + 1, 1 << 32, 1 << 32, 1, 0), ARG),
     ((0, 4, None, None, 64, 64, 1, 0), OK), ((2, 4, None, None, 0, 64, 1, 0), OK),
     ((2, 4, None, None, 64, 64, 0, 0), OK)])
 def test_reorder_rows_refuses(args, want):
@@ -175,6 +179,12 @@ def test_reorder_pages_refuses_pages(kw, want):
     ((70000, 1, FAKE, FAKE, FAKE, 4, FAKE), ARG), ((1, 2, None, FAKE, FAKE, 4, FAKE), NULL),
     ((1, 2, FAKE, None, FAKE, 4, FAKE), NULL), ((1, 2, FAKE, FAKE, None, 4, FAKE), NULL),
     ((1, 2, FAKE, FAKE, FAKE, 4, None), NULL), ((1, 2, FAKE, FAKE, FAKE, 1 << 31, FAKE), ARG),
+    ((1, 2, FAKE, FAKE, FAKE, 1 << 30, FAKE), ARG),
     ((0, 2, None, None, None, 4, None), OK)])
 def test_reorder_pages_refuses(args, want):
     assert hip.lib().syn_hip_beam_reorder_pages(C.byref(pages()), *args, None) == want
+
+
+def test_reorder_pages_refuses_more_layers_than_a_launch_holds():
+    pg = pages(n_layers=1 << 24)
+    assert hip.lib().syn_hip_beam_reorder_pages(C.byref(pg), 1, 2, FAKE, FAKE, FAKE, 4, FAKE, None) == ARG

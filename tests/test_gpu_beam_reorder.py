@@ -100,6 +100,33 @@ def test_pages(dtype, page, kv, hd, layers, groups, w, cols, held):
         assert np.array_equal(k, pool.k) and np.array_equal(v, pool.v)
 
 
+def test_pages_past_32_bits():
+    """a pool of over 2^32 elements: the last pages"""
+    page, kv, hd, w = 512, 8, 128, 3
+    far = 2 * w
+    pages = (1 << 32) // (page * kv * hd) + far
+    step = page * kv * hd * 2
+    dk, dv = hip.DeviceBuffer(pages * step), hip.DeviceBuffer(pages * step)
+    near = R.Pool("f16", page, far, 1, kv, hd, rng=np.random.default_rng(9))
+    first = pages - far
+    for d, x in ((dk, near.pack_k(near.k)), (dv, near.pack_v(near.v))):
+        hip.check(hip.lib().syn_hip_memcpy_h2d(d.ptr + first * step, hip.ptr(x), x.nbytes))
+    desc = hip.KvPages(hip.KV_F16, page, pages, 1, kv, hd, dk.ptr, dv.ptr)
+    table, spare = R.i32(np.arange(w)[:, None]), R.i32(w + np.arange(w))
+    parent, held = R.i32([2, 0, 0]), R.i32([301])
+    d = [R.dev(a) for a in (parent, held, table + first, spare + first)]
+    hip.check(hip.lib().syn_hip_beam_reorder_pages(C.byref(desc), 1, w, d[0].ptr, d[1].ptr, d[2].ptr, 1,
+                                                   d[3].ptr, None))
+    R.sync()
+    pages_step(near, parent, held, table, spare, w)
+    assert np.array_equal(d[2].download(table.shape, np.int32), table + first)
+    assert np.array_equal(d[3].download(spare.shape, np.int32), spare + first)
+    for b, want in ((dk, near.pack_k(near.k)), (dv, near.pack_v(near.v))):
+        got = np.empty_like(want)
+        hip.check(hip.lib().syn_hip_memcpy_d2h(hip.ptr(got), b.ptr + first * step, got.nbytes))
+        assert np.array_equal(got, want)
+
+
 def test_pages_outside_the_pool():
     rng = np.random.default_rng(5)
     pool = R.Pool("f16", 16, 10, 1, 1, 16, rng=rng)

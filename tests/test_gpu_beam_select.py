@@ -129,6 +129,16 @@ def test_first_step_scores_and_dead_beams():
     c.check()
 
 
+@pytest.mark.parametrize("w,n,vocab", [(64, 128, 3), (2, 5, 9000)])
+def test_no_live_beam_in_a_group(w, n, vocab):
+    """the first continuations in order, all of -inf"""
+    c = Case(10, 2, w, n, vocab, finished=False)
+    c.scores[:w] = -np.inf
+    c.call()
+    R.sync()
+    c.check()
+
+
 def test_fewer_live_words_than_asked_for():
     c = Case(6, 3, 2, 9, 50, finished=False)
     c.x[0, 3:] = -np.inf

@@ -160,6 +160,57 @@ def test_places_past_the_lengths_are_not_read_into_the_result(dtype):
     c.check()
 
 
+@pytest.mark.parametrize("dtype,size", [("f16", 2.0 ** -20), ("f16", 2.0 ** -15), ("bf16", 2.0 ** -60),
+                                        ("f32", 2.0 ** -60)])
+def test_small_stored_values(dtype, size):
+    """keys and values of f16 mostly below its normal range (2^-14)"""
+    c = Case(11, dtype, 16, 2, 64, 4, 1, 5, 90, 33)
+    c.pool.k, c.pool.v = (R.store((R.values(x, dtype) * size).astype(np.float32), dtype)
+                          for x in (c.pool.k, c.pool.v))
+    c.pool.upload()
+    c.q *= np.float32(1 / size)
+    c.call()
+    R.sync()
+    hd, pool = c.pool.hd, c.pool
+    got = c.bufs["out"].download((5, 4 * hd + 4), np.float32)[:, :4 * hd].reshape(5, 4, hd)
+    for r in range(5):
+        k, v = (np.concatenate([pool.rows(x, c.layer, c.ptable[0], 90), pool.rows(x, c.layer, c.table[r], 33)])
+                for x in "kv")
+        q = c.q[r].astype(np.float64).reshape(4, hd)
+        want, mag, qk = R.attention(q, k, v, 1 / np.sqrt(hd))
+        tol = (2 * (hd + 8) * 2.0 ** -24 * qk / np.sqrt(hd) + (123 + 64) * 2.0 ** -24) * mag
+        assert (np.abs(got[r] - want) <= tol).all()
+
+
+@pytest.mark.parametrize("plen", [70, 1500])
+def test_pool_past_32_bits(plen):
+    """over 2^32 elements: a prefix and suffixes in the last pages (in one launch, and split)"""
+    page, kv, hd, nh = 512, 8, 128, 16
+    cols, rows = -(-plen // page), 3
+    far = cols + rows
+    pages = (1 << 32) // (page * kv * hd) + far
+    step = page * kv * hd * 2
+    dk, dv = hip.DeviceBuffer(pages * step), hip.DeviceBuffer(pages * step)
+    near = R.Pool("f16", page, far, 1, kv, hd, rng=np.random.default_rng(12))
+    for d, x in ((dk, near.pack_k(near.k)), (dv, near.pack_v(near.v))):
+        hip.check(hip.lib().syn_hip_memcpy_h2d(d.ptr + (pages - far) * step, hip.ptr(x), x.nbytes))
+    c = Case(13, "f16", page, kv, hd, nh, 1, rows, 1, 1)
+    c.pool, c.layer = near, 0
+    c.plen, c.slen = R.i32([plen]), R.i32([9, 33, 0])
+    c.max_prefix, c.max_suffix = plen, 40
+    c.ptable = R.i32(np.arange(cols)[None])
+    c.table = R.i32(cols + np.arange(rows)[:, None])
+    first = pages - far
+    c.ptable += first
+    c.table += first
+    c.pool.desc = hip.KvPages(hip.KV_F16, page, pages, 1, kv, hd, dk.ptr, dv.ptr)
+    c.call()
+    R.sync()
+    c.ptable -= first
+    c.table -= first
+    c.check()
+
+
 def test_pages_outside_the_pool_and_odd_lengths():
     c = Case(5, "f16", 16, 2, 64, 4, 2, 2, [100, 40], [30, 20, 33, 7], max_prefix=80, max_suffix=32)
     c.plen[1], c.slen[1] = -3, -2147483648
