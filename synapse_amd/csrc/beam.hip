@@ -17,6 +17,13 @@ namespace {
 // are formed, n values at least are not below the least of the groups' maxima,
 // and few are; those go to LDS, where each counts the ones before it.
 //
+// Bytes and exponentials bound it: every logit is read once and costs about ten
+// instructions, one of them an exponential, which together take as long as the
+// read.  128 rows of 151936 logits, 16 to choose: 28.9 us, the chunks 20 (3.9
+// TB/s), the join of 16 lists of 19 a group 8; 32 rows of 128256: 13.4 us; 4
+// rows of 32000: 8.9, two launches.  A single launch would need counters that
+// are zero at the start, which a caller's workspace is not.
+//
 // Equal values go to the lower (beam, token).  A value of -inf is a candidate
 // only when a group has fewer than n_select others, so the chunks leave those
 // out and the second kernel fills up with them in order.
@@ -125,8 +132,10 @@ __device__ __forceinline__ Cand cand_of(uint64_t key) {
 constexpr int kChunkNT = 256;
 constexpr int kWaveCap = 256;  // of a wave's candidates
 
-template <int PER>  // values a thread
-__global__ void __launch_bounds__(kChunkNT) k_beam_chunks(SelectArgs a) {
+// PER values a thread, which stay in registers; six waves a SIMD (28.9 us at 128
+// rows of 151936, five 30.0, seven 30.7).
+template <int PER>
+__global__ void __launch_bounds__(kChunkNT, 6) k_beam_chunks(SelectArgs a) {
   __shared__ __align__(16) uint64_t list[4][kWaveCap];
   __shared__ float wtop[4], wsum[4], wgroup[4][64];
   __shared__ int count[4], ri[4];
@@ -142,13 +151,17 @@ __global__ void __launch_bounds__(kChunkNT) k_beam_chunks(SelectArgs a) {
   const int first = chunk * (kChunkNT * PER), left = min(a.vocab - first, kChunkNT * PER);
   const float *x0 = a.logits + (size_t)row * a.ld + first;
   float x[PER];
-  if (a.aligned && left == kChunkNT * PER) {
+  if (a.aligned && left % 4 == 0) {
 #pragma unroll
     for (int i = 0; i < PER; i += 4) {
-      const f32x4 v = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(x0 + i * kChunkNT + tid * 4));
+      const int at4 = min(i * kChunkNT + tid * 4, left - 4);
+      const f32x4 v = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(x0 + at4));
 #pragma unroll
       for (int j = 0; j < 4; j++) x[i + j] = v[j];
     }
+    if (left < kChunkNT * PER)
+#pragma unroll
+      for (int i = 0; i < PER; i++) x[i] = i / 4 * 4 * kChunkNT + tid * 4 < left ? x[i] : kNone;
   } else {  // (no load behind a branch: all are in flight together)
 #pragma unroll
     for (int i = 0; i < PER; i++) x[i] = x0[min((i / 4 * kChunkNT + tid) * 4 + i % 4, left - 1)];
@@ -251,7 +264,9 @@ __global__ void __launch_bounds__(kChunkNT) k_beam_chunks(SelectArgs a) {
 constexpr int kMergeNT = 1024;
 constexpr int kMergeCap = 1024;
 
-// one workgroup a group
+// One workgroup a group: the sums of a beam's chunks joined in f64, then the
+// best of all lists.  4 us for one group of 4 beams, 8 for 16 groups of 128
+// lists at once: latency (f64 logarithms, four barriers, the ranks in LDS).
 __global__ void __launch_bounds__(kMergeNT) k_beam_merge(SelectArgs a) {
   struct Pick {
     double v;
@@ -444,8 +459,11 @@ struct SelectSpace {
 SelectSpace select_space(const syn_hip_beam_select_params &p) {
   const size_t rows = (size_t)p.n_groups * p.n_beams;
   SelectSpace s;
-  // chunks of 8192 logits; of 2048 where those would not fill the chip
-  s.per = rows * cdiv(p.vocab, kChunkNT * 32) >= 256 ? 32 : 8;
+  // Chunks of 8192 logits; of 2048 where fewer than 128 would be at work (4 rows
+  // of 32000, 16 chunks: 11.0 us against 10.1; 4 of 128256, 64: 11.4 and 10.9;
+  // 8 of 128256, 128: 12.2 and 12.8; 32: 13.4 and 16.5).  4096 a chunk take 36 us
+  // where 8192 take 29, 16384 35: the lists that are joined, and registers.
+  s.per = rows * cdiv(p.vocab, kChunkNT * 32) >= 128 ? 32 : 8;
   s.chunks = (int)cdiv(p.vocab, (size_t)kChunkNT * s.per);
   s.stat = 0;
   s.cand = round_up(rows * s.chunks * sizeof(ChunkStat), 16);
@@ -455,7 +473,9 @@ SelectSpace select_space(const syn_hip_beam_select_params &p) {
 
 // ---------------------------------------------------------------- reordering
 // One workgroup moves 64 units (of U bytes) of every row of a group: a unit's
-// rows are all read before any is written, so the move is in place.
+// rows are all read before any is written, so the move is in place.  Bound by
+// its bytes: 8 rows of 128 KiB in 48 buffers 11.2 us, 4.5 TB/s (a large copy
+// reaches 4.8).
 template <class U>
 __global__ void __launch_bounds__(64)
     k_reorder_rows(const int32_t *parent, int W, uint8_t *rows, size_t units, size_t row_stride,
@@ -497,7 +517,10 @@ __device__ __forceinline__ void held(const PagesArgs &a, int g, size_t *full, in
   *rest = (int)(n & (a.ps - 1));
 }
 
-// grid (layer * kv head, row): the parent's part of a page into the spare page
+// grid (layer * kv head, row): the parent's part of a page into the spare page.
+// Bound by its bytes, 5.5 to 6 TB/s: 32 rows of 43 positions, 28 layers of 8 kv
+// heads of 128, f16: 25 us, and 4 for the tables (parents are read by several
+// rows, once from HBM).
 __global__ void __launch_bounds__(256) k_copy_pages(PagesArgs a) {
   const int row = blockIdx.y, g = row / a.W, b = row - g * a.W;
   const int p = a.parent[row];

@@ -89,6 +89,17 @@ def test_select(case):
     c.check()
 
 
+@pytest.mark.parametrize("rows", [3, 64])
+@pytest.mark.parametrize("vocab,pad", [(8195, 1), (8196, 4), (30001, 3), (2050, 2), (4, 4)])
+def test_rows_that_end_inside_a_chunk(rows, vocab, pad):
+    """rows 16 bytes apart, with large values between them"""
+    c = Case(11, rows, 2, 4, vocab, pad=pad)
+    c.x[:, vocab:] = 100.0
+    c.call()
+    R.sync()
+    c.check()
+
+
 def test_without_flags_or_eos():
     c = Case(2, 2, 4, 4, 5000, eos=-1, null_flags=True)
     c.call()
