@@ -48,13 +48,13 @@ struct AttnArgs {
   size_t ldq, ldo, ld_ptable, ld_table;
   int nh, rep, group_size, n_seqs, max_prefix, max_suffix;
   float scale;  // times log2(e): exponentials are powers of two
-  // the split: positions of a part (a multiple of kTile * kWaves), parts of
+  // the split: positions of a part (a multiple of kTile), parts of
   // the longest prefix and suffix; parts of query row (sequence, head) are
   // po[(sequence * nh + head) * (npp + nsp) + part][hd], pml[..][2] (max, sum)
   int pchunk, schunk, npp, nsp, prefix_wgs;
   int prw, srw;  // tiles of 16 rows of a prefix and of a suffix workgroup: 1, 2 or 4
   float *po, *pml;
-  bool joined, q16;  // rows of queries are 16-byte aligned
+  bool joined, solo, q16;  // solo: a wave for a sequence's rows; rows of queries are 16-byte aligned
 };
 
 // ---------------------------------------------------------------- products
@@ -376,14 +376,16 @@ template <class T, int NC, bool FULL> struct Rows {
     for (int d = 0; d < DT; d++) o[d] = F::mma(v[d], p, o[d]);
   }
 
-  // ---- 16 rows in all: the waves take the tiles of a run in turn, K and V in
-  // registers.  One set of them: the next tile's K is requested when this
-  // one's scores are formed, its V when this one's product is.
+  // ---- 16 rows in all: `waves` waves (a power of two) take the tiles of a run
+  // in turn, K and V in registers.  One set of them: the next tile's K is
+  // requested when this one's scores are formed, its V when this one's product
+  // is.
   template <bool WIDE>
-  __device__ __forceinline__ void run_alone(const KvPool<T> &pool, const HeadBase &hb, const Run &r) {
-    constexpr int kStep = kTile * kWaves;
+  __device__ __forceinline__ void run_alone(const KvPool<T> &pool, const HeadBase &hb, const Run &r,
+                                            int waves) {
+    const int kStep = kTile * waves;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int k0 = r.from + ((wave - r.first) & (kWaves - 1)) * kTile;
+    int k0 = r.from + ((wave - r.first) & (waves - 1)) * kTile;
     if (k0 >= r.to) return;
     // (FULL: the fragments' offsets are even steps from the first)
     const uint32_t k_first = koff(pool, 0), v_first = voff(pool, 0);
@@ -554,6 +556,30 @@ template <class T, int NC, bool FULL> struct Rows {
     }
   }
 
+  // A wave's own results to the output, or to its part of the workspace.
+  __device__ __forceinline__ void finish_alone(const AttnArgs &a, int hd, int seq0, int head, int row0,
+                                               int rows, int part) {
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const float sum = groups_sum(l);
+    if (n >= rows) return;
+    const int row = row0 + n, member = row / a.rep;
+    const size_t qh = (size_t)head * a.rep + (row - member * a.rep), seq = seq0 + member;
+    float *out = a.out + seq * a.ldo + qh * hd;
+    const size_t at = part < 0 ? 0 : (seq * a.nh + qh) * (a.npp + a.nsp) + part;
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+      const int c = d * 16 + g * 4;
+      if (c >= hd) continue;
+      if (part < 0) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) out[c + k] = sum == 0.0f ? 0.0f : o[d][k] / sum;
+      } else {
+        *reinterpret_cast<f32x4 *>(a.po + at * hd + c) = o[d];
+      }
+    }
+    if (part >= 0 && g == 0) a.pml[at * 2] = m, a.pml[at * 2 + 1] = sum;
+  }
+
   // The results of the waves that share rows joined, in the order of the
   // waves; a row's goes to the output, or to its part of the workspace.  RW
   // tiles of rows: wave w has tile w % RW.
@@ -622,7 +648,11 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, NC, FULL>)) k_atten
   const int parts = a.joined ? 1 : (prefix ? a.npp : a.nsp);
   // workgroup i runs on XCD i % 8: the blocks of rows that read the same
   // positions come 8 apart and share that XCD's L2
-  const int j = i >> 3, unit = (j / blocks) * 8 + (i & 7), block = j % blocks;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool solo = !prefix && a.solo;  // nothing below waits for the other waves then
+  const int j = i >> 3, block = j % blocks;
+  int unit = (j / blocks) * 8 + (i & 7);
+  if (solo) unit = unit * kWaves + wave;
   const int head = unit % pool.nkv, u = unit / pool.nkv;
   const int part = u % parts, owner = u / parts;  // group or sequence
   if (owner * members >= a.n_seqs) return;
@@ -638,7 +668,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, NC, FULL>)) k_atten
     r.to = min(r.from + chunk, len);
     at = prefix ? part : a.npp + part;
     if (r.from >= len) {  // nothing here: no rows to write, a sum of 0
-      for (int k = threadIdx.x; k < rows; k += 64 * kWaves) {
+      for (int k = solo ? (int)threadIdx.x & 63 : (int)threadIdx.x; k < rows; k += 64 * kWaves) {
         const int row = row0 + k, member = row / a.rep;
         const size_t p = ((size_t)(seq0 + member) * a.nh + (size_t)head * a.rep + (row - member * a.rep)) *
                              (a.npp + a.nsp) + at;
@@ -662,7 +692,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, NC, FULL>)) k_atten
       ok = wide ? W::template start_shared<true, 2>(pool, hb, r, lds)
                 : W::template start_shared<false, 2>(pool, hb, r, lds);
   W w;
-  const int tile = (int)(threadIdx.x >> 6) & (RW - 1);
+  const int tile = wave & (RW - 1);
   w.load_queries(a, pool.hd, seq0, head, row0 + tile * 16, row0 + rows - 1);
   if (RW == 1) {
     // joined: the prefix first, its next tile's wave begins the suffix
@@ -671,9 +701,13 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, NC, FULL>)) k_atten
       if (k == 0) x = Run{a.ptable + (size_t)group * a.ld_ptable, 0, plen, 0};
       if (k == 1 && a.joined) x.first = (plen + kTile - 1) / kTile;
       if (wide)
-        w.template run_alone<true>(pool, hb, x);
+        w.template run_alone<true>(pool, hb, x, solo ? 1 : kWaves);
       else
-        w.template run_alone<false>(pool, hb, x);
+        w.template run_alone<false>(pool, hb, x, solo ? 1 : kWaves);
+    }
+    if (solo) {
+      w.finish_alone(a, pool.hd, seq0, head, row0, rows, at);
+      return;
     }
   } else if (RW == 4) {
     if (wide)
@@ -747,7 +781,7 @@ __global__ void __launch_bounds__(256) k_join_parts(AttnArgs a, int hd) {
 
 // ---------------------------------------------------------------- host
 struct Plan {
-  bool joined;
+  bool joined, solo;
   int nc, prw, srw;
   int pchunk, schunk, npp, nsp;
   size_t prefix_wgs, wgs, rows, po_bytes, pml_bytes;
@@ -762,7 +796,7 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_prefix_attention_params
   // two, their blocks read K and V once each, the second time from L2.
   const bool small = w.nc * (pg.dtype == SYN_HIP_KV_F32 ? 2 : 1) <= 4;
   auto tiles = [&](size_t rows) { return rows <= 16 ? 1 : (rows <= 32 ? (small ? 2 : 1) : 4); };
-  const size_t step = kTile * kWaves, seqs = (size_t)p.n_groups * p.group_size;
+  const size_t seqs = (size_t)p.n_groups * p.group_size;
   // One launch, each sequence's rows whole, where a second launch would cost
   // more than the prefix read again for every sequence (from L2): 24 heads of
   // 128, 8 sequences, f16: 900 positions 11.2 us against 12.2 in parts, 1600
@@ -770,33 +804,63 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_prefix_attention_params
   // twice the bytes and four times the matrix instructions' time: 500 positions
   // 17.9 us, 900 in parts 12.8.
   const size_t whole = pg.dtype == SYN_HIP_KV_F32 ? 2 : (seqs * nkv <= 512 ? 8 : 4);
-  w.joined = (size_t)p.max_prefix + p.max_suffix <= whole * step;
+  w.joined = (size_t)p.max_prefix + p.max_suffix <= whole * kTile * kWaves;
   w.prw = tiles((size_t)p.group_size * rep);
   w.srw = w.joined ? 1 : tiles(rep);
   const size_t sblocks = cdiv(rep, 16 * w.srw), sunits = seqs * nkv;
-  if (w.joined) {
-    w.wgs = round_up(sunits, 8) * sblocks;
-    return w;
-  }
   // Parts of about equal work for as many workgroups as the chip holds at
   // once, four a CU, two, or one.  (512 workgroups of 64 dims in 16 bits,
   // 48 sequences of 1500 positions over a shared 8200: 45 us, 1024: 40; of 128
   // dims, 64 sequences over four prefixes of 32768: 110 and 127.)
   const size_t want = w.nc == 8 ? 256 : (w.nc == 4 || pg.dtype == SYN_HIP_KV_F32 ? 512 : 1024);
-  const size_t pblocks = cdiv((size_t)p.group_size * rep, 16 * w.prw), punits = (size_t)p.n_groups * nkv;
-  const size_t psteps = cdiv(p.max_prefix, step), ssteps = cdiv(p.max_suffix, step);
-  const size_t total = punits * pblocks * psteps + sunits * sblocks * ssteps;
-  const size_t per = std::max<size_t>(1, cdiv(total, want));
-  auto cut = [&](size_t steps, int *chunk, int *n) {
-    const size_t k = cdiv(steps, per);  // as many parts, of equal length
-    const size_t each = k ? cdiv(steps, k) : 0;
-    *chunk = (int)(each * step);
-    *n = each ? (int)cdiv(steps, each) : 0;
+  const size_t ptiles = cdiv(p.max_prefix, kTile), stiles = cdiv(p.max_suffix, kTile);
+  // Many short runs of a sequence's own: a wave for each, where the rounds of
+  // workgroups with their latency (of about kFix tiles) come to less so (246
+  // sequences of 20 positions, 8 kv heads of 128, f32: 19 us against 36 with
+  // four waves; 100 over shared prefixes of 559: 32 and 48).
+  constexpr size_t kFix = 6;
+  auto alone = [&](size_t units, size_t tiles) {
+    return w.srw == 1 && cdiv(cdiv(units, kWaves) * sblocks, want) * (kFix + tiles) <
+                             cdiv(units * sblocks, want) * (kFix + cdiv(tiles, kWaves));
   };
-  cut(psteps, &w.pchunk, &w.npp);
-  cut(ssteps, &w.schunk, &w.nsp);
-  w.prefix_wgs = round_up(punits * w.npp, 8) * pblocks;
-  w.wgs = w.prefix_wgs + round_up(sunits * w.nsp, 8) * sblocks;
+  auto groups_of = [&](size_t units) { return round_up(w.solo ? cdiv(units, kWaves) : units, 8) * sblocks; };
+  if (w.joined) {
+    w.solo = alone(sunits, ptiles + stiles);
+    w.wgs = groups_of(sunits);
+    return w;
+  }
+  const size_t pblocks = cdiv((size_t)p.group_size * rep, 16 * w.prw), punits = (size_t)p.n_groups * nkv;
+  const size_t total = punits * pblocks * ptiles + sunits * sblocks * stiles;
+  auto cut = [&](size_t tiles, size_t each, size_t grain, int *chunk, int *n) {
+    const size_t k = cdiv(tiles, round_up(each, grain));  // as many parts, of equal length
+    each = k ? round_up(cdiv(tiles, k), grain) : 0;
+    *chunk = (int)(each * kTile);
+    *n = each ? (int)cdiv(tiles, each) : 0;
+  };
+  // Waves that share tiles take them all, so a part may be short: two tiles (32
+  // rows of f32 over 512 positions 13.7 us, 16.3 with four; one tile takes 15.2
+  // where two take 13.5 at 24 rows of f16 over 4001: the join).
+  constexpr size_t kGrain = 2;
+  for (size_t per = std::max<size_t>(1, cdiv(total, want));; per += kGrain + per / 16) {
+    cut(ptiles, per, w.prw == 1 ? kWaves : kGrain, &w.pchunk, &w.npp);
+    cut(stiles, per, kWaves, &w.schunk, &w.nsp);
+    w.solo = alone(sunits * w.nsp, std::min<size_t>(stiles, w.schunk / kTile));
+    w.prefix_wgs = round_up(punits * w.npp, 8) * pblocks;
+    const size_t suffix_wgs = groups_of(sunits * w.nsp);
+    w.wgs = w.prefix_wgs + suffix_wgs;
+    // A second round for an eighth or more of them costs more than longer parts
+    // (24 sequences of 16 heads of 64 over eight prefixes of 3876: 18.0 us, 15.5
+    // so), and so do 1.5 of them a CU (52 of 16 heads of 128, f32, over four of
+    // 6918: 384 workgroups 82 us, 256 64); suffixes count by their length.
+    // Where they alone make rounds, the order hides it.
+    constexpr size_t kCus = 256;
+    const bool uneven = w.prefix_wgs > kCus && 4 * round_up(w.prefix_wgs, kCus) > 5 * w.prefix_wgs;
+    auto waves_take = [&](int chunk, int rw) { return kFix + cdiv((size_t)chunk / kTile * rw, kWaves); };
+    const size_t stiles_part = std::min<size_t>(stiles, w.schunk / kTile);
+    const size_t suffix = suffix_wgs * (w.solo ? kFix + stiles_part : waves_take(w.schunk, w.srw)) /
+                          waves_take(w.pchunk, w.prw);
+    if (w.npp <= 1 || (w.prefix_wgs + suffix <= want + want / 8 && !uneven) || 2 * suffix > want) break;
+  }
   const size_t n = w.rows * (size_t)(w.npp + w.nsp);
   w.po_bytes = round_up(n * hd * 4, 16);
   w.pml_bytes = round_up(n * 8, 16);
@@ -910,6 +974,7 @@ extern "C" syn_status_t syn_hip_prefix_attention(
   a.prw = w.prw;
   a.srw = w.srw;
   a.joined = w.joined;
+  a.solo = w.solo;
   a.q16 = aligned16(d_q) && p->ldq % 4 == 0;
   a.po = static_cast<float *>(d_workspace);
   a.pml = reinterpret_cast<float *>(static_cast<uint8_t *>(d_workspace) + w.po_bytes);

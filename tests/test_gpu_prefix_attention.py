@@ -121,6 +121,24 @@ def test_attention(case):
     c.check()
 
 
+MANY = [  # more sequences' heads than workgroups run at once, little work in each
+    ("f32", 16, 8, 128, 32, 2, 50, [18, 5], 2), ("f16", 8, 8, 64, 16, 3, 47, [300, 0, 9], 21),
+    ("bf16", 32, 16, 40, 16, 1, 64, 0, 30), ("f16", 16, 8, 128, 24, 3, 46, [1650, 1, 900], 27),
+    ("f32", 64, 8, 64, 32, 4, 60, [700, 300, 0, 33], 70), ("bf16", 16, 8, 128, 128, 2, 40, 1500, 1),
+    ("bf16", 8, 32, 8, 32, 1, 40, 260, 5), ("f16", 64, 16, 256, 32, 1, 24, 80, 9)]
+
+
+@pytest.mark.parametrize("case", MANY, ids=str)
+def test_many_short_sequences(case):
+    print("case", case, flush=True)
+    c = Case(14, *case)
+    c.slen[:] = c.rng.integers(0, case[-1] + 1, len(c.slen))
+    c.slen[-1] = case[-1]
+    c.call()
+    R.sync()
+    c.check()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_long_prefix_and_suffix(dtype):
     """long enough for any split"""
