@@ -634,7 +634,7 @@ template <class T, int NC, bool FULL> constexpr int kResident = NC == 8 || (NC *
 
 // Joined: a workgroup has both runs of a sequence's rows whole.  Else the
 // first workgroups have the parts of the prefixes, the others those of the
-// suffixes.
+// suffixes.  Solo: a wave has what else a sequence's workgroup has.
 template <class T, int NC, bool FULL>
 __global__ void __launch_bounds__(64 * kWaves, (kResident<T, NC, FULL>)) k_attend(AttnArgs a, KvPool<T> pool) {
   using W = Rows<T, NC, FULL>;

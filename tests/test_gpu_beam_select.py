@@ -90,11 +90,29 @@ def test_select(case):
 
 
 @pytest.mark.parametrize("rows", [3, 64])
-@pytest.mark.parametrize("vocab,pad", [(8195, 1), (8196, 4), (30001, 3), (2050, 2), (4, 4)])
+@pytest.mark.parametrize("vocab,pad", [(8195, 1), (8196, 4), (30001, 3), (2050, 2), (4, 4), (8198, 0), (8199, 2),
+                                       (2055, 0), (4111, 1), (8194, 3)])
 def test_rows_that_end_inside_a_chunk(rows, vocab, pad):
     """rows 16 bytes apart, with large values between them"""
     c = Case(11, rows, 2, 4, vocab, pad=pad)
     c.x[:, vocab:] = 100.0
+    c.call()
+    R.sync()
+    c.check()
+
+
+@pytest.mark.parametrize("shift", [1, 2, 3])
+def test_logits_that_begin_off_16_bytes(shift):
+    c = Case(12, 5, 3, 6, 16390)
+    c.call()
+    R.sync()
+    raw = R.dev(np.concatenate([np.full(shift, 100, np.float32), c.x.reshape(-1)]))
+
+    class Moved:
+        ptr = raw.ptr + 4 * shift
+    c.bufs["x"] = Moved
+    for k in "ptv":
+        c.bufs[k] = R.dev(np.full(c.g * c.n + 5, -7, np.int32))
     c.call()
     R.sync()
     c.check()
