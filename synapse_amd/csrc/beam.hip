@@ -20,7 +20,7 @@ namespace {
 // Bytes and exponentials bound it: every logit is read once and costs about ten
 // instructions, one of them an exponential, which together take as long as the
 // read.  128 rows of 151936 logits, 16 to choose: 28.9 us, the chunks 20 (3.9
-// TB/s), the join of 16 lists of 19 a group 8; 32 rows of 128256: 13.4 us; 4
+// TB/s), the join of 152 lists of 16 a group 8; 32 rows of 128256: 13.4 us; 4
 // rows of 32000: 8.9, two launches.  A single launch would need counters that
 // are zero at the start, which a caller's workspace is not.
 //
@@ -276,7 +276,7 @@ constexpr int kMergeNT = 1024;
 constexpr int kMergeCap = 1024;
 
 // One workgroup a group: the sums of a beam's chunks joined in f64, then the
-// best of all lists.  4 us for one group of 4 beams, 8 for 16 groups of 128
+// best of all lists.  4 us for one group of 4 beams, 8 for 16 groups of 152
 // lists at once: latency (f64 logarithms, four barriers, the ranks in LDS).
 __global__ void __launch_bounds__(kMergeNT) k_beam_merge(SelectArgs a) {
   struct Pick {
