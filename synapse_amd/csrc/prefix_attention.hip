@@ -15,7 +15,10 @@
 // Precision: queries and weights are f32 and stay so: for a 16-bit pool each
 // is split into parts of the pool's type (two f16 carry 22 bits, three bf16
 // carry 24) whose products with the stored K and V are exact in the f32
-// accumulators; an f32 pool takes the f32 matrix instructions.
+// accumulators; an f32 pool takes the f32 matrix instructions.  f16 has 40
+// binary orders where f32 has 277, so weights far below a row's maximum, which
+// are all that counts where its value is zero, are lifted into f16's range by
+// powers of two and summed apart.
 //
 // What bounds it (a large copy reaches 4.8 TB/s here, a stream of reads alone
 // more, large products 1115 TFLOP/s in f16 and 152 in f32): up to 16 rows of a
@@ -38,7 +41,6 @@ namespace {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr int kWaves = 4;
-constexpr float kSlack = 8.0f;
 constexpr int kTile = 32;  // positions a wave takes at a time
 
 struct AttnArgs {
@@ -68,21 +70,24 @@ template <class T> struct Frag;
 template <> struct Frag<_Float16> {
   using V = f16x8;
   static constexpr int kParts = 2;
-  // A weight is 2^kBias where its score is the reference maximum (and at most
-  // 2^(kBias + kSlack), within f16), so that the second part of small ones
-  // is still a normal f16.
-  static constexpr float kBias = 6.0f;
+  // A weight is 2^kBias where its score is the reference maximum, and at most
+  // 2^(kBias + kSlack), within f16.  From kLeast = 2^kLeastLog on, two parts
+  // hold it to 2^-22 of itself (f16's steps end at 2^-24); a smaller one
+  // takes part in multiples of kLift (add_small), up to 2^15 again.
+  static constexpr float kBias = 12.0f, kSlack = 3.0f;
+  static constexpr float kLeastLog = -3.0f, kLeast = 0.125f, kLift = 262144.0f;
   static __device__ __forceinline__ V load(const _Float16 *p) {
     return *reinterpret_cast<const V *>(p);
   }
-  // both parts cut toward zero: the second holds what the first leaves to
-  // within 2^-21 of x
+  // both parts to nearest: together within 2^-22 of x, or within 2^-25
   static __device__ __forceinline__ void split(const float *x, V *p) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
-      const auto h = __builtin_amdgcn_cvt_pkrtz(x[j], x[j + 1]);
-      const auto r = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], -1.0f, x[j]),
-                                                __builtin_fmaf((float)h[1], -1.0f, x[j + 1]));
+      const f16x2 h = __builtin_convertvector((f32x2{x[j], x[j + 1]}), f16x2);
+      const f16x2 r = __builtin_convertvector((f32x2{__builtin_fmaf((float)h[0], -1.0f, x[j]),
+                                                     __builtin_fmaf((float)h[1], -1.0f, x[j + 1])}), f16x2);
       p[0][j] = h[0], p[0][j + 1] = h[1], p[1][j] = r[0], p[1][j + 1] = r[1];
     }
   }
@@ -95,7 +100,7 @@ template <> struct Frag<_Float16> {
 template <> struct Frag<__bf16> {
   using V = bf16x8;
   static constexpr int kParts = 3;
-  static constexpr float kBias = 0.0f;
+  static constexpr float kBias = 0.0f, kSlack = 8.0f;
   static __device__ __forceinline__ V load(const __bf16 *p) {
     return *reinterpret_cast<const V *>(p);
   }
@@ -129,7 +134,7 @@ template <> struct Frag<__bf16> {
 template <> struct Frag<float> {
   using V = f32x8;
   static constexpr int kParts = 1;
-  static constexpr float kBias = 0.0f;
+  static constexpr float kBias = 0.0f, kSlack = 8.0f;
   static __device__ __forceinline__ V load(const float *p) {
     return V{*reinterpret_cast<const f32x4 *>(p), *reinterpret_cast<const f32x4 *>(p + 4)};
   }
@@ -358,7 +363,7 @@ template <class T, int NC, bool FULL> struct Rows {
     top = groups_max(top) * unscale;
     // weights are relative to m, a maximum of earlier: the accumulators are
     // rescaled only when a score is 2^kSlack times above it
-    if (__any(top > m + kSlack)) {
+    if (__any(top > m + F::kSlack)) {
       const float up = fmaxf(m, top);
       const float back = __builtin_amdgcn_exp2f(m - (up == kNegInf ? 0.0f : up));
       m = up;
@@ -368,12 +373,68 @@ template <class T, int NC, bool FULL> struct Rows {
     }
     const float ref = F::kBias - (m == kNegInf ? 0.0f : m);
 #pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], unscale, ref));
+    for (int j = 0; j < 8; j++) x[j] = __builtin_fmaf(x[j], unscale, ref);
+    bool small = false;
+    if constexpr (F::kParts == 2) {
+      float least = fminf(x[0], x[1]);
+#pragma unroll
+      for (int j = 2; j < 8; j += 2) least = fminf(fminf(x[j], x[j + 1]), least);
+      small = __any(least < F::kLeastLog);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = __builtin_amdgcn_exp2f(x[j]);
     l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+    float y[8];  // the weights below kLeast
+    if constexpr (F::kParts == 2)
+      if (small)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          y[j] = x[j] < F::kLeast ? x[j] : 0.0f;
+          x[j] = x[j] < F::kLeast ? 0.0f : x[j];
+        }
     V p[F::kParts];
     F::split(x, p);
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = F::mma(v[d], p, o[d]);
+    if constexpr (F::kParts == 2)
+      if (small) {
+#pragma unroll
+        for (int d = 0; d < DT; d++) asm volatile("" : "+v"(o[d]));  // as in scores()
+        add_small(y, v);
+      }
+  }
+  // Weights of which two parts would keep few bits or none: lifted until they are
+  // not, their products are added to the sums in f32.  (At most nine rounds: no
+  // weight is below 2^-149.)  Calls without such weights pay for the test and the
+  // registers, 0 to 1 % at 128 dims (four prefixes of 32768 under 64 rows 109.8
+  // us, 108.7 without), 10 % at 64 (48 sequences over 8200: 37.9, 34.4); scores
+  // spread over 36 binary orders take 215 us where 109 do without.
+  __device__ __forceinline__ void add_small(float *y, const V *v) {
+    float back = 1.0f;
+    bool left = false;
+#pragma unroll
+    for (int j = 0; j < 8; j++) left |= y[j] > 0.0f;
+    while (__any(left)) {
+      float z[8];
+      left = false;
+      back *= 1.0f / F::kLift;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        y[j] *= F::kLift;
+        z[j] = y[j] < F::kLeast ? 0.0f : y[j];
+        y[j] = y[j] < F::kLeast ? y[j] : 0.0f;
+        left |= y[j] > 0.0f;
+      }
+      V p[F::kParts];
+      F::split(z, p);
+#pragma unroll
+      for (int d = 0; d < DT; d++) {
+        f32x4 t = F::mma(v[d], p, f32x4{0, 0, 0, 0});
+        asm volatile("" : "+v"(t));
+#pragma unroll
+        for (int k = 0; k < 4; k++) o[d][k] = __builtin_fmaf(t[k], back, o[d][k]);
+      }
+    }
   }
 
   // ---- 16 rows in all: `waves` waves (a power of two) take the tiles of a run
