@@ -118,9 +118,9 @@ template <class F> __device__ __forceinline__ F least_group(F x, int G) {
 }
 
 // keys that order as (value descending, index ascending) when the larger is
-// first; no key is 0
+// first; no key is 0 (-0.0 + 0.0 is 0.0: zeros are equal, and so are their keys)
 __device__ __forceinline__ uint64_t key_of(float x, int i) {
-  const uint32_t u = __float_as_uint(x);
+  const uint32_t u = __float_as_uint(x + 0.0f);
   return (uint64_t)(u >> 31 ? ~u : u | 0x80000000u) << 32 | (uint32_t)~i;
 }
 __device__ __forceinline__ Cand cand_of(uint64_t key) {
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kMergeNT) k_beam_merge(SelectArgs a) {
   if (K <= kMergeCap) {
     for (int k = tid; k < K + 4; k += kMergeNT) {
       const Pick p = list[max(min(k, K - 1), 0)];
-      const uint64_t u = (uint64_t)__double_as_longlong(p.v);
+      const uint64_t u = (uint64_t)__double_as_longlong(p.v + 0.0);  // (as in key_of)
       keys[k] = k < K ? (u >> 63 ? ~u : u | 1ull << 63) : 0;
       index[k] = ~((uint64_t)p.b << 32 | (uint32_t)p.t);
     }
