@@ -707,9 +707,10 @@ syn_status_t syn_hip_prefix_attention(const syn_hip_kv_pages *pages,
  * n_beams * vocab continuations, best first.  The value of token t after beam
  * b is d_scores[b] + d_logits[b][t] - log(sum of exp(d_logits[b])), with
  * d_scores and d_finished [n_groups * n_beams] and d_logits rows ld_logits
- * floats apart.  Equal values go to the lower beam, then the lower token; the
- * tokens of one beam are ordered by their logits, beams against each other by
- * values formed in f64 (d_score: rounded once to f32).  A NaN logit counts as
+ * floats apart.  Beams are ordered against each other by values formed in f64
+ * (d_score: rounded once to f32), equal ones the lower beam first; the tokens
+ * of one beam by their logits, equal ones (0.0 and -0.0 are) the lower token
+ * first.  A NaN logit counts as
  * -inf; a row whose largest logit is +inf shares its probability among the
  * infinities; every continuation of a beam whose score is NaN or infinite is
  * -inf.  A beam whose d_finished is not 0 (NULL: none) is not

@@ -24,9 +24,11 @@ namespace {
 // rows of 32000: 8.9, two launches.  A single launch would need counters that
 // are zero at the start, which a caller's workspace is not.
 //
-// Equal values go to the lower (beam, token).  A value of -inf is a candidate
-// only when a group has fewer than n_select others, so the chunks leave those
-// out and the second kernel fills up with them in order.
+// Equal values go to the lower beam; within a beam the order is that of the
+// logits everywhere (f64 may hold two of them as the same value), equal ones
+// by token.  A value of -inf is a candidate only when a group has fewer than
+// n_select others, so the chunks leave those out and the second kernel fills
+// up with them in order.
 struct Cand {
   float x;
   int i;  // token
@@ -119,9 +121,12 @@ template <class F> __device__ __forceinline__ F least_group(F x, int G) {
 
 // keys that order as (value descending, index ascending) when the larger is
 // first; no key is 0 (-0.0 + 0.0 is 0.0: zeros are equal, and so are their keys)
-__device__ __forceinline__ uint64_t key_of(float x, int i) {
+__device__ __forceinline__ uint32_t ordered(float x) {  // larger for larger x
   const uint32_t u = __float_as_uint(x + 0.0f);
-  return (uint64_t)(u >> 31 ? ~u : u | 0x80000000u) << 32 | (uint32_t)~i;
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t key_of(float x, int i) {
+  return (uint64_t)ordered(x) << 32 | (uint32_t)~i;
 }
 __device__ __forceinline__ Cand cand_of(uint64_t key) {
   const uint32_t u = (uint32_t)(key >> 32);
@@ -281,7 +286,8 @@ constexpr int kMergeCap = 1024;
 __global__ void __launch_bounds__(kMergeNT) k_beam_merge(SelectArgs a) {
   struct Pick {
     double v;
-    int b, t;
+    int b, t, j;  // j: the place among the beam's candidates, which goes up with t where x is the same
+    float x;
   };
   __shared__ Pick list[kMergeCap];
   __shared__ uint64_t keys[kMergeCap + 4], index[kMergeCap + 4];
@@ -335,10 +341,14 @@ __global__ void __launch_bounds__(kMergeNT) k_beam_merge(SelectArgs a) {
   // candidate j: the lists' places (those of beams that do not live are empty)
   auto pick = [&](int j, const Cand &c) {
     const int b = (int)((uint32_t)j / (uint32_t)n / (uint32_t)C);
-    return Pick{value(b, c.x), b, c.i};
+    return Pick{value(b, c.x), b, c.i, j - b * C * n, c.x};
   };
+  auto closed = [&](int b) { return Pick{(double)score[b], b, a.pad, 0, 0.0f}; };  // a finished beam's
+  // two logits of a beam may be so close that their values are the same
   auto ahead = [](const Pick &p, const Pick &q) {
-    return p.v > q.v || (p.v == q.v && (p.b < q.b || (p.b == q.b && p.t < q.t)));
+    if (p.v != q.v) return p.v > q.v;
+    if (p.b != q.b) return p.b < q.b;
+    return p.x > q.x || (p.x == q.x && p.t < q.t);
   };
   double key = none;
   for (int q = tid; q < L; q += kMergeNT) {
@@ -360,7 +370,7 @@ __global__ void __launch_bounds__(kMergeNT) k_beam_merge(SelectArgs a) {
   for (int k = 0; k < kHeld; k++)
     if (tid + k * kMergeNT < T) offer(pick(tid + k * kMergeNT, mine[k]));
   for (int j = tid + kHeld * kMergeNT; j < T; j += kMergeNT) offer(pick(j, cand[j]));
-  if (tid < W && state[tid] == 1) offer(Pick{(double)score[tid], tid, a.pad});
+  if (tid < W && state[tid] == 1) offer(closed(tid));
   __syncthreads();
   const int K = count;
   auto emit = [&](int r, const Pick &p) {
@@ -375,7 +385,8 @@ __global__ void __launch_bounds__(kMergeNT) k_beam_merge(SelectArgs a) {
       const Pick p = list[max(min(k, K - 1), 0)];
       const uint64_t u = (uint64_t)__double_as_longlong(p.v + 0.0);  // (as in key_of)
       keys[k] = k < K ? (u >> 63 ? ~u : u | 1ull << 63) : 0;
-      index[k] = ~((uint64_t)p.b << 32 | (uint32_t)p.t);
+      // (places of a beam are below 2^26: at most 2^18 chunks of 128)
+      index[k] = ~((uint64_t)p.b << 58 | (uint64_t)~ordered(p.x) << 26 | (uint32_t)p.j);
     }
     __syncthreads();
     for (int k = tid; k < K; k += kMergeNT) {
@@ -392,20 +403,20 @@ __global__ void __launch_bounds__(kMergeNT) k_beam_merge(SelectArgs a) {
     }
     if (tid == 0) chosen = min(K, n);
   } else {
-    Pick last{__builtin_huge_val(), -1, -1};
+    Pick last{__builtin_huge_val(), -1, -1, 0, 0.0f};
     for (int r = 0; r < n; r++) {
-      Pick p{none, 0x7fffffff, 0};
+      Pick p{none, 0x7fffffff, 0, 0, 0.0f};
       for (int j = tid; j < T + W; j += kMergeNT) {
-        Pick q{none, 0, 0};
+        Pick q{none, 0, 0, 0, 0.0f};
         if (j < T)
           q = pick(j, cand[j]);
         else if (state[j - T] == 1)
-          q = Pick{(double)score[j - T], j - T, a.pad};
+          q = closed(j - T);
         if (q.v > none && ahead(last, q) && ahead(q, p)) p = q;
       }
       // the first of the wave, of the workgroup
       for (int o = 32; o > 0; o >>= 1) {
-        const Pick q{__shfl_xor(p.v, o), __shfl_xor(p.b, o), __shfl_xor(p.t, o)};
+        const Pick q{__shfl_xor(p.v, o), __shfl_xor(p.b, o), __shfl_xor(p.t, o), 0, __shfl_xor(p.x, o)};
         if (ahead(q, p)) p = q;
       }
       __syncthreads();
@@ -439,7 +450,7 @@ __global__ void __launch_bounds__(kMergeNT) k_beam_merge(SelectArgs a) {
         all += rj[w];
       }
       at += __popcll(who & ((1ull << lane) - 1));
-      if (in && at < n) emit(at, Pick{none, b, t});
+      if (in && at < n) emit(at, Pick{none, b, t, 0, 0.0f});
       have += all;
     }
 }

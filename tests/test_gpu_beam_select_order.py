@@ -78,3 +78,42 @@ def test_finished_and_live_beams_at_zero(first):
     c.scores[:] = -c.scores
     c.bufs = None
     check(c)
+
+
+def tight(c, row, at, large=1e18):
+    """logits that differ in f32, next to one so large that their values do not in f64"""
+    c.x[row] = -np.inf
+    c.x[row, at] = np.float32(1 + np.arange(len(at)) % 7)
+    c.x[row, at[len(at) // 2]] = large
+
+
+@pytest.mark.parametrize("vocab,many", [(50, 20), (9000, 60), (9000, 3000), (40000, 1500)])
+@pytest.mark.parametrize("n", [1, 2, 8, 40, 128])
+def test_logits_whose_values_are_equal(vocab, many, n):
+    """in a chunk, over chunks, and more of them than are ranked at once"""
+    c = Case(4, 2, 2, min(n, many), vocab, finished=False)
+    for row in range(4):
+        tight(c, row, np.sort(c.rng.permutation(vocab)[:many]))
+    c.scores[:] = -3.0
+    c.scores[3] = -4.0
+    check(c)
+
+
+def test_equal_values_of_beams_live_and_finished():
+    """the beams' best words meet at one value"""
+    c = Case(5, 1, 5, 10, 2100, finished=False)
+    c.fin[[1, 3]] = 1
+    for row in (0, 2, 4):
+        tight(c, row, np.sort(c.rng.permutation(2100)[:30]), large=1e17)
+    c.scores[:] = -3.0
+    check(c)
+
+
+@pytest.mark.parametrize("n", [16, 128])
+def test_every_beam_the_same(n):
+    """64 beams with equal words and scores: more candidates than are ranked at once"""
+    c = Case(6, 1, 64, n, 5000, finished=False)
+    c.x[:] = np.where(np.arange(5000) % 11 == 0, 2.0, -1.0)
+    c.x[:, 4000] = np.float32(2.0000002)
+    c.scores[:] = -7.0
+    check(c)
