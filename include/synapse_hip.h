@@ -679,8 +679,8 @@ syn_status_t syn_hip_kv_append(const syn_hip_kv_pages *pages, const syn_hip_kv_a
  * apart, n_heads a multiple of n_kv_heads (query head h reads kv head
  * h / (n_heads / n_kv_heads)); scale 0: 1 / sqrt(head_dim).  max_prefix and
  * max_suffix bound the lengths, which are cut to them (they and the table
- * widths decide the split of the work, so a captured call keeps them);
- * a negative length is 0.  Positions in pages outside the pool are left out;
+ * widths decide the split of the work, so a captured call keeps them) and are
+ * at most 2^31 - 2^16; a negative length is 0.  Positions in pages outside the pool are left out;
  * a sequence with no position gives zeros.  Scores, softmax and sums are f32;
  * 16-bit pools are read as stored.  d_q and the keys and values of the
  * positions that count are finite (an infinity among them may give NaN where

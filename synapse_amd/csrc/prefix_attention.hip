@@ -726,7 +726,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, NC, FULL>)) k_atten
   if (!a.joined) {
     const int len = prefix ? plen : slen, chunk = prefix ? a.pchunk : a.schunk;
     r.from = part * chunk;
-    r.to = min(r.from + chunk, len);
+    r.to = r.from + min(chunk, len - r.from);  // (the sum of the two may pass 2^31)
     at = prefix ? part : a.npp + part;
     if (r.from >= len) {  // nothing here: no rows to write, a sum of 0
       for (int k = solo ? (int)threadIdx.x & 63 : (int)threadIdx.x; k < rows; k += 64 * kWaves) {
@@ -938,8 +938,10 @@ syn_status_t check_attention(const syn_hip_kv_pages *pages,
     set_error("prefix_attention: layer outside the pool, or n_heads no multiple of n_kv_heads");
     return SYN_ERR_INVALID_ARG;
   }
-  if (rows > 65535u || p->max_prefix > 0x7fffff00u || p->max_suffix > 0x7fffff00u) {
-    set_error("prefix_attention: more than 65535 sequences or 2^31 positions");
+  // (kernels look two rounds of tiles past a length, in 32 bits)
+  constexpr uint32_t kMaxLength = 0x7fff0000u;
+  if (rows > 65535u || p->max_prefix > kMaxLength || p->max_suffix > kMaxLength) {
+    set_error("prefix_attention: more than 65535 sequences or 2^31 - 2^16 positions");
     return SYN_ERR_INVALID_ARG;
   }
   if (p->ldq < p->n_heads * hd || p->ldo < p->n_heads * hd ||
