@@ -720,7 +720,7 @@ syn_status_t syn_hip_prefix_attention(const syn_hip_kv_pages *pages,
  * 1 <= n_beams <= 64, 1 <= n_select <= 128, n_select <= n_beams * vocab;
  * d_score may be d_scores and d_finished_out d_finished when n_select ==
  * n_beams.  n_groups * n_beams is at most 65535, and n_beams * n_select *
- * ceil(vocab / 2048) below 2^31.  The workspace (16-byte aligned) is needed by
+ * ceil(vocab / 2048) at most 2^31 - 2^16.  The workspace (16-byte aligned) is needed by
  * every call. */
 typedef struct {
   uint32_t n_groups, n_beams, n_select;

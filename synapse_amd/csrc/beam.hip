@@ -463,7 +463,8 @@ syn_status_t check_select(const syn_hip_beam_select_params *p) {
   }
   if (!p->vocab || p->vocab > 0x7ff00000u || (uint64_t)p->n_select > p->n_beams * (uint64_t)p->vocab ||
       (uint64_t)p->n_groups * p->n_beams > 65535u ||
-      (uint64_t)p->n_beams * p->n_select * cdiv(p->vocab, 2048) > 0x7ffffff0u) {
+      // (the join steps over the lists' places by 1024 in 32 bits)
+      (uint64_t)p->n_beams * p->n_select * cdiv(p->vocab, 2048) > 0x7fff0000u) {
     set_error("beam_select: fewer continuations than n_select, or too many rows or candidates");
     return SYN_ERR_INVALID_ARG;
   }

@@ -26,3 +26,12 @@ def attention_workspace(**kw):
 def test_attention_lengths(which, length, want, members):
     """kernels step past a length, by less than 2^16, in 32 bits"""
     assert attention_workspace(**{which: length}, group_size=members) == want
+
+
+@pytest.mark.parametrize("chunks,want", [(262136, OK), (262137, ARG), (262143, ARG)])
+def test_select_candidates(chunks, want):
+    """64 beams, 128 of each chunk: 2^31 - 2^16 places, which the join steps over
+    by 1024 in 32 bits"""
+    p = hip.BeamSelect(n_groups=1, n_beams=64, n_select=128, eos=0, pad=0, vocab=2048 * chunks,
+                       ld_logits=2048 * chunks)
+    assert hip.lib().syn_hip_beam_select_workspace(C.byref(p), C.byref(C.c_size_t())) == want
