@@ -300,6 +300,8 @@ extern "C" syn_status_t syn_hip_kv_append(
     set_error("kv_append: d_q_out may be d_q with ldo == ldq only");
     return SYN_ERR_INVALID_ARG;
   }
+  // (every token is skipped: the tables have no row that a kernel may read)
+  if (p->n_positions == 0) return SYN_OK;
   SYN_TRY(ensure_init());
   AppendArgs a{d_q,      d_k,    d_v,    d_q_norm, d_k_norm, d_cos,       d_sin,
                d_pos,    d_seq,  d_index, d_table, d_q_out,  p->ldq,      p->ldk,

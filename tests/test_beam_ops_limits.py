@@ -35,3 +35,12 @@ def test_select_candidates(chunks, want):
     p = hip.BeamSelect(n_groups=1, n_beams=64, n_select=128, eos=0, pad=0, vocab=2048 * chunks,
                        ld_logits=2048 * chunks)
     assert hip.lib().syn_hip_beam_select_workspace(C.byref(p), C.byref(C.c_size_t())) == want
+
+
+def test_append_without_positions():
+    """every token is skipped: nothing is launched that would read a row of empty tables"""
+    pages = hip.KvPages(hip.KV_F16, 16, 8, 1, 2, 8, FAKE, FAKE)
+    p = hip.KvAppend(layer=0, n_heads=2, n_seqs=1, rotary_dim=8, interleaved=0, n_positions=0, eps=0,
+                     ldq=32, ldk=32, ldv=32, ldo=16, ld_table=1)
+    assert hip.lib().syn_hip_kv_append(C.byref(pages), C.byref(p), 3, FAKE, FAKE, FAKE, None, None, FAKE,
+                                       FAKE, FAKE, None, FAKE, FAKE, 2 * FAKE, None) == OK
