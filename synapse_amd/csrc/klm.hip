@@ -65,6 +65,7 @@ struct syn_hip_klm_s {
   HostPos hp;
   hipGraphExec_t graph = nullptr;
   bool finalized = false;
+  bool fitted = false;    // scratch and plans are those of the weights that are there
   bool use_graph = true;  // replay the captured decode step, else launch eagerly
   bool use_fused = true;  // five-kernel decode layers (klm_fused.hip) when the model fits
   // fused decode step: split plans, the fixed-point residual r [h] and QKV
@@ -75,9 +76,47 @@ struct syn_hip_klm_s {
   std::unique_ptr<BeamSpace> beams;  // of the last beam search
 
   ~syn_hip_klm_s() {
+    drop_captured();
+    if (stream) (void)hipStreamDestroy(stream);
+  }
+  // The captured steps hold the addresses of weights and scratch.
+  void drop_captured() {
+    if (stream) (void)hipStreamSynchronize(stream);
     if (graph) (void)hipGraphExecDestroy(graph);
     if (draft_graph) (void)hipGraphExecDestroy(draft_graph);
-    if (stream) (void)hipStreamDestroy(stream);
+    graph = draft_graph = nullptr;
+    beams.reset();
+  }
+  // before a weight's buffer is freed for another
+  void weights_change() {
+    drop_captured();
+    fitted = false;
+  }
+  syn_status_t complete() const {
+    if (!have_embed || !have_lm) {
+      set_error("embed_tokens or lm_head not set");
+      return SYN_ERR_INVALID_ARG;
+    }
+    for (size_t l = 0; l < L; l++)
+      if (layers[l].have != 0x7f) {
+        set_error("layer " + std::to_string(l) + " incomplete");
+        return SYN_ERR_INVALID_ARG;
+      }
+    return SYN_OK;
+  }
+  syn_status_t fit() {
+    SYN_TRY(complete());
+    drop_captured();
+    for (auto &Ly : layers) {
+      SYN_TRY(Ly.qkv.prepare(S));
+      SYN_TRY(Ly.o.prepare(S));
+      SYN_TRY(Ly.gu.prepare(S));
+      SYN_TRY(Ly.down.prepare(S));
+    }
+    SYN_TRY(lm_head.prepare(1));
+    SYN_TRY(setup_fused());
+    fitted = true;
+    return SYN_OK;
   }
   // per-layer KV caches in the decode attention's tiled layout (layer_ops.hpp)
   size_t k_elems() const { return kv_k_elems((int)(kvd / hd), (int)hd, (int)S); }
@@ -149,6 +188,8 @@ struct syn_hip_klm_s {
   syn_status_t set_proj(size_t l, int proj, const uint8_t *bytes) {
     Layer &Ly = layers[l];
     const size_t nbytes = proj_bytes(proj);
+    weights_change();
+    if (proj == 3 || proj == 6) Ly.have &= ~(1 << proj);
     if (proj == 3) {
       SYN_TRY(Ly.o.upload(fmt_of(3), bytes, h, qd));
     } else if (proj == 6) {
@@ -777,7 +818,7 @@ static syn_status_t check_klm(syn_hip_klm_t *m) {
     set_error("model not finalized");
     return SYN_ERR_INVALID_ARG;
   }
-  return SYN_OK;
+  return m->fitted ? SYN_OK : m->fit();  // (weights set since the last call)
 }
 
 extern "C" {
@@ -828,7 +869,8 @@ syn_status_t syn_hip_klm_create(const syn_hip_klm_config *cfg, syn_hip_klm_t **o
 
 syn_status_t syn_hip_klm_set_embed(syn_hip_klm_t *m, const float *embed) {
   if (!m || !embed) return SYN_ERR_NULL_PTR;
-  m->beams.reset();  // its captured step holds the buffers' addresses
+  m->weights_change();
+  m->have_embed = false;
   SYN_TRY(m->embed.alloc(m->vocab * m->h * 4));
   SYN_HIP(hipMemcpy(m->embed.p, embed, m->vocab * m->h * 4, hipMemcpyHostToDevice));
   m->have_embed = true;
@@ -839,13 +881,13 @@ syn_status_t syn_hip_klm_set_proj(syn_hip_klm_t *m, uint32_t layer, int proj,
                                   const uint8_t *gguf_bytes) {
   if (!m || !gguf_bytes) return SYN_ERR_NULL_PTR;
   if (layer >= m->L || proj < 0 || proj > 6) return SYN_ERR_INVALID_ARG;
-  m->beams.reset();
   return m->set_proj(layer, proj, gguf_bytes);
 }
 
 syn_status_t syn_hip_klm_set_lm_head(syn_hip_klm_t *m, const uint8_t *gguf_bytes) {
   if (!m || !gguf_bytes) return SYN_ERR_NULL_PTR;
-  m->beams.reset();
+  m->weights_change();
+  m->have_lm = false;
   SYN_TRY(m->lm_head.upload(m->c.fmt_lm_head, gguf_bytes, m->vocab, m->h));
   m->have_lm = true;
   return SYN_OK;
@@ -895,15 +937,7 @@ syn_status_t syn_hip_klm_init_synthetic(syn_hip_klm_t *m, uint64_t seed_base, fl
 
 syn_status_t syn_hip_klm_finalize(syn_hip_klm_t *m) {
   if (!m) return SYN_ERR_NULL_PTR;
-  if (!m->have_embed || !m->have_lm) {
-    set_error("embed_tokens or lm_head not set");
-    return SYN_ERR_INVALID_ARG;
-  }
-  for (size_t l = 0; l < m->L; l++)
-    if (m->layers[l].have != 0x7f) {
-      set_error("layer " + std::to_string(l) + " incomplete");
-      return SYN_ERR_INVALID_ARG;
-    }
+  SYN_TRY(m->complete());
   const size_t half = m->hd / 2;
   std::vector<float> cs(m->S * half), sn(m->S * half);
   const float fb = (float)m->c.base.rope_theta;
@@ -917,14 +951,7 @@ syn_status_t syn_hip_klm_finalize(syn_hip_klm_t *m) {
     }
   SYN_HIP(hipMemcpy(m->rope_cos.p, cs.data(), cs.size() * 4, hipMemcpyHostToDevice));
   SYN_HIP(hipMemcpy(m->rope_sin.p, sn.data(), sn.size() * 4, hipMemcpyHostToDevice));
-  for (auto &Ly : m->layers) {
-    SYN_TRY(Ly.qkv.prepare(m->S));
-    SYN_TRY(Ly.o.prepare(m->S));
-    SYN_TRY(Ly.gu.prepare(m->S));
-    SYN_TRY(Ly.down.prepare(m->S));
-  }
-  SYN_TRY(m->lm_head.prepare(1));
-  SYN_TRY(m->setup_fused());
+  SYN_TRY(m->fit());
   m->finalized = true;
   SYN_TRY(m->set_state(0, 0, 0));
   return SYN_OK;
