@@ -461,6 +461,9 @@ typedef struct {
 
 typedef struct syn_hip_klm_s syn_hip_klm_t;
 syn_status_t syn_hip_klm_create(const syn_hip_klm_config *cfg, syn_hip_klm_t **out);
+/* Weights may be set again at any time.  q, k and v of a layer are stored as
+ * one matrix, and so are gate and up: where one of them is set again the layer
+ * is incomplete, and the model refuses to run, until the others are too. */
 syn_status_t syn_hip_klm_set_embed(syn_hip_klm_t *m, const float *embed);
 syn_status_t syn_hip_klm_set_proj(syn_hip_klm_t *m, uint32_t layer, int proj,
                                   const uint8_t *gguf_bytes);

@@ -195,7 +195,10 @@ struct syn_hip_klm_s {
     } else if (proj == 6) {
       SYN_TRY(Ly.down.upload(fmt_of(6), bytes, h, inter));
     } else {
+      // Members of a stack, q, k, v or gate, up: set again, all of them are.
       const int slot = proj <= 2 ? proj : proj - 1;  // q,k,v,gate,up -> 0..4
+      const int stack = proj <= 2 ? 7 : 0x30;
+      if ((Ly.have & stack) == stack) Ly.have &= ~stack;
       Ly.pending[slot].assign(bytes, bytes + nbytes);
     }
     Ly.have |= 1 << proj;

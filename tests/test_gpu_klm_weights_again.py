@@ -76,3 +76,45 @@ def test_finalized_twice():
     first = everything(g)
     g.finalize()
     same(everything(g), first)
+
+
+@pytest.mark.parametrize("order", [(0, 1, 2, 3, 4, 5, 6), (2, 1, 0, 6, 5, 4, 3), (5, 0, 4, 2, 1)])
+@pytest.mark.parametrize("finalize", [True, False])
+def test_stacked_projections_again(order, finalize):
+    """q, k and v are one matrix, and gate and up: refused while one of them is missing"""
+    _, g = build()
+    first = everything(g)
+    _, want = build()
+    for i, p in enumerate(order):
+        g.set_proj(0, p, proj(p, 70 + p))
+        want.set_proj(0, p, proj(p, 70 + p))
+        done = set(order[:i + 1])
+        partial = (len(done & {0, 1, 2}) % 3, len(done & {4, 5}) % 2) != (0, 0)
+        ids, out = PROMPT.copy(), np.zeros(TINY["vocab"], np.float32)
+        call = hip.lib().syn_hip_klm_forward_prefill(g.h, hip.ptr(ids), ids.size, hip.ptr(out))
+        assert call == (2 if partial else 0)
+        if partial:
+            assert hip.lib().syn_hip_klm_finalize(g.h) == 2
+    want.finalize()
+    if finalize:
+        g.finalize()
+    now = everything(g)
+    same(now, everything(want))
+    assert not np.array_equal(now[-1], first[-1])
+
+
+def test_all_weights_again():
+    """as a file loaded a second time sets them"""
+    _, g = build()
+    first = everything(g)
+    for seed in (0x5EED1000, 0x5EED0000):
+        _, other = build(seed=seed)
+        g.set_embed(O.normal(TINY["vocab"] * H, seed, 0.5).reshape(TINY["vocab"], H))
+        for layer in range(TINY["n_layers"]):
+            for p in range(7):
+                g.set_proj(layer, p, proj(p, seed + 1 + 8 * layer + p))
+        w = O.normal(TINY["vocab"] * H, seed + 1 + 8 * TINY["n_layers"], 0.2).reshape(TINY["vocab"], H)
+        g.set_lm_head(hip.kquant_encode(F6, w))
+        g.finalize()
+        same(everything(g), everything(other))
+    same(everything(g), first)
