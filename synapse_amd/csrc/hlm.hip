@@ -659,6 +659,12 @@ syn_status_t syn_hip_hlm_init_synthetic(syn_hip_hlm_t *m, uint64_t seed_base, fl
   if (!m) return SYN_ERR_NULL_PTR;
   const size_t H = m->H, I = m->I, F = m->F, V = m->V, hd = m->hd, ck = m->ck;
   const size_t qd = m->qd, kvd = m->kvd, S = m->S, nkv_ = m->nkv;
+  SYN_HIP(hipStreamSynchronize(m->stream));
+  if (m->graph) {  // weights replaced: the captured step is stale
+    (void)hipGraphExecDestroy(m->graph);
+    m->graph = nullptr;
+  }
+  m->ready = false;
   auto up = [](DevBuf &b, const std::vector<float> &v) -> syn_status_t {
     SYN_TRY(b.alloc(v.size() * 4));
     SYN_HIP(hipMemcpy(b.p, v.data(), v.size() * 4, hipMemcpyHostToDevice));
@@ -768,10 +774,6 @@ syn_status_t syn_hip_hlm_init_synthetic(syn_hip_hlm_t *m, uint64_t seed_base, fl
   SYN_TRY(m->history.alloc((S + 1) * 4));
   SYN_TRY(m->mhist.alloc((S + 1) * 4));
   SYN_TRY(m->setup_fused());
-  if (m->graph) {  // weights replaced: the captured step is stale
-    (void)hipGraphExecDestroy(m->graph);
-    m->graph = nullptr;
-  }
   m->ready = true;
   return m->reset();
 }

@@ -940,6 +940,12 @@ syn_status_t syn_hip_mamba_create(const syn_hip_mamba_config *cfg, syn_hip_mamba
 syn_status_t syn_hip_mamba_init_synthetic(syn_hip_mamba_t *m, uint64_t seed_base, float stddev) {
   if (!m) return SYN_ERR_NULL_PTR;
   const size_t dm = m->dm, di = m->di, ds = m->ds, dc = m->dc, dr = m->dr, nx = m->nx;
+  SYN_HIP(hipStreamSynchronize(m->stream));
+  if (m->graph) {  // weights replaced: the captured step is stale
+    (void)hipGraphExecDestroy(m->graph);
+    m->graph = nullptr;
+  }
+  m->ready = false;
   {
     std::vector<float> emb(m->vocab * dm);
     fill_normal_parallel(emb.data(), emb.size(), seed_base, stddev);

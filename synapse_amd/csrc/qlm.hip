@@ -60,6 +60,7 @@ struct syn_hip_qlm_s {
   HostPos hp;
   hipGraphExec_t graph = nullptr;
   bool finalized = false;
+  bool fitted = false;  // scratch and plans are those of the weights that are there
   // per-launch event pairs of an eager fused step (syn_hip_qlm_time_step_kernels)
   struct TraceEntry {
     int kind;
@@ -96,8 +97,28 @@ struct syn_hip_qlm_s {
   DevBuf u_draws;
 
   ~syn_hip_qlm_s() {
-    if (graph) (void)hipGraphExecDestroy(graph);
+    weights_change();
     if (stream) (void)hipStreamDestroy(stream);
+  }
+  // before a weight's buffer is freed for another: the captured step holds its
+  // address, and so does the fused step's plan
+  void weights_change() {
+    if (stream) (void)hipStreamSynchronize(stream);
+    if (graph) (void)hipGraphExecDestroy(graph);
+    graph = nullptr;
+    fitted = false;
+  }
+  syn_status_t fit() {
+    for (auto &Ly : layers) {
+      SYN_TRY(Ly.qkv.prepare(S));
+      SYN_TRY(Ly.o.prepare(S));
+      SYN_TRY(Ly.gu.prepare(S));
+      SYN_TRY(Ly.down.prepare(S));
+    }
+    SYN_TRY(lm_head.prepare(1));
+    SYN_TRY(prepare_fused());
+    fitted = true;
+    return SYN_OK;
   }
   // per-layer KV caches in the decode attention's tiled layout (layer_ops.hpp)
   size_t k_elems() const { return kv_k_elems((int)(kvd / hd), (int)hd, (int)S); }
@@ -169,6 +190,7 @@ struct syn_hip_qlm_s {
   syn_status_t set_layer(size_t l, const float *wq, const float *wk, const float *wv,
                          const float *wo, const float *wg, const float *wu, const float *wd) {
     QLayer &Ly = layers[l];
+    weights_change();
     // q,k,v rows stacked: per-row scales make the fused GEMV exact
     {
       std::vector<float> sc(n_qkv);
@@ -583,7 +605,7 @@ static syn_status_t check_model(syn_hip_qlm_t *m) {
     set_error("model not finalized");
     return SYN_ERR_INVALID_ARG;
   }
-  return SYN_OK;
+  return m->fitted ? SYN_OK : m->fit();  // (weights set since the last call)
 }
 
 extern "C" {
@@ -630,6 +652,7 @@ syn_status_t syn_hip_qlm_set_embed(syn_hip_qlm_t *m, const float *embed) {
   if (!m || !embed) return SYN_ERR_NULL_PTR;
   const size_t n = m->vocab * m->h;
   m->host_embed.assign(embed, embed + n);
+  m->weights_change();
   SYN_TRY(m->embed.alloc(n * 4));
   SYN_HIP(hipMemcpy(m->embed.p, embed, n * 4, hipMemcpyHostToDevice));
   return SYN_OK;
@@ -839,6 +862,7 @@ syn_status_t syn_hip_qlm_finalize(syn_hip_qlm_t *m) {
       set_error("layer " + std::to_string(l) + " not set");
       return SYN_ERR_INVALID_ARG;
     }
+  m->weights_change();
   // lm_head quantized from its own weight, else tied to embed_tokens
   // (int8.rs:125-139)
   const std::vector<float> &lm = m->host_lm_head.empty() ? m->host_embed : m->host_lm_head;
@@ -859,14 +883,7 @@ syn_status_t syn_hip_qlm_finalize(syn_hip_qlm_t *m) {
     }
   SYN_HIP(hipMemcpy(m->rope_cos.p, cs.data(), cs.size() * 4, hipMemcpyHostToDevice));
   SYN_HIP(hipMemcpy(m->rope_sin.p, sn.data(), sn.size() * 4, hipMemcpyHostToDevice));
-  for (auto &Ly : m->layers) {
-    SYN_TRY(Ly.qkv.prepare(m->S));
-    SYN_TRY(Ly.o.prepare(m->S));
-    SYN_TRY(Ly.gu.prepare(m->S));
-    SYN_TRY(Ly.down.prepare(m->S));
-  }
-  SYN_TRY(m->lm_head.prepare(1));
-  SYN_TRY(m->prepare_fused());
+  SYN_TRY(m->fit());
   m->fused = m->fused_supported();
   m->finalized = true;
   SYN_TRY(m->set_state(0, 0, 0));
