@@ -711,7 +711,10 @@ syn_status_t syn_hip_prefix_attention(const syn_hip_kv_pages *pages,
  * b is d_scores[b] + d_logits[b][t] - log(sum of exp(d_logits[b])), with
  * d_scores and d_finished [n_groups * n_beams] and d_logits rows ld_logits
  * floats apart.  Beams are ordered against each other by values formed in f64
- * (d_score: rounded once to f32), equal ones the lower beam first; the tokens
+ * (d_score: rounded once to f32), equal ones the lower beam first, but the sum
+ * of exponentials is f32 within 8192 tokens, so that its logarithm is off by
+ * less than 2^-18 (as a rule by 2^-23) and beams' values closer than that may
+ * change places; the tokens
  * of one beam by their logits, equal ones (0.0 and -0.0 are) the lower token
  * first.  A NaN logit counts as
  * -inf; a row whose largest logit is +inf shares its probability among the

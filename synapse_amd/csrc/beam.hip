@@ -12,8 +12,13 @@ namespace {
 // Rows are cut into chunks over the whole chip: a workgroup reads its chunk
 // once into registers, forms max and sum of exp, and keeps the n_select best
 // logits (the order within a beam is that of its logits); one workgroup a
-// group then joins the sums and chooses among the chunks' candidates by their
-// values in f64.  The selection itself never sorts: if G >= n groups of values
+// group then joins the sums in f64 and chooses among the chunks' candidates by
+// their values in f64.  A chunk's sum is f32: in units of 2^-24 of it, its
+// terms' arguments, up to ln 8192 below the top where they weigh, are off by 23
+// at most, the exponential by 2, the additions (31 in a thread, 8 over lanes and
+// waves) by 39, so that a row's logarithm is off by less than 2^-18.  (f64
+// exponentials, a polynomial of degree 8, take 39.4 us where these take 29.2, 128
+// rows of 151936.)  The selection itself never sorts: if G >= n groups of values
 // are formed, n values at least are not below the least of the groups' maxima,
 // and few are; those go to LDS, where each counts the ones before it.
 //
