@@ -677,21 +677,23 @@ syn_status_t syn_hip_kv_append(const syn_hip_kv_pages *pages, const syn_hip_kv_a
  * group's prefix (d_prefix_len[g] positions found through row g of
  * d_prefix_table [n_groups][ld_prefix_table]) and the sequence's own suffix
  * (d_len[s] positions, from slot 0 of the first page of row s of d_table
- * [n_groups * group_size][ld_table]).  The prefix is read once for the whole
- * group.  d_q and d_out [sequences][n_heads][head_dim], rows ldq and ldo
- * apart, n_heads a multiple of n_kv_heads (query head h reads kv head
- * h / (n_heads / n_kv_heads)); scale 0: 1 / sqrt(head_dim).  max_prefix and
- * max_suffix bound the lengths, which are cut to them (they and the table
+ * [n_groups * group_size][ld_table]).  The prefix is read for the whole group
+ * at once (again for every 64 rows of a kv head, and in short calls for every
+ * sequence, from cache).  d_q and d_out [sequences][n_heads][head_dim], rows
+ * ldq and ldo apart, n_heads a multiple of n_kv_heads (query head h reads kv
+ * head h / (n_heads / n_kv_heads)); scale 0: 1 / sqrt(head_dim).  max_prefix
+ * and max_suffix bound the lengths, which are cut to them (they and the table
  * widths decide the split of the work, so a captured call keeps them) and are
- * at most 2^31 - 2^16; a negative length is 0.  Positions in pages outside the pool are left out;
- * a sequence with no position gives zeros.  Scores, softmax and sums are f32;
- * 16-bit pools are read as stored.  d_q and the keys and values of the
- * positions that count are finite (an infinity among them may give NaN where
- * the formula has a limit); what lies behind a length or in slots that no
- * length reaches may hold anything.  d_out is apart from d_q.  At most 65535
- * sequences, and sequences * n_heads below 2^24.  The workspace holds the parts of a split
- * prefix or suffix (size from syn_hip_prefix_attention_workspace, which may
- * be 0; 16-byte aligned). */
+ * at most 2^31 - 2^16; a negative length is 0.  Positions in pages outside the
+ * pool are left out; a sequence with no position gives zeros.  Scores, softmax
+ * and sums are f32; 16-bit pools are read as stored (an f16 pool's products
+ * take a query's elements to 2^-22 of themselves or 2^-36 of the row's
+ * largest).  d_q and the keys and values of the positions that count are finite
+ * (an infinity among them may give NaN where the formula has a limit); what
+ * lies behind a length or in slots that no length reaches may hold anything.
+ * d_out is apart from d_q.  At most 65535 sequences, and sequences * n_heads
+ * below 2^24.  The workspace holds the parts of a split prefix or suffix (size
+ * from syn_hip_prefix_attention_workspace, which may be 0; 16-byte aligned). */
 typedef struct {
   uint32_t layer, n_heads, n_groups, group_size, max_prefix, max_suffix;
   float scale;

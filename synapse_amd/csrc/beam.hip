@@ -22,12 +22,14 @@ namespace {
 // are formed, n values at least are not below the least of the groups' maxima,
 // and few are; those go to LDS, where each counts the ones before it.
 //
-// Bytes and exponentials bound it: every logit is read once and costs about ten
-// instructions, one of them an exponential, which together take as long as the
-// read.  128 rows of 151936 logits, 16 to choose: 28.9 us, the chunks 20 (3.9
-// TB/s), the join of 152 lists of 16 a group 8; 32 rows of 128256: 13.4 us; 4
-// rows of 32000: 8.9, two launches.  A single launch would need counters that
-// are zero at the start, which a caller's workspace is not.
+// 128 rows of 151936 logits, 16 to choose: 29.4 us, the chunks 20 (3.9 TB/s),
+// the join of 152 lists of 16 a group 9; 32 rows of 128256: 13.5 us; 4 rows of
+// 32000: 9.2, two launches.  The chunks are bound neither by the read (16 us at a
+// copy's rate) nor by their instructions (vector instructions in 45 % of the
+// SIMDs' cycles): a workgroup has loaded all of its chunk before it computes and
+// has nothing in flight then, and 2432 workgroups at six a CU are 1.6 rounds.  A
+// single launch would need counters that are zero at the start, which a caller's
+// workspace is not.
 //
 // Equal values go to the lower beam; within a beam the order is that of the
 // logits everywhere (f64 may hold two of them as the same value), equal ones
@@ -141,8 +143,8 @@ __device__ __forceinline__ Cand cand_of(uint64_t key) {
 constexpr int kChunkNT = 256;
 constexpr int kWaveCap = 256;  // of a wave's candidates
 
-// PER values a thread, which stay in registers; six waves a SIMD (28.9 us at 128
-// rows of 151936, five 30.0, seven 30.7).
+// PER values a thread, which stay in registers; six waves a SIMD (29.5 us at 128
+// rows of 151936, five 29.9, seven 30.8).
 template <int PER>
 __global__ void __launch_bounds__(kChunkNT, 6) k_beam_chunks(SelectArgs a) {
   __shared__ __align__(16) uint64_t list[4][kWaveCap];
@@ -161,8 +163,8 @@ __global__ void __launch_bounds__(kChunkNT, 6) k_beam_chunks(SelectArgs a) {
   const float *x0 = a.logits + (size_t)row * a.ld + first;
   float x[PER];
   if (left >= 4) {
-    // (a 16-byte load needs 4-byte alignment only: 128 rows of 151935, 8 to
-    // choose, 20.5 us; 25.6 with 4-byte loads)
+    // (a 16-byte load needs 4-byte alignment only: 128 rows of 151935, 80 of them
+    // live, 8 to choose, 20.5 us; 25.6 with 4-byte loads)
     typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll
     for (int i = 0; i < PER; i += 4) {
@@ -286,7 +288,7 @@ constexpr int kMergeNT = 1024;
 constexpr int kMergeCap = 1024;
 
 // One workgroup a group: the sums of a beam's chunks joined in f64, then the
-// best of all lists.  4 us for one group of 4 beams, 8 for 16 groups of 152
+// best of all lists.  4.3 us for one group of 4 beams, 9 for 16 groups of 152
 // lists at once: latency (f64 logarithms, four barriers, the ranks in LDS).
 __global__ void __launch_bounds__(kMergeNT) k_beam_merge(SelectArgs a) {
   struct Pick {
@@ -488,9 +490,10 @@ SelectSpace select_space(const syn_hip_beam_select_params &p) {
   const size_t rows = (size_t)p.n_groups * p.n_beams;
   SelectSpace s;
   // Chunks of 8192 logits; of 2048 where fewer than 128 would be at work (4 rows
-  // of 32000, 16 chunks: 11.0 us against 10.1; 4 of 128256, 64: 11.4 and 10.9;
-  // 8 of 128256, 128: 12.2 and 12.8; 32: 13.4 and 16.5).  4096 a chunk take 36 us
-  // where 8192 take 29, 16384 35: the lists that are joined, and registers.
+  // of 32000, 16 chunks: 10.6 us against 9.5; 4 of 128256, 64: 10.6 and 10.1; 8 of
+  // 128256, 128: 12.7 and 13.6; 32: 14.7 and 17.4).  At 128 rows of 151936 4096 a
+  // chunk take 38 us where 8192 take 29.5, 16384 35: the lists that are joined,
+  // and registers.
   s.per = rows * cdiv(p.vocab, kChunkNT * 32) >= 128 ? 32 : 8;
   s.chunks = (int)cdiv(p.vocab, (size_t)kChunkNT * s.per);
   s.stat = 0;

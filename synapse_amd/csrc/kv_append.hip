@@ -44,8 +44,8 @@ __device__ __forceinline__ float row_sum(float x) {
 // comes from the token's row in LDS, which only its own wave writes.  The next
 // head is requested before this one is worked on.  Bound by its bytes, read
 // once and written once: 8192 tokens of 32 + 2 * 8 heads of 128 into f16 pages
-// 88 us, 4.1 TB/s (a large copy reaches 4.8); 517 tokens of 40 heads into bf16
-// 8.4 us, three dependent loads (place, page, angles) and one round of heads; 4
+// 89 us, 4.1 TB/s (a large copy reaches 4.8); 517 tokens of 16 + 2 * 8 heads into
+// bf16 8.5 us, three dependent loads (place, page, angles) and one round of heads; 8
 // tokens 4.7, a launch.  KD: 64 dims each (hd <= 64 KD).
 template <class T, int KD>
 __global__ void __launch_bounds__(kThreads) k_kv_append(AppendArgs a, KvPool<T> pool) {
@@ -313,8 +313,8 @@ extern "C" syn_status_t syn_hip_kv_append(
   a.vec_rot = aligned16(d_cos) && aligned16(d_sin) && p->rotary_dim % 8 == 0;
   a.vec_gain = aligned16(d_q_norm) && aligned16(d_k_norm);
   // Workgroups enough to fill the chip, then heads in turn, whose angles are
-  // there already (8192 tokens of 48 heads: 97 us with 1024 workgroups, 95 with
-  // 2048, 107 with 512 and 4096; 517: 9.9, 11.3, 10.3, 11.2).
+  // there already (8192 tokens of 48 heads: 89 us with 1024 workgroups, 87 with
+  // 2048, 103 with 512, 98 with 4096; 517 of 32: 8.6, 8.7, 9.2, 8.7).
   const size_t tiles = cdiv(n_tokens, kTok), heads = nh + 2 * nkv;
   const dim3 grid((unsigned)tiles, (unsigned)std::min(heads, std::max<size_t>(1, cdiv(1024, tiles))));
   return kv_dispatch(pages->dtype, [&](auto t) -> syn_status_t {

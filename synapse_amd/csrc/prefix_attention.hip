@@ -22,11 +22,11 @@
 //
 // What bounds it (a large copy reaches 4.8 TB/s here, a stream of reads alone
 // more, large products 1115 TFLOP/s in f16 and 152 in f32): up to 16 rows of a
-// kv head, bytes: 64 sequences of up to 4000 positions, 8 kv heads of 128, f16,
-// 186 us, 5.6 TB/s; a shared prefix of 4 * 32768 under 4 to 16 rows 98 to 101
-// us, 5.5 to 5.3 TB/s.  32 rows 5.1, 64 rows 4.6 TB/s and 290 TFLOP/s of the
+// kv head, bytes: 64 sequences of 4000 positions, 8 kv heads of 128, f16, 191
+// us, 5.5 TB/s; a shared prefix of 4 * 32768 under 4 to 16 rows 99 to 101 us,
+// 5.4 to 5.3 TB/s.  32 rows 5.0, 64 rows 4.6 TB/s and 290 TFLOP/s of the
 // formula, 580 in matrix instructions with the operands' second parts; 128 rows
-// 370 and 740.  f32, 64 rows: 2.6 TB/s, 84 TFLOP/s, the matrix instructions.
+// 380 and 760.  f32, 64 rows: 3.0 TB/s, 97 TFLOP/s, the matrix instructions.
 // Short calls are latency: 4 sequences of 113 positions 7.5 us.
 #include <algorithm>
 #include <cmath>
@@ -206,8 +206,8 @@ template <class T, int NC, bool FULL> struct Rows {
   float m, l, unscale;
 
   // The rows' queries times scale, each row for an f16 pool times the power of
-  // two that puts its largest element into [2^11, 2^12): both parts of every
-  // element that matters are normal.  Rows past the last repeat it.
+  // two that puts its largest element into [2^11, 2^12): an element is held to
+  // 2^-22 of itself, or 2^-36 of the row's largest.  Rows past the last repeat it.
   __device__ __forceinline__ void load_queries(const AttnArgs &a, int hd, int seq0, int head, int row,
                                                int last) {
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
@@ -860,10 +860,11 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_prefix_attention_params
   const size_t seqs = (size_t)p.n_groups * p.group_size;
   // One launch, each sequence's rows whole, where a second launch would cost
   // more than the prefix read again for every sequence (from L2): 24 heads of
-  // 128, 8 sequences, f16: 900 positions 11.2 us against 12.2 in parts, 1600
-  // 14.7 against 12.9; 128 sequences of 900, 32.6 against 31.0.  An f32 tile has
-  // twice the bytes and four times the matrix instructions' time: 500 positions
-  // 17.9 us, 900 in parts 12.8.
+  // 128, 8 sequences, f16: 200 positions 7.2 us against 10.5 in parts, 600 9.0
+  // against 10.6, 900 10.9 against 10.7, 1600 14.0 against 11.2; 128 sequences of
+  // 200 15.0 against 18.4, of 400 20.4 against 18.8.  An f32 tile has twice the
+  // bytes and four times the matrix instructions' time: 200 positions 10.4 us
+  // against 11.6, 500 17.8 against 11.7.
   const size_t whole = pg.dtype == SYN_HIP_KV_F32 ? 2 : (seqs * nkv <= 512 ? 8 : 4);
   w.joined = (size_t)p.max_prefix + p.max_suffix <= whole * kTile * kWaves;
   w.prw = tiles((size_t)p.group_size * rep);
@@ -871,8 +872,9 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_prefix_attention_params
   const size_t sblocks = cdiv(rep, 16 * w.srw), sunits = seqs * nkv;
   // Parts of about equal work for as many workgroups as the chip holds at
   // once, four a CU, two, or one.  (512 workgroups of 64 dims in 16 bits,
-  // 48 sequences of 1500 positions over a shared 8200: 45 us, 1024: 40; of 128
-  // dims, 64 sequences over four prefixes of 32768: 110 and 127.)
+  // 48 sequences of 1500 positions over a shared 8200: 45 us, 1024: 38.7 in bf16,
+  // 37.8 in f16; of 128 dims, 64 sequences over four prefixes of 32768: 111 and
+  // 119.)
   const size_t want = w.nc == 8 ? 256 : (w.nc == 4 || pg.dtype == SYN_HIP_KV_F32 ? 512 : 1024);
   const size_t ptiles = cdiv(p.max_prefix, kTile), stiles = cdiv(p.max_suffix, kTile);
   // Many short runs of a sequence's own: a wave for each, where the rounds of
@@ -898,9 +900,9 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_prefix_attention_params
     *chunk = (int)(each * kTile);
     *n = each ? (int)cdiv(tiles, each) : 0;
   };
-  // Waves that share tiles take them all, so a part may be short: two tiles (32
-  // rows of f32 over 512 positions 13.7 us, 16.3 with four; one tile takes 15.2
-  // where two take 13.5 at 24 rows of f16 over 4001: the join).
+  // Waves that share tiles take them all, so a part may be short: two tiles (160
+  // rows of f16 over 4001 positions 25.6 us, 26.8 with four, 24.7 with one; up to
+  // 64 rows over 300 to 4001 the three are alike).
   constexpr size_t kGrain = 2;
   for (size_t per = std::max<size_t>(1, cdiv(total, want));; per += kGrain + per / 16) {
     cut(ptiles, per, w.prw == 1 ? kWaves : kGrain, &w.pchunk, &w.npp);
