@@ -130,3 +130,11 @@ def test_rows_of_which_some_have_a_sink():
     c.q[1::3, ::64] = -4.0   # the sink is far below the rest
     c.q[2::3, ::64] = 0.0
     compare(c)
+
+
+@pytest.mark.parametrize("dtype,orders", [("f16", 22), ("f16", 110), ("bf16", 90), ("f32", 110)])
+@pytest.mark.parametrize("layout", LAYOUTS, ids=str)
+def test_what_a_sink_leaves_in_pages_of_whole_tiles(layout, dtype, orders):
+    """(a weight's third bf16 part is 2^-16 of it, so a bf16 pool's weights keep
+    f32's bits down to 2^-110)"""
+    compare(sink(dtype, *layout, orders, 0, page=64))
