@@ -406,9 +406,11 @@ template <class T, int NC, bool FULL> struct Rows {
   // Weights of which two parts would keep few bits or none: lifted until they are
   // not, their products are added to the sums in f32.  (At most nine rounds: no
   // weight is below 2^-149.)  Calls without such weights pay for the test and the
-  // registers, 0 to 1 % at 128 dims (four prefixes of 32768 under 64 rows 109.8
-  // us, 108.7 without), 10 % at 64 (48 sequences over 8200: 37.9, 34.4); scores
-  // spread over 36 binary orders take 215 us where 109 do without.
+  // registers: at 128 dims 1 % (four prefixes of 32768 under 64 rows 109.8 us,
+  // 108.7 without) to 7 % (two of 8000 under 128 rows 38.8, 36.4), at 64, where a CU
+  // then holds three workgroups and not four, 10 % (48 sequences over 8200: 37.9,
+  // 34.4).  Scores spread over 36 binary orders, where most tiles come here, take
+  // 215 us where 109 do without.
   __device__ __forceinline__ void add_small(float *y, const V *v) {
     float back = 1.0f;
     bool left = false;
