@@ -162,6 +162,7 @@ CASES = [(4, 8, 20, "f32", False, 0, -1, F32), (4, 8, 20, "f32", False, 1, 219, 
          (4, 8, 20, "f16", True, 0, -1, PAGES), (4, 8, 20, "f16", True, 40, 252, PAGES),
          (8, 7, 18, "bf16", False, 2, -1, PAGES), (8, 7, 18, "bf16", False, 82, 60, PAGES),
          (2, 1, 40, "f16", False, 40, -1, PAGES), (2, 1, 40, "f16", False, 1, 135, PAGES),
+         (2, 1, 40, "f16", False, 1, 280, PAGES),  # all beams end, and the search with them
          (7, 1, 17, "bf16", True, 34, -1, PAGES), (7, 1, 17, "bf16", True, 5, 99, PAGES),
          (12, 33, 6, "f32", True, 33, -1, ROWS), (12, 33, 6, "f32", True, 33, 75, ROWS),
          (4, 21, 12, "f16", False, 4, -1, ROWS), (4, 21, 12, "f16", False, 2, 167, ROWS),
