@@ -791,6 +791,127 @@ syn_status_t syn_hip_klm_generate_beams(syn_hip_klm_t *m, const uint32_t *prompt
                                         uint32_t *out_tokens, uint32_t *out_lengths,
                                         float *out_scores);
 
+/* =====================================================================
+ * 4. Sampling with drafts over a paged cache (no reference counterpart: its
+ *    speculative loop accepts every draft): attention of several new tokens of
+ *    a sequence, verification of drafted tokens, and the pages of sequences
+ *    that grow, are cut back, and continue one another.  As in section 3: the
+ *    caller's buffers on the current device, calls asynchronous on `stream`
+ *    that allocate nothing and may be captured, a workspace for each of two
+ *    calls that overlap.
+ * =================================================================== */
+
+/* Causal attention of the new tokens of each of n_seqs sequences over its
+ * pages: one token (decoding), a few (drafts), many (a chunk of a prompt).
+ * Rows d_start[s] .. d_start[s + 1] - 1 of d_q and d_out (d_start [n_seqs + 1],
+ * never falling, cut to [0, n_tokens]; NULL: max_new rows each) are sequence
+ * s's n new tokens, at most max_new (what is above that is left out, its rows
+ * as they are).  Their keys and values are in the pages already, the last n of
+ * the sequence's d_len[s] positions (cut to [0, max_len]), found through row s
+ * of d_table [n_seqs][ld_table].  Row j sees the positions up to its own,
+ * d_len[s] - n + j, with a window (0: none) the last `window` of those; a row
+ * that sees none gives zeros.  d_q and d_out [n_tokens][n_heads][head_dim],
+ * rows ldq and ldo apart; rows of no sequence are left as they are.  Heads,
+ * scale, pages outside the pool, values behind a length, precision: as
+ * syn_hip_prefix_attention.  max_new, max_len and n_tokens decide the split of
+ * the work, so a captured call keeps them.  d_out is apart from d_q.  At most
+ * 65535 sequences, max_len 2^31 - 2^16, max_new * n_heads below 2^30.  The
+ * workspace (which may be 0; 16-byte aligned) holds the parts of split runs. */
+typedef struct {
+  uint32_t layer, n_heads, n_seqs, n_tokens, max_new, max_len, window;
+  float scale;
+  size_t ldq, ldo, ld_table;
+} syn_hip_paged_attention_params;
+syn_status_t syn_hip_paged_attention_workspace(const syn_hip_kv_pages *pages,
+                                               const syn_hip_paged_attention_params *p,
+                                               size_t *bytes);
+syn_status_t syn_hip_paged_attention(const syn_hip_kv_pages *pages,
+                                     const syn_hip_paged_attention_params *p, const float *d_q,
+                                     const int32_t *d_start, const int32_t *d_len,
+                                     const int32_t *d_table, float *d_out, void *d_workspace,
+                                     size_t workspace_bytes, void *stream);
+
+/* Verification of drafted tokens.  Sequence s has n = d_n_draft[s] drafts (NULL:
+ * max_draft; cut to it), d_drafted [n_seqs][max_draft].  p_i is the softmax of
+ * logits row i of the target at s * target_stride + i * ld_target floats (0 to n;
+ * a stride may be 0), divided by the temperature d_temperature[s] (NULL: 1), q_i
+ * that of the draft's row at s * draft_stride + i * ld_draft (0 to n - 1; d_draft
+ * NULL: drafts that were certain, q 1 at the draft and 0 elsewhere).  Draft x_i
+ * is accepted when all before it are and u_i q_i(x_i) < p_i(x_i), u_i being
+ * d_u[s * (max_draft + 1) + i], in [0, 1).  Then one token is drawn, after r
+ * accepted drafts from max(p_r - q_r, 0) when r < n (where that is 0 everywhere,
+ * from p_r), else from p_n: the lowest t whose weights up to t sum to more than u
+ * times all, u = d_u[s * (max_draft + 1) + max_draft].  With max_draft 0 this
+ * draws a token from each row.  A temperature that is not above 0, or is not
+ * finite, is a greedy sequence: a draft is accepted when it is its row's first
+ * largest logit, and that of row r follows; its draft rows are not read.
+ * d_token [n_seqs][max_draft + 1] gets the accepted drafts, the token, then pad;
+ * d_count[s] the number of tokens before pad (r + 1).  n < 0: the sequence is
+ * not read, its count is 0.  d_logp (nullable) [n_seqs][max_draft + 1]: the
+ * tokens' log-probabilities under p_i (0 when greedy, and at pad).  A NaN logit
+ * counts as -inf; a row whose largest is +inf shares its probability among the
+ * infinities; a draft outside the vocabulary is not accepted; where row r has no
+ * logit above -inf the token is pad (and counted) with log-probability -inf.
+ * Exponentials and sums are f64: a token differs from the formula's only where u
+ * falls within 2^-40 of a border.  d_token is apart from the other buffers.  At most 64 drafts, n_seqs *
+ * (2 max_draft + 1) at most 65535.  The workspace (16-byte aligned) is needed by
+ * every call. */
+typedef struct {
+  uint32_t n_seqs, max_draft, pad;
+  size_t vocab, ld_target, target_stride, ld_draft, draft_stride;
+} syn_hip_draft_verify_params;
+syn_status_t syn_hip_draft_verify_workspace(const syn_hip_draft_verify_params *p, size_t *bytes);
+syn_status_t syn_hip_draft_verify(const syn_hip_draft_verify_params *p, const float *d_target,
+                                  const float *d_draft, const uint32_t *d_drafted,
+                                  const int32_t *d_n_draft, const float *d_temperature,
+                                  const float *d_u, uint32_t *d_token, int32_t *d_count,
+                                  float *d_logp, void *d_workspace, size_t workspace_bytes,
+                                  void *stream);
+
+/* The page tables of n_seqs sequences over a pool of n_pages pages, on the
+ * device: row s of table [n_seqs][ld_table] holds held[s] pages, -1 behind
+ * them; refs[page] counts the entries that name a page, and a page of count 0
+ * is free (one that the caller keeps for itself has a count that it gave it).
+ * To begin: table all -1, held and refs all 0.  Where pages are taken, the free
+ * pages of lowest number are, the rows in order and a row's columns in order;
+ * where there are too few, held tells what a row got.  Entries outside
+ * [0, n_pages) name no page.  At most 2^24 pages, 65535 rows, n_seqs *
+ * ld_table below 2^31. */
+typedef struct {
+  uint32_t page_size, n_pages, n_seqs;
+  size_t ld_table;
+  int32_t *table, *held, *refs;
+} syn_hip_kv_tables;
+/* the workspace of a call on these tables (16-byte aligned) */
+syn_status_t syn_hip_kv_tables_workspace(const syn_hip_kv_tables *t, size_t *bytes);
+/* Every row holds the pages of d_len[s] positions (as many as the row has room
+ * for; a negative length: the row stays as it is): those above are given back,
+ * then missing ones are taken.  So a sequence grows, is cut back to what was
+ * accepted, or ends (0). */
+syn_status_t syn_hip_kv_resize(const syn_hip_kv_tables *t, const int32_t *d_len, void *d_workspace,
+                               size_t workspace_bytes, void *stream);
+/* Row s continues row d_parent[s]: it gives back its pages, then holds those of
+ * the parent's first d_len[s] positions (at most what the parent's pages hold;
+ * below 0: 0): full pages are shared, one that is not full is copied, every
+ * layer, positions up to the next multiple of 8, into a page that is taken for
+ * it (where none is free, the row ends with the full ones).  A row whose
+ * d_parent is itself or outside [0, n_seqs), or whose parent continues another
+ * row, stays as it is.  pages and t have the same n_pages and page_size. */
+syn_status_t syn_hip_kv_fork(const syn_hip_kv_pages *pages, const syn_hip_kv_tables *t,
+                             const int32_t *d_parent, const int32_t *d_len, void *d_workspace,
+                             size_t workspace_bytes, void *stream);
+/* The pages of a count above 0, every layer, to the front of another pool in
+ * the order of their numbers, with their counts; the tables' rows rename them,
+ * -1 behind what a row holds.  *d_live (device) is how many there are: those
+ * that the other pool has no page for are left out, and entries that name them
+ * become -1.  The pools have the same pages but for their number, and overlap
+ * nowhere; the tables have the same rows, u at least as many columns.  The
+ * workspace is t's. */
+syn_status_t syn_hip_kv_compact(const syn_hip_kv_pages *from, const syn_hip_kv_tables *t,
+                                const syn_hip_kv_pages *to, const syn_hip_kv_tables *u,
+                                int32_t *d_live, void *d_workspace, size_t workspace_bytes,
+                                void *stream);
+
 /* -- harness helpers (no reference counterpart) -- */
 /* Encode f32 [n,k] into Q8_0 / Q4_K / Q6_K block bytes.  The reference has no
  * encoder for these formats (only dequantizers); any encoding is valid since

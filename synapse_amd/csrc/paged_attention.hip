@@ -1,0 +1,296 @@
+// Causal attention of the new tokens of each sequence over its pages: one token
+// (decoding), a few (drafts to be verified), many (a prompt's chunk).
+//
+// Row j of a sequence's n new tokens, which are the last n of its len positions,
+// is softmax(scale q k_i) over i from len - n + j back, as far as the window
+// reaches.  The rows of a kv head, all tokens' query heads that read it, are the
+// columns of the two products of attend_rows.hpp, 16, 32 or 64 to a workgroup: a
+// key or value that several tokens see is read for all of them at once.
+#include <algorithm>
+#include <cmath>
+
+#include "attend_rows.hpp"
+
+namespace syn {
+
+namespace {
+
+struct PagedArgs : RowArgs {
+  const int32_t *start, *len, *table;
+  size_t ld_table;
+  int n_seqs, n_tokens, max_new, max_len, window;
+  int chunk;   // positions of a part (a multiple of kTile)
+  int rw;      // tiles of 16 rows of a workgroup: 1, 2 or 4
+  int blocks;  // workgroups for the rows of the longest sequence
+  bool solo;   // a wave for a sequence's rows
+};
+
+__device__ __forceinline__ int scalar(const int32_t *p, int i) {
+  const auto *t = (const __attribute__((address_space(4))) int32_t *)(uintptr_t)p;  // a scalar load
+  return t[i];
+}
+// a sequence's new tokens: the first one's row, and how many
+__device__ __forceinline__ int first_of(const PagedArgs &a, int s) {
+  return a.start ? min(max(scalar(a.start, s), 0), a.n_tokens) : s * a.max_new;
+}
+__device__ __forceinline__ int count_of(const PagedArgs &a, int s, int first) {
+  const int end = a.start ? min(max(scalar(a.start, s + 1), first), a.n_tokens) : first + a.max_new;
+  return min(end - first, a.max_new);
+}
+
+template <class T, int NC, bool FULL>
+__global__ void __launch_bounds__(64 * kWaves, (kResident<T, NC, FULL>)) k_attend_new(PagedArgs a, KvPool<T> pool) {
+  using W = Rows<T, NC, FULL, true>;
+  __shared__ __align__(16) uint8_t lds[W::kLdsBytes];
+  __shared__ float ml[kWaves * 16 * 2];
+  // workgroup i runs on XCD i % 8: the blocks of rows that read the same
+  // positions come 8 apart and share that XCD's L2; the last rows, which see
+  // most, go first
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = blockIdx.x, j = i >> 3, block = a.blocks - 1 - j % a.blocks;
+  int unit = (j / a.blocks) * 8 + (i & 7);
+  if (a.solo) unit = unit * kWaves + wave;
+  const int head = unit % pool.nkv, u = unit / pool.nkv;
+  const int part = u % a.parts, s = u / a.parts;
+  if (s >= a.n_seqs) return;
+  const int first = first_of(a, s), count = count_of(a, s, first), all = count * a.rep;
+  const int RW = a.rw, row0 = block * RW * 16, rows = min(RW * 16, all - row0);
+  if (rows <= 0) return;
+  const int len = min(max(scalar(a.len, s), 0), a.max_len);
+  // token j sees the positions below lim_of(j), from lo_of(j) on
+  auto lim_of = [&](int token) { return len - count + token + 1; };
+  auto lo_of = [&](int token) { return a.window && lim_of(token) > a.window ? lim_of(token) - a.window : 0; };
+  const int last = row0 + rows - 1;
+  const int to = max(0, lim_of(last / a.rep)), from = min(lo_of(row0 / a.rep) & ~(kTile - 1), to);
+  Run r{a.table + (size_t)s * a.ld_table, from, to, 0};
+  int at = -1;
+  if (a.parts > 1) {
+    at = part;
+    const int64_t begin = from + (int64_t)part * a.chunk;
+    if (begin >= to) {  // nothing here: no rows to write, a sum of 0
+      for (int k = a.solo ? (int)threadIdx.x & 63 : (int)threadIdx.x; k < rows; k += 64 * kWaves) {
+        const int row = row0 + k, token = row / a.rep;
+        const size_t p = ((size_t)(first + token) * a.nh + (size_t)head * a.rep + (row - token * a.rep)) * a.parts + at;
+        a.pml[p * 2] = kNegInf;
+        a.pml[p * 2 + 1] = 0.0f;
+      }
+      return;
+    }
+    r.from = (int)begin;
+    r.to = r.from + min(a.chunk, to - r.from);
+  }
+  const size_t head_bytes = (size_t)pool.hd * pool.ps * sizeof(T);
+  const HeadBase hb{reinterpret_cast<const uint8_t *>(pool.k) + head * head_bytes,
+                    reinterpret_cast<const uint8_t *>(pool.v) + head * head_bytes,
+                    (uint32_t)(pool.nkv * head_bytes)};
+  const bool wide = pool.ps >= kTile;
+  uint32_t ok = 0;
+  if (RW == 4)
+    ok = wide ? W::template start_shared<true, 1>(pool, hb, r, lds)
+              : W::template start_shared<false, 1>(pool, hb, r, lds);
+  if constexpr (W::kRing == 4)
+    if (RW == 2)
+      ok = wide ? W::template start_shared<true, 2>(pool, hb, r, lds)
+                : W::template start_shared<false, 2>(pool, hb, r, lds);
+  W w;
+  const int mine = row0 + (wave & (RW - 1)) * 16;
+  w.load_queries(a, pool.hd, first, head, mine, last);
+  {
+    const int token = min(mine + (int)(threadIdx.x & 15), last) / a.rep;
+    w.see(lo_of(token), lim_of(token), lo_of(min(mine + 15, last) / a.rep), lim_of(min(mine, last) / a.rep));
+  }
+  if (RW == 1) {
+    if (wide)
+      w.template run_alone<true>(pool, hb, r, a.solo ? 1 : kWaves);
+    else
+      w.template run_alone<false>(pool, hb, r, a.solo ? 1 : kWaves);
+    if (a.solo) {
+      w.finish_alone(a, pool.hd, first, head, row0, rows, at);
+      return;
+    }
+  } else if (RW == 4) {
+    if (wide)
+      w.template run_shared<true, 1>(pool, hb, r, lds, ok);
+    else
+      w.template run_shared<false, 1>(pool, hb, r, lds, ok);
+  } else if constexpr (W::kRing == 4) {
+    if (wide)
+      w.template run_shared<true, 2>(pool, hb, r, lds, ok);
+    else
+      w.template run_shared<false, 2>(pool, hb, r, lds, ok);
+  }
+  w.finish(a, pool.hd, first, head, row0, rows, RW, at, reinterpret_cast<float *>(lds), ml);
+}
+
+// one workgroup for a query row of a sequence (those past its last token leave)
+template <int LANES> __global__ void __launch_bounds__(256) k_join_new(PagedArgs a, int hd) {
+  const size_t row = blockIdx.x / a.nh;
+  const int head = blockIdx.x - row * a.nh, s = row / a.max_new, token = row - (size_t)s * a.max_new;
+  const int first = first_of(a, s);
+  if (token >= count_of(a, s, first)) return;
+  join_parts<LANES>(a, hd, (size_t)(first + token) * a.nh + head);
+}
+
+// ---------------------------------------------------------------- host
+struct Plan {
+  bool solo;
+  int nc, rw, blocks, chunk, parts;
+  size_t wgs, rows, po_bytes, pml_bytes;
+};
+
+Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_paged_attention_params &p) {
+  Plan w{};
+  const int hd = (int)pg.head_dim, nkv = (int)pg.n_kv_heads;
+  const size_t rep = p.n_heads / nkv, rows = p.max_new * rep;
+  w.nc = hd <= 64 ? 2 : (hd <= 128 ? 4 : 8);
+  const bool small = w.nc * (pg.dtype == SYN_HIP_KV_F32 ? 2 : 1) <= 4;  // (a ring of four tiles)
+  w.rw = rows <= 16 ? 1 : (rows <= 32 ? (small ? 2 : 1) : 4);
+  w.blocks = (int)cdiv(rows, 16 * w.rw);
+  w.rows = (size_t)p.n_seqs * p.max_new * p.n_heads;
+  // the positions of a workgroup's rows
+  const size_t tokens = std::min<size_t>(p.max_new, 16 * w.rw / rep + 2);
+  const size_t span = p.window ? std::min<size_t>(p.max_len, (size_t)p.window + tokens + kTile) : p.max_len;
+  const size_t tiles = cdiv(span, kTile), units = (size_t)p.n_seqs * nkv;
+  const size_t want = w.nc == 8 ? 256 : (w.nc == 4 || pg.dtype == SYN_HIP_KV_F32 ? 512 : 1024);
+  const size_t whole = pg.dtype == SYN_HIP_KV_F32 ? 2 : (units <= 512 ? 8 : 4);
+  constexpr size_t kFix = 6;
+  auto alone = [&](size_t units, size_t tiles) {
+    return w.rw == 1 && cdiv(cdiv(units, kWaves) * w.blocks, want) * (kFix + tiles) <
+                            cdiv(units * w.blocks, want) * (kFix + cdiv(tiles, kWaves));
+  };
+  w.parts = 1;
+  w.chunk = (int)(tiles * kTile);
+  const size_t each = std::max<size_t>(1, cdiv(units * w.blocks * tiles, want));
+  const size_t grain = w.rw == 1 ? kWaves : 2;
+  if (tiles > whole * kWaves && each < tiles) {
+    const size_t k = cdiv(tiles, round_up(each, grain));
+    const size_t per = round_up(cdiv(tiles, k), grain);
+    w.chunk = (int)(per * kTile);
+    w.parts = (int)cdiv(tiles, per);
+  }
+  w.solo = alone(units * w.parts, w.chunk / kTile);
+  const size_t work = units * w.parts;
+  w.wgs = round_up(w.solo ? cdiv(work, kWaves) : work, 8) * w.blocks;
+  if (w.parts > 1) {
+    const size_t n = (size_t)p.n_tokens * p.n_heads * w.parts;
+    w.po_bytes = round_up(n * hd * 4, 16);
+    w.pml_bytes = round_up(n * 8, 16);
+  }
+  return w;
+}
+
+syn_status_t check(const syn_hip_kv_pages *pages, const syn_hip_paged_attention_params *p) {
+  if (!p) return SYN_ERR_NULL_PTR;
+  SYN_TRY(check_pages(pages, "paged_attention"));
+  const size_t hd = pages->head_dim;
+  if (p->layer >= pages->n_layers || !p->n_heads || p->n_heads % pages->n_kv_heads || p->n_heads > 65535u) {
+    set_error("paged_attention: layer outside the pool, or n_heads no multiple of n_kv_heads");
+    return SYN_ERR_INVALID_ARG;
+  }
+  // (kernels look two rounds of tiles past a length, and count rows, in 32 bits)
+  if (p->n_seqs > 65535u || p->max_len > 0x7fff0000u || p->n_tokens > 0x7fffffffu ||
+      p->max_new > p->n_tokens || (uint64_t)p->max_new * p->n_heads > 0x3fffffffu) {
+    set_error("paged_attention: more than 65535 sequences, 2^31 - 2^16 positions or 2^30 - 1 query rows of "
+              "a sequence, or max_new above n_tokens");
+    return SYN_ERR_INVALID_ARG;
+  }
+  if (p->ldq < p->n_heads * hd || p->ldo < p->n_heads * hd || p->ld_table < cdiv(p->max_len, pages->page_size)) {
+    set_error("paged_attention: rows or page tables shorter than the heads or the lengths");
+    return SYN_ERR_SHAPE_MISMATCH;
+  }
+  if (!p->n_seqs || !p->max_new) return SYN_OK;
+  const Plan w = make_plan(*pages, *p);
+  if (w.wgs > kMaxThreads / (64 * kWaves) || (w.parts > 1 && w.rows > kMaxThreads / 256)) {
+    set_error("paged_attention: more workgroups than a launch takes");
+    return SYN_ERR_INVALID_ARG;
+  }
+  return SYN_OK;
+}
+
+template <class T, int NC>
+syn_status_t launch(const Plan &w, const PagedArgs &a, const KvPool<T> &pool, hipStream_t s) {
+  const dim3 grid((unsigned)w.wgs), block(64 * kWaves);
+  if (pool.hd == 32 * NC)
+    hipLaunchKernelGGL((k_attend_new<T, NC, true>), grid, block, 0, s, a, pool);
+  else
+    hipLaunchKernelGGL((k_attend_new<T, NC, false>), grid, block, 0, s, a, pool);
+  SYN_LAUNCH_CHECK();
+  if (w.parts == 1) return SYN_OK;
+  const dim3 rows((unsigned)w.rows);
+  hipLaunchKernelGGL((k_join_new<8 * NC>), rows, dim3(256), 0, s, a, pool.hd);
+  SYN_LAUNCH_CHECK();
+  return SYN_OK;
+}
+
+}  // namespace
+
+}  // namespace syn
+
+using namespace syn;
+
+extern "C" syn_status_t syn_hip_paged_attention_workspace(const syn_hip_kv_pages *pages,
+                                                          const syn_hip_paged_attention_params *p,
+                                                          size_t *bytes) {
+  if (!bytes) return SYN_ERR_NULL_PTR;
+  SYN_TRY(check(pages, p));
+  *bytes = 0;
+  if (!p->n_seqs || !p->max_new) return SYN_OK;
+  const Plan w = make_plan(*pages, *p);
+  *bytes = w.po_bytes + w.pml_bytes;
+  return SYN_OK;
+}
+
+extern "C" syn_status_t syn_hip_paged_attention(const syn_hip_kv_pages *pages,
+                                                const syn_hip_paged_attention_params *p, const float *d_q,
+                                                const int32_t *d_start, const int32_t *d_len,
+                                                const int32_t *d_table, float *d_out, void *d_workspace,
+                                                size_t workspace_bytes, void *stream) {
+  SYN_TRY(check(pages, p));
+  if (!d_start && (uint64_t)p->n_seqs * p->max_new != p->n_tokens) {
+    set_error("paged_attention: without d_start every sequence has max_new tokens");
+    return SYN_ERR_SHAPE_MISMATCH;
+  }
+  if (!p->n_seqs || !p->max_new) return SYN_OK;
+  if (!d_q || !d_out || !d_len || (p->max_len && !d_table)) return SYN_ERR_NULL_PTR;
+  const Plan w = make_plan(*pages, *p);
+  const size_t need = w.po_bytes + w.pml_bytes;
+  if (need && !d_workspace) return SYN_ERR_NULL_PTR;
+  if (need && (!aligned16(d_workspace) || workspace_bytes < need)) {
+    set_error("paged_attention: workspace unaligned or too small");
+    return SYN_ERR_INVALID_ARG;
+  }
+  SYN_TRY(ensure_init());
+  PagedArgs a{};
+  a.q = d_q;
+  a.out = d_out;
+  a.ldq = p->ldq;
+  a.ldo = p->ldo;
+  a.nh = (int)p->n_heads;
+  a.rep = (int)(p->n_heads / pages->n_kv_heads);
+  a.scale = (p->scale != 0.0f ? p->scale : 1.0f / sqrtf((float)pages->head_dim)) * kLog2e;
+  a.parts = w.parts;
+  a.po = static_cast<float *>(d_workspace);
+  a.pml = reinterpret_cast<float *>(static_cast<uint8_t *>(d_workspace) + w.po_bytes);
+  a.q16 = aligned16(d_q) && p->ldq % 4 == 0;
+  a.start = d_start;
+  a.len = d_len;
+  a.table = d_table;
+  a.ld_table = p->ld_table;
+  a.n_seqs = (int)p->n_seqs;
+  a.n_tokens = (int)p->n_tokens;
+  a.max_new = (int)p->max_new;
+  a.max_len = (int)p->max_len;
+  a.window = p->window < p->max_len ? (int)p->window : 0;
+  a.chunk = w.chunk;
+  a.rw = w.rw;
+  a.blocks = w.blocks;
+  a.solo = w.solo;
+  hipStream_t s = pick_stream(stream);
+  return kv_dispatch(pages->dtype, [&](auto t) -> syn_status_t {
+    using T = decltype(t);
+    const KvPool<T> pool = kv_pool<T>(*pages, p->layer);
+    if (w.nc == 2) return launch<T, 2>(w, a, pool, s);
+    if (w.nc == 4) return launch<T, 4>(w, a, pool, s);
+    return launch<T, 8>(w, a, pool, s);
+  });
+}

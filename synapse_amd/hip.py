@@ -97,6 +97,28 @@ class BeamSelect(C.Structure):
                 ("ld_logits", C.c_size_t)]
 
 
+class PagedAttention(C.Structure):
+    """syn_hip_paged_attention_params"""
+    _fields_ = [("layer", C.c_uint32), ("n_heads", C.c_uint32), ("n_seqs", C.c_uint32),
+                ("n_tokens", C.c_uint32), ("max_new", C.c_uint32), ("max_len", C.c_uint32),
+                ("window", C.c_uint32), ("scale", C.c_float), ("ldq", C.c_size_t),
+                ("ldo", C.c_size_t), ("ld_table", C.c_size_t)]
+
+
+class DraftVerify(C.Structure):
+    """syn_hip_draft_verify_params"""
+    _fields_ = [("n_seqs", C.c_uint32), ("max_draft", C.c_uint32), ("pad", C.c_uint32),
+                ("vocab", C.c_size_t), ("ld_target", C.c_size_t), ("target_stride", C.c_size_t),
+                ("ld_draft", C.c_size_t), ("draft_stride", C.c_size_t)]
+
+
+class KvTables(C.Structure):
+    """syn_hip_kv_tables: the page tables of sequences, on the device."""
+    _fields_ = [("page_size", C.c_uint32), ("n_pages", C.c_uint32), ("n_seqs", C.c_uint32),
+                ("ld_table", C.c_size_t), ("table", C.c_void_p), ("held", C.c_void_p),
+                ("refs", C.c_void_p)]
+
+
 class BeamSearch(C.Structure):
     """syn_hip_beam_search"""
     _fields_ = [("n_beams", C.c_uint32), ("eos", C.c_int32), ("kv_dtype", C.c_int32),
@@ -173,6 +195,17 @@ SIGNATURES = {
     "syn_hip_beam_select": (ST, [C.POINTER(BeamSelect)] + [P] * 8 + [SZ, P]),
     "syn_hip_beam_reorder_rows": (ST, [SZ, SZ, P, P, SZ, SZ, SZ, SZ, P]),
     "syn_hip_beam_reorder_pages": (ST, [C.POINTER(KvPages), SZ, SZ, P, P, P, SZ, P, P]),
+    "syn_hip_paged_attention_workspace": (ST, [C.POINTER(KvPages), C.POINTER(PagedAttention),
+                                               C.POINTER(SZ)]),
+    "syn_hip_paged_attention": (ST, [C.POINTER(KvPages), C.POINTER(PagedAttention)] + [P] * 6
+                                + [SZ, P]),
+    "syn_hip_draft_verify_workspace": (ST, [C.POINTER(DraftVerify), C.POINTER(SZ)]),
+    "syn_hip_draft_verify": (ST, [C.POINTER(DraftVerify)] + [P] * 10 + [SZ, P]),
+    "syn_hip_kv_tables_workspace": (ST, [C.POINTER(KvTables), C.POINTER(SZ)]),
+    "syn_hip_kv_resize": (ST, [C.POINTER(KvTables), P, P, SZ, P]),
+    "syn_hip_kv_fork": (ST, [C.POINTER(KvPages), C.POINTER(KvTables), P, P, P, SZ, P]),
+    "syn_hip_kv_compact": (ST, [C.POINTER(KvPages), C.POINTER(KvTables), C.POINTER(KvPages),
+                                C.POINTER(KvTables), P, P, SZ, P]),
     "syn_hip_stdrng_f32": (ST, [C.c_uint64, SZ, P]),
     "syn_hip_qlm_time_lm_head_rotating": (ST, [P, SZ, C.POINTER(C.c_float)]),
     "syn_hip_qlm_time_step_kernels": (ST, [P, SZ, P, P]),
