@@ -912,6 +912,34 @@ syn_status_t syn_hip_kv_compact(const syn_hip_kv_pages *from, const syn_hip_kv_t
                                 int32_t *d_live, void *d_workspace, size_t workspace_bytes,
                                 void *stream);
 
+/* Samples of a prompt's continuation with the K-quant decoder over the operators
+ * above: the prompt is prefilled once, n_samples rows of one page table continue
+ * it, and each round draws n_draft tokens of every sample from the first
+ * draft_layers layers (0: a third of them), verifies all of them in one forward
+ * pass, and keeps what was accepted and the token after it; a replayed HIP graph
+ * a round, no host work in it.  The tokens are distributed as ones drawn one by
+ * one from the softmax of the logits over `temperature` (not above 0 or not
+ * finite: greedy), whatever the drafts.  n_draft 0: one token a round.  A sample
+ * ends with `eos` (-1: none) or max_new tokens: out_tokens [n_samples][max_new]
+ * (places behind the eos hold it), out_lengths [n_samples] (nullable; with the
+ * eos), out_rounds (nullable) the rounds that were run.  The random numbers are
+ * the first n_samples + max_new * n_samples * (2 n_draft + 1) of
+ * syn_hip_stdrng_f32(seed): one for each sample's first token, then by round and
+ * sample n_draft for the drafts, n_draft for their acceptance, one for the token
+ * after them.  Keys and values are kept in kv_dtype.  1 to 64 samples, at most 16
+ * drafts, n_samples * (n_draft + 1) <= max_seq, n_prompt + max_new - 1 + n_draft
+ * <= max_seq.  Afterwards the model's own cache holds the prompt. */
+typedef struct {
+  uint32_t n_samples, n_draft, draft_layers;
+  int32_t eos, kv_dtype; /* SYN_HIP_KV_* */
+  float temperature;
+  uint64_t seed;
+} syn_hip_draft_sampling;
+syn_status_t syn_hip_klm_generate_samples(syn_hip_klm_t *m, const uint32_t *prompt, size_t n_prompt,
+                                          size_t max_new, const syn_hip_draft_sampling *p,
+                                          uint32_t *out_tokens, uint32_t *out_lengths,
+                                          uint32_t *out_rounds);
+
 /* -- harness helpers (no reference counterpart) -- */
 /* Encode f32 [n,k] into Q8_0 / Q4_K / Q6_K block bytes.  The reference has no
  * encoder for these formats (only dequantizers); any encoding is valid since

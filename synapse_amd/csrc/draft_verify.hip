@@ -22,6 +22,7 @@ namespace {
 
 constexpr int kNT = 256;
 constexpr int kBlock = 8 * kNT;  // tokens that a workgroup has in registers at a time
+constexpr int kDraws = 4;  // blocks of a workgroup that sums weights, at most
 constexpr float kNone = -__builtin_huge_valf();
 constexpr double kLog2e = 1.44269504088896340736;
 constexpr uint32_t kMaxDraft = 64;
@@ -35,6 +36,16 @@ struct Stat {
   int at;
 };
 
+// The draw that is left of a sequence when its drafts are decided on: weights
+// max(p / sum - q / sum, 0) from the logits of a target row, and of a draft row.
+struct Draw {
+  double ip, iq;    // 1 / sum
+  float pref, qref;
+  int r;            // drafts accepted; -1: nothing to draw
+  uint32_t except;  // a draft that was certain, and rejected
+  int32_t plain;    // p alone
+};
+
 struct VerifyArgs {
   const float *target, *draft, *heat, *u;
   const uint32_t *token;
@@ -43,10 +54,11 @@ struct VerifyArgs {
   int32_t *count;
   float *logp;
   Stat *stat;      // [n_seqs][target rows, then draft rows][chunks]
-  double *weight;  // [n_seqs][chunks]
-  int32_t *done;   // [n_seqs] chunks whose weights are summed
+  Draw *draw;      // [n_seqs]
+  uint64_t *weight;  // [n_seqs][blocks] sums (f64)
+  int32_t *done;     // [n_seqs] workgroups that have theirs
   size_t ld_target, target_stride, ld_draft, draft_stride;
-  int n_seqs, K, rows, vocab, chunks, per;
+  int n_seqs, K, rows, vocab, chunks, per, blocks, draws;  // per: tokens of a chunk, whole blocks
   uint32_t pad;
 };
 
@@ -155,7 +167,6 @@ __global__ void __launch_bounds__(kNT) k_verify_rows(VerifyArgs a) {
   const int s = blockIdx.y / a.rows, r = blockIdx.y - s * a.rows, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6, n = drafts_of(a, s);
   const double c32 = scale_of(a, s);
-  if (r == 0 && blockIdx.x == 0 && tid == 0) a.done[s] = 0;
   if (r > a.K ? r - a.K - 1 >= n || c32 == 0.0 : r > n) return;
   const int first = blockIdx.x * a.per, left = min(a.per, a.vocab - first);
   const float *x = row_of(a, s, r) + first;
@@ -217,263 +228,305 @@ __global__ void __launch_bounds__(kNT) k_verify_rows(VerifyArgs a) {
   a.stat[(size_t)blockIdx.y * a.chunks + blockIdx.x] = all;
 }
 
-// A wave joins the chunks of a row.
-__device__ __forceinline__ Stat join(const VerifyArgs &a, int s, int r, double c32, const uint64_t *tab) {
-  const Stat *st = a.stat + ((size_t)s * a.rows + r) * a.chunks;
-  const int lane = threadIdx.x & 63;
-  const Stat q0 = st[min(lane, a.chunks - 1)];
-  Stat all{0.0, kNone, 0x7fffffff};
-  for (int i = lane; i < a.chunks; i += 64) {
-    const Stat q = i == lane ? q0 : st[i];
-    if (q.ref > all.ref) all.ref = q.ref, all.at = q.at;
-  }
-  if (c32 == 0.0) {
-    first_top(&all.ref, &all.at);
-    return all;
-  }
-  all.ref = wave_max(all.ref);
-  const Exps e(all.ref, c32);
-  for (int i = lane; i < a.chunks; i += 64) {
-    const Stat q = i == lane ? q0 : st[i];
-    if (q.ref > kNone) all.sum += q.sum * e.of(q.ref, tab);
-  }
-  all.sum = wave_sum(all.sum);
-  return all;
+// over the 16 lanes of a row
+template <class F, class Op> __device__ __forceinline__ F over_16(F x, Op op) {
+  x = op(x, partner<8>(x));
+  x = op(x, partner<4>(x));
+  x = op(x, partner<2>(x));
+  return op(x, partner<1>(x));
 }
 
-// What is decided of a sequence: drafts accepted, and the rows' statistics.
-struct Choice {
-  Stat row[kMaxDraft + 1], of[kMaxDraft];  // target rows, draft rows
-  double p[kMaxDraft];                     // of the drafts
-  int fine[kMaxDraft];
-};
+constexpr int kDecideNT = 512;
 
-// The workgroup decides on the n drafts of a sequence: how many are accepted.
-__device__ __forceinline__ int decide(const VerifyArgs &a, int s, int n, double c32, const uint64_t *tab,
-                                      Choice *d) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int i = wave; i <= n; i += kNT / 64) {
-    const bool last = i == n, drafted = !last && a.draft && c32 != 0.0;
-    const uint32_t t = last ? 0xffffffffu : a.token[(size_t)s * a.K + i];
-    const bool known = t < (uint32_t)a.vocab;
-    // (asked for ahead of the sums)
-    const float lp = known ? row_of(a, s, i)[t] : kNone;
-    const float lq = known && drafted ? row_of(a, s, a.K + 1 + i)[t] : kNone;
-    const float u = last ? 0.0f : a.u[(size_t)s * (a.K + 1) + i];
-    const Stat p = join(a, s, i, c32, tab);
-    Stat q{0.0, kNone, 0};
-    if (drafted) q = join(a, s, a.K + 1 + i, c32, tab);
-    double pt = 0.0, qt = known && !a.draft ? 1.0 : 0.0;
-    bool fine;
-    if (c32 == 0.0) {
-      fine = p.ref > kNone && t == (uint32_t)p.at;
-      pt = 1.0;
+// One workgroup a sequence: 16 lanes join the chunks of a row, all rows at once,
+// and a lane a draft says whether it is accepted.
+__global__ void __launch_bounds__(kDecideNT) k_verify_decide(VerifyArgs a) {
+  __shared__ uint64_t tab[32];
+  __shared__ Stat row[2 * kMaxDraft + 1];    // target rows, then draft rows
+  __shared__ double prob[2 * kMaxDraft + 1]; // of the row's draft
+  __shared__ int accepted;
+  const int s = blockIdx.x, n = drafts_of(a, s), tid = threadIdx.x, l = tid & 15;
+  const double c32 = scale_of(a, s);
+  const bool greedy = c32 == 0.0;
+  uint32_t *out = a.out + (size_t)s * (a.K + 1);
+  float *logp = a.logp ? a.logp + (size_t)s * (a.K + 1) : nullptr;
+  if (n < 0) {
+    if (tid <= a.K) {
+      out[tid] = a.pad;
+      if (logp) logp[tid] = 0.0f;
+    }
+    if (tid == 0) a.count[s] = 0, a.draw[s].r = -1;
+    return;
+  }
+  copy_table(tab);
+  __syncthreads();
+  const int rows = n + 1 + (a.draft && !greedy ? n : 0);
+  for (int k = tid >> 4; k < rows; k += kDecideNT / 16) {
+    const bool of_draft = k > n;
+    const int i = of_draft ? k - n - 1 : k, r = of_draft ? a.K + 1 + i : i;
+    const Stat *st = a.stat + ((size_t)s * a.rows + r) * a.chunks;
+    const Stat q0 = st[min(l, a.chunks - 1)];
+    float x = kNone;
+    if (i < n && !greedy) {
+      const uint32_t t = a.token[(size_t)s * a.K + i];
+      if (t < (uint32_t)a.vocab) x = row_of(a, s, r)[t];
+    }
+    Stat all{0.0, kNone, 0x7fffffff};
+    for (int c = l; c < a.chunks; c += 16) {
+      const Stat q = c == l ? q0 : st[c];
+      if (q.ref > all.ref) all.ref = q.ref, all.at = q.at;
+    }
+    if (greedy) {
+      for (int o = 8; o > 0; o >>= 1) {
+        const float t = __shfl_xor(all.ref, o);
+        const int at = __shfl_xor(all.at, o);
+        if (t > all.ref || (t == all.ref && at < all.at)) all.ref = t, all.at = at;
+      }
     } else {
-      if (p.sum > 0.0) pt = Exps(p.ref, c32).of(lp, tab) / p.sum;
-      if (q.sum > 0.0) qt = Exps(q.ref, c32).of(lq, tab) / q.sum;
-      fine = known && (double)u * qt < pt;
+      all.ref = over_16(all.ref, [](float p, float q) { return fmaxf(p, q); });
+      const Exps e(all.ref, c32);
+      for (int c = l; c < a.chunks; c += 16) {
+        const Stat q = c == l ? q0 : st[c];
+        if (q.ref > kNone) all.sum += q.sum * e.of(q.ref, tab);
+      }
+      all.sum = over_16(all.sum, [](double p, double q) { return p + q; });
+      if (l == 0) prob[k] = all.sum > 0.0 ? e.of(x, tab) / all.sum : 0.0;
     }
-    if (lane == 0) {
-      d->row[i] = p;
-      if (!last) d->of[i] = q, d->p[i] = pt, d->fine[i] = fine;
-    }
+    if (l == 0) row[k] = all;
   }
   __syncthreads();
-  int r = 0;
-  while (r < n && d->fine[r]) r++;
-  return r;
+  if (tid < 64) {  // (at most 64 drafts)
+    bool fine = true;
+    if (tid < n) {
+      const uint32_t t = a.token[(size_t)s * a.K + tid];
+      const double u = (double)a.u[(size_t)s * (a.K + 1) + tid];
+      if (greedy)
+        fine = row[tid].ref > kNone && t == (uint32_t)row[tid].at;
+      else
+        fine = t < (uint32_t)a.vocab && u * (a.draft ? prob[n + 1 + tid] : 1.0) < prob[tid];
+    }
+    const uint64_t wrong = __ballot(!fine);
+    if (tid == 0) accepted = wrong ? __ffsll((unsigned long long)wrong) - 1 : n;
+  }
+  __syncthreads();
+  const int r = accepted;
+  const Stat p = row[r];
+  const bool none = greedy ? p.ref == kNone : !(p.sum > 0.0);
+  if (tid <= a.K) {  // (a token that is drawn comes later)
+    out[tid] = tid < r ? a.token[(size_t)s * a.K + tid] : (tid == r && greedy && !none ? (uint32_t)p.at : a.pad);
+    if (logp)
+      logp[tid] = tid == r && none ? kNone : (tid < r && !greedy ? (float)log(prob[tid]) : 0.0f);
+  }
+  if (tid == 0) {
+    a.count[s] = r + 1;
+    Draw d{};
+    d.r = greedy || none ? -1 : r;
+    d.pref = p.ref;
+    d.ip = 1.0 / p.sum;
+    d.plain = r == n;
+    if (r < n) {
+      d.except = a.token[(size_t)s * a.K + r];
+      if (a.draft && !greedy) {
+        const Stat q = row[n + 1 + r];
+        d.qref = q.ref;
+        d.iq = 1.0 / q.sum;
+        d.plain = !(q.sum > 0.0);  // (a draft row of -inf: q is 0)
+      }
+    }
+    a.draw[s] = d;
+    a.done[s] = 0;
+  }
 }
 
-// The weights after r accepted drafts; PLAIN: of p_r alone.
 struct Weights {
-  const float *x, *y;
+  const float *x, *y;  // y: null where the weights are p's alone
   Exps p, q;
   double ip, iq;
-  uint32_t except;  // a draft that was certain, and rejected
-  __device__ __forceinline__ double of(int t, float lx, float ly, bool plain, const uint64_t *tab) const {
-    const double w = p.of(lx, tab) * ip;
-    if (plain) return w;
-    if (!y) return (uint32_t)t == except ? 0.0 : w;
-    return fmax(w - q.of(ly, tab) * iq, 0.0);
-  }
-  __device__ __forceinline__ double at(int t, bool plain, const uint64_t *tab) const {
-    return of(t, x[t], plain || !y ? 0.0f : y[t], plain, tab);
+  uint32_t except;  // a draft that was certain, and rejected; the vocabulary: none
+  bool infinite;    // a row's largest logit is +inf
+  // of token t with logits lx and ly
+  template <bool INF> __device__ __forceinline__ double of(int t, float lx, float ly, const uint64_t *tab) const {
+    double w = (INF ? p.of(lx, tab) : p.at_least(lx, tab)) * ip;
+    if (y)
+      w -= (INF ? q.of(ly, tab) : q.at_least(ly, tab)) * iq;
+    else
+      w = (uint32_t)t == except ? 0.0 : w;
+    return w > 1e-290 ? w : 0.0;  // (2^-1000 is nothing)
   }
 };
 
-// The first token of [first, end) whose weights up to it, and `before`, are above
+// wsum[block][wave]: the sums of the weights of the blocks of [first, first + n)
+template <bool INF>
+__device__ __forceinline__ void block_sums(const Weights &w, int first, int n, const uint64_t *tab,
+                                           double (*wsum)[4]) {
+  const float *yr = w.y ? w.y + first : nullptr;
+  float y[8] = {}, ynext[8] = {};
+  if (yr) load_block(yr, n, ynext);
+  over_blocks(w.x + first, n, [&](int b, const float *v) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) y[i] = ynext[i];
+    if (yr && b + kBlock < n) load_block(yr + b + kBlock, n - b - kBlock, ynext);
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      sum += w.of<INF>(first + b + i / 4 * (kBlock / 2) + (int)threadIdx.x * 4 + i % 4, v[i], y[i], tab);
+    sum = wave_sum(sum);
+    if ((threadIdx.x & 63) == 0) wsum[b / kBlock][threadIdx.x >> 6] = sum;
+  });
+}
+__device__ __forceinline__ void sum_blocks(const Weights &w, int first, int n, const uint64_t *tab,
+                                           double (*wsum)[4]) {
+  if (w.infinite)
+    block_sums<true>(w, first, n, tab, wsum);
+  else
+    block_sums<false>(w, first, n, tab, wsum);
+}
+
+// The first token of a block whose weights up to it, and `before`, are above
 // `border`; where rounding leaves none, the last one that has a weight.
-__device__ __forceinline__ int pick(const Weights &w, bool plain, int first, int end, double before,
-                                    double border, const uint64_t *tab) {
+__device__ __forceinline__ int pick(const Weights &w, int first, int left, double before, double border,
+                                    const uint64_t *tab) {
   __shared__ double wsum[4];
-  __shared__ int wfound[4], wlast[4], chosen;
-  __shared__ double base_of;
+  __shared__ int wfound[4], wlast[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int each = (end - first + kNT - 1) / kNT;  // a thread's tokens, next to each other
-  const int t0 = first + min(tid * each, end - first), t1 = min(end, t0 + each);
-  double sum = 0.0;
-  int last = -1;
-  for (int t = t0; t < t1; t++) {
-    const double x = w.at(t, plain, tab);
+  float v[8], y[8] = {};  // of 8 tokens next to each other
+#pragma unroll
+  for (int i = 0; i < 8; i++) v[i] = w.x[first + min(8 * tid + i, left - 1)];
+  if (w.y)
+#pragma unroll
+    for (int i = 0; i < 8; i++) y[i] = w.y[first + min(8 * tid + i, left - 1)];
+  double up[8], sum = 0.0;
+  uint32_t some = 0;  // that have a weight
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const int t = first + 8 * tid + i;
+    const double in = w.infinite ? w.of<true>(t, v[i], y[i], tab) : w.of<false>(t, v[i], y[i], tab);
+    const double x = 8 * tid + i < left ? in : 0.0;
     sum += x;
-    if (x > 0.0) last = t;
+    up[i] = sum;
+    some |= x > 0.0 ? 1u << i : 0u;
   }
   double base = wave_before(sum);
   if (lane == 63) wsum[wave] = base + sum;
   __syncthreads();
   for (int i = 0; i < wave; i++) base += wsum[i];
   base += before;
-  const uint64_t over = __ballot(sum > 0.0 && base + sum > border), some = __ballot(last >= 0);
-  if (lane == 0) {
-    wfound[wave] = over ? wave * 64 + __ffsll((unsigned long long)over) - 1 : kNT;
-    wlast[wave] = some ? wave * 64 + 63 - __clzll((long long)some) : -1;
+  int found = 0x7fffffff;
+#pragma unroll
+  for (int i = 7; i >= 0; i--)
+    if ((some >> i & 1) && base + up[i] > border) found = 8 * tid + i;
+  int last = some ? 8 * tid + 31 - __clz(some) : -1;
+  for (int o = 32; o > 0; o >>= 1) {
+    found = min(found, __shfl_xor(found, o));
+    last = max(last, __shfl_xor(last, o));
   }
+  if (lane == 0) wfound[wave] = found, wlast[wave] = last;
   __syncthreads();
-  int who = min(min(wfound[0], wfound[1]), min(wfound[2], wfound[3]));
-  if (who == kNT) who = max(max(wlast[0], wlast[1]), max(wlast[2], wlast[3]));
-  if (tid == who) base_of = base, chosen = last;
-  __syncthreads();
-  if (who < 0) return -1;
-  // that thread's tokens again, by the first wave's lanes
-  if (wave == 0) {
-    double x = base_of;
-    const int f = first + who * each, g = min(end, f + each);
-    for (int b = f; b < g; b += 64) {
-      const double v = b + lane < g ? w.at(b + lane, plain, tab) : 0.0;
-      const double up = x + wave_before(v) + v;
-      const uint64_t hit = __ballot(v > 0.0 && up > border);
-      if (hit) {
-        if (lane == 0) chosen = b + __ffsll((unsigned long long)hit) - 1;
-        break;
-      }
-      x = __shfl(up, 63);
-    }
-  }
-  __syncthreads();
-  return chosen;
+  found = min(min(wfound[0], wfound[1]), min(wfound[2], wfound[3]));
+  last = max(max(wlast[0], wlast[1]), max(wlast[2], wlast[3]));
+  return first + (found < left ? found : last);
 }
 
-// grid (chunk, sequence): every workgroup of a sequence decides on its drafts and
-// sums its chunk of the weights; the last one to have done so draws.
+// grid (some blocks, sequence): the sums of the weights by blocks; the last workgroup of
+// a sequence to have its sum draws.
 __global__ void __launch_bounds__(kNT) k_verify_draw(VerifyArgs a) {
   __shared__ uint64_t tab[32];
-  __shared__ Choice d;
-  __shared__ double wsum[4];
-  __shared__ int mine;
-  const int s = blockIdx.y, n = drafts_of(a, s), tid = threadIdx.x;
-  uint32_t *out = a.out + (size_t)s * (a.K + 1);
-  float *logp = a.logp ? a.logp + (size_t)s * (a.K + 1) : nullptr;
+  __shared__ double wsum[kDraws][4];
+  __shared__ int mine, block_of;
+  __shared__ double before_of, border_of;
+  const int s = blockIdx.y, tid = threadIdx.x;
+  const Draw d = a.draw[s];
+  if (d.r < 0) return;
   const double c32 = scale_of(a, s);
-  if (blockIdx.x && (n < 0 || c32 == 0.0)) return;
-  if (n < 0) {
-    for (int i = tid; i <= a.K; i += kNT) {
-      out[i] = a.pad;
-      if (logp) logp[i] = 0.0f;
-    }
-    if (tid == 0) a.count[s] = 0;
-    return;
-  }
   copy_table(tab);
   __syncthreads();
-  const int r = decide(a, s, n, c32, tab, &d);
-  const Stat p = d.row[r];
-  int t = -1;
-  double pt = 1.0;
-  if (c32 == 0.0) {
-    t = p.ref > kNone ? p.at : -1;
-  } else {
-    const Stat q = r == n ? Stat{0.0, kNone, 0} : d.of[r];
-    const bool plain = r == n || (a.draft && !(q.sum > 0.0));  // (a draft row of -inf: q is 0)
-    const Weights w{row_of(a, s, r),
-                    plain || !a.draft ? nullptr : row_of(a, s, a.K + 1 + r),
-                    Exps(p.ref, c32),
-                    Exps(q.ref, c32),
-                    p.sum > 0.0 ? 1.0 / p.sum : 0.0,
-                    q.sum > 0.0 ? 1.0 / q.sum : 0.0,
-                    r == n ? 0 : a.token[(size_t)s * a.K + r]};
-    const int first = blockIdx.x * a.per, left = min(a.per, a.vocab - first);
-    double sum = 0.0;
-    if (p.sum > 0.0) {
-      float y[8], ynext[8];
-      const float *yr = w.y ? w.y + first : nullptr;
-      if (yr) load_block(yr, left, ynext);
-      over_blocks(w.x + first, left, [&](int b, const float *v) {
-        if (yr) {
-#pragma unroll
-          for (int i = 0; i < 8; i++) y[i] = ynext[i];
-          if (b + kBlock < left) load_block(yr + b + kBlock, left - b - kBlock, ynext);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-          sum += w.of(first + b + i / 4 * (kBlock / 2) + tid * 4 + i % 4, v[i], yr ? y[i] : 0.0f, plain, tab);
-      });
+  Weights w{row_of(a, s, d.r),
+            d.plain || !a.draft ? nullptr : row_of(a, s, a.K + 1 + d.r),
+            Exps(d.pref, c32),
+            Exps(d.qref, c32),
+            d.ip,
+            d.iq,
+            d.plain ? (uint32_t)a.vocab : d.except,
+            fmaxf(d.pref, d.qref) == __builtin_huge_valf()};
+  const int first = blockIdx.x * a.draws * kBlock;
+  sum_blocks(w, first, min(a.draws * kBlock, a.vocab - first), tab, wsum);
+  __syncthreads();
+  uint64_t *sums = a.weight + (size_t)s * a.blocks;
+  if (tid < 64) {
+    // As in split_k.hpp: an exchange that has returned is at the point where every
+    // XCD's atomics are, so relaxed ones suffice (an acquire and a release each
+    // write back and drop an L2: 142 us where this kernel took 53).
+    const int b = blockIdx.x * a.draws + tid;
+    if (tid < a.draws && b < a.blocks) {
+      const double x = (wsum[tid][0] + wsum[tid][1]) + (wsum[tid][2] + wsum[tid][3]);
+      const uint64_t seen = __hip_atomic_exchange(sums + b, (uint64_t)__double_as_longlong(x), __ATOMIC_RELAXED,
+                                                  __HIP_MEMORY_SCOPE_AGENT);
+      asm volatile("" ::"v"(seen));
     }
-    sum = wave_sum(sum);
-    if ((tid & 63) == 0) wsum[tid >> 6] = sum;
-    __syncthreads();
-    double *sums = a.weight + (size_t)s * a.chunks;
-    if (tid == 0) {
-      __hip_atomic_store(sums + blockIdx.x, (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]), __ATOMIC_RELAXED,
-                         __HIP_MEMORY_SCOPE_AGENT);
-      mine = __hip_atomic_fetch_add(a.done + s, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == a.chunks - 1;
-    }
-    __syncthreads();
-    if (!mine) return;
-    // the chunk that the draw falls into, by the first wave
-    __shared__ double before_of, border_of;
-    __shared__ int chunk_of;
-    if (tid < 64) {
-      double total = 0.0;
-      for (int i0 = 0; i0 < a.chunks; i0 += 64) {
-        const double x = i0 + tid < a.chunks ? __hip_atomic_load(sums + i0 + tid, __ATOMIC_RELAXED,
-                                                                 __HIP_MEMORY_SCOPE_AGENT)
-                                             : 0.0;
-        total += __shfl(wave_before(x) + x, 63);
-      }
-      const double u = (double)a.u[(size_t)s * (a.K + 1) + a.K], border = u * total;
-      double base = 0.0, before = 0.0;
-      int at = -1;
-      for (int i0 = 0; i0 < a.chunks; i0 += 64) {
-        const double x = i0 + tid < a.chunks ? __hip_atomic_load(sums + i0 + tid, __ATOMIC_RELAXED,
-                                                                 __HIP_MEMORY_SCOPE_AGENT)
-                                             : 0.0;
-        const double lo = base + wave_before(x);
-        const uint64_t some = __ballot(x > 0.0), over = __ballot(x > 0.0 && lo + x > border);
-        // the first above the border, or the last that has a weight
-        const uint64_t from = over ? over : some;
-        if (from) {
-          const int l = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
-          at = i0 + l;
-          before = __shfl(lo, l);
-        }
-        if (over) break;
-        base = __shfl(lo + x, 63);
-      }
-      if (tid == 0) before_of = before, border_of = at < 0 ? u : border, chunk_of = at;
-    }
-    __syncthreads();
-    const int at = chunk_of;
-    if (at >= 0)
-      t = pick(w, plain, at * a.per, at * a.per + min(a.per, a.vocab - at * a.per), before_of, border_of, tab);
-    else if (p.sum > 0.0)  // p_r is nowhere above q_r: from p_r
-      t = pick(w, true, 0, a.vocab, 0.0, border_of, tab);
-    if (t >= 0) pt = w.p.of(w.x[t], tab) * w.ip;
+    if (tid == 0)
+      mine = __hip_atomic_fetch_add(a.done + s, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
   }
-  for (int i = tid; i <= a.K; i += kNT) {
-    out[i] = i < r ? a.token[(size_t)s * a.K + i] : (i == r && t >= 0 ? (uint32_t)t : a.pad);
-    if (!logp) continue;
-    double l = 0.0;
-    if (i < r) l = log(d.p[i]);
-    if (i == r) l = t < 0 ? -__builtin_huge_val() : log(pt);
-    logp[i] = (float)l;
+  __syncthreads();
+  if (!mine) return;
+  const double u = (double)a.u[(size_t)s * (a.K + 1) + a.K];
+  if (tid < 64) {  // the block that the draw falls into
+    auto load = [&](int i) {
+      return i < a.blocks ? __longlong_as_double((long long)__hip_atomic_load(
+                                sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+                          : 0.0;
+    };
+    const double held[2] = {load(tid), load(64 + tid)};
+    double total = held[0] + held[1];
+    for (int i0 = 128; i0 < a.blocks; i0 += 64) total += load(i0 + tid);
+    const double border = u * wave_sum(total);
+    double base = 0.0, before = 0.0;
+    int at = -1;
+    for (int i0 = 0; i0 < a.blocks; i0 += 64) {
+      const double x = i0 == 0 ? held[0] : (i0 == 64 ? held[1] : load(i0 + tid)), lo = base + wave_before(x);
+      const uint64_t some = __ballot(x > 0.0), over = __ballot(x > 0.0 && lo + x > border);
+      if (over | some) {  // the first above the border, or the last that has a weight
+        const int k = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
+        at = i0 + k;
+        before = __shfl(lo, k);
+      }
+      if (over) break;
+      base = __shfl(lo + x, 63);
+    }
+    if (tid == 0) before_of = before, border_of = border, block_of = at;
   }
-  if (tid == 0) a.count[s] = r + 1;
+  __syncthreads();
+  int at = block_of;
+  double before = before_of, border = border_of;
+  if (at < 0) {  // p_r is nowhere above q_r: from p_r, whose weights sum to 1
+    w.y = nullptr;
+    w.except = (uint32_t)a.vocab;
+    border = u;
+    before = 0.0;
+    double in = 0.0;
+    for (int b = 0; b < a.blocks; b++) {
+      __syncthreads();
+      sum_blocks(w, b * kBlock, min(kBlock, a.vocab - b * kBlock), tab, wsum);
+      __syncthreads();
+      const double x = (wsum[0][0] + wsum[0][1]) + (wsum[0][2] + wsum[0][3]);
+      if (!(x > 0.0)) continue;
+      before += in;
+      in = x;
+      at = b;
+      if (before + x > border) break;
+    }
+  }
+  const int t = pick(w, at * kBlock, min(kBlock, a.vocab - at * kBlock), before, border, tab);
+  if (tid == 0) {
+    const size_t o = (size_t)s * (a.K + 1) + d.r;
+    a.out[o] = (uint32_t)t;
+    if (a.logp) a.logp[o] = (float)log(w.p.of(w.x[t], tab) * w.ip);
+  }
 }
 
 // ---------------------------------------------------------------- host
 struct Space {
-  int per, chunks, rows;
-  size_t stat, weight, done, total;
+  int per, chunks, rows, draws;
+  size_t stat, draw, weight, done, total;
 };
 Space space_of(const syn_hip_draft_verify_params &p) {
   Space s;
@@ -482,9 +535,12 @@ Space space_of(const syn_hip_draft_verify_params &p) {
   s.per = kBlock;
   while (s.per < 8 * kBlock && p.n_seqs * (size_t)s.rows * cdiv(p.vocab, 2 * s.per) >= 2048) s.per *= 2;
   s.chunks = (int)cdiv(p.vocab, s.per);
+  s.draws = 1;
+  while (s.draws < kDraws && p.n_seqs * cdiv(p.vocab, 2 * s.draws * kBlock) >= 1024) s.draws *= 2;
   s.stat = 0;
-  s.weight = (size_t)p.n_seqs * s.rows * s.chunks * sizeof(Stat);
-  s.done = s.weight + (size_t)p.n_seqs * s.chunks * 8;
+  s.draw = (size_t)p.n_seqs * s.rows * s.chunks * sizeof(Stat);
+  s.weight = s.draw + p.n_seqs * sizeof(Draw);
+  s.done = s.weight + (size_t)p.n_seqs * cdiv(p.vocab, kBlock) * 8;
   s.total = round_up(s.done + (size_t)p.n_seqs * 4, 16);
   return s;
 }
@@ -553,8 +609,9 @@ syn_status_t syn_hip_draft_verify(const syn_hip_draft_verify_params *p, const fl
   a.count = d_count;
   a.logp = d_logp;
   a.stat = reinterpret_cast<Stat *>(ws + sp.stat);
-  a.weight = reinterpret_cast<double *>(ws + sp.weight);
+  a.weight = reinterpret_cast<uint64_t *>(ws + sp.weight);
   a.done = reinterpret_cast<int32_t *>(ws + sp.done);
+  a.draw = reinterpret_cast<Draw *>(ws + sp.draw);
   a.ld_target = p->ld_target;
   a.target_stride = p->target_stride;
   a.ld_draft = p->ld_draft;
@@ -565,11 +622,15 @@ syn_status_t syn_hip_draft_verify(const syn_hip_draft_verify_params *p, const fl
   a.vocab = (int)p->vocab;
   a.chunks = sp.chunks;
   a.per = sp.per;
+  a.blocks = (int)cdiv(p->vocab, kBlock);
+  a.draws = sp.draws;
   a.pad = p->pad;
   hipStream_t s = pick_stream(stream);
   hipLaunchKernelGGL(k_verify_rows, dim3(a.chunks, p->n_seqs * a.rows), dim3(kNT), 0, s, a);
   SYN_LAUNCH_CHECK();
-  hipLaunchKernelGGL(k_verify_draw, dim3(a.chunks, p->n_seqs), dim3(kNT), 0, s, a);
+  hipLaunchKernelGGL(k_verify_decide, dim3(p->n_seqs), dim3(kDecideNT), 0, s, a);
+  SYN_LAUNCH_CHECK();
+  hipLaunchKernelGGL(k_verify_draw, dim3((unsigned)cdiv(a.blocks, a.draws), p->n_seqs), dim3(kNT), 0, s, a);
   SYN_LAUNCH_CHECK();
   return SYN_OK;
 }

@@ -19,8 +19,16 @@
 #include "kv_pages.hpp"
 #include "kquant.hpp"
 #include "layer_ops.hpp"
+#include "samples.hpp"
 
 using namespace syn;
+
+// Where a prompt's keys and values are stored beside the decoder's own cache.
+struct PromptPages {
+  const syn_hip_kv_pages *pages;
+  const int32_t *iota, *zeros, *table;
+  size_t cols;
+};
 
 // What a beam search of one shape keeps on the device: pages for the prompt and
 // for each beam's tokens (and its spare), tables, counters, per-beam rows, and
@@ -41,6 +49,30 @@ struct BeamSpace {
   }
   bool is(size_t np, size_t mn, size_t w, const syn_hip_beam_search &p) const {
     return n_prompt == np && max_new == mn && W == w && eos == p.eos && dtype == p.kv_dtype;
+  }
+};
+
+// What drawing samples of one shape keeps on the device: pages for the prompt and
+// what the samples add to it, their tables, the state of a round, its rows of
+// logits, and the captured round.
+struct SampleSpace {
+  size_t n_prompt = 0, max_new = 0, n = 0, k = 0, draft_layers = 0, ld = 0;
+  int32_t eos = -1, dtype = SYN_HIP_KV_F32;
+  syn_hip_kv_pages pages{};
+  syn_hip_kv_tables tables{};
+  size_t rows() const { return n * (k + 1); }
+  size_t most() const { return n_prompt + max_new + k; }  // positions of a sample
+  DevBuf kp, vp, table, held, refs, ints, iota, zeros, history, draws, u;
+  DevBuf target, draft, token, count, heat, lens, parent, attn_ws, verify_ws, table_ws;
+  size_t attn_bytes = 0, verify_bytes = 0, table_bytes = 0;
+  SampleState st{};
+  hipGraphExec_t graph = nullptr;
+  ~SampleSpace() {
+    if (graph) (void)hipGraphExecDestroy(graph);
+  }
+  bool is(size_t np, size_t mn, size_t layers, const syn_hip_draft_sampling &p) const {
+    return n_prompt == np && max_new == mn && n == p.n_samples && k == p.n_draft &&
+           draft_layers == layers && eos == p.eos && dtype == p.kv_dtype;
   }
 };
 
@@ -73,7 +105,8 @@ struct syn_hip_klm_s {
   bool fused_ok = false;
   KqfPlan fp_qkv, fp_o, fp_gu, fp_down, fp_lm;
   DevBuf f_r, f_qkv, f_ao, f_aml, f_pv, f_pi, f_pv2;
-  std::unique_ptr<BeamSpace> beams;  // of the last beam search
+  std::unique_ptr<BeamSpace> beams;      // of the last beam search
+  std::unique_ptr<SampleSpace> samples;  // of the last samples
 
   ~syn_hip_klm_s() {
     drop_captured();
@@ -86,6 +119,7 @@ struct syn_hip_klm_s {
     if (draft_graph) (void)hipGraphExecDestroy(draft_graph);
     graph = draft_graph = nullptr;
     beams.reset();
+    samples.reset();
   }
   // before a weight's buffer is freed for another
   void weights_change() {
@@ -220,7 +254,7 @@ struct syn_hip_klm_s {
   // cache_off (prefill only): cache row of the first of `rows` tokens; with
   // `prompt` set, the rows' keys and values go to its pages too
   syn_status_t layer(size_t l, int rows, bool prefill, hipStream_t s, int cache_off = 0,
-                     BeamSpace *prompt = nullptr) {
+                     const PromptPages *prompt = nullptr) {
     Layer &Ly = layers[l];
     const float eps = c.base.eps;
     const int nh = (int)c.base.n_heads, nkv = (int)c.base.n_kv_heads;
@@ -231,12 +265,11 @@ struct syn_hip_klm_s {
                                  nullptr, normed.as<float>(), s));
     SYN_TRY(Ly.qkv.gemv(rows, normed.as<float>(), h, qkv.as<float>(), n_qkv, s));
     if (prompt) {
-      const syn_hip_kv_append_params p = append_params(l, 0, 1, prompt->prefix_cols);
+      const syn_hip_kv_append_params p = append_params(l, 0, 1, prompt->cols);
       const float *k = qkv.as<float>() + qd;
-      SYN_TRY(syn_hip_kv_append(&prompt->pages, &p, rows, nullptr, k, k + kvd, nullptr, kn,
-                                rope_cos.as<float>(), rope_sin.as<float>(), prompt->iota.as<int32_t>(),
-                                prompt->zeros.as<int32_t>(), prompt->iota.as<int32_t>(),
-                                prompt->ptable.as<int32_t>(), nullptr, s));
+      SYN_TRY(syn_hip_kv_append(prompt->pages, &p, rows, nullptr, k, k + kvd, nullptr, kn,
+                                rope_cos.as<float>(), rope_sin.as<float>(), prompt->iota, prompt->zeros,
+                                prompt->iota, prompt->table, nullptr, s));
     }
     if (!prefill && fused_attention_fits((int)hd, (int)S)) {
       // one kernel per query head: head norms, RoPE, KV append and attention
@@ -466,7 +499,7 @@ struct syn_hip_klm_s {
 
   // the layers of CausalLM::forward_prefill (causal_lm.rs:195-224) over n
   // tokens whose ids are on the device, appended at cache rows cache_off ..
-  syn_status_t prefill_rows(const uint32_t *d_ids, int n, int cache_off, BeamSpace *prompt = nullptr) {
+  syn_status_t prefill_rows(const uint32_t *d_ids, int n, int cache_off, const PromptPages *prompt = nullptr) {
     SYN_TRY(launch_embed(embed.as<float>(), d_ids, n, (int)h, (int)vocab, x.as<float>(), stream));
     for (size_t l = 0; l < L; l++) SYN_TRY(layer(l, n, true, stream, cache_off, prompt));
     return SYN_OK;
@@ -539,6 +572,7 @@ struct syn_hip_klm_s {
     if (beams && beams->is(n_prompt, max_new, W, bs)) return SYN_OK;
     SYN_HIP(hipStreamSynchronize(stream));
     beams.reset();
+    samples.reset();  // (the head's scratch may grow: a captured round holds its address)
     auto b = std::make_unique<BeamSpace>();
     constexpr size_t kPage = 16;  // positions; a step copies half of one a beam at most on average
     b->n_prompt = n_prompt;
@@ -707,7 +741,9 @@ struct syn_hip_klm_s {
     hp.known = false;
     SYN_HIP(hipMemcpyAsync(ids.p, prompt, n_prompt * 4, hipMemcpyHostToDevice, stream));
     SYN_TRY(set_state(0, 0, 0));
-    SYN_TRY(prefill_rows(ids.as<uint32_t>(), (int)n_prompt, 0, &b));
+    const PromptPages pp{&b.pages, b.iota.as<int32_t>(), b.zeros.as<int32_t>(), b.ptable.as<int32_t>(),
+                         b.prefix_cols};
+    SYN_TRY(prefill_rows(ids.as<uint32_t>(), (int)n_prompt, 0, &pp));
     SYN_TRY(head((int)n_prompt - 1, (int)n_prompt, stream));
     syn_hip_beam_select_params first = b.select;
     first.n_beams = 1;
@@ -757,6 +793,293 @@ struct syn_hip_klm_s {
       if (out_lengths) out_lengths[r] = (uint32_t)len[i];
       if (out_scores) out_scores[r] = score[i];
     }
+    return SYN_OK;
+  }
+
+  // ---- samples: the prompt is prefilled as ever and its keys and values stored
+  // once; each sample's row of the page table continues them.
+  syn_status_t make_samples(size_t n_prompt, size_t max_new, size_t draft_layers,
+                            const syn_hip_draft_sampling &sp) {
+    if (samples && samples->is(n_prompt, max_new, draft_layers, sp)) return SYN_OK;
+    SYN_HIP(hipStreamSynchronize(stream));
+    samples.reset();
+    beams.reset();  // (the head's scratch may grow: a captured step holds its address)
+    auto b = std::make_unique<SampleSpace>();
+    constexpr size_t kPage = 16;  // positions; half of one a sample is copied on average
+    const size_t n = sp.n_samples, k = sp.n_draft, rows = n * (k + 1);
+    b->n_prompt = n_prompt;
+    b->max_new = max_new;
+    b->n = n;
+    b->k = k;
+    b->draft_layers = draft_layers;
+    b->ld = round_up(vocab, 4);  // 16-byte rows
+    b->eos = sp.eos;
+    b->dtype = sp.kv_dtype;
+    // a sample's pages but the prompt's whole ones are its own
+    const size_t cols = cdiv(b->most(), kPage), shared = n_prompt / kPage;
+    syn_hip_kv_pages &pg = b->pages;
+    pg.dtype = sp.kv_dtype;
+    pg.page_size = kPage;
+    pg.n_pages = (uint32_t)(shared + n * (cols - shared));
+    pg.n_layers = (uint32_t)L;
+    pg.n_kv_heads = c.base.n_kv_heads;
+    pg.head_dim = (uint32_t)hd;
+    SYN_TRY(b->kp.alloc(kv_pool_bytes(pg)));
+    SYN_TRY(b->vp.alloc(kv_pool_bytes(pg)));
+    pg.k = b->kp.p;
+    pg.v = b->vp.p;
+    SYN_TRY(check_pages(&pg, "klm_generate_samples"));
+    SYN_TRY(b->table.alloc(n * cols * 4));
+    SYN_TRY(b->held.alloc(n * 4));
+    SYN_TRY(b->refs.alloc(pg.n_pages * 4));
+    b->tables = syn_hip_kv_tables{(uint32_t)kPage,        pg.n_pages,           (uint32_t)n, cols,
+                                  b->table.as<int32_t>(), b->held.as<int32_t>(), b->refs.as<int32_t>()};
+    SampleState &st_ = b->st;
+    st_.n = (int)n;
+    st_.k = (int)k;
+    st_.eos = sp.eos;
+    st_.max_new = (int)max_new;
+    SYN_TRY(b->ints.alloc((1 + 6 * n + 3 * rows + 3 * k * n) * 4));
+    int32_t *at = b->ints.as<int32_t>();
+    auto ints = [&](size_t m) {
+      int32_t *p = at;
+      at += m;
+      return p;
+    };
+    st_.round = ints(1);
+    st_.len = ints(n);
+    st_.out = ints(n);
+    st_.drafting = ints(n);
+    st_.drafts = ints(n);
+    st_.room = ints(n);
+    st_.last = reinterpret_cast<uint32_t *>(ints(n));
+    st_.pos = ints(rows);
+    st_.seq = ints(rows);
+    st_.ids = reinterpret_cast<uint32_t *>(ints(rows));
+    st_.draft_pos = ints(k * n);
+    st_.draft_len = ints(k * n);
+    st_.drafted = reinterpret_cast<uint32_t *>(ints(k * n));
+    SYN_TRY(b->history.alloc(n * max_new * 4));
+    SYN_TRY(b->draws.alloc((n + max_new * n * (2 * k + 1)) * 4));
+    SYN_TRY(b->u.alloc((k * n + rows) * 4));
+    st_.history = b->history.as<uint32_t>();
+    st_.draws = b->draws.as<float>();
+    st_.u_draft = b->u.as<float>();
+    st_.u = st_.u_draft + k * n;
+    SYN_TRY(b->iota.alloc(n_prompt * 4));
+    SYN_TRY(b->zeros.alloc(std::max(n_prompt, n) * 4));
+    SYN_TRY(b->target.alloc(rows * b->ld * 4));
+    SYN_TRY(b->draft.alloc(k * n * b->ld * 4));
+    SYN_TRY(b->token.alloc(rows * 4));
+    SYN_TRY(b->count.alloc(n * 4));
+    SYN_TRY(b->heat.alloc(n * 4));
+    SYN_TRY(b->lens.alloc(n * 4));
+    SYN_TRY(b->parent.alloc(n * 4));
+    for (const size_t m : {(size_t)1, k + 1}) {
+      const syn_hip_paged_attention_params ap = sample_attention(*b, 0, m);
+      size_t bytes = 0;
+      SYN_TRY(syn_hip_paged_attention_workspace(&pg, &ap, &bytes));
+      b->attn_bytes = std::max(b->attn_bytes, bytes);
+    }
+    const syn_hip_draft_verify_params vp = sample_verify(*b, k), dp = sample_verify(*b, 0);
+    size_t bytes = 0;
+    SYN_TRY(syn_hip_draft_verify_workspace(&vp, &b->verify_bytes));
+    SYN_TRY(syn_hip_draft_verify_workspace(&dp, &bytes));
+    b->verify_bytes = std::max(b->verify_bytes, bytes);
+    SYN_TRY(syn_hip_kv_tables_workspace(&b->tables, &b->table_bytes));
+    SYN_TRY(b->attn_ws.alloc(b->attn_bytes));
+    SYN_TRY(b->verify_ws.alloc(b->verify_bytes));
+    SYN_TRY(b->table_ws.alloc(b->table_bytes));
+    SYN_TRY(lm_head.prepare(rows));
+    samples = std::move(b);
+    return SYN_OK;
+  }
+  syn_hip_paged_attention_params sample_attention(const SampleSpace &b, size_t l, size_t each) const {
+    syn_hip_paged_attention_params p{};
+    p.layer = (uint32_t)l;
+    p.n_heads = c.base.n_heads;
+    p.n_seqs = (uint32_t)b.n;
+    p.n_tokens = (uint32_t)(b.n * each);
+    p.max_new = (uint32_t)each;
+    p.max_len = (uint32_t)b.most();
+    p.ldq = p.ldo = qd;
+    p.ld_table = b.tables.ld_table;
+    return p;
+  }
+  syn_hip_draft_verify_params sample_verify(const SampleSpace &b, size_t drafts) const {
+    syn_hip_draft_verify_params p{};
+    p.n_seqs = (uint32_t)b.n;
+    p.max_draft = (uint32_t)drafts;
+    p.pad = (uint32_t)std::max(b.eos, 0);
+    p.vocab = vocab;
+    p.ld_target = b.ld;
+    p.target_stride = (drafts + 1) * b.ld;
+    p.ld_draft = b.n * b.ld;  // draft steps one after the other
+    p.draft_stride = b.ld;
+    return p;
+  }
+
+  // the state at the beginning: row 0 holds the prompt's pages, no token is drawn
+  syn_status_t reset_samples(SampleSpace &b, float temperature, uint64_t seed) {
+    const size_t n = b.n, n_draws = n + b.max_new * n * (2 * b.k + 1);
+    std::vector<float> draws(n_draws), heat(n, temperature);
+    SYN_TRY(syn_hip_stdrng_f32(seed, n_draws, draws.data()));
+    std::vector<int32_t> iota(b.n_prompt), zeros(std::max(b.n_prompt, n), 0), lens(n, 0);
+    for (size_t i = 0; i < b.n_prompt; i++) iota[i] = (int32_t)i;
+    lens[0] = (int32_t)b.n_prompt;
+    std::vector<int32_t> none(n * b.tables.ld_table, -1), free(b.pages.n_pages, 0);
+    std::vector<int32_t> ints(b.ints.bytes / 4, 0);
+    for (size_t s = 0; s < n; s++) ints[1 + s] = (int32_t)b.n_prompt;  // len
+    auto put = [&](void *dst, const void *src, size_t bytes) -> syn_status_t {
+      SYN_HIP(hipMemcpyAsync(dst, src, bytes, hipMemcpyHostToDevice, stream));
+      return SYN_OK;
+    };
+    SYN_TRY(put(b.draws.p, draws.data(), n_draws * 4));
+    SYN_TRY(put(b.heat.p, heat.data(), n * 4));
+    SYN_TRY(put(b.iota.p, iota.data(), b.n_prompt * 4));
+    SYN_TRY(put(b.zeros.p, zeros.data(), zeros.size() * 4));
+    SYN_TRY(put(b.lens.p, lens.data(), n * 4));
+    SYN_TRY(put(b.table.p, none.data(), none.size() * 4));
+    SYN_TRY(put(b.held.p, zeros.data(), n * 4));
+    SYN_TRY(put(b.refs.p, free.data(), free.size() * 4));
+    SYN_TRY(put(b.ints.p, ints.data(), ints.size() * 4));
+    SYN_TRY(put(b.parent.p, zeros.data(), n * 4));
+    SYN_HIP(hipStreamSynchronize(stream));
+    return syn_hip_kv_resize(&b.tables, b.lens.as<int32_t>(), b.table_ws.p, b.table_bytes, stream);
+  }
+
+  // `each` tokens of every sample through a layer, at d_pos of its sequence, which
+  // has d_len positions with them
+  syn_status_t sample_layer(SampleSpace &b, size_t l, size_t each, const int32_t *d_pos, const int32_t *d_seq,
+                            const int32_t *d_len, hipStream_t s) {
+    Layer &Ly = layers[l];
+    const size_t rows = b.n * each;
+    const float eps = c.base.eps;
+    SYN_TRY(launch_rmsnorm_quant(x.as<float>(), l == 0 ? nullptr : down.as<float>(),
+                                 attn_nw.as<float>() + l * h, eps, (int)rows, (int)h, nullptr, 0, nullptr,
+                                 normed.as<float>(), s));
+    SYN_TRY(Ly.qkv.gemv(rows, normed.as<float>(), h, qkv.as<float>(), n_qkv, s));
+    const syn_hip_kv_append_params ap = append_params(l, c.base.n_heads, b.n, b.tables.ld_table);
+    const float *q = qkv.as<float>();
+    SYN_TRY(syn_hip_kv_append(&b.pages, &ap, rows, q, q + qd, q + qd + kvd,
+                              c.qk_norm ? q_nw.as<float>() + l * hd : nullptr,
+                              c.qk_norm ? k_nw.as<float>() + l * hd : nullptr, rope_cos.as<float>(),
+                              rope_sin.as<float>(), d_pos, d_seq, d_pos, b.table.as<int32_t>(),
+                              qrot.as<float>(), s));
+    const syn_hip_paged_attention_params tp = sample_attention(b, l, each);
+    SYN_TRY(syn_hip_paged_attention(&b.pages, &tp, qrot.as<float>(), nullptr, d_len, b.table.as<int32_t>(),
+                                    attn.as<float>(), b.attn_ws.p, b.attn_bytes, s));
+    SYN_TRY(Ly.o.gemv(rows, attn.as<float>(), qd, o.as<float>(), h, s));
+    SYN_TRY(launch_rmsnorm_quant(x.as<float>(), o.as<float>(), ffn_nw.as<float>() + l * h, eps, (int)rows,
+                                 (int)h, nullptr, 0, nullptr, normed.as<float>(), s));
+    SYN_TRY(Ly.gu.gemv(rows, normed.as<float>(), h, gu.as<float>(), 2 * inter, s));
+    SYN_TRY(launch_swiglu_f32(gu.as<float>(), (int)(2 * inter), (int)rows, (int)inter, hbuf.as<float>(),
+                              (int)inter, s));
+    return Ly.down.gemv(rows, hbuf.as<float>(), inter, down.as<float>(), h, s);
+  }
+  syn_status_t sample_logits(size_t rows, float *out, size_t ld, hipStream_t s) {
+    SYN_TRY(launch_rmsnorm_quant(x.as<float>(), down.as<float>(), final_nw.as<float>(), c.base.eps, (int)rows,
+                                 (int)h, nullptr, 0, nullptr, normed.as<float>(), s));
+    return lm_head.gemv(rows, normed.as<float>(), h, out, ld, s);
+  }
+
+  // One round: pages for it, the drafts one after the other, all of them verified
+  // at once, and what follows.
+  syn_status_t sample_round(SampleSpace &b, hipStream_t s) {
+    const SampleState &st_ = b.st;
+    const size_t n = b.n, k = b.k;
+    SYN_TRY(syn_hip_kv_resize(&b.tables, st_.room, b.table_ws.p, b.table_bytes, s));
+    const syn_hip_draft_verify_params draw = sample_verify(b, 0), all = sample_verify(b, k);
+    for (size_t i = 0; i < k; i++) {
+      SYN_TRY(launch_embed(embed.as<float>(), i ? b.token.as<uint32_t>() : st_.last, (int)n, (int)h,
+                           (int)vocab, x.as<float>(), s));
+      for (size_t l = 0; l < b.draft_layers; l++)
+        SYN_TRY(sample_layer(b, l, 1, st_.draft_pos + i * n, nullptr, st_.draft_len + i * n, s));
+      float *row = b.draft.as<float>() + i * n * b.ld;
+      SYN_TRY(sample_logits(n, row, b.ld, s));
+      SYN_TRY(syn_hip_draft_verify(&draw, row, nullptr, nullptr, st_.drafting, b.heat.as<float>(),
+                                   st_.u_draft + i * n, b.token.as<uint32_t>(), b.count.as<int32_t>(), nullptr,
+                                   b.verify_ws.p, b.verify_bytes, s));
+      SYN_TRY(launch_sample_drafted(st_, (int)i, b.token.as<uint32_t>(), s));
+    }
+    SYN_TRY(launch_embed(embed.as<float>(), st_.ids, (int)b.rows(), (int)h, (int)vocab, x.as<float>(), s));
+    for (size_t l = 0; l < L; l++) SYN_TRY(sample_layer(b, l, k + 1, st_.pos, st_.seq, st_.room, s));
+    SYN_TRY(sample_logits(b.rows(), b.target.as<float>(), b.ld, s));
+    SYN_TRY(syn_hip_draft_verify(&all, b.target.as<float>(), k ? b.draft.as<float>() : nullptr, st_.drafted,
+                                 st_.drafts, b.heat.as<float>(), st_.u, b.token.as<uint32_t>(),
+                                 b.count.as<int32_t>(), nullptr, b.verify_ws.p, b.verify_bytes, s));
+    return launch_sample_advance(st_, b.token.as<uint32_t>(), (int)(k + 1), b.count.as<int32_t>(), s);
+  }
+
+  syn_status_t generate_samples(const uint32_t *prompt, size_t n_prompt, size_t max_new,
+                                const syn_hip_draft_sampling &sp, size_t draft_layers, uint32_t *out_tokens,
+                                uint32_t *out_lengths, uint32_t *out_rounds) {
+    SYN_TRY(make_samples(n_prompt, max_new, draft_layers, sp));
+    SampleSpace &b = *samples;
+    const size_t n = b.n;
+    SYN_TRY(reset_samples(b, sp.temperature, sp.seed));
+    if (use_graph && !b.graph && max_new > 1) {
+      hipGraph_t g;
+      SYN_HIP(hipStreamBeginCapture(stream, hipStreamCaptureModeThreadLocal));
+      const syn_status_t st_ = sample_round(b, stream);
+      hipError_t e = hipStreamEndCapture(stream, &g);
+      if (st_ != SYN_OK) {
+        if (e == hipSuccess) (void)hipGraphDestroy(g);
+        return st_;
+      }
+      if (e != hipSuccess) return hip_fail(e, "hipStreamEndCapture", __FILE__, __LINE__);
+      e = hipGraphInstantiate(&b.graph, g, nullptr, nullptr, 0);
+      (void)hipGraphDestroy(g);
+      if (e != hipSuccess) {
+        b.graph = nullptr;
+        return hip_fail(e, "hipGraphInstantiate", __FILE__, __LINE__);
+      }
+    }
+    // the prompt into row 0's pages, the other rows continue it, and the first
+    // token of each is drawn from the prompt's one row of logits
+    hp.known = false;
+    SYN_HIP(hipMemcpyAsync(ids.p, prompt, n_prompt * 4, hipMemcpyHostToDevice, stream));
+    SYN_TRY(set_state(0, 0, 0));
+    const PromptPages pp{&b.pages, b.iota.as<int32_t>(), b.zeros.as<int32_t>(), b.table.as<int32_t>(),
+                         b.tables.ld_table};
+    SYN_TRY(prefill_rows(ids.as<uint32_t>(), (int)n_prompt, 0, &pp));
+    SYN_TRY(head((int)n_prompt - 1, (int)n_prompt, stream));
+    SYN_TRY(syn_hip_kv_fork(&b.pages, &b.tables, b.parent.as<int32_t>(), b.st.len, b.table_ws.p,
+                            b.table_bytes, stream));
+    syn_hip_draft_verify_params first = sample_verify(b, 0);
+    first.ld_target = vocab;
+    first.target_stride = 0;
+    SYN_TRY(syn_hip_draft_verify(&first, logits.as<float>(), nullptr, nullptr, nullptr, b.heat.as<float>(),
+                                 b.draws.as<float>(), b.token.as<uint32_t>(), b.count.as<int32_t>(), nullptr,
+                                 b.verify_ws.p, b.verify_bytes, stream));
+    SYN_TRY(launch_sample_advance(b.st, b.token.as<uint32_t>(), 1, b.count.as<int32_t>(), stream));
+    std::vector<int32_t> ended(n, 0);
+    size_t rounds = 0;
+    const size_t least = cdiv(max_new - 1, b.k + 1);  // rounds that draw max_new tokens
+    for (; rounds + 1 < max_new;) {
+      if (use_graph)
+        SYN_HIP(hipGraphLaunch(b.graph, stream));
+      else
+        SYN_TRY(sample_round(b, stream));
+      rounds++;
+      if (rounds + 1 < max_new && (rounds >= least || (b.eos >= 0 && rounds % 8 == 0))) {  // all ended?
+        SYN_HIP(hipMemcpyAsync(ended.data(), b.st.drafting, n * 4, hipMemcpyDeviceToHost, stream));
+        SYN_HIP(hipStreamSynchronize(stream));
+        if (std::all_of(ended.begin(), ended.end(), [](int32_t e) { return e < 0; })) break;
+      }
+    }
+    std::vector<uint32_t> hist(n * max_new);
+    std::vector<int32_t> len(n);
+    SYN_HIP(hipMemcpyAsync(hist.data(), b.history.p, hist.size() * 4, hipMemcpyDeviceToHost, stream));
+    SYN_HIP(hipMemcpyAsync(len.data(), b.st.out, n * 4, hipMemcpyDeviceToHost, stream));
+    SYN_HIP(hipStreamSynchronize(stream));
+    for (size_t i = 0; i < n; i++) {
+      for (size_t t = 0; t < max_new; t++)
+        out_tokens[i * max_new + t] =
+            t < (size_t)len[i] ? hist[i * max_new + t] : (uint32_t)std::max(b.eos, 0);
+      if (out_lengths) out_lengths[i] = (uint32_t)len[i];
+    }
+    if (out_rounds) *out_rounds = (uint32_t)rounds;
     return SYN_OK;
   }
 
@@ -1078,6 +1401,48 @@ syn_status_t syn_hip_klm_generate_beams(syn_hip_klm_t *m, const uint32_t *prompt
     return m->generate_beams(prompt, n_prompt, max_new, *p, out_tokens, out_lengths, out_scores);
   } catch (const std::bad_alloc &) {
     set_error("beam search: host memory");
+    return SYN_ERR_OUT_OF_MEMORY;
+  }
+}
+
+syn_status_t syn_hip_klm_generate_samples(syn_hip_klm_t *m, const uint32_t *prompt, size_t n_prompt,
+                                          size_t max_new, const syn_hip_draft_sampling *p,
+                                          uint32_t *out_tokens, uint32_t *out_lengths,
+                                          uint32_t *out_rounds) {
+  SYN_TRY(check_klm(m));
+  if (!prompt || !p || !out_tokens) return SYN_ERR_NULL_PTR;
+  if (max_new == 0) return SYN_OK;
+  if (p->n_samples == 0 || p->n_samples > kMaxBeams || p->n_draft > 16 ||
+      (size_t)p->n_samples * (p->n_draft + 1) > m->S) {
+    set_error("samples: 1 to 64 with at most 16 drafts, max_seq rows of them a round");
+    return SYN_ERR_INVALID_ARG;
+  }
+  if (n_prompt == 0 || n_prompt > m->S || max_new - 1 > m->S - n_prompt ||
+      p->n_draft > m->S - n_prompt - (max_new - 1)) {
+    set_error("samples: prompt + generated tokens + drafts must be in [1, max_seq]");
+    return SYN_ERR_INVALID_ARG;
+  }
+  if (p->eos >= 0 && (size_t)p->eos >= m->vocab) {
+    set_error("samples: eos outside the vocabulary");
+    return SYN_ERR_INVALID_ARG;
+  }
+  if (p->draft_layers > m->L) {
+    set_error("samples: more draft layers than the model has");
+    return SYN_ERR_INVALID_ARG;
+  }
+  if (p->kv_dtype != SYN_HIP_KV_F32 && p->kv_dtype != SYN_HIP_KV_F16 && p->kv_dtype != SYN_HIP_KV_BF16) {
+    set_error("samples: unknown cache dtype");
+    return SYN_ERR_INVALID_ARG;
+  }
+  if (m->hd % 8 || m->hd > kKvMaxHeadDim) {
+    set_error("samples: head_dim must be a multiple of 8 up to 256");
+    return SYN_ERR_INVALID_ARG;
+  }
+  const size_t layers = p->draft_layers ? p->draft_layers : std::max<size_t>(1, m->L / 3);
+  try {
+    return m->generate_samples(prompt, n_prompt, max_new, *p, layers, out_tokens, out_lengths, out_rounds);
+  } catch (const std::bad_alloc &) {
+    set_error("samples: host memory");
     return SYN_ERR_OUT_OF_MEMORY;
   }
 }

@@ -119,6 +119,13 @@ class KvTables(C.Structure):
                 ("refs", C.c_void_p)]
 
 
+class DraftSampling(C.Structure):
+    """syn_hip_draft_sampling"""
+    _fields_ = [("n_samples", C.c_uint32), ("n_draft", C.c_uint32), ("draft_layers", C.c_uint32),
+                ("eos", C.c_int32), ("kv_dtype", C.c_int32), ("temperature", C.c_float),
+                ("seed", C.c_uint64)]
+
+
 class BeamSearch(C.Structure):
     """syn_hip_beam_search"""
     _fields_ = [("n_beams", C.c_uint32), ("eos", C.c_int32), ("kv_dtype", C.c_int32),
@@ -186,6 +193,7 @@ SIGNATURES = {
     "syn_hip_qlm_set_sampler": (ST, [P, C.POINTER(SamplerParams), C.c_uint64]),
     "syn_hip_sample": (ST, [P, SZ, P, SZ, C.POINTER(SamplerParams), C.c_float, P, P, P]),
     "syn_hip_klm_generate_beams": (ST, [P, P, SZ, SZ, C.POINTER(BeamSearch), P, P, P]),
+    "syn_hip_klm_generate_samples": (ST, [P, P, SZ, SZ, C.POINTER(DraftSampling), P, P, P]),
     "syn_hip_kv_append": (ST, [C.POINTER(KvPages), C.POINTER(KvAppend), SZ] + [P] * 13),
     "syn_hip_prefix_attention_workspace": (ST, [C.POINTER(KvPages), C.POINTER(PrefixAttention),
                                                 C.POINTER(SZ)]),
@@ -830,6 +838,19 @@ class KQuantCausalLM:
                                                ptr(toks), ptr(lens), ptr(scores)),
               "klm_generate_beams")
         return toks, lens, scores
+
+    def generate_samples(self, prompt, max_new: int, n_samples: int, n_draft: int = 4,
+                         draft_layers: int = 0, temperature: float = 1.0, eos: int = -1,
+                         kv_dtype: int = KV_F32, seed: int = 0):
+        """Samples drawn with drafts: (tokens [n_samples, max_new], lengths, rounds)."""
+        prompt = np.ascontiguousarray(prompt, np.uint32)
+        toks, lens = np.zeros((n_samples, max_new), np.uint32), np.zeros(n_samples, np.uint32)
+        p, rounds = DraftSampling(n_samples, n_draft, draft_layers, eos, kv_dtype, temperature,
+                                  seed), C.c_uint32()
+        check(lib().syn_hip_klm_generate_samples(self.h, ptr(prompt), prompt.size, max_new, C.byref(p),
+                                                 ptr(toks), ptr(lens), C.byref(rounds)),
+              "klm_generate_samples")
+        return toks, lens, rounds.value
 
     def time(self, prompt, steps: int):
         prompt = np.ascontiguousarray(prompt, np.uint32)
