@@ -28,6 +28,7 @@ struct TableArgs {
   int32_t *need;    // [n_seqs] pages that a row takes
   int32_t *before;  // [n_seqs + 1] those of the rows before it
   int32_t *count;   // [chunks] free (or live) pages of a chunk
+  int32_t *col;     // [n_seqs] the column that a row's first one goes to
   __device__ __forceinline__ bool has(int page) const { return (uint32_t)page < n_pages; }
   __device__ __forceinline__ int holds(int row) const {
     return (int)min((size_t)max(0, held[row]), ld);
@@ -57,6 +58,7 @@ __device__ __forceinline__ void resize_row(const TableArgs &a, int row) {
   if ((threadIdx.x & 63) == 0) {
     if (len >= 0) a.held[row] = min(held, want);
     a.need[row] = max(0, want - held);
+    a.col[row] = held;
   }
 }
 
@@ -90,6 +92,7 @@ __device__ __forceinline__ void fork_row(const TableArgs &a, int row) {
   if (lane == 0) {
     a.held[row] = full;
     a.need[row] = (n & (a.ps - 1)) != 0;
+    a.col[row] = full;
   }
 }
 
@@ -119,16 +122,40 @@ template <int NT> __device__ __forceinline__ int sum_before(int x, int *all) {
   return s;
 }
 
-// the wanted pages among a thread's: bit j for page first + j
-template <bool LIVE> __device__ __forceinline__ uint32_t wanted(const TableArgs &a, uint32_t first) {
+// the wanted pages among a thread's: bit j for page first + j (PER of them, a
+// multiple of 4; counts are read where the atomics are)
+template <bool LIVE, int PER>
+__device__ __forceinline__ uint32_t wanted(const int32_t *refs, uint32_t first, uint32_t n_pages) {
   uint32_t on = 0;
+  int n[PER];
+  if (first + PER <= n_pages && (reinterpret_cast<uintptr_t>(refs) & 15) == 0) {
 #pragma unroll
-  for (int j = 0; j < kPer; j++)
-    if (first + j < a.n_pages) {
-      const int n = a.refs[first + j];
-      on |= (LIVE ? n > 0 : n == 0) ? 1u << j : 0u;
+    for (int j = 0; j < PER; j += 4) {
+      const i32x4 x = *reinterpret_cast<const i32x4 *>(refs + first + j);
+#pragma unroll
+      for (int k = 0; k < 4; k++) n[j + k] = x[k];
     }
+  } else {
+#pragma unroll
+    for (int j = 0; j < PER; j++) n[j] = first + j < n_pages ? refs[first + j] : -1;
+  }
+#pragma unroll
+  for (int j = 0; j < PER; j++) on |= (LIVE ? n[j] > 0 : n[j] == 0) ? 1u << j : 0u;
   return on;
+}
+
+// the last row with before[row] <= rank (rows that need none have the same sum as
+// the row after them)
+__device__ __forceinline__ int row_of(const int32_t *before, int n, int rank) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (before[mid] <= rank)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
 }
 
 // workgroup 0: the rows' needs added up; the others: a chunk's wanted pages
@@ -137,18 +164,19 @@ template <bool LIVE> __global__ void __launch_bounds__(kNT) k_count(TableArgs a)
   int all;
   if (blockIdx.x == 0) {
     if (LIVE) return;
-    int base = 0;
-    for (int r0 = 0; r0 < a.n_seqs; r0 += kNT) {
-      const int r = r0 + tid, n = r < a.n_seqs ? a.need[r] : 0;
-      const int s = sum_before<kNT>(n, &all);
-      if (r < a.n_seqs) a.before[r] = base + s;
-      base += all;
+    const int each = (a.n_seqs + kNT - 1) / kNT, r0 = min(tid * each, a.n_seqs), r1 = min(r0 + each, a.n_seqs);
+    int sum = 0;
+    for (int r = r0; r < r1; r++) sum += a.need[r];
+    int at = sum_before<kNT>(sum, &all);
+    for (int r = r0; r < r1; r++) {
+      a.before[r] = at;
+      at += a.need[r];
     }
-    if (tid == 0) a.before[a.n_seqs] = base;
+    if (tid == 0) a.before[a.n_seqs] = all;
     return;
   }
   const uint32_t chunk = blockIdx.x - 1;
-  (void)sum_before<kNT>(__popc(wanted<LIVE>(a, chunk * kChunk + tid * kPer)), &all);
+  (void)sum_before<kNT>(__popc(wanted<LIVE, kPer>(a.refs, chunk * kChunk + tid * kPer, a.n_pages)), &all);
   if (tid == 0) a.count[chunk] = all;
 }
 
@@ -165,36 +193,117 @@ __device__ __forceinline__ int chunks_before(const TableArgs &a, int chunk, int 
   return sum;
 }
 
-// The i-th free page goes to the i-th place that needs one.
+constexpr int kLdsRows = 4096;  // rows whose sums a workgroup searches in LDS
+
+// The i-th free page goes to the i-th place that needs one: a chunk's free pages
+// are listed in LDS, so that each thread has one of them in turn.
 __global__ void __launch_bounds__(kNT) k_take(TableArgs a) {
+  __shared__ uint16_t list[kChunk];
+  __shared__ int32_t sums[kLdsRows];
   const int chunk = blockIdx.x, tid = threadIdx.x;
   int free, in;
   const int base = chunks_before(a, chunk, &free);
   const int needed = a.before[a.n_seqs];
   if (chunk == 0)
-    for (int r = tid; r < a.n_seqs; r += kNT)
-      a.held[r] += max(0, min(a.need[r], free - a.before[r]));
-  if (base >= needed) return;
-  const uint32_t first = chunk * (uint32_t)kChunk + tid * kPer;
-  uint32_t on = wanted<false>(a, first);
-  int rank = base + sum_before<kNT>(__popc(on), &in);
-  for (; on && rank < needed; on &= on - 1, rank++) {
-    const int page = (int)first + __ffs(on) - 1;
-    int lo = 0, hi = a.n_seqs;  // the last row with before[row] <= rank
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (a.before[mid] <= rank)
-        lo = mid;
-      else
-        hi = mid;
+    for (int r = tid; r < a.n_seqs; r += kNT) {
+      const int n = max(0, min(a.need[r], free - a.before[r]));
+      if (n) a.held[r] += n;
     }
-    // (rows that need none have the same sum as the row after them)
-    const int len = a.len[lo], i = rank - a.before[lo];
-    const int end = a.parent ? (int)(taken_over(a, lo, parent_of(a, lo)) >> a.ps_shift) + 1
-                             : (int)min((size_t)a.pages_of(len), a.ld);
-    a.table[(size_t)lo * a.ld + (end - a.need[lo] + i)] = page;
+  if (base >= needed) return;
+  const uint32_t on = wanted<false, kPer>(a.refs, chunk * (uint32_t)kChunk + tid * kPer, a.n_pages);
+  int rank = sum_before<kNT>(__popc(on), &in);
+  for (uint32_t m = on; m; m &= m - 1) list[rank++] = (uint16_t)(tid * kPer + __ffs(m) - 1);
+  const bool lds = a.n_seqs <= kLdsRows;
+  if (lds)
+    for (int r = tid; r < a.n_seqs; r += kNT) sums[r] = a.before[r];
+  __syncthreads();
+  const int most = min(in, needed - base);
+  for (int i = tid; i < most; i += kNT) {
+    const int row = row_of(lds ? sums : a.before, a.n_seqs, base + i);
+    const int page = chunk * kChunk + list[i];
+    a.table[(size_t)row * a.ld + a.col[row] + (base + i - a.before[row])] = page;
     a.refs[page] = 1;
   }
+}
+
+// ---- the whole of it by one workgroup, where little is to be done: a launch and
+// five steps with a barrier between, their entries dealt to all threads.
+constexpr int kSmallNT = 1024;
+constexpr int kSmallRows = 1024, kSmallEntries = 16384;
+constexpr uint32_t kSmallPages = 65536;
+
+template <bool FORK> __global__ void __launch_bounds__(kSmallNT) k_tables_small(TableArgs a) {
+  // entries that a row gives back, shares, and takes: sums over the rows before
+  __shared__ int32_t back[kSmallRows], share[FORK ? kSmallRows : 1], take[kSmallRows];
+  __shared__ int32_t first[kSmallRows], col[kSmallRows], from[FORK ? kSmallRows : 1];
+  const int tid = threadIdx.x, n = a.n_seqs;
+  int n_back = 0, n_share = 0, n_take = 0, keep = 0, parent = -1;
+  bool changed = false;
+  if (tid < n) {
+    const int held = a.holds(tid);
+    if (FORK) {
+      parent = parent_of(a, tid);
+      if (parent >= 0) {
+        const long long m = taken_over(a, tid, parent);
+        n_back = held;
+        n_share = keep = (int)(m >> a.ps_shift);
+        n_take = (m & (a.ps - 1)) != 0;
+        first[tid] = 0;
+        changed = true;
+      }
+      from[tid] = parent;
+    } else {
+      const int len = a.len[tid], want = len < 0 ? held : (int)min((size_t)a.pages_of(len), a.ld);
+      keep = min(held, want);
+      n_back = held - keep;
+      n_take = want - keep;
+      first[tid] = keep;
+      changed = len >= 0;
+    }
+    col[tid] = keep;
+  }
+  int all_back, all_share = 0, all_take;
+  const int b0 = sum_before<kSmallNT>(n_back, &all_back), t0 = sum_before<kSmallNT>(n_take, &all_take);
+  if (tid < n) back[tid] = b0, take[tid] = t0;
+  if (FORK) {
+    const int s0 = sum_before<kSmallNT>(n_share, &all_share);
+    if (tid < n) share[tid] = s0;
+  }
+  __syncthreads();
+  for (int e = tid; e < all_back; e += kSmallNT) {
+    const int row = row_of(back, n, e);
+    int32_t *t = a.table + (size_t)row * a.ld + first[row] + (e - back[row]);
+    drop(a, *t);
+    *t = -1;
+  }
+  if (FORK) {
+    __syncthreads();
+    for (int e = tid; e < all_share; e += kSmallNT) {
+      const int row = row_of(share, n, e), c = e - share[row];
+      const int page = a.table[(size_t)from[row] * a.ld + c];
+      if (a.has(page)) atomicAdd(a.refs + page, 1);
+      a.table[(size_t)row * a.ld + c] = page;
+    }
+  }
+  // every count has changed where it is read next (an agent's fence would write
+  // the L2 back and drop it)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  int given = 0;
+  constexpr int kEach = 8;
+  for (uint32_t p0 = 0; p0 < a.n_pages && given < all_take; p0 += kSmallNT * kEach) {
+    int in;
+    const uint32_t p = p0 + tid * kEach;
+    uint32_t on = wanted<false, kEach>(a.refs, p, a.n_pages);
+    int rank = given + sum_before<kSmallNT>(__popc(on), &in);
+    for (; on && rank < all_take; on &= on - 1, rank++) {
+      const int page = (int)p + __ffs(on) - 1, row = row_of(take, n, rank);
+      a.table[(size_t)row * a.ld + col[row] + (rank - take[row])] = page;
+      a.refs[page] = 1;
+    }
+    given += in;
+  }
+  if (changed) a.held[tid] = keep + max(0, min(n_take, given - t0));
 }
 
 // ---------------------------------------------------------------- copies
@@ -220,16 +329,30 @@ __global__ void __launch_bounds__(kNT) k_copy_tails(TableArgs a, CopyArgs c) {
   const int layer = blockIdx.x / c.nkv, h = blockIdx.x - layer * c.nkv;
   const size_t head = (size_t)c.hd * c.ps * c.esz, off = (size_t)layer * c.n_pages;
   const size_t so = ((off + src) * c.nkv + h) * head, to = ((off + dst) * c.nkv + h) * head;
-  const int v16 = n8 * c.hd * c.esz / 2;  // 16-byte units: 8 elements of each dim, whole groups
-  for (int i = threadIdx.x; i < v16; i += kNT)
-    *reinterpret_cast<uint4 *>(c.to_v + to + (size_t)i * 16) =
-        *reinterpret_cast<const uint4 *>(c.v + so + (size_t)i * 16);
-  const int run = n8 * 4 * c.esz;  // 16-byte units of n8 * 8 positions at 8 dims
+  // 16-byte units of 8 elements: V whole groups of 8 positions of every dim, K n8 * 8
+  // positions of every 8 dims
+  const int units = n8 * c.hd * c.esz / 2, run = n8 * 4 * c.esz;
   const size_t pitch = (size_t)c.ps * 8 * c.esz;
-  for (int i = threadIdx.x; i < run * (c.hd >> 3); i += kNT) {
-    const int d8 = i / run;
-    const size_t o = d8 * pitch + (size_t)(i - d8 * run) * 16;
-    *reinterpret_cast<uint4 *>(c.to_k + to + o) = *reinterpret_cast<const uint4 *>(c.k + so + o);
+  auto at = [&](int i) {
+    if (i < units) return (size_t)i * 16;
+    const int k = i - units, d8 = k / run;
+    return d8 * pitch + (size_t)(k - d8 * run) * 16;
+  };
+  constexpr int kAtOnce = 4;
+  for (int i0 = threadIdx.x; i0 < 2 * units; i0 += kAtOnce * kNT) {
+    u32x4 x[kAtOnce];
+    size_t o[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++) {
+      const int i = min(i0 + j * kNT, 2 * units - 1);
+      o[j] = at(i);
+      x[j] = *reinterpret_cast<const u32x4 *>((i < units ? c.v : c.k) + so + o[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++) {
+      const int i = i0 + j * kNT;
+      if (i < 2 * units) *reinterpret_cast<u32x4 *>((i < units ? c.to_v : c.to_k) + to + o[j]) = x[j];
+    }
   }
 }
 
@@ -248,7 +371,7 @@ __global__ void __launch_bounds__(kNT) k_number(TableArgs a, CopyArgs c, MoveArg
   for (uint32_t p = live + chunk * kNT + tid; p < c.to_pages; p += gridDim.x * kNT) m.to_refs[p] = 0;
   if (chunk >= a.chunks) return;
   const uint32_t first = chunk * (uint32_t)kChunk + tid * kPer;
-  const uint32_t on = wanted<true>(a, first);
+  const uint32_t on = wanted<true, kPer>(a.refs, first, a.n_pages);
   int rank = base + sum_before<kNT>(__popc(on), &in);
   for (int j = 0; j < kPer; j++) {
     if (first + j >= a.n_pages) break;
@@ -259,6 +382,45 @@ __global__ void __launch_bounds__(kNT) k_number(TableArgs a, CopyArgs c, MoveArg
       m.to_refs[rank] = a.refs[first + j];
     }
     rank += is;
+  }
+}
+
+// The same and the tables by one workgroup, where little is to be done.
+__global__ void __launch_bounds__(kSmallNT) k_rename_small(TableArgs a, CopyArgs c, MoveArgs m) {
+  const int tid = threadIdx.x;
+  constexpr int kEach = 8;
+  int live = 0, in;
+  for (uint32_t p0 = 0; p0 < a.n_pages; p0 += kSmallNT * kEach) {
+    const uint32_t p = p0 + tid * kEach;
+    const uint32_t on = wanted<true, kEach>(a.refs, p, a.n_pages);
+    int rank = live + sum_before<kSmallNT>(__popc(on), &in);
+#pragma unroll
+    for (int j = 0; j < kEach; j++) {
+      if (p + j >= a.n_pages) break;
+      const bool is = on >> j & 1, fits = (uint32_t)rank < c.to_pages;
+      m.number[p + j] = is && fits ? rank : -1;
+      if (is && fits) {
+        m.order[rank] = (int)(p + j);
+        m.to_refs[rank] = a.refs[p + j];
+      }
+      rank += is;
+    }
+    live += in;
+  }
+  if (tid == 0) *m.live = live;
+  for (uint32_t p = live + tid; p < c.to_pages; p += kSmallNT) m.to_refs[p] = 0;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the numbers are read below
+  __syncthreads();
+  for (int r = tid; r < a.n_seqs; r += kSmallNT) m.to_held[r] = a.holds(r);
+  const uint32_t entries = (uint32_t)(a.n_seqs * m.to_ld);
+  for (uint32_t e = tid; e < entries; e += kSmallNT) {
+    const uint32_t row = e / (uint32_t)m.to_ld, col = e - row * (uint32_t)m.to_ld;
+    int to = -1;
+    if ((int)col < a.holds((int)row)) {
+      const int page = a.table[(size_t)row * a.ld + col];
+      if (a.has(page)) to = m.number[page];
+    }
+    m.to_table[e] = to;
   }
 }
 
@@ -276,7 +438,7 @@ __global__ void __launch_bounds__(kNT) k_rename(TableArgs a, MoveArgs m) {
   m.to_table[(size_t)row * m.to_ld + col] = to;
 }
 
-constexpr int kSlice = 32768;  // bytes that a workgroup moves at a time
+constexpr int kSlice = 16384;  // bytes that a workgroup moves at a time
 
 // Pages of every layer, keys then values, in slices.
 __global__ void __launch_bounds__(kNT) k_move_pages(CopyArgs c, MoveArgs m) {
@@ -290,14 +452,21 @@ __global__ void __launch_bounds__(kNT) k_move_pages(CopyArgs c, MoveArgs m) {
     const uint8_t *src = (kind & 1 ? c.v : c.k) + ((size_t)layer * c.n_pages + m.order[page]) * bytes + at;
     uint8_t *dst = (kind & 1 ? c.to_v : c.to_k) + ((size_t)layer * c.to_pages + page) * bytes + at;
     const int n = (int)min((size_t)kSlice, bytes - at) / 16;
-    for (int u = threadIdx.x; u < n; u += kNT)
-      reinterpret_cast<uint4 *>(dst)[u] = reinterpret_cast<const uint4 *>(src)[u];
+    constexpr int kAtOnce = kSlice / 16 / kNT;  // all of a slice in flight
+    u32x4 x[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++)
+      x[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src) + min((int)threadIdx.x + j * kNT, n - 1));
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++)
+      if ((int)threadIdx.x + j * kNT < n)
+        __builtin_nontemporal_store(x[j], reinterpret_cast<u32x4 *>(dst) + threadIdx.x + j * kNT);
   }
 }
 
 // ---------------------------------------------------------------- host
 struct Space {
-  size_t need, before, count, number, order, total;
+  size_t need, before, count, col, number, order, total;
   int chunks;
 };
 Space space_of(const syn_hip_kv_tables &t) {
@@ -306,7 +475,8 @@ Space space_of(const syn_hip_kv_tables &t) {
   s.need = 0;
   s.before = s.need + (size_t)t.n_seqs * 4;
   s.count = s.before + ((size_t)t.n_seqs + 1) * 4;
-  s.number = s.count + (size_t)s.chunks * 4;
+  s.col = s.count + (size_t)s.chunks * 4;
+  s.number = s.col + (size_t)t.n_seqs * 4;
   s.order = s.number + (size_t)t.n_pages * 4;
   s.total = round_up(s.order + (size_t)t.n_pages * 4, 16);
   return s;
@@ -368,10 +538,16 @@ TableArgs table_args(const syn_hip_kv_tables &t, const int32_t *parent, const in
   a.need = reinterpret_cast<int32_t *>(w + s.need);
   a.before = reinterpret_cast<int32_t *>(w + s.before);
   a.count = reinterpret_cast<int32_t *>(w + s.count);
+  a.col = reinterpret_cast<int32_t *>(w + s.col);
   return a;
 }
 
 template <bool FORK> syn_status_t launch_take(const TableArgs &a, hipStream_t s) {
+  if (a.n_seqs <= kSmallRows && a.n_pages <= kSmallPages && a.n_seqs * a.ld <= kSmallEntries) {
+    hipLaunchKernelGGL(k_tables_small<FORK>, dim3(1), dim3(kSmallNT), 0, s, a);
+    SYN_LAUNCH_CHECK();
+    return SYN_OK;
+  }
   hipLaunchKernelGGL(k_rows<FORK>, dim3((unsigned)cdiv(a.n_seqs, kNT / 64)), dim3(kNT), 0, s, a);
   SYN_LAUNCH_CHECK();
   hipLaunchKernelGGL(k_count<false>, dim3(a.chunks + 1), dim3(kNT), 0, s, a);
@@ -468,13 +644,18 @@ syn_status_t syn_hip_kv_compact(const syn_hip_kv_pages *from, const syn_hip_kv_t
   uint8_t *w = static_cast<uint8_t *>(d_workspace);
   const MoveArgs m{reinterpret_cast<int32_t *>(w + sp.number), reinterpret_cast<int32_t *>(w + sp.order),
                    u->table, u->held, u->refs, d_live, u->ld_table};
-  hipLaunchKernelGGL(k_count<true>, dim3(a.chunks + 1), dim3(kNT), 0, s, a);
-  SYN_LAUNCH_CHECK();
-  hipLaunchKernelGGL(k_number, dim3(a.chunks), dim3(kNT), 0, s, a, c, m);
-  SYN_LAUNCH_CHECK();
-  hipLaunchKernelGGL(k_rename, dim3((unsigned)std::max<size_t>(1, cdiv(u->ld_table, kNT)), t->n_seqs),
-                     dim3(kNT), 0, s, a, m);
-  SYN_LAUNCH_CHECK();
+  if (std::max(from->n_pages, to->n_pages) <= kSmallPages && t->n_seqs * u->ld_table <= kSmallEntries) {
+    hipLaunchKernelGGL(k_rename_small, dim3(1), dim3(kSmallNT), 0, s, a, c, m);
+    SYN_LAUNCH_CHECK();
+  } else {
+    hipLaunchKernelGGL(k_count<true>, dim3(a.chunks + 1), dim3(kNT), 0, s, a);
+    SYN_LAUNCH_CHECK();
+    hipLaunchKernelGGL(k_number, dim3(a.chunks), dim3(kNT), 0, s, a, c, m);
+    SYN_LAUNCH_CHECK();
+    hipLaunchKernelGGL(k_rename, dim3((unsigned)std::max<size_t>(1, cdiv(u->ld_table, kNT)), t->n_seqs),
+                       dim3(kNT), 0, s, a, m);
+    SYN_LAUNCH_CHECK();
+  }
   hipLaunchKernelGGL(k_move_pages, dim3(2048), dim3(kNT), 0, s, c, m);
   SYN_LAUNCH_CHECK();
   return SYN_OK;
