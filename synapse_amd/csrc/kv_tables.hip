@@ -15,8 +15,9 @@ namespace syn {
 namespace {
 
 constexpr int kNT = 256;
-constexpr int kPer = 16;              // pages of a thread
-constexpr int kChunk = kNT * kPer;    // pages of a workgroup
+constexpr int kPoolNT = 1024;           // of a workgroup that looks through a chunk of the pool
+constexpr int kPer = 4;                 // pages of a thread
+constexpr int kChunk = kPoolNT * kPer;  // pages of a workgroup
 constexpr uint32_t kMaxTablePages = 1u << 24;
 
 struct TableArgs {
@@ -159,15 +160,15 @@ __device__ __forceinline__ int row_of(const int32_t *before, int n, int rank) {
 }
 
 // workgroup 0: the rows' needs added up; the others: a chunk's wanted pages
-template <bool LIVE> __global__ void __launch_bounds__(kNT) k_count(TableArgs a) {
+template <bool LIVE> __global__ void __launch_bounds__(kPoolNT) k_count(TableArgs a) {
   const int tid = threadIdx.x;
   int all;
   if (blockIdx.x == 0) {
     if (LIVE) return;
-    const int each = (a.n_seqs + kNT - 1) / kNT, r0 = min(tid * each, a.n_seqs), r1 = min(r0 + each, a.n_seqs);
+    const int each = (a.n_seqs + kPoolNT - 1) / kPoolNT, r0 = min(tid * each, a.n_seqs), r1 = min(r0 + each, a.n_seqs);
     int sum = 0;
     for (int r = r0; r < r1; r++) sum += a.need[r];
-    int at = sum_before<kNT>(sum, &all);
+    int at = sum_before<kPoolNT>(sum, &all);
     for (int r = r0; r < r1; r++) {
       a.before[r] = at;
       at += a.need[r];
@@ -176,20 +177,20 @@ template <bool LIVE> __global__ void __launch_bounds__(kNT) k_count(TableArgs a)
     return;
   }
   const uint32_t chunk = blockIdx.x - 1;
-  (void)sum_before<kNT>(__popc(wanted<LIVE, kPer>(a.refs, chunk * kChunk + tid * kPer, a.n_pages)), &all);
+  (void)sum_before<kPoolNT>(__popc(wanted<LIVE, kPer>(a.refs, chunk * kChunk + tid * kPer, a.n_pages)), &all);
   if (tid == 0) a.count[chunk] = all;
 }
 
 // wanted pages of the chunks before this one, and of all
 __device__ __forceinline__ int chunks_before(const TableArgs &a, int chunk, int *all) {
   int below = 0, total = 0, sum;
-  for (int c = threadIdx.x; c < a.chunks; c += kNT) {
+  for (int c = threadIdx.x; c < a.chunks; c += kPoolNT) {
     const int n = a.count[c];
     total += n;
     below += c < chunk ? n : 0;
   }
-  (void)sum_before<kNT>(total, all);
-  (void)sum_before<kNT>(below, &sum);
+  (void)sum_before<kPoolNT>(total, all);
+  (void)sum_before<kPoolNT>(below, &sum);
   return sum;
 }
 
@@ -197,7 +198,7 @@ constexpr int kLdsRows = 4096;  // rows whose sums a workgroup searches in LDS
 
 // The i-th free page goes to the i-th place that needs one: a chunk's free pages
 // are listed in LDS, so that each thread has one of them in turn.
-__global__ void __launch_bounds__(kNT) k_take(TableArgs a) {
+__global__ void __launch_bounds__(kPoolNT) k_take(TableArgs a) {
   __shared__ uint16_t list[kChunk];
   __shared__ int32_t sums[kLdsRows];
   const int chunk = blockIdx.x, tid = threadIdx.x;
@@ -205,20 +206,20 @@ __global__ void __launch_bounds__(kNT) k_take(TableArgs a) {
   const int base = chunks_before(a, chunk, &free);
   const int needed = a.before[a.n_seqs];
   if (chunk == 0)
-    for (int r = tid; r < a.n_seqs; r += kNT) {
+    for (int r = tid; r < a.n_seqs; r += kPoolNT) {
       const int n = max(0, min(a.need[r], free - a.before[r]));
       if (n) a.held[r] += n;
     }
   if (base >= needed) return;
   const uint32_t on = wanted<false, kPer>(a.refs, chunk * (uint32_t)kChunk + tid * kPer, a.n_pages);
-  int rank = sum_before<kNT>(__popc(on), &in);
+  int rank = sum_before<kPoolNT>(__popc(on), &in);
   for (uint32_t m = on; m; m &= m - 1) list[rank++] = (uint16_t)(tid * kPer + __ffs(m) - 1);
   const bool lds = a.n_seqs <= kLdsRows;
   if (lds)
-    for (int r = tid; r < a.n_seqs; r += kNT) sums[r] = a.before[r];
+    for (int r = tid; r < a.n_seqs; r += kPoolNT) sums[r] = a.before[r];
   __syncthreads();
   const int most = min(in, needed - base);
-  for (int i = tid; i < most; i += kNT) {
+  for (int i = tid; i < most; i += kPoolNT) {
     const int row = row_of(lds ? sums : a.before, a.n_seqs, base + i);
     const int page = chunk * kChunk + list[i];
     a.table[(size_t)row * a.ld + a.col[row] + (base + i - a.before[row])] = page;
@@ -363,16 +364,16 @@ struct MoveArgs {
 };
 
 // The live pages numbered; the other pool's counts.
-__global__ void __launch_bounds__(kNT) k_number(TableArgs a, CopyArgs c, MoveArgs m) {
+__global__ void __launch_bounds__(kPoolNT) k_number(TableArgs a, CopyArgs c, MoveArgs m) {
   const int chunk = blockIdx.x, tid = threadIdx.x;
   int live, in;
   const int base = chunks_before(a, chunk, &live);
   if (chunk == 0 && tid == 0) *m.live = live;
-  for (uint32_t p = live + chunk * kNT + tid; p < c.to_pages; p += gridDim.x * kNT) m.to_refs[p] = 0;
+  for (uint32_t p = live + chunk * kPoolNT + tid; p < c.to_pages; p += gridDim.x * kPoolNT) m.to_refs[p] = 0;
   if (chunk >= a.chunks) return;
   const uint32_t first = chunk * (uint32_t)kChunk + tid * kPer;
   const uint32_t on = wanted<true, kPer>(a.refs, first, a.n_pages);
-  int rank = base + sum_before<kNT>(__popc(on), &in);
+  int rank = base + sum_before<kPoolNT>(__popc(on), &in);
   for (int j = 0; j < kPer; j++) {
     if (first + j >= a.n_pages) break;
     const bool is = on >> j & 1, fits = (uint32_t)rank < c.to_pages;
@@ -550,9 +551,9 @@ template <bool FORK> syn_status_t launch_take(const TableArgs &a, hipStream_t s)
   }
   hipLaunchKernelGGL(k_rows<FORK>, dim3((unsigned)cdiv(a.n_seqs, kNT / 64)), dim3(kNT), 0, s, a);
   SYN_LAUNCH_CHECK();
-  hipLaunchKernelGGL(k_count<false>, dim3(a.chunks + 1), dim3(kNT), 0, s, a);
+  hipLaunchKernelGGL(k_count<false>, dim3(a.chunks + 1), dim3(kPoolNT), 0, s, a);
   SYN_LAUNCH_CHECK();
-  hipLaunchKernelGGL(k_take, dim3(a.chunks), dim3(kNT), 0, s, a);
+  hipLaunchKernelGGL(k_take, dim3(a.chunks), dim3(kPoolNT), 0, s, a);
   SYN_LAUNCH_CHECK();
   return SYN_OK;
 }
@@ -648,9 +649,9 @@ syn_status_t syn_hip_kv_compact(const syn_hip_kv_pages *from, const syn_hip_kv_t
     hipLaunchKernelGGL(k_rename_small, dim3(1), dim3(kSmallNT), 0, s, a, c, m);
     SYN_LAUNCH_CHECK();
   } else {
-    hipLaunchKernelGGL(k_count<true>, dim3(a.chunks + 1), dim3(kNT), 0, s, a);
+    hipLaunchKernelGGL(k_count<true>, dim3(a.chunks + 1), dim3(kPoolNT), 0, s, a);
     SYN_LAUNCH_CHECK();
-    hipLaunchKernelGGL(k_number, dim3(a.chunks), dim3(kNT), 0, s, a, c, m);
+    hipLaunchKernelGGL(k_number, dim3(a.chunks), dim3(kPoolNT), 0, s, a, c, m);
     SYN_LAUNCH_CHECK();
     hipLaunchKernelGGL(k_rename, dim3((unsigned)std::max<size_t>(1, cdiv(u->ld_table, kNT)), t->n_seqs),
                        dim3(kNT), 0, s, a, m);
