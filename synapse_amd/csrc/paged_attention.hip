@@ -122,13 +122,54 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, NC, FULL>)) k_atten
   w.finish(a, pool.hd, first, head, row0, rows, RW, at, reinterpret_cast<float *>(lds), ml);
 }
 
-// one workgroup for a query row of a sequence (those past its last token leave)
+// a query row of a sequence to a workgroup (those past its last token leave)
 template <int LANES> __global__ void __launch_bounds__(256) k_join_new(PagedArgs a, int hd) {
   const size_t row = blockIdx.x / a.nh;
   const int head = blockIdx.x - row * a.nh, s = row / a.max_new, token = row - (size_t)s * a.max_new;
   const int first = first_of(a, s);
   if (token >= count_of(a, s, first)) return;
   join_parts<LANES>(a, hd, (size_t)(first + token) * a.nh + head);
+}
+
+constexpr int kFewParts = 16;
+
+// ... or, of few parts, to LANES lanes with four dims each, all parts in flight
+// together (6144 rows of three parts of 128 dims 13.6 us with a workgroup each).
+template <int LANES> __global__ void __launch_bounds__(256) k_join_few(PagedArgs a, int hd, uint32_t rows) {
+  const uint32_t at = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  if (at >= rows) return;
+  const uint32_t row = at / a.nh, head = at - row * a.nh;
+  const int s = row / a.max_new, token = row - (uint32_t)s * a.max_new, c4 = 4 * (threadIdx.x % LANES);
+  const int start = a.start ? a.start[s] : 0, end = a.start ? a.start[s + 1] : 0;
+  const int first = a.start ? min(max(start, 0), a.n_tokens) : s * a.max_new;
+  const int count = a.start ? min(min(max(end, first), a.n_tokens) - first, a.max_new) : a.max_new;
+  if (token >= count || c4 >= hd) return;
+  const size_t q = (size_t)(first + token) * a.nh + head;
+  const float *ml = a.pml + q * a.parts * 2, *po = a.po + q * a.parts * hd + c4;
+  const int n = a.parts;
+  float m[kFewParts], l[kFewParts], top = kNegInf, sum = 0.0f;
+  f32x4 y[kFewParts], x{0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < kFewParts; i++)
+    if (i < n) {
+      m[i] = ml[2 * i];
+      l[i] = ml[2 * i + 1];
+      y[i] = *reinterpret_cast<const f32x4 *>(po + (size_t)i * hd);
+    }
+#pragma unroll
+  for (int i = 0; i < kFewParts; i++)
+    if (i < n) top = fmaxf(top, m[i]);
+#pragma unroll
+  for (int i = 0; i < kFewParts; i++)
+    if (i < n && l[i] != 0.0f) {  // (a part with no position has left its row unwritten)
+      const float f = __builtin_amdgcn_exp2f(m[i] - top);
+      sum = __builtin_fmaf(l[i], f, sum);
+#pragma unroll
+      for (int c = 0; c < 4; c++) x[c] = __builtin_fmaf(y[i][c], f, x[c]);
+    }
+  float *out = a.out + (size_t)(first + token) * a.ldo + (size_t)head * hd + c4;
+#pragma unroll
+  for (int c = 0; c < 4; c++) out[c] = sum == 0.0f ? 0.0f : x[c] / sum;
 }
 
 // ---------------------------------------------------------------- host
@@ -216,8 +257,11 @@ syn_status_t launch(const Plan &w, const PagedArgs &a, const KvPool<T> &pool, hi
     hipLaunchKernelGGL((k_attend_new<T, NC, false>), grid, block, 0, s, a, pool);
   SYN_LAUNCH_CHECK();
   if (w.parts == 1) return SYN_OK;
-  const dim3 rows((unsigned)w.rows);
-  hipLaunchKernelGGL((k_join_new<8 * NC>), rows, dim3(256), 0, s, a, pool.hd);
+  if (w.parts <= kFewParts)
+    hipLaunchKernelGGL((k_join_few<8 * NC>), dim3((unsigned)cdiv(w.rows, 256 / (8 * NC))), dim3(256), 0, s, a,
+                       pool.hd, (uint32_t)w.rows);
+  else
+    hipLaunchKernelGGL((k_join_new<8 * NC>), dim3((unsigned)w.rows), dim3(256), 0, s, a, pool.hd);
   SYN_LAUNCH_CHECK();
   return SYN_OK;
 }
