@@ -173,6 +173,8 @@ template <int LANES> __global__ void __launch_bounds__(256) k_join_few(PagedArgs
 }
 
 // ---------------------------------------------------------------- host
+constexpr double kMostSpace = 192 << 20;  // of a workspace, where runs need not be split
+
 struct Plan {
   bool solo;
   int nc, rw, blocks, chunk, parts;
@@ -201,13 +203,37 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_paged_attention_params 
   };
   w.parts = 1;
   w.chunk = (int)(tiles * kTile);
-  const size_t each = std::max<size_t>(1, cdiv(units * w.blocks * tiles, want));
-  const size_t grain = w.rw == 1 ? kWaves : 2;
-  if (tiles > whole * kWaves && each < tiles) {
-    const size_t k = cdiv(tiles, round_up(each, grain));
-    const size_t per = round_up(cdiv(tiles, k), grain);
+  auto cut = [&](size_t parts) {
+    const size_t grain = w.rw == 1 ? kWaves : 2, per = round_up(cdiv(tiles, parts), grain);
     w.chunk = (int)(per * kTile);
     w.parts = (int)cdiv(tiles, per);
+  };
+  const size_t all = units * w.blocks;
+  if (tiles > whole * kWaves && w.rw == 1 && all < want) {
+    // few rows are bound by their bytes: as many workgroups as the chip holds
+    cut(cdiv(want, all));
+  } else if (tiles > whole * kWaves && w.rw > 1) {
+    // Many rows are bound by their steps of a tile: of the ways to cut a run, the
+    // one with the fewest, counted in rounds of workgroups (half a round of them,
+    // one a CU, takes 0.8 of one), a fixed time each, and the join, which reads and
+    // writes every part (4.5 TB/s; a step takes 0.9 us, of an f32 pool 3.5).  One
+    // chunk of 1536 tokens at 12001, 24 heads of 128, f16: 576 workgroups 693 us,
+    // four parts 506; two such sequences 976 whole, 883 in two parts; 512 tokens at
+    // 8000, f32, 602 whole, 435 in five; 16 tokens of four sequences at 8200 175 and
+    // 43.
+    const double step = pg.dtype == SYN_HIP_KV_F32 ? 3.5e-6 : 0.9e-6;
+    double least = 0;
+    size_t best = 1;
+    for (size_t parts = 1; parts <= 64; parts++) {
+      cut(parts);
+      const size_t wgs = all * w.parts, rest = wgs % want;
+      const double rounds = (double)(wgs / want) + (rest == 0 ? 0.0 : (rest <= want / 2 ? 0.8 : 1.0));
+      const double join = (double)p.n_tokens * p.n_heads * w.parts * 8 * (hd + 2) / 4.5e12 / step + 5;
+      const double steps = rounds * (kFix + w.chunk / kTile) + (w.parts > 1 ? join : 0.0);
+      const bool fits = (double)p.n_tokens * p.n_heads * w.parts * 4 * (hd + 2) <= kMostSpace;
+      if (parts == 1 || (fits && steps < least)) least = steps, best = parts;
+    }
+    cut(best);
   }
   w.solo = alone(units * w.parts, w.chunk / kTile);
   const size_t work = units * w.parts;
