@@ -406,8 +406,9 @@ __device__ __forceinline__ int pick(const Weights &w, int first, int left, doubl
     up[i] = sum;
     some |= x > 0.0 ? 1u << i : 0u;
   }
-  double base = wave_before(sum);
-  if (lane == 63) wsum[wave] = base + sum;
+  const double upto = wave_upto(sum);
+  double base = wave_shifted(upto);
+  if (lane == 63) wsum[wave] = upto;
   __syncthreads();
   for (int i = 0; i < wave; i++) base += wsum[i];
   base += before;
@@ -416,10 +417,8 @@ __device__ __forceinline__ int pick(const Weights &w, int first, int left, doubl
   for (int i = 7; i >= 0; i--)
     if ((some >> i & 1) && base + up[i] > border) found = 8 * tid + i;
   int last = some ? 8 * tid + 31 - __clz(some) : -1;
-  for (int o = 32; o > 0; o >>= 1) {
-    found = min(found, __shfl_xor(found, o));
-    last = max(last, __shfl_xor(last, o));
-  }
+  found = over_wave(found, [](int p, int q) { return min(p, q); });
+  last = over_wave(last, [](int p, int q) { return max(p, q); });
   if (lane == 0) wfound[wave] = found, wlast[wave] = last;
   __syncthreads();
   found = min(min(wfound[0], wfound[1]), min(wfound[2], wfound[3]));
@@ -437,7 +436,7 @@ __global__ void __launch_bounds__(kNT) k_verify_draw(VerifyArgs a) {
   const int s = blockIdx.y, tid = threadIdx.x;
   const Draw d = a.draw[s];
   if (d.r < 0) return;
-  const double c32 = scale_of(a, s);
+  const double c32 = scale_of(a, s), u = (double)a.u[(size_t)s * (a.K + 1) + a.K];
   copy_table(tab);
   __syncthreads();
   Weights w{row_of(a, s, d.r),
@@ -468,7 +467,6 @@ __global__ void __launch_bounds__(kNT) k_verify_draw(VerifyArgs a) {
   }
   __syncthreads();
   if (!mine) return;
-  const double u = (double)a.u[(size_t)s * (a.K + 1) + a.K];
   if (tid < 64) {  // the block that the draw falls into
     auto load = [&](int i) {
       return i < a.blocks ? __longlong_as_double((long long)__hip_atomic_load(
@@ -482,7 +480,8 @@ __global__ void __launch_bounds__(kNT) k_verify_draw(VerifyArgs a) {
     double base = 0.0, before = 0.0;
     int at = -1;
     for (int i0 = 0; i0 < a.blocks; i0 += 64) {
-      const double x = i0 == 0 ? held[0] : (i0 == 64 ? held[1] : load(i0 + tid)), lo = base + wave_before(x);
+      const double x = i0 == 0 ? held[0] : (i0 == 64 ? held[1] : load(i0 + tid));
+      const double upto = wave_upto(x), lo = base + wave_shifted(upto);
       const uint64_t some = __ballot(x > 0.0), over = __ballot(x > 0.0 && lo + x > border);
       if (over | some) {  // the first above the border, or the last that has a weight
         const int k = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
@@ -490,7 +489,7 @@ __global__ void __launch_bounds__(kNT) k_verify_draw(VerifyArgs a) {
         before = __shfl(lo, k);
       }
       if (over) break;
-      base = __shfl(lo + x, 63);
+      base += __shfl(upto, 63);
     }
     if (tid == 0) before_of = before, border_of = border, block_of = at;
   }

@@ -110,9 +110,10 @@ template <bool FORK> __global__ void __launch_bounds__(kNT) k_rows(TableArgs a) 
 template <int NT> __device__ __forceinline__ int sum_before(int x, int *all) {
   __shared__ int w[NT / 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int s = wave_before(x);
+  const int upto = wave_upto(x);
+  int s = wave_shifted(upto);
   __syncthreads();
-  if (lane == 63) w[wave] = s + x;
+  if (lane == 63) w[wave] = upto;
   __syncthreads();
   int t = 0;
   for (int i = 0; i < NT / 64; i++) {

@@ -19,6 +19,7 @@ template <int STEP> __device__ __forceinline__ uint32_t partner(uint32_t x) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctl, 0xf, 0xf, false);
   }
 }
+template <int STEP> __device__ __forceinline__ int partner(int x) { return (int)partner<STEP>((uint32_t)x); }
 template <int STEP> __device__ __forceinline__ float partner(float x) {
   return __uint_as_float(partner<STEP>(__float_as_uint(x)));
 }
@@ -46,16 +47,30 @@ template <class F> __device__ __forceinline__ F wave_sum(F x) {
   return over_wave(x, [](F a, F b) { return a + b; });
 }
 
-// the sum over the lanes below this one
-template <class F> __device__ __forceinline__ F wave_before(F x) {
-  const int lane = threadIdx.x & 63;
-  F sum = x;
-  for (int o = 1; o < 64; o <<= 1) {
-    const F y = __shfl_up(sum, o);
-    if (lane >= o) sum += y;
-  }
-  const F before = __shfl_up(sum, 1);
-  return lane ? before : F(0);
+// x of the lane that a DPP control names, 0 where there is none
+template <int CTL, int ROWS> __device__ __forceinline__ uint32_t from_lane(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTL, ROWS, 0xf, false);
 }
+template <int CTL, int ROWS> __device__ __forceinline__ int from_lane(int x) {
+  return (int)from_lane<CTL, ROWS>((uint32_t)x);
+}
+template <int CTL, int ROWS> __device__ __forceinline__ double from_lane(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x);
+  const uint64_t lo = from_lane<CTL, ROWS>((uint32_t)u), hi = from_lane<CTL, ROWS>((uint32_t)(u >> 32));
+  return __longlong_as_double((long long)(hi << 32 | lo));
+}
+// the sum over the lanes up to this one: within the rows of 16 by shifts of 1, 2, 4
+// and 8, then row 0's to row 1 and 2's to 3, then that of both to the upper two
+template <class F> __device__ __forceinline__ F wave_upto(F x) {
+  x += from_lane<0x111, 0xf>(x);
+  x += from_lane<0x112, 0xf>(x);
+  x += from_lane<0x114, 0xf>(x);
+  x += from_lane<0x118, 0xf>(x);
+  x += from_lane<0x142, 0xa>(x);
+  return x + from_lane<0x143, 0xc>(x);
+}
+// the sum over the lanes below this one, given that up to it
+template <class F> __device__ __forceinline__ F wave_shifted(F upto) { return from_lane<0x138, 0xf>(upto); }
+template <class F> __device__ __forceinline__ F wave_before(F x) { return wave_shifted(wave_upto(x)); }
 
 }  // namespace syn
