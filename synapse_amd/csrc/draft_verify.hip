@@ -9,8 +9,15 @@
 // drawn from the target one by one.
 //
 // Precision: a draw's borders between tokens lie as close as a vocabulary's
-// probabilities are small, so exponentials and sums are f64 throughout: in f32
-// one in a hundred draws over 150000 tokens would fall to a neighbour.
+// probabilities are small, so exponentials and sums are f64 throughout: with
+// sums off by 2^-24 one in a hundred draws over 150000 tokens would fall to a
+// neighbour.
+//
+// Three launches: every row read once (the statistics), the decisions, and the
+// weights of one target and one draft row of a sequence summed by blocks, whose
+// last workgroup draws.  64 sequences of up to 8 drafts, 151936 tokens, 506 MB of
+// rows: 101 us (5.0 TB/s, a large copy reaches 4.7), 5.6 and 30; one of 4 drafts and
+// 32000 tokens 3.4, 3.2 and 8.1, each a chain of dependent loads.
 #include <algorithm>
 
 #include "kv_pages.hpp"
@@ -87,8 +94,8 @@ struct Exps {
   __device__ __forceinline__ Exps(float ref_, double c32_) : ref(ref_), c32(c32_), least(-32000.0 / c32_) {}
   // how far above ref a logit may be: 2^400 (finite, so that +inf is above it)
   __device__ __forceinline__ float limit() const { return fminf((float)(ref + 12800.0 / c32), 3.402823466e38f); }
-  // of d = x - ref, 2^-1000 where that is less (or x NaN)
-  __device__ __forceinline__ double at(double d, const uint64_t *tab) const {
+  // of d = x - ref, 2^-1000 where that is less (or x NaN), plus sum
+  __device__ __forceinline__ double at(double d, const uint64_t *tab, double sum = 0.0) const {
     const double kShift = 0x1.8p+52;
     d = fmax(d, least);
     double kd = __builtin_fma(d, c32, kShift);
@@ -101,10 +108,10 @@ struct Exps {
     y = __builtin_fma(y, f, 0x1.62e42fef6d01bp-6);
     y = __builtin_fma(y, f, 1.0);
     const uint64_t t = tab[k & 31u] + ((uint64_t)k << 47);
-    return y * __longlong_as_double((long long)t);
+    return __builtin_fma(y, __longlong_as_double((long long)t), sum);
   }
-  __device__ __forceinline__ double at_least(float x, const uint64_t *tab) const {
-    return at((double)x - ref, tab);
+  __device__ __forceinline__ double at_least(float x, const uint64_t *tab, double sum = 0.0) const {
+    return at((double)x - ref, tab, sum);
   }
   __device__ __forceinline__ double of(float x, const uint64_t *tab) const {
     if (ref == __builtin_huge_val()) return x == __builtin_huge_valf() ? 1.0 : 0.0;
@@ -160,7 +167,9 @@ __device__ __forceinline__ void first_top(float *top, int *at) {
 
 // grid (chunk, sequence and row): the statistics of a chunk of a row, in one pass:
 // each wave's sum is relative to the largest logit of its first block that has
-// one, until one is 2^400 above that.
+// one, until one is 2^400 above that.  Bound by its bytes, with vector instructions
+// in some 80 % of the SIMDs' cycles beside them (a tenth more of those, 101 us as
+// before).
 __global__ void __launch_bounds__(kNT) k_verify_rows(VerifyArgs a) {
   __shared__ uint64_t tab[32];
   __shared__ Stat part[4];
@@ -201,7 +210,7 @@ __global__ void __launch_bounds__(kNT) k_verify_rows(VerifyArgs a) {
       }
       if (mine.ref == kNone || above) return;
 #pragma unroll
-      for (int i = 0; i < 8; i++) sum += e.at_least(v[i], tab);
+      for (int i = 0; i < 8; i++) sum = e.at_least(v[i], tab, sum);
     });
     if (__any(above)) {
       sum = 0.0;
@@ -239,7 +248,8 @@ template <class F, class Op> __device__ __forceinline__ F over_16(F x, Op op) {
 constexpr int kDecideNT = 512;
 
 // One workgroup a sequence: 16 lanes join the chunks of a row, all rows at once,
-// and a lane a draft says whether it is accepted.
+// and a lane a draft says whether it is accepted.  (Done again by every workgroup
+// that sums weights instead, 64 sequences of 8 drafts took 179 us and not 141.)
 __global__ void __launch_bounds__(kDecideNT) k_verify_decide(VerifyArgs a) {
   __shared__ uint64_t tab[32];
   __shared__ Stat row[2 * kMaxDraft + 1];    // target rows, then draft rows
@@ -426,8 +436,9 @@ __device__ __forceinline__ int pick(const Weights &w, int first, int left, doubl
   return first + (found < left ? found : last);
 }
 
-// grid (some blocks, sequence): the sums of the weights by blocks; the last workgroup of
-// a sequence to have its sum draws.
+// grid (some blocks, sequence): the sums of the weights by blocks; the last
+// workgroup of a sequence to have its sums draws.  As many blocks a workgroup as
+// leave 1024 of them (64 sequences of 151936 tokens: one block each 50 us, four 30).
 __global__ void __launch_bounds__(kNT) k_verify_draw(VerifyArgs a) {
   __shared__ uint64_t tab[32];
   __shared__ double wsum[kDraws][4];
@@ -454,7 +465,7 @@ __global__ void __launch_bounds__(kNT) k_verify_draw(VerifyArgs a) {
   if (tid < 64) {
     // As in split_k.hpp: an exchange that has returned is at the point where every
     // XCD's atomics are, so relaxed ones suffice (an acquire and a release each
-    // write back and drop an L2: 142 us where this kernel took 53).
+    // write back and drop an L2: 142 us where this kernel then took 53).
     const int b = blockIdx.x * a.draws + tid;
     if (tid < a.draws && b < a.blocks) {
       const double x = (wsum[tid][0] + wsum[tid][1]) + (wsum[tid][2] + wsum[tid][3]);
@@ -530,7 +541,8 @@ struct Space {
 Space space_of(const syn_hip_draft_verify_params &p) {
   Space s;
   s.rows = 2 * (int)p.max_draft + 1;
-  // chunks of 2048 to 16384 tokens, as long as there are workgroups for the chip
+  // Chunks of 2048 tokens, of up to 16384 as long as 2048 workgroups, all that the
+  // chip holds at eight a CU, are left: a row's chunks are joined one by one.
   s.per = kBlock;
   while (s.per < 8 * kBlock && p.n_seqs * (size_t)s.rows * cdiv(p.vocab, 2 * s.per) >= 2048) s.per *= 2;
   s.chunks = (int)cdiv(p.vocab, s.per);

@@ -5,6 +5,12 @@
 // count 0 is free, so there is no list of free pages to keep in order: whoever
 // needs pages gets the free ones of lowest number, the rows in order and the
 // columns of a row in order, whatever order the workgroups run in.
+//
+// Pages that are copied are bound by their bytes: all of a pool of 768 live pages
+// of 28 layers to another, 7 GB read and written, 1367 us, 5.2 TB/s (a large copy
+// reaches 4.7); the last pages of 96 rows that continue 32 others 111 us, 4.2 TB/s
+// of what HBM has to read (a parent's page once) and write.  The tables are a few
+// dependent loads: 16 rows 4 us, 1024 rows over 262144 pages 3 + 2.5 + 7.5.
 #include <algorithm>
 
 #include "kv_pages.hpp"
@@ -229,7 +235,10 @@ __global__ void __launch_bounds__(kPoolNT) k_take(TableArgs a) {
 }
 
 // ---- the whole of it by one workgroup, where little is to be done: a launch and
-// five steps with a barrier between, their entries dealt to all threads.
+// five steps with a barrier between, their entries dealt to all threads.  (Two calls
+// for 16 rows of 44 entries: 8.1 us, by the launches above 20.  128 rows of 24
+// entries that all change: 16 us in the kernel, 14.5 in the three.)  The bound on
+// entries is for calls that change all of them; most change few.
 constexpr int kSmallNT = 1024;
 constexpr int kSmallRows = 1024, kSmallEntries = 16384;
 constexpr uint32_t kSmallPages = 65536;

@@ -5,7 +5,18 @@
 // is softmax(scale q k_i) over i from len - n + j back, as far as the window
 // reaches.  The rows of a kv head, all tokens' query heads that read it, are the
 // columns of the two products of attend_rows.hpp, 16, 32 or 64 to a workgroup: a
-// key or value that several tokens see is read for all of them at once.
+// key or value that several tokens see is read for all of them at once.  A row's
+// own limits only mask its scores, in the tiles that some row of the wave does not
+// see whole; positions that no row of the workgroup sees are not read.
+//
+// What bounds it (a large copy reaches 4.7 TB/s here, large products 1100 TFLOP/s
+// in f16): up to 32 rows of a kv head, bytes: 64 sequences of one token at up to
+// 12000 positions, 32 heads of 64, bf16, 211 us, 5.6 TB/s; 24 of up to 8 tokens at
+// 8200, 32 heads of 128, f16, 131 to 143 us, 4.7 to 4.3 TB/s.  Chunks, their steps
+// of a tile: two of 1536 tokens at 12001, 24 heads of 128, f16, 815 us, 450 TFLOP/s
+// of the formula and 900 in matrix instructions with the operands' second parts,
+// which keep 35 % of the SIMDs' cycles, the vector ones 43 %.  Four sequences of
+// five tokens at 213, f32: 10.4 us, one launch and dependent loads.
 #include <algorithm>
 #include <cmath>
 
@@ -224,7 +235,7 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_paged_attention_params 
     const double step = pg.dtype == SYN_HIP_KV_F32 ? 3.5e-6 : 0.9e-6;
     double least = 0;
     size_t best = 1;
-    for (size_t parts = 1; parts <= 64; parts++) {
+    for (size_t parts = 1; parts <= 8 || parts * all <= 4 * want; parts += 1 + parts / 16) {
       cut(parts);
       const size_t wgs = all * w.parts, rest = wgs % want;
       const double rounds = (double)(wgs / want) + (rest == 0 ? 0.0 : (rest <= want / 2 ? 0.8 : 1.0));

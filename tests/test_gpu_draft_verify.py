@@ -269,6 +269,15 @@ def test_ties_go_to_the_lowest_token():
     assert emitted.tolist() == [2, 1, 2] and (token[:, 0] == 0).all() and token[0, 1] == 0
 
 
+@pytest.mark.parametrize("seqs,drafts", [(1, 0), (2, 3)])
+def test_many_blocks(seqs, drafts):
+    """a vocabulary of 342 blocks: more chunks and sums than a wave has lanes"""
+    c = Case(36, seqs, drafts, 700001)
+    c.call()
+    R.sync()
+    c.check()
+
+
 def test_captured_and_replayed():
     a, b = Case(33, 6, 4, 9001), Case(34, 3, 2, 500)
     graphs = []

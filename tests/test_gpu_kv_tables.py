@@ -53,7 +53,7 @@ class Device:
 SHAPES = [  # page, pages, rows, columns
     (16, 2048, 16, 48), (8, 5, 3, 4), (16, 1, 1, 1), (64, 300, 7, 33), (16, 9000, 130, 65),
     (1024, 100, 9, 8), (16, 70000, 1030, 61), (8, 4096, 300, 13), (8, 4097, 2, 2000), (32, 250000, 40, 300),
-    (8, 40, 4000, 2)]
+    (8, 40, 4000, 2), (16, 30000, 8000, 3)]
 
 
 @pytest.mark.parametrize("page,pages,rows,cols", SHAPES)
@@ -74,6 +74,23 @@ def test_resize(page, pages, rows, cols):
         R.sync()
         ref.resize(lens)
         dev.check()
+
+
+def test_counts_of_any_alignment():
+    """counts that begin 4 bytes behind a 16-byte boundary"""
+    rng = np.random.default_rng(5)
+    for rows, cols, pages in ((9, 20, 210), (40, 500, 21001)):
+        ref = D.Tables(16, pages, rows, cols)
+        dev = Device(ref)
+        buf = R.dev(np.zeros(pages + 1, np.int32))
+        dev.desc.refs = buf.ptr + 4
+        for _ in range(3):
+            lens = R.i32(rng.integers(0, cols * 16, rows))
+            dev.resize(R.dev(lens))
+            R.sync()
+            ref.resize(lens)
+            assert (buf.download((pages + 1,), np.int32)[1:] == ref.refs).all()
+            assert (dev.b["table"].download(ref.table.shape, np.int32) == ref.table).all()
 
 
 def fill(ref, rng, most):
@@ -203,6 +220,66 @@ def test_compact(dtype, page, pages, layers, kv, hd, rows, cols, to_pages, to_co
     for a, b in moves:
         other.k[:, b], other.v[:, b] = pool.k[:, a], pool.v[:, a]
     same(other, [])
+
+
+def test_pools_past_32_bits():
+    """pages whose bytes lie more than 2^32 behind the pool's, copied from and into"""
+    layers, kv, hd, page, pages = 2, 8, 128, 64, 20500  # 128 KiB a page, 5.2 GiB a pool
+    each = kv * hd * page * 2
+    k, v, to_k, to_v = (hip.DeviceBuffer(n * each) for n in (layers * pages,) * 2 + (layers * 3,) * 2)
+    pool = hip.KvPages(hip.KV_F16, page, pages, layers, kv, hd, k.ptr, v.ptr)
+    rng = np.random.default_rng(3)
+    ref, to = D.Tables(page, pages, 2, 4), D.Tables(page, 3, 2, 4)
+    ref.table[0, :2], ref.held[0] = [pages - 1, pages - 3], 2
+    ref.refs[:] = 1  # (all the caller's own, but for the last but one)
+    ref.refs[pages - 2] = 0
+    dev = Device(ref)
+
+    def at(buf, layer, p):
+        return buf.ptr + (layer * pages + p) * each
+
+    data = {}
+    for buf in (k, v):
+        for layer in range(layers):
+            for p in (pages - 1, pages - 2, pages - 3):
+                x = rng.integers(0, 256, each, dtype=np.uint8)
+                data[buf.ptr, layer, p] = x
+                hip.check(hip.lib().syn_hip_memcpy_h2d(at(buf, layer, p), hip.ptr(x), each))
+
+    def read(address):
+        x = np.empty(each, np.uint8)
+        hip.check(hip.lib().syn_hip_memcpy_d2h(hip.ptr(x), address, each))
+        return x
+
+    parent, lens = R.i32([0, 0]), R.i32([0, page + 24])
+    d_parent, d_lens = R.dev(parent), R.dev(lens)
+    hip.check(hip.lib().syn_hip_kv_fork(C.byref(pool), C.byref(dev.desc), d_parent.ptr, d_lens.ptr,
+                                        dev.ws.ptr, dev.need, None))
+    R.sync()
+    assert ref.fork(parent, lens) == [(pages - 3, pages - 2, 24)]
+    dev.check()
+    for layer in range(layers):
+        for buf, shape, take in ((k, (kv, hd // 8, page, 16), np.s_[:, :, :24]),
+                                 (v, (kv, page // 8, hd, 16), np.s_[:, :3])):
+            want = data[buf.ptr, layer, pages - 2].reshape(shape).copy()
+            want[take] = data[buf.ptr, layer, pages - 3].reshape(shape)[take]
+            assert (read(at(buf, layer, pages - 2)) == want.reshape(-1)).all()
+            data[buf.ptr, layer, pages - 2] = want.reshape(-1)
+    # the last three pages alone are live
+    ref.refs[:pages - 3] = 0
+    dev.upload()
+    into, live = Device(to), R.dev(np.zeros(1, np.int32))
+    other = hip.KvPages(hip.KV_F16, page, 3, layers, kv, hd, to_k.ptr, to_v.ptr)
+    hip.check(hip.lib().syn_hip_kv_compact(C.byref(pool), C.byref(dev.desc), C.byref(other), C.byref(into.desc),
+                                           live.ptr, dev.ws.ptr, dev.need, None))
+    R.sync()
+    assert ref.compact(to)[0] == 3 == live.download((1,), np.int32)[0]
+    into.check()
+    for layer in range(layers):
+        for i in range(3):
+            for a, b in ((k, to_k), (v, to_v)):
+                got = read(b.ptr + (layer * 3 + i) * each)
+                assert (got == data[a.ptr, layer, pages - 3 + i]).all()
 
 
 def test_captured_and_replayed():

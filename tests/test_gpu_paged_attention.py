@@ -191,6 +191,15 @@ def test_rows_that_see_nothing(dtype, max_len):
     assert np.abs(got[2:5, :8 * 64]).min(1).max() > 0
 
 
+def test_no_position_at_all():
+    c = Case(14, "f16", 8, 2, 64, 4, [3, 1], [0, 0])
+    assert c.max_len == 0
+    c.call()
+    R.sync()
+    c.check()
+    assert (c.got()[:4, :256] == 0).all()
+
+
 def test_starts_outside_the_rows():
     """offsets below 0, above n_tokens or falling are cut, and their rows stay"""
     c = Case(5, "f16", 16, 1, 64, 2, [4, 3, 5], [20, 30, 40])
