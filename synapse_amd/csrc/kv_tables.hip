@@ -6,7 +6,7 @@
 // needs pages gets the free ones of lowest number, the rows in order and the
 // columns of a row in order, whatever order the workgroups run in.
 //
-// Pages that are copied are bound by their bytes: all of a pool of 768 live pages
+// Pages that are copied are bound by their bytes: all of a pool of 480 live pages
 // of 28 layers to another, 7 GB read and written, 1367 us, 5.2 TB/s (a large copy
 // reaches 4.7); the last pages of 96 rows that continue 32 others 111 us, 4.2 TB/s
 // of what HBM has to read (a parent's page once) and write.  The tables are a few
