@@ -160,8 +160,8 @@ struct HeadBase {
 
 // One wave's part of the work: 16 query rows of a kv head.  FULL: hd is 32 NC.
 // CAUSAL: a row sees positions of its own, lo to lim (see()), of those that the
-// run has.
-template <class T, int NC, bool FULL, bool CAUSAL = false> struct Rows {
+// run has.  RING: tiles that the ring in LDS holds, if not as many as below.
+template <class T, int NC, bool FULL, bool CAUSAL = false, int RING = 0> struct Rows {
   using F = Frag<T>;
   using V = typename F::V;
   static constexpr int DT = 2 * NC;           // tiles of 16 dims (hd <= 32 NC)
@@ -169,7 +169,9 @@ template <class T, int NC, bool FULL, bool CAUSAL = false> struct Rows {
   static constexpr int kLoads = kFrags * (int)sizeof(V) / 16;  // 1 KiB direct loads of a tile
   static constexpr int kTileBytes = kLoads * 1024;
   // tiles that the ring in LDS holds: 32 to 64 KiB, 128 where a tile has 64
-  static constexpr int kRing = kTileBytes <= 16384 ? 4 : 2;
+  static constexpr int kRing = RING ? RING : (kTileBytes <= 16384 ? 4 : 2);
+  // V asked for when the scores are formed, where registers are short
+  static constexpr bool kLate = sizeof(V) != 16 || (RING == 3 && F::kParts == 3);
   static constexpr int kLd = 32 * NC + 4;     // f32 rows on different banks
   static constexpr int kJoinBytes = kWaves * 16 * kLd * 4;
   static constexpr int kLdsBytes = kRing * kTileBytes > kJoinBytes ? kRing * kTileBytes : kJoinBytes;
@@ -583,7 +585,7 @@ template <class T, int NC, bool FULL, bool CAUSAL = false> struct Rows {
         for (int j = 0; j < 2 * NC; j++) kf[j] = frag(j);
         // all of the tile is asked for before the first product waits (V of an
         // f32 pool after it: two workgroups a CU need the registers)
-        if constexpr (sizeof(V) == 16)
+        if constexpr (!kLate)
 #pragma unroll
           for (int j = 0; j < DT; j++) vf[j] = frag(2 * NC + j);
         __builtin_amdgcn_sched_barrier(0);
@@ -598,7 +600,7 @@ template <class T, int NC, bool FULL, bool CAUSAL = false> struct Rows {
       if (on) {
         f32x4 s[2];
         scores(kf, s);
-        if constexpr (sizeof(V) != 16)
+        if constexpr (kLate)
 #pragma unroll
           for (int j = 0; j < DT; j++) vf[j] = frag(2 * NC + j);
         weigh(s, vf, kt, r.to, here);

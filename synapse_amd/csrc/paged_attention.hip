@@ -31,7 +31,6 @@ struct PagedArgs : RowArgs {
   size_t ld_table;
   int n_seqs, n_tokens, max_new, max_len, window;
   int chunk;   // positions of a part (a multiple of kTile)
-  int rw;      // tiles of 16 rows of a workgroup: 1, 2 or 4
   int blocks;  // workgroups for the rows of the longest sequence
   bool solo;   // a wave for a sequence's rows
 };
@@ -49,9 +48,15 @@ __device__ __forceinline__ int count_of(const PagedArgs &a, int s, int first) {
   return min(end - first, a.max_new);
 }
 
-template <class T, int NC, bool FULL>
-__global__ void __launch_bounds__(64 * kWaves, (kResident<T, NC, FULL>)) k_attend_new(PagedArgs a, KvPool<T> pool) {
-  using W = Rows<T, NC, FULL, true>;
+// 64 rows of 128 dims in 16 bits: a ring of three tiles and 168 registers leave
+// room for three workgroups a CU.
+template <class T, int NC, int RW> constexpr bool kThree = RW == 4 && NC == 4 && sizeof(T) == 2;
+
+// RW: tiles of 16 rows of a workgroup
+template <class T, int NC, bool FULL, int RW>
+__global__ void __launch_bounds__(64 * kWaves, (kThree<T, NC, RW> ? 3 : kResident<T, NC, FULL>))
+    k_attend_new(PagedArgs a, KvPool<T> pool) {
+  using W = Rows<T, NC, FULL, true, kThree<T, NC, RW> ? 3 : 0>;
   __shared__ __align__(16) uint8_t lds[W::kLdsBytes];
   __shared__ float ml[kWaves * 16 * 2];
   // workgroup i runs on XCD i % 8: the blocks of rows that read the same
@@ -65,7 +70,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, NC, FULL>)) k_atten
   const int part = u % a.parts, s = u / a.parts;
   if (s >= a.n_seqs) return;
   const int first = first_of(a, s), count = count_of(a, s, first), all = count * a.rep;
-  const int RW = a.rw, row0 = block * RW * 16, rows = min(RW * 16, all - row0);
+  const int row0 = block * RW * 16, rows = min(RW * 16, all - row0);
   if (rows <= 0) return;
   const int len = min(max(scalar(a.len, s), 0), a.max_len);
   // token j sees the positions below lim_of(j), from lo_of(j) on
@@ -96,13 +101,9 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, NC, FULL>)) k_atten
                     (uint32_t)(pool.nkv * head_bytes)};
   const bool wide = pool.ps >= kTile;
   uint32_t ok = 0;
-  if (RW == 4)
-    ok = wide ? W::template start_shared<true, 1>(pool, hb, r, lds)
-              : W::template start_shared<false, 1>(pool, hb, r, lds);
-  if constexpr (W::kRing == 4)
-    if (RW == 2)
-      ok = wide ? W::template start_shared<true, 2>(pool, hb, r, lds)
-                : W::template start_shared<false, 2>(pool, hb, r, lds);
+  if constexpr (RW > 1)
+    ok = wide ? W::template start_shared<true, 4 / RW>(pool, hb, r, lds)
+              : W::template start_shared<false, 4 / RW>(pool, hb, r, lds);
   W w;
   const int mine = row0 + (wave & (RW - 1)) * 16;
   w.load_queries(a, pool.hd, first, head, mine, last);
@@ -110,7 +111,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, NC, FULL>)) k_atten
     const int token = min(mine + (int)(threadIdx.x & 15), last) / a.rep;
     w.see(lo_of(token), lim_of(token), lo_of(min(mine + 15, last) / a.rep), lim_of(min(mine, last) / a.rep));
   }
-  if (RW == 1) {
+  if constexpr (RW == 1) {
     if (wide)
       w.template run_alone<true>(pool, hb, r, a.solo ? 1 : kWaves);
     else
@@ -119,16 +120,10 @@ __global__ void __launch_bounds__(64 * kWaves, (kResident<T, NC, FULL>)) k_atten
       w.finish_alone(a, pool.hd, first, head, row0, rows, at);
       return;
     }
-  } else if (RW == 4) {
-    if (wide)
-      w.template run_shared<true, 1>(pool, hb, r, lds, ok);
-    else
-      w.template run_shared<false, 1>(pool, hb, r, lds, ok);
-  } else if constexpr (W::kRing == 4) {
-    if (wide)
-      w.template run_shared<true, 2>(pool, hb, r, lds, ok);
-    else
-      w.template run_shared<false, 2>(pool, hb, r, lds, ok);
+  } else if (wide) {
+    w.template run_shared<true, 4 / RW>(pool, hb, r, lds, ok);
+  } else {
+    w.template run_shared<false, 4 / RW>(pool, hb, r, lds, ok);
   }
   w.finish(a, pool.hd, first, head, row0, rows, RW, at, reinterpret_cast<float *>(lds), ml);
 }
@@ -205,7 +200,9 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_paged_attention_params 
   const size_t tokens = std::min<size_t>(p.max_new, 16 * w.rw / rep + 2);
   const size_t span = p.window ? std::min<size_t>(p.max_len, (size_t)p.window + tokens + kTile) : p.max_len;
   const size_t tiles = cdiv(span, kTile), units = (size_t)p.n_seqs * nkv;
-  const size_t want = w.nc == 8 ? 256 : (w.nc == 4 || pg.dtype == SYN_HIP_KV_F32 ? 512 : 1024);
+  // workgroups that the chip holds at once
+  const bool f32 = pg.dtype == SYN_HIP_KV_F32;
+  const size_t want = w.nc == 8 ? 256 : (w.nc == 2 && !f32 ? 1024 : (w.rw == 4 && !f32 ? 768 : 512));
   const size_t whole = pg.dtype == SYN_HIP_KV_F32 ? 2 : (units <= 512 ? 8 : 4);
   constexpr size_t kFix = 6;
   auto alone = [&](size_t units, size_t tiles) {
@@ -285,13 +282,22 @@ syn_status_t check(const syn_hip_kv_pages *pages, const syn_hip_paged_attention_
   return SYN_OK;
 }
 
-template <class T, int NC>
-syn_status_t launch(const Plan &w, const PagedArgs &a, const KvPool<T> &pool, hipStream_t s) {
+template <class T, int NC, int RW>
+void launch_rows(const Plan &w, const PagedArgs &a, const KvPool<T> &pool, hipStream_t s) {
   const dim3 grid((unsigned)w.wgs), block(64 * kWaves);
   if (pool.hd == 32 * NC)
-    hipLaunchKernelGGL((k_attend_new<T, NC, true>), grid, block, 0, s, a, pool);
+    hipLaunchKernelGGL((k_attend_new<T, NC, true, RW>), grid, block, 0, s, a, pool);
   else
-    hipLaunchKernelGGL((k_attend_new<T, NC, false>), grid, block, 0, s, a, pool);
+    hipLaunchKernelGGL((k_attend_new<T, NC, false, RW>), grid, block, 0, s, a, pool);
+}
+template <class T, int NC>
+syn_status_t launch(const Plan &w, const PagedArgs &a, const KvPool<T> &pool, hipStream_t s) {
+  if (w.rw == 1)
+    launch_rows<T, NC, 1>(w, a, pool, s);
+  else if (w.rw == 4)
+    launch_rows<T, NC, 4>(w, a, pool, s);
+  else if constexpr (Rows<T, NC, true, true>::kRing == 4)
+    launch_rows<T, NC, 2>(w, a, pool, s);
   SYN_LAUNCH_CHECK();
   if (w.parts == 1) return SYN_OK;
   if (w.parts <= kFewParts)
@@ -363,7 +369,6 @@ extern "C" syn_status_t syn_hip_paged_attention(const syn_hip_kv_pages *pages,
   a.max_len = (int)p->max_len;
   a.window = p->window < p->max_len ? (int)p->window : 0;
   a.chunk = w.chunk;
-  a.rw = w.rw;
   a.blocks = w.blocks;
   a.solo = w.solo;
   hipStream_t s = pick_stream(stream);
