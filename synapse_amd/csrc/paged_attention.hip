@@ -13,10 +13,11 @@
 // in f16): up to 32 rows of a kv head, bytes: 64 sequences of one token at up to
 // 12000 positions, 32 heads of 64, bf16, 211 us, 5.6 TB/s; 24 of up to 8 tokens at
 // 8200, 32 heads of 128, f16, 131 to 143 us, 4.7 to 4.3 TB/s.  Chunks, their steps
-// of a tile: two of 1536 tokens at 12001, 24 heads of 128, f16, 815 us, 450 TFLOP/s
-// of the formula and 900 in matrix instructions with the operands' second parts,
-// which keep 35 % of the SIMDs' cycles, the vector ones 43 %.  Four sequences of
-// five tokens at 213, f32: 10.4 us, one launch and dependent loads.
+// of a tile: two of 1536 tokens at 12001, 24 heads of 128, f16, 661 to 734 us, 500
+// to 555 TFLOP/s of the formula and twice that in matrix instructions with the
+// operands' second parts, which take 51 % of the SIMDs' cycles, the vector ones 60 %
+// (with two workgroups a CU 815 to 893 us, 41 and 48 %).  Four sequences of
+// five tokens at 213, f32: 10.1 us, one launch and dependent loads.
 #include <algorithm>
 #include <cmath>
 
@@ -49,7 +50,9 @@ __device__ __forceinline__ int count_of(const PagedArgs &a, int s, int first) {
 }
 
 // 64 rows of 128 dims in 16 bits: a ring of three tiles and 168 registers leave
-// room for three workgroups a CU.
+// room for three workgroups a CU (30 chunks of 100 tokens at 1000, 32 heads of 128,
+// f16, 92 us, 107 with two; two of 1200 at 9000, bf16, 752 and 789).  Four in f16
+// would have to spill.
 template <class T, int NC, int RW> constexpr bool kThree = RW == 4 && NC == 4 && sizeof(T) == 2;
 
 // RW: tiles of 16 rows of a workgroup
@@ -225,10 +228,10 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_paged_attention_params 
     // one with the fewest, counted in rounds of workgroups (half a round of them,
     // one a CU, takes 0.8 of one), a fixed time each, and the join, which reads and
     // writes every part (4.5 TB/s; a step takes 0.9 us, of an f32 pool 3.5).  One
-    // chunk of 1536 tokens at 12001, 24 heads of 128, f16: 576 workgroups 693 us,
-    // four parts 506; two such sequences 976 whole, 883 in two parts; 512 tokens at
-    // 8000, f32, 602 whole, 435 in five; 16 tokens of four sequences at 8200 175 and
-    // 43.
+    // chunk of 1536 tokens at 12001, 24 heads of 128, f16: whole 526 us, in four parts
+    // 449; two such sequences 844, in two 790; 200 tokens at 20000, 32 heads, 564, 222
+    // in three, 151 as chosen; 512 tokens at 8000, f32, 602, in five 435; 16 tokens of
+    // four sequences at 8200, bf16, 176, in five 51, 40 as chosen.
     const double step = pg.dtype == SYN_HIP_KV_F32 ? 3.5e-6 : 0.9e-6;
     double least = 0;
     size_t best = 1;
@@ -264,7 +267,7 @@ syn_status_t check(const syn_hip_kv_pages *pages, const syn_hip_paged_attention_
   }
   // (kernels look two rounds of tiles past a length, and count rows, in 32 bits)
   if (p->n_seqs > 65535u || p->max_len > 0x7fff0000u || p->n_tokens > 0x7fffffffu ||
-      p->max_new > p->n_tokens || (uint64_t)p->max_new * p->n_heads > 0x3fffffffu) {
+      (p->n_tokens && p->max_new > p->n_tokens) || (uint64_t)p->max_new * p->n_heads > 0x3fffffffu) {
     set_error("paged_attention: more than 65535 sequences, 2^31 - 2^16 positions or 2^30 - 1 query rows of "
               "a sequence, or max_new above n_tokens");
     return SYN_ERR_INVALID_ARG;
@@ -273,7 +276,7 @@ syn_status_t check(const syn_hip_kv_pages *pages, const syn_hip_paged_attention_
     set_error("paged_attention: rows or page tables shorter than the heads or the lengths");
     return SYN_ERR_SHAPE_MISMATCH;
   }
-  if (!p->n_seqs || !p->max_new) return SYN_OK;
+  if (!p->n_seqs || !p->max_new || !p->n_tokens) return SYN_OK;
   const Plan w = make_plan(*pages, *p);
   if (w.wgs > kMaxThreads / (64 * kWaves) || (w.parts > 1 && w.rows > kMaxThreads / 256)) {
     set_error("paged_attention: more workgroups than a launch takes");
@@ -321,7 +324,7 @@ extern "C" syn_status_t syn_hip_paged_attention_workspace(const syn_hip_kv_pages
   if (!bytes) return SYN_ERR_NULL_PTR;
   SYN_TRY(check(pages, p));
   *bytes = 0;
-  if (!p->n_seqs || !p->max_new) return SYN_OK;
+  if (!p->n_seqs || !p->max_new || !p->n_tokens) return SYN_OK;
   const Plan w = make_plan(*pages, *p);
   *bytes = w.po_bytes + w.pml_bytes;
   return SYN_OK;
@@ -337,7 +340,7 @@ extern "C" syn_status_t syn_hip_paged_attention(const syn_hip_kv_pages *pages,
     set_error("paged_attention: without d_start every sequence has max_new tokens");
     return SYN_ERR_SHAPE_MISMATCH;
   }
-  if (!p->n_seqs || !p->max_new) return SYN_OK;
+  if (!p->n_seqs || !p->max_new || !p->n_tokens) return SYN_OK;
   if (!d_q || !d_out || !d_len || (p->max_len && !d_table)) return SYN_ERR_NULL_PTR;
   const Plan w = make_plan(*pages, *p);
   const size_t need = w.po_bytes + w.pml_bytes;

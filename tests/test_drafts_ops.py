@@ -46,8 +46,8 @@ def test_attention_refuses(kw, want):
 @pytest.mark.parametrize("kw,want", [
     (dict(ptrs=dict(q=None)), NULL), (dict(ptrs=dict(len=None)), NULL), (dict(ptrs=dict(t=None)), NULL),
     (dict(ptrs=dict(out=None)), NULL), (dict(ptrs=dict(start=None)), SHAPE),
-    (dict(n_seqs=0), OK), (dict(max_new=0), OK),
-    (dict(n_seqs=0, ptrs=dict(q=None, out=None)), OK)])
+    (dict(n_seqs=0), OK), (dict(max_new=0), OK), (dict(n_tokens=0), OK),
+    (dict(n_seqs=0, ptrs=dict(q=None, out=None)), OK), (dict(n_tokens=0, ptrs=dict(q=None)), OK)])
 def test_attention_refuses_calls(kw, want):
     assert attention(**kw)[1] == want
 
