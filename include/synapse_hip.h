@@ -813,7 +813,8 @@ syn_status_t syn_hip_klm_generate_beams(syn_hip_klm_t *m, const uint32_t *prompt
  * that sees none gives zeros.  d_q and d_out [n_tokens][n_heads][head_dim],
  * rows ldq and ldo apart; rows of no sequence are left as they are.  Heads,
  * scale, pages outside the pool, values behind a length, precision: as
- * syn_hip_prefix_attention.  max_new, max_len and n_tokens decide the split of
+ * syn_hip_prefix_attention (all keys and values within a length are finite, for
+ * the rows that do not see them too).  max_new, max_len and n_tokens decide the split of
  * the work, so a captured call keeps them.  d_out is apart from d_q.  At most
  * 65535 sequences, max_len 2^31 - 2^16, max_new * n_heads below 2^30.  The
  * workspace (which may be 0; 16-byte aligned) holds the parts of split runs. */
@@ -887,7 +888,9 @@ syn_status_t syn_hip_kv_tables_workspace(const syn_hip_kv_tables *t, size_t *byt
 /* Every row holds the pages of d_len[s] positions (as many as the row has room
  * for; a negative length: the row stays as it is): those above are given back,
  * then missing ones are taken.  So a sequence grows, is cut back to what was
- * accepted, or ends (0). */
+ * accepted, or ends (0).  A page that several rows name is not to be written: a
+ * row cut back into the middle of one goes on in another row that continues it
+ * (syn_hip_kv_fork copies the part that it holds). */
 syn_status_t syn_hip_kv_resize(const syn_hip_kv_tables *t, const int32_t *d_len, void *d_workspace,
                                size_t workspace_bytes, void *stream);
 /* Row s continues row d_parent[s]: it gives back its pages, then holds those of
