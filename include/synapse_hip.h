@@ -813,11 +813,12 @@ syn_status_t syn_hip_klm_generate_beams(syn_hip_klm_t *m, const uint32_t *prompt
  * that sees none gives zeros.  d_q and d_out [n_tokens][n_heads][head_dim],
  * rows ldq and ldo apart; rows of no sequence are left as they are.  Heads,
  * scale, pages outside the pool, values behind a length, precision: as
- * syn_hip_prefix_attention (all keys and values within a length are finite, for
- * the rows that do not see them too).  max_new, max_len and n_tokens decide the split of
- * the work, so a captured call keeps them.  d_out is apart from d_q.  At most
- * 65535 sequences, max_len 2^31 - 2^16, max_new * n_heads below 2^30.  The
- * workspace (which may be 0; 16-byte aligned) holds the parts of split runs. */
+ * syn_hip_prefix_attention (a row that sees a key or value that is not finite may
+ * be NaN in every dim; one that does not see it stays what it is).  max_new,
+ * max_len and n_tokens decide the split of the work, so a captured call keeps
+ * them.  d_out is apart from d_q.  At most 65535 sequences, max_len 2^31 - 2^16,
+ * max_new * n_heads below 2^30.  The workspace (which may be 0; 16-byte aligned)
+ * holds the parts of split runs. */
 typedef struct {
   uint32_t layer, n_heads, n_seqs, n_tokens, max_new, max_len, window;
   float scale;

@@ -319,6 +319,35 @@ template <class T, int NC, bool FULL, bool CAUSAL = false, int RING = 0> struct 
     return below & (down <= 0 ? 0xff : (down >= 8 ? 0 : 0xffu << down));
   }
 
+  // those of the positions 8g .. 8g+7 at which some dim of V is not finite, a bit each
+  static __device__ __forceinline__ uint32_t odd(const V *v) {
+    constexpr int kWords = (int)sizeof(V) / 4, kEach = kWords == 4 ? 2 : 1;
+    // elements without their signs, the largest of all dims (above another in a word)
+    uint32_t hi[kWords] = {}, lo[kWords] = {};
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+      uint32_t w[kWords];
+      __builtin_memcpy(w, &v[d], sizeof(V));
+#pragma unroll
+      for (int k = 0; k < kWords; k++) {
+        hi[k] = max(hi[k], w[k] & 0x7fffffffu);
+        if (kEach == 2) lo[k] = max(lo[k], w[k] << 16 & 0x7fffffffu);
+      }
+    }
+    constexpr uint32_t kInf = F::kParts == 2 ? 0x7c000000u : 0x7f800000u;
+    uint32_t on = 0;
+#pragma unroll
+    for (int k = 0; k < kWords; k++)
+      on |= (hi[k] >= kInf ? 1u << (kEach * k + kEach - 1) : 0u) | (kEach == 2 && lo[k] >= kInf ? 1u << 2 * k : 0u);
+    // over the 16 lanes of the group, each of which has other dims
+    auto with = [&](int x) { on |= (uint32_t)x; };
+    with(__builtin_amdgcn_update_dpp(0, (int)on, 0xb1, 0xf, 0xf, false));
+    with(__builtin_amdgcn_update_dpp(0, (int)on, 0x4e, 0xf, 0xf, false));
+    with(__builtin_amdgcn_update_dpp(0, (int)on, 0x141, 0xf, 0xf, false));
+    with(__builtin_amdgcn_update_dpp(0, (int)on, 0x140, 0xf, 0xf, false));
+    return on;
+  }
+
   // ---- the two products of a tile
   __device__ __forceinline__ void scores(const V *k, f32x4 *s) const {
     s[0] = s[1] = f32x4{0, 0, 0, 0};
@@ -338,11 +367,23 @@ template <class T, int NC, bool FULL, bool CAUSAL = false, int RING = 0> struct 
     for (int j = 0; j < 4; j++) x[j] = s[0][j], x[j + 4] = s[1][j];
     const bool cut = k0 + kTile > to || ok != 15;
     if (cut || (CAUSAL && (k0 + kTile > all_to || k0 < all_from))) {
-      const uint32_t there = which(k0, to, ok), mine = CAUSAL ? there & seen(k0) : there;
+      uint32_t there = which(k0, to, ok);
+      const uint32_t mine = CAUSAL ? there & seen(k0) : there;
+      bool clear = !CAUSAL || cut;
+      if constexpr (CAUSAL) {
+        // A value that is not finite is none of the rows' that do not see it; those
+        // that do are NaN.
+        const uint32_t none = odd(v) & there;
+        if (__any(none)) {
+          if (none & mine) l = __builtin_nanf("");
+          there &= ~none;
+          clear = true;
+        }
+      }
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         x[j] = mine >> j & 1 ? x[j] : kNegInf;
-        if (CAUSAL && !cut) continue;
+        if (!clear) continue;
 #pragma unroll
         for (int d = 0; d < DT; d++)  // what is not there may hold anything: 0 times NaN is NaN
           if (!(there >> j & 1)) F::clear(v[d], j);

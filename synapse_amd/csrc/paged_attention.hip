@@ -7,7 +7,10 @@
 // columns of the two products of attend_rows.hpp, 16, 32 or 64 to a workgroup: a
 // key or value that several tokens see is read for all of them at once.  A row's
 // own limits only mask its scores, in the tiles that some row of the wave does not
-// see whole; positions that no row of the workgroup sees are not read.
+// see whole; positions that no row of the workgroup sees are not read.  The second
+// product multiplies values by weights of 0 there, so in those tiles values that are
+// not finite are taken out of it, and the rows that do see them made NaN (no more
+// than 1.5 % of a call; most measure no difference).
 //
 // What bounds it (a large copy reaches 4.7 TB/s here, large products 1100 TFLOP/s
 // in f16): up to 32 rows of a kv head, bytes: 64 sequences of one token at up to
@@ -55,9 +58,14 @@ __device__ __forceinline__ int count_of(const PagedArgs &a, int s, int first) {
 // would have to spill.
 template <class T, int NC, int RW> constexpr bool kThree = RW == 4 && NC == 4 && sizeof(T) == 2;
 
+// 16 rows of 64 dims in f16: 128 registers, four workgroups a CU (130 without the bound)
+template <class T, int NC, int RW> constexpr bool kFour = RW == 1 && NC == 2 && Frag<T>::kParts == 2;
+
 // RW: tiles of 16 rows of a workgroup
 template <class T, int NC, bool FULL, int RW>
-__global__ void __launch_bounds__(64 * kWaves, (kThree<T, NC, RW> ? 3 : kResident<T, NC, FULL>))
+__global__ void __launch_bounds__(64 * kWaves, (kThree<T, NC, RW>          ? 3
+                                                : kFour<T, NC, RW> && FULL ? 4
+                                                                           : kResident<T, NC, FULL>))
     k_attend_new(PagedArgs a, KvPool<T> pool) {
   using W = Rows<T, NC, FULL, true, kThree<T, NC, RW> ? 3 : 0>;
   __shared__ __align__(16) uint8_t lds[W::kLdsBytes];

@@ -260,6 +260,36 @@ def test_future_positions_do_not_count():
     assert (before[:4] == after[:4]).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("hd,new,length", [(64, 9, 100), (128, 9, 1500), (72, 40, 90), (128, 40, 2000)])
+def test_rows_that_see_what_is_not_finite(dtype, bad, hd, new, length):
+    """one dim of one value (or key) of a late token: the rows before it are as they were"""
+    c = Case(15, dtype, 16, 2, hd, 4, [new, 3], [length, 50])
+    c.call()
+    R.sync()
+    before = c.got()
+    at, w = length - 4, 2 * hd  # seen by the last four tokens; kv head 0's rows come first
+    rows = np.r_[0:new - 4, new:len(before)]
+    for which in ("v", "k"):
+        x = getattr(c.pool, which)
+        kept = x.copy()
+        x[:, c.table[0, at // 16], 1, at % 16, 5] = R.store(np.float32(bad).reshape(1), dtype)[0]
+        c.pool.upload()
+        c.call()
+        R.sync()
+        after = c.got()
+        setattr(c.pool, which, kept)
+        assert np.isfinite(after[rows]).all(), which
+        if which == "v":
+            assert (after[rows] == before[rows]).all()
+            assert (after[new - 4:new, :w] == before[new - 4:new, :w]).all()
+            assert (~np.isfinite(after[new - 4:new, w + 5])).all()
+        else:  # (a score of +inf in a row has the others of its wave rescaled: 2e-5 as in check())
+            off = np.linalg.norm(after[rows] - before[rows])
+            assert off <= 4e-5 * np.linalg.norm(before[rows])
+
+
 def test_one_token_is_the_prefix_operator():
     """a token a sequence: the attention of one query with an empty prefix"""
     c = Case(10, "f16", 16, 8, 128, 16, [1] * 5, [700, 33, 1, 4000, 128])
