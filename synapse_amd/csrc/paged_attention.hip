@@ -191,11 +191,16 @@ template <int LANES> __global__ void __launch_bounds__(256) k_join_few(PagedArgs
 
 // ---------------------------------------------------------------- host
 constexpr double kMostSpace = 192 << 20;  // of a workspace, where runs need not be split
+constexpr size_t kMostWgs = kMaxThreads / (64 * kWaves);  // of a launch, of either kernel
 
 struct Plan {
   bool solo;
   int nc, rw, blocks, chunk, parts;
-  size_t wgs, rows, po_bytes, pml_bytes;
+  size_t seqs;  // of a launch; 0: not even one
+  size_t po_bytes, pml_bytes;
+  size_t wgs(size_t n, size_t nkv) const {
+    return round_up(solo ? cdiv(n * nkv * parts, kWaves) : n * nkv * parts, 8) * blocks;
+  }
 };
 
 Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_paged_attention_params &p) {
@@ -206,7 +211,6 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_paged_attention_params 
   const bool small = w.nc * (pg.dtype == SYN_HIP_KV_F32 ? 2 : 1) <= 4;  // (a ring of four tiles)
   w.rw = rows <= 16 ? 1 : (rows <= 32 ? (small ? 2 : 1) : 4);
   w.blocks = (int)cdiv(rows, 16 * w.rw);
-  w.rows = (size_t)p.n_seqs * p.max_new * p.n_heads;
   // the positions of a workgroup's rows
   const size_t tokens = std::min<size_t>(p.max_new, 16 * w.rw / rep + 2);
   const size_t span = p.window ? std::min<size_t>(p.max_len, (size_t)p.window + tokens + kTile) : p.max_len;
@@ -255,8 +259,12 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_paged_attention_params 
     cut(best);
   }
   w.solo = alone(units * w.parts, w.chunk / kTile);
-  const size_t work = units * w.parts;
-  w.wgs = round_up(w.solo ? cdiv(work, kWaves) : work, 8) * w.blocks;
+  // Most calls are one launch.  Every sequence counts as max_new tokens here, so a
+  // batch with few tokens may need more workgroups, or more rows joined, than a
+  // launch takes: then some sequences at a time.
+  w.seqs = kMostWgs / w.blocks / 8 * 8 * (w.solo ? kWaves : 1) / ((size_t)nkv * w.parts);
+  if (w.parts > 1) w.seqs = std::min(w.seqs, kMostWgs / ((size_t)p.max_new * p.n_heads));
+  w.seqs = std::min<size_t>(w.seqs, p.n_seqs);
   if (w.parts > 1) {
     const size_t n = (size_t)p.n_tokens * p.n_heads * w.parts;
     w.po_bytes = round_up(n * hd * 4, 16);
@@ -285,17 +293,16 @@ syn_status_t check(const syn_hip_kv_pages *pages, const syn_hip_paged_attention_
     return SYN_ERR_SHAPE_MISMATCH;
   }
   if (!p->n_seqs || !p->max_new || !p->n_tokens) return SYN_OK;
-  const Plan w = make_plan(*pages, *p);
-  if (w.wgs > kMaxThreads / (64 * kWaves) || (w.parts > 1 && w.rows > kMaxThreads / 256)) {
-    set_error("paged_attention: more workgroups than a launch takes");
+  if (!make_plan(*pages, *p).seqs) {
+    set_error("paged_attention: a sequence of more rows than a launch takes");
     return SYN_ERR_INVALID_ARG;
   }
   return SYN_OK;
 }
 
 template <class T, int NC, int RW>
-void launch_rows(const Plan &w, const PagedArgs &a, const KvPool<T> &pool, hipStream_t s) {
-  const dim3 grid((unsigned)w.wgs), block(64 * kWaves);
+void launch_rows(size_t wgs, const PagedArgs &a, const KvPool<T> &pool, hipStream_t s) {
+  const dim3 grid((unsigned)wgs), block(64 * kWaves);
   if (pool.hd == 32 * NC)
     hipLaunchKernelGGL((k_attend_new<T, NC, true, RW>), grid, block, 0, s, a, pool);
   else
@@ -303,21 +310,40 @@ void launch_rows(const Plan &w, const PagedArgs &a, const KvPool<T> &pool, hipSt
 }
 template <class T, int NC>
 syn_status_t launch(const Plan &w, const PagedArgs &a, const KvPool<T> &pool, hipStream_t s) {
+  const size_t wgs = w.wgs(a.n_seqs, pool.nkv);
   if (w.rw == 1)
-    launch_rows<T, NC, 1>(w, a, pool, s);
+    launch_rows<T, NC, 1>(wgs, a, pool, s);
   else if (w.rw == 4)
-    launch_rows<T, NC, 4>(w, a, pool, s);
+    launch_rows<T, NC, 4>(wgs, a, pool, s);
   else if constexpr (Rows<T, NC, true, true>::kRing == 4)
-    launch_rows<T, NC, 2>(w, a, pool, s);
+    launch_rows<T, NC, 2>(wgs, a, pool, s);
   SYN_LAUNCH_CHECK();
   if (w.parts == 1) return SYN_OK;
+  const size_t rows = (size_t)a.n_seqs * a.max_new * a.nh;
   if (w.parts <= kFewParts)
-    hipLaunchKernelGGL((k_join_few<8 * NC>), dim3((unsigned)cdiv(w.rows, 256 / (8 * NC))), dim3(256), 0, s, a,
-                       pool.hd, (uint32_t)w.rows);
+    hipLaunchKernelGGL((k_join_few<8 * NC>), dim3((unsigned)cdiv(rows, 256 / (8 * NC))), dim3(256), 0, s, a,
+                       pool.hd, (uint32_t)rows);
   else
-    hipLaunchKernelGGL((k_join_new<8 * NC>), dim3((unsigned)w.rows), dim3(256), 0, s, a, pool.hd);
+    hipLaunchKernelGGL((k_join_new<8 * NC>), dim3((unsigned)rows), dim3(256), 0, s, a, pool.hd);
   SYN_LAUNCH_CHECK();
   return SYN_OK;
+}
+
+// sequences first .. first + n - 1 of a call
+PagedArgs some_of(const PagedArgs &a, int hd, size_t first, size_t n) {
+  PagedArgs b = a;
+  b.n_seqs = (int)n;
+  b.len += first;
+  if (b.table) b.table += first * a.ld_table;
+  if (b.start) {
+    b.start += first;
+  } else {
+    const size_t rows = first * a.max_new, parts = rows * a.nh * a.parts;
+    b.q += rows * a.ldq;
+    b.out += rows * a.ldo;
+    if (a.parts > 1) b.po += parts * hd, b.pml += parts * 2;
+  }
+  return b;
 }
 
 }  // namespace
@@ -386,8 +412,11 @@ extern "C" syn_status_t syn_hip_paged_attention(const syn_hip_kv_pages *pages,
   return kv_dispatch(pages->dtype, [&](auto t) -> syn_status_t {
     using T = decltype(t);
     const KvPool<T> pool = kv_pool<T>(*pages, p->layer);
-    if (w.nc == 2) return launch<T, 2>(w, a, pool, s);
-    if (w.nc == 4) return launch<T, 4>(w, a, pool, s);
-    return launch<T, 8>(w, a, pool, s);
+    for (size_t i = 0; i < p->n_seqs; i += w.seqs) {
+      const PagedArgs b = some_of(a, pool.hd, i, std::min<size_t>(w.seqs, p->n_seqs - i));
+      SYN_TRY(w.nc == 2 ? (launch<T, 2>(w, b, pool, s))
+                        : (w.nc == 4 ? (launch<T, 4>(w, b, pool, s)) : (launch<T, 8>(w, b, pool, s))));
+    }
+    return SYN_OK;
   });
 }
