@@ -855,8 +855,10 @@ syn_status_t syn_hip_paged_attention(const syn_hip_kv_pages *pages,
  * counts as -inf; a row whose largest is +inf shares its probability among the
  * infinities; a draft outside the vocabulary is not accepted; where row r has no
  * logit above -inf the token is pad (and counted) with log-probability -inf.
- * Exponentials and sums are f64: a token differs from the formula's only where u
- * falls within 2^-40 of a border.  d_token is apart from the other buffers.  At most 64 drafts, n_seqs *
+ * Exponentials and sums are f64, p_i and q_i within 2^-42 of themselves: a token
+ * differs from the formula's only where u falls within 2^-40 of a border, or, after
+ * a rejected draft, within 2^-40 / S of one, S being the sum of max(p_r - q_r, 0).
+ * d_token is apart from the other buffers.  At most 64 drafts, n_seqs *
  * (2 max_draft + 1) at most 65535.  The workspace (16-byte aligned) is needed by
  * every call. */
 typedef struct {
