@@ -902,8 +902,9 @@ syn_status_t syn_hip_kv_resize(const syn_hip_kv_tables *t, const int32_t *d_len,
  * below 0: 0): full pages are shared, one that is not full is copied, every
  * layer, positions up to the next multiple of 8, into a page that is taken for
  * it (where none is free, the row ends with the full ones).  A row whose
- * d_parent is itself or outside [0, n_seqs), or whose parent continues another
- * row, stays as it is.  pages and t have the same n_pages and page_size. */
+ * d_parent is itself or outside [0, n_seqs) stays as it is, and so does one whose
+ * parent's own d_parent is not the parent: the rows that others continue name
+ * themselves.  pages and t have the same n_pages and page_size. */
 syn_status_t syn_hip_kv_fork(const syn_hip_kv_pages *pages, const syn_hip_kv_tables *t,
                              const int32_t *d_parent, const int32_t *d_len, void *d_workspace,
                              size_t workspace_bytes, void *stream);
