@@ -913,7 +913,9 @@ syn_status_t syn_hip_kv_fork(const syn_hip_kv_pages *pages, const syn_hip_kv_tab
  * -1 behind what a row holds.  *d_live (device) is how many there are: those
  * that the other pool has no page for are left out, and entries that name them
  * become -1.  The pools have the same pages but for their number, and overlap
- * nowhere; the tables have the same rows, u at least as many columns.  The
+ * nowhere; the tables have the same rows, u at least as many columns.  Tables of
+ * no rows (n_seqs 0): nothing is done, *d_live is not written; pages that are kept
+ * by the caller's own counts alone are moved with one row that holds none.  The
  * workspace is t's. */
 syn_status_t syn_hip_kv_compact(const syn_hip_kv_pages *from, const syn_hip_kv_tables *t,
                                 const syn_hip_kv_pages *to, const syn_hip_kv_tables *u,
