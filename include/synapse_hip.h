@@ -817,6 +817,7 @@ syn_status_t syn_hip_klm_generate_beams(syn_hip_klm_t *m, const uint32_t *prompt
  * be NaN in every dim; one that does not see it stays what it is).  max_new,
  * max_len and n_tokens decide the split of the work, so a captured call keeps
  * them.  d_out is apart from d_q.  At most 65535 sequences, max_len 2^31 - 2^16,
+ * max_new n_tokens (n_tokens may count rows of no sequence),
  * the rows of max_new tokens below 2^30 - 63 (n_kv_heads up to the next multiple of
  * 8 times max_new * n_heads / n_kv_heads up to one of 64).  The workspace (which may
  * be 0; 16-byte aligned) holds the parts of split runs. */
@@ -837,7 +838,7 @@ syn_status_t syn_hip_paged_attention(const syn_hip_kv_pages *pages,
 /* Verification of drafted tokens.  Sequence s has n = d_n_draft[s] drafts (NULL:
  * max_draft; cut to it), d_drafted [n_seqs][max_draft].  p_i is the softmax of
  * logits row i of the target at s * target_stride + i * ld_target floats (0 to n;
- * a stride may be 0), divided by the temperature d_temperature[s] (NULL: 1), q_i
+ * a stride may be 0, ld_target, and ld_draft where it is used, vocab or more), divided by the temperature d_temperature[s] (NULL: 1), q_i
  * that of the draft's row at s * draft_stride + i * ld_draft (0 to n - 1; d_draft
  * NULL: drafts that were certain, q 1 at the draft and 0 elsewhere).  Draft x_i
  * is accepted when all before it are and u_i q_i(x_i) < p_i(x_i), u_i being
