@@ -939,7 +939,8 @@ syn_status_t syn_hip_kv_compact(const syn_hip_kv_pages *from, const syn_hip_kv_t
  * sample n_draft for the drafts, n_draft for their acceptance, one for the token
  * after them.  Keys and values are kept in kv_dtype.  1 to 64 samples, at most 16
  * drafts, n_samples * (n_draft + 1) <= max_seq, n_prompt + max_new - 1 + n_draft
- * <= max_seq.  Afterwards the model's own cache holds the prompt. */
+ * <= max_seq.  Afterwards the model's own cache holds the prompt.  max_new 0: nothing
+ * is run, lengths and rounds are 0. */
 typedef struct {
   uint32_t n_samples, n_draft, draft_layers;
   int32_t eos, kv_dtype; /* SYN_HIP_KV_* */

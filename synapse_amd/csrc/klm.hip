@@ -1411,14 +1411,13 @@ syn_status_t syn_hip_klm_generate_samples(syn_hip_klm_t *m, const uint32_t *prom
                                           uint32_t *out_rounds) {
   SYN_TRY(check_klm(m));
   if (!prompt || !p || !out_tokens) return SYN_ERR_NULL_PTR;
-  if (max_new == 0) return SYN_OK;
   if (p->n_samples == 0 || p->n_samples > kMaxBeams || p->n_draft > 16 ||
       (size_t)p->n_samples * (p->n_draft + 1) > m->S) {
     set_error("samples: 1 to 64 with at most 16 drafts, max_seq rows of them a round");
     return SYN_ERR_INVALID_ARG;
   }
-  if (n_prompt == 0 || n_prompt > m->S || max_new - 1 > m->S - n_prompt ||
-      p->n_draft > m->S - n_prompt - (max_new - 1)) {
+  const size_t fed = max_new ? max_new - 1 : 0;  // tokens that follow the prompt through the model
+  if (n_prompt == 0 || n_prompt > m->S || fed > m->S - n_prompt || p->n_draft > m->S - n_prompt - fed) {
     set_error("samples: prompt + generated tokens + drafts must be in [1, max_seq]");
     return SYN_ERR_INVALID_ARG;
   }
@@ -1437,6 +1436,11 @@ syn_status_t syn_hip_klm_generate_samples(syn_hip_klm_t *m, const uint32_t *prom
   if (m->hd % 8 || m->hd > kKvMaxHeadDim) {
     set_error("samples: head_dim must be a multiple of 8 up to 256");
     return SYN_ERR_INVALID_ARG;
+  }
+  if (max_new == 0) {
+    if (out_lengths) std::fill_n(out_lengths, p->n_samples, 0u);
+    if (out_rounds) *out_rounds = 0;
+    return SYN_OK;
   }
   const size_t layers = p->draft_layers ? p->draft_layers : std::max<size_t>(1, m->L / 3);
   try {
