@@ -780,7 +780,8 @@ syn_status_t syn_hip_beam_reorder_pages(const syn_hip_kv_pages *pages, size_t n_
  * score the sum of the tokens' log-probabilities).  A beam ends with `eos`
  * (-1: none) and competes with its score from then on.  The keys and values of
  * prompt and beams are kept in kv_dtype; n_prompt + max_new - 1 <= max_seq.
- * Afterwards the model's own cache holds the prompt. */
+ * Afterwards the model's own cache holds the prompt.  max_new 0: nothing is run,
+ * lengths and scores are 0. */
 typedef struct {
   uint32_t n_beams;
   int32_t eos, kv_dtype; /* SYN_HIP_KV_* */

@@ -1372,8 +1372,7 @@ syn_status_t syn_hip_klm_generate_beams(syn_hip_klm_t *m, const uint32_t *prompt
                                         float *out_scores) {
   SYN_TRY(check_klm(m));
   if (!prompt || !p || !out_tokens) return SYN_ERR_NULL_PTR;
-  if (max_new == 0) return SYN_OK;
-  if (n_prompt == 0 || n_prompt > m->S || max_new - 1 > m->S - n_prompt) {
+  if (n_prompt == 0 || n_prompt > m->S || (max_new ? max_new - 1 : 0) > m->S - n_prompt) {
     set_error("beam search: prompt + generated tokens must be in [1, max_seq]");
     return SYN_ERR_INVALID_ARG;
   }
@@ -1396,6 +1395,11 @@ syn_status_t syn_hip_klm_generate_beams(syn_hip_klm_t *m, const uint32_t *prompt
   if (m->hd % 8 || m->hd > kKvMaxHeadDim) {
     set_error("beam search: head_dim must be a multiple of 8 up to 256");
     return SYN_ERR_INVALID_ARG;
+  }
+  if (max_new == 0) {
+    if (out_lengths) std::fill_n(out_lengths, p->n_beams, 0u);
+    if (out_scores) std::fill_n(out_scores, p->n_beams, 0.0f);
+    return SYN_OK;
   }
   try {
     return m->generate_beams(prompt, n_prompt, max_new, *p, out_tokens, out_lengths, out_scores);
