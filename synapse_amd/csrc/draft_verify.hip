@@ -65,7 +65,7 @@ struct VerifyArgs {
   uint64_t *weight;  // [n_seqs][blocks] sums (f64)
   int32_t *done;     // [n_seqs] workgroups that have theirs
   size_t ld_target, target_stride, ld_draft, draft_stride;
-  int n_seqs, K, rows, vocab, chunks, per, blocks, draws;  // per: tokens of a chunk, whole blocks
+  int K, rows, vocab, chunks, per, blocks, draws;  // per: tokens of a chunk, whole blocks
   uint32_t pad;
 };
 
@@ -627,7 +627,6 @@ syn_status_t syn_hip_draft_verify(const syn_hip_draft_verify_params *p, const fl
   a.target_stride = p->target_stride;
   a.ld_draft = p->ld_draft;
   a.draft_stride = p->draft_stride;
-  a.n_seqs = (int)p->n_seqs;
   a.K = (int)p->max_draft;
   a.rows = a.draft ? sp.rows : a.K + 1;
   a.vocab = (int)p->vocab;

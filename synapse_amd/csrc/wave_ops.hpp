@@ -71,6 +71,5 @@ template <class F> __device__ __forceinline__ F wave_upto(F x) {
 }
 // the sum over the lanes below this one, given that up to it
 template <class F> __device__ __forceinline__ F wave_shifted(F upto) { return from_lane<0x138, 0xf>(upto); }
-template <class F> __device__ __forceinline__ F wave_before(F x) { return wave_shifted(wave_upto(x)); }
 
 }  // namespace syn
