@@ -541,8 +541,11 @@ struct Space {
 Space space_of(const syn_hip_draft_verify_params &p) {
   Space s;
   s.rows = 2 * (int)p.max_draft + 1;
-  // Chunks of 2048 tokens, of up to 16384 as long as 2048 workgroups, all that the
-  // chip holds at eight a CU, are left: a row's chunks are joined one by one.
+  // Chunks of 2048 tokens, of up to 16384 as long as 2048 workgroups are left: a row's
+  // chunks are joined one by one.  (64 sequences of up to 8 drafts, 151936 tokens, 124
+  // us, 203 in chunks of 2048 alone; 32000 tokens 47 and 65.  The chip holds 1280, five
+  // a CU by their 90 registers: down to as many, 8 sequences of 4 drafts and 151936
+  // tokens 32.0 where this takes 33.3, the rest the same.)
   s.per = kBlock;
   while (s.per < 8 * kBlock && p.n_seqs * (size_t)s.rows * cdiv(p.vocab, 2 * s.per) >= 2048) s.per *= 2;
   s.chunks = (int)cdiv(p.vocab, s.per);

@@ -16,11 +16,12 @@
 // in f16): up to 32 rows of a kv head, bytes: 64 sequences of one token at up to
 // 12000 positions, 32 heads of 64, bf16, 211 us, 5.6 TB/s; 24 of up to 8 tokens at
 // 8200, 32 heads of 128, f16, 131 to 143 us, 4.7 to 4.3 TB/s.  Chunks, their steps
-// of a tile: two of 1536 tokens at 12001, 24 heads of 128, f16, 661 to 734 us, 500
+// of a tile: two of 1536 tokens at 12001, 24 heads of 128, f16, 661 to 760 us, 483
 // to 555 TFLOP/s of the formula and twice that in matrix instructions with the
 // operands' second parts, which take 51 % of the SIMDs' cycles, the vector ones 60 %
-// (with two workgroups a CU 815 to 893 us, 41 and 48 %).  Four sequences of
-// five tokens at 213, f32: 10.1 us, one launch and dependent loads.
+// (with two workgroups a CU 815 to 893 us, 41 and 48 %): a wave's scores, weights and
+// values of a tile come one after the other.  Four sequences of five tokens at 213,
+// f32: 10.1 us, one launch and dependent loads.
 #include <algorithm>
 #include <cmath>
 
@@ -55,7 +56,8 @@ __device__ __forceinline__ int count_of(const PagedArgs &a, int s, int first) {
 // 64 rows of 128 dims in 16 bits: a ring of three tiles and 168 registers leave
 // room for three workgroups a CU (30 chunks of 100 tokens at 1000, 32 heads of 128,
 // f16, 92 us, 107 with two; two of 1200 at 9000, bf16, 752 and 789).  Four in f16
-// would have to spill.
+// would have to spill.  (Of all instances one does: f32, heads of 136 to 248, 16 rows
+// to a workgroup, 98 registers, 216 bytes a lane.)
 template <class T, int NC, int RW> constexpr bool kThree = RW == 4 && NC == 4 && sizeof(T) == 2;
 
 // 16 rows of 64 dims in f16: 128 registers, four workgroups a CU (130 without the bound)
@@ -215,7 +217,8 @@ Plan make_plan(const syn_hip_kv_pages &pg, const syn_hip_paged_attention_params 
   const size_t tokens = std::min<size_t>(p.max_new, 16 * w.rw / rep + 2);
   const size_t span = p.window ? std::min<size_t>(p.max_len, (size_t)p.window + tokens + kTile) : p.max_len;
   const size_t tiles = cdiv(span, kTile), units = (size_t)p.n_seqs * nkv;
-  // workgroups that the chip holds at once
+  // workgroups that the chip holds at once (with 16 rows each one a CU fewer where
+  // heads do not fill their tiles, f32 or f16, and of 64 dims in bf16)
   const bool f32 = pg.dtype == SYN_HIP_KV_F32;
   const size_t want = w.nc == 8 ? 256 : (w.nc == 2 && !f32 ? 1024 : (w.rw == 4 && !f32 ? 768 : 512));
   const size_t whole = pg.dtype == SYN_HIP_KV_F32 ? 2 : (units <= 512 ? 8 : 4);
