@@ -817,11 +817,11 @@ syn_status_t syn_hip_klm_generate_beams(syn_hip_klm_t *m, const uint32_t *prompt
  * syn_hip_prefix_attention (a row that sees a key or value that is not finite may
  * be NaN in every dim; one that does not see it stays what it is).  max_new,
  * max_len and n_tokens decide the split of the work, so a captured call keeps
- * them.  d_out is apart from d_q.  At most 65535 sequences, max_len 2^31 - 2^16,
- * max_new n_tokens (n_tokens may count rows of no sequence),
- * the rows of max_new tokens below 2^30 - 63 (n_kv_heads up to the next multiple of
- * 8 times max_new * n_heads / n_kv_heads up to one of 64).  The workspace (which may
- * be 0; 16-byte aligned) holds the parts of split runs. */
+ * them.  d_out is apart from d_q.  At most 65535 sequences, max_len at most 2^31 -
+ * 2^16, max_new at most n_tokens (which may count rows of no sequence), the query rows
+ * of max_new tokens at most 2^30 - 64 (max_new * n_heads / n_kv_heads up to the next
+ * multiple of 64, times n_kv_heads up to one of 8).  The workspace (which may be 0;
+ * 16-byte aligned) holds the parts of split runs. */
 typedef struct {
   uint32_t layer, n_heads, n_seqs, n_tokens, max_new, max_len, window;
   float scale;

@@ -50,6 +50,14 @@ def test_more_than_one_launch(case):
     c.call()
     R.sync()
     c.check()
+    first = c.got()
+    g = R.Graph(lambda s: c.call(s))  # the same, captured and replayed
+    for _ in range(3):
+        c.bufs["out"].upload(np.full(first.shape, 7.0, np.float32))
+        R.sync()
+        g.replay()
+        assert (c.got() == first).all()
+    g.close()
 
 
 def test_more_kv_heads_than_a_launch_holds_without_starts():
